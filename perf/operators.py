@@ -145,6 +145,11 @@ def _heads_data(shape, gen, dtype):
     return (x * size).to(dtype)
 
 
+def _pow2(e):
+    """2**e in fp32 for whole numbers e in [-126, 128), by its bits."""
+    return ((e.to(torch.int32) + 127) << 23).view(torch.float32)
+
+
 def _quantize(x, dtype):
     """(codes, scales) of x [..., D], by comparisons with the code borders."""
     blocks = x.float().unflatten(-1, (-1, 32))
@@ -153,7 +158,7 @@ def _quantize(x, dtype):
     e = exp - 3 + (mant >= 0.875).to(exp.dtype)
     lo, hi = (-23, 13) if dtype == torch.float16 else (-100, 125)
     e = torch.where(a == 0, lo, e).clamp(lo, hi)
-    y = torch.ldexp(blocks, -e.unsqueeze(-1))
+    y = blocks * _pow2(-e).unsqueeze(-1)
     mag = y.abs()
     # ties go to the even code: above 1/4, from 3/4, above 5/4, from 7/4, ...
     code = ((mag > 0.25).to(torch.uint8) + (mag >= 0.75) + (mag > 1.25) + (mag >= 1.75)
@@ -339,7 +344,7 @@ def _plain_values(codes, scales):
     lut = torch.tensor(_E2M1 + tuple(-v for v in _E2M1), device=codes.device)
     nib = torch.stack([codes & 15, codes >> 4], -1).flatten(-2)
     x = lut[nib.int()].unflatten(-1, (-1, 32))
-    f = torch.where(scales == 255, math.nan, torch.ldexp(torch.ones((), device=codes.device), scales.int() - 127))
+    f = torch.where(scales == 255, math.nan, _pow2(scales.int() - 127))
     return (x * f.unsqueeze(-1)).flatten(-2)
 
 
@@ -396,6 +401,10 @@ def work(case):
 # in 64 bits
 # ---------------------------------------------------------------------------
 
+def _power(e):
+    return ((e + 1023) << 52).view(torch.float64)
+
+
 def _exact_values(codes, scales):
     """E2M1 by its fields: s eem -> (-1)^s 2^(ee-1) (1 + m/2), 0 and 1/2 below."""
     nib = torch.empty(codes.shape[:-1] + (2 * codes.shape[-1],), dtype=torch.float64, device="cuda")
@@ -403,7 +412,7 @@ def _exact_values(codes, scales):
         ee, mm = ((n >> 1) & 3).double(), (n & 1).double()
         mag = torch.where(ee == 0, 0.5 * mm, 2.0 ** (ee - 1) * (1 + 0.5 * mm))
         nib[..., i::2] = torch.where(n >= 8, -mag, mag)
-    f = torch.pow(2.0, scales.double() - 127)
+    f = torch.where(scales == 255, math.nan, _power(scales.long() - 127))
     return nib * f.repeat_interleave(32, -1)
 
 
@@ -412,17 +421,15 @@ def _exact_round(x, dtype):
     the block's scale, the even code where two are as near."""
     y = x.double().unflatten(-1, (-1, 32))
     a = y.abs().amax(-1, keepdim=True)
-    fl = torch.floor(torch.log2(torch.where(a > 0, a, 1.0)))
-    fl = torch.where(torch.pow(2.0, fl) > a, fl - 1, fl)
-    fl = torch.where(torch.pow(2.0, fl + 1) <= a, fl + 1, fl)
-    e = fl - 2 + (a >= 1.75 * torch.pow(2.0, fl)).double()
-    lo, hi = (-23.0, 13.0) if dtype == torch.float16 else (-100.0, 125.0)
+    fl = (a.view(torch.int64) >> 52) - 1023  # floor(log2 a)
+    e = fl - 2 + (a >= 1.75 * _power(fl)).long()
+    lo, hi = (-23, 13) if dtype == torch.float16 else (-100, 125)
     e = torch.where(a > 0, e, lo).clamp(lo, hi)
-    r = (y / torch.pow(2.0, e)).abs().clamp(max=6.0)
+    r = (y * _power(-e)).abs().clamp(max=6.0)
     # the grid's step: 1/2 below 2, 1 below 4, 2 above; round() ties to even
     step = torch.where(r < 2, 0.5, torch.where(r < 4, 1.0, 2.0))
     r = torch.round(r / step) * step
-    return (torch.sign(y) * r * torch.pow(2.0, e)).flatten(-2)
+    return (torch.sign(y) * r * _power(e)).flatten(-2)
 
 
 def _exact_of_rows(s, cache, table, lens, start):
