@@ -1,0 +1,254 @@
+"""paged_kv_append_fp4 and paged_kv_gather_fp4: exact, against the quantiser in
+64 bits (fp4_ref)."""
+
+import math
+
+import pytest
+import torch
+
+import fp4_ref as R
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.float16, torch.bfloat16, torch.float32]
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.fail("GPU tests need an MI355X")
+
+
+def tables(lens, page, seed, spare=2):
+    """Two shuffled block tables over one pool, padding -1."""
+    g = torch.Generator().manual_seed(seed)
+    need = [-(-n // page) for n in lens]
+    pages, width = sum(need) + spare, max(need + [1])
+    out = []
+    for _ in range(2):
+        perm, t, at = torch.randperm(pages, generator=g), torch.full((len(lens), width), -1), 0
+        for b, n in enumerate(need):
+            t[b, :n] = perm[at:at + n]
+            at += n
+        out.append(t.to(torch.int32))
+    return out[0], out[1], pages
+
+
+def place(table, b, n, page):
+    return table[b, n // page].item(), n % page
+
+
+def rows_of(T, H, D, dtype, seed):
+    """Blocks of many sizes, with ties, signed zeros and blocks of zeros."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(T, H, D, generator=g)
+    x = x * torch.exp2(torch.randint(-9, 9, (T, H, D // 32), generator=g).float()
+                       ).repeat_interleave(32, -1)
+    x[0] = 0.0
+    x[0, 0, 1] = -0.0
+    ties = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0] * 4)
+    x[-1, :, :32] = ties
+    x[-1, :, 32:64] = -ties * 2.0 ** -7
+    x[T // 2, 0, :32] = torch.linspace(-7, 7, 32)         # the step's border is 7
+    x[T // 2, 0, 32:64] = torch.linspace(-6.999, 6.999, 32)
+    return x.to(dtype)
+
+
+def indptr(lens):
+    return torch.tensor([0] + list(lens)).cumsum(0).to(torch.int32)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,H,page", [(64, 1, 16), (64, 3, 5), (128, 8, 16), (128, 2, 1),
+                                      (128, 5, 64), (256, 2, 16), (256, 1, 7)])
+def test_append_then_gather(dtype, D, H, page):
+    from kernels import allocate_fp4_cache, paged_kv_append_fp4, paged_kv_gather_fp4
+    lens, start = [1, 0, 37, 70, 5], [0, 9, 3, 130, 15]
+    T = sum(lens)
+    k, v = rows_of(T, H, D, dtype, 1), rows_of(T, H, D, dtype, 2)
+    kt, vt, pages = tables([a + b for a, b in zip(lens, start)], page, 3)
+    kc, vc = (allocate_fp4_cache(pages, page, H, D) for _ in range(2))
+    ip, sp = indptr(lens).cuda(), torch.tensor(start, dtype=torch.int32).cuda()
+    paged_kv_append_fp4(kc, vc, kt.cuda(), vt.cuda(), k.cuda(), v.cuda(), ip, start_pos=sp)
+    for x, cache, table in ((k, kc, kt), (v, vc, vt)):
+        val, nib, scale = R.quantize(x)
+        codes, scales = torch.zeros_like(cache.codes.cpu()), torch.zeros_like(cache.scales.cpu())
+        t = 0
+        for b, n in enumerate(lens):
+            for j in range(n):
+                pg, off = place(table, b, start[b] + j, page)
+                codes[pg, :, off], scales[pg, :, off] = R.pack(nib[t]), scale[t]
+                t += 1
+        assert torch.equal(cache.codes.cpu(), codes)
+        assert torch.equal(cache.scales.cpu(), scales)
+    for to in DTYPES:
+        if dtype != to and to == torch.float16:
+            continue  # (values of other types need not be exact in fp16)
+        gk, gv = paged_kv_gather_fp4(kc, vc, kt.cuda(), vt.cuda(), ip, T, sp, dtype=to)
+        assert gk.dtype == to
+        assert torch.equal(gk.cpu().double(), R.quantize(k)[0])
+        assert torch.equal(gv.cpu().double(), R.quantize(v)[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_extreme_values(dtype):
+    """The largest, the smallest, infinities and NaN; error within 1/7 of the
+    block's largest inside the type's range of powers."""
+    from kernels import allocate_fp4_cache, paged_kv_append_fp4, paged_kv_gather_fp4
+    f = torch.finfo(dtype)
+    x = torch.zeros(12, 1, 64)
+    x = x.to(torch.float64)
+    x[0, 0, :] = f.max
+    x[1, 0, :] = torch.linspace(-1, 1, 64, dtype=torch.float64) * f.max
+    x[2, 0, :] = f.smallest_normal
+    x[3, 0, 5] = f.smallest_normal * f.eps                # the smallest number
+    x[4, 0, 3] = math.inf
+    x[5, 0, 40] = -math.inf
+    x[6, 0, 63] = math.nan
+    x[7, 0, :32] = 2.0 ** -14
+    x[8, 0, :] = torch.linspace(-1, 1, 64, dtype=torch.float64) * 2.0 ** -100 if dtype != torch.float16 else 0
+    x[9, 0, :] = 49152.0
+    x[10, 0, :] = torch.randn(64, generator=torch.Generator().manual_seed(0), dtype=torch.float64)
+    x[11, 0, ::2] = -f.max
+    x = x.to(dtype)
+    kt = torch.zeros(1, 1, dtype=torch.int32).cuda()
+    kc = allocate_fp4_cache(1, 12, 1, 64)
+    ip = indptr([12]).cuda()
+    paged_kv_append_fp4(kc, None, kt, None, x.cuda(), None, ip)
+    val, nib, scale = R.quantize(x)
+    assert torch.equal(kc.codes[0, 0].cpu(), R.pack(nib)[:, 0])
+    assert torch.equal(kc.scales[0, 0].cpu(), scale[:, 0])
+    got, none = paged_kv_gather_fp4(kc, None, kt, None, ip, 12, dtype=dtype)
+    assert none is None
+    got = got.cpu().double()
+    assert torch.equal(torch.isnan(got), torch.isnan(val))
+    assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(val))
+    assert torch.isnan(got[4, 0, :32]).all() and (got[4, 0, 32:] == 0).all()
+    a = x[10].double().unflatten(-1, (-1, 32))
+    err = (got[10].unflatten(-1, (-1, 32)) - a).abs().amax(-1)
+    assert (err <= a.abs().amax(-1) / 7).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_without_a_place(dtype):
+    """Pages past the table or outside the pool are skipped by the writer and
+    zeros to the reader; rows that no sequence holds stay as they are."""
+    from kernels import allocate_fp4_cache, paged_kv_append_fp4, paged_kv_gather_fp4
+    H, D, page = 2, 64, 4
+    x = rows_of(20, H, D, dtype, 4)
+    kt = torch.tensor([[2, -1, 7], [0, 3, 1]], dtype=torch.int32)  # pages 0..3
+    kc = allocate_fp4_cache(4, page, H, D)
+    ip = torch.tensor([2, 12, 18], dtype=torch.int32)  # rows 0, 1, 18, 19: nobody's
+    sp = torch.tensor([0, 8], dtype=torch.int32)
+    args = (kc, None, kt.cuda(), None)
+    paged_kv_append_fp4(*args, x.cuda(), None, ip.cuda(), start_pos=sp.cuda())
+    want = torch.zeros(4, H, page, D // 2, dtype=torch.uint8)
+    nib = R.pack(R.quantize(x)[1])
+    for j in range(4):
+        want[2, :, j] = nib[2 + j]       # sequence 0: page 2, then none
+        want[1, :, j] = nib[12 + j]      # sequence 1: page 1, then past the table
+    assert torch.equal(kc.codes.cpu(), want)
+    out = torch.full((20, H, D), 7.0, dtype=dtype, device="cuda")
+    got, _ = paged_kv_gather_fp4(*args, ip.cuda(), 20, sp.cuda(), out=(out, None))
+    assert got is out
+    got, val = got.cpu().double(), R.quantize(x)[0]
+    for t in range(20):
+        exp = (torch.full((H, D), 7.0, dtype=torch.float64) if t < 2 or t >= 18
+               else val[t] if 2 <= t < 6 or 12 <= t < 16 else torch.zeros(H, D).double())
+        assert torch.equal(got[t], exp), t
+
+
+def test_strides_and_index_types():
+    """K and V views of one projection with strides of their own, unaligned rows,
+    int64 indices, tables that are slices."""
+    from kernels import allocate_fp4_cache, paged_kv_append_fp4
+    H, D, page, lens = 4, 128, 16, [3, 40]
+    T = sum(lens)
+    kt, vt, pages = tables(lens, page, 5)
+    wide = torch.cat([kt, kt + 100], 1).cuda()
+    qkv = rows_of(T, 3 * H, D, torch.bfloat16, 6).cuda()
+    k, v = qkv[:, H:2 * H], qkv[:, 2 * H:]
+    ip = indptr(lens).cuda()
+    want = [allocate_fp4_cache(pages, page, H, D) for _ in range(2)]
+    paged_kv_append_fp4(*want, kt.cuda(), vt.cuda(), k.contiguous(), v.contiguous(), ip)
+    off = torch.empty(T * H * D + 1, dtype=k.dtype, device="cuda")[1:].view(T, H, D).copy_(v)
+    for kk, vv in ((k, v), (k.contiguous(), v), (k, off),
+                   (k.transpose(0, 2).contiguous().transpose(0, 2), v)):
+        got = [allocate_fp4_cache(pages, page, H, D) for _ in range(2)]
+        paged_kv_append_fp4(*got, wide[:, :kt.shape[1]], vt.long().cuda(), kk, vv, ip.long())
+        for a, b in zip(got, want):
+            assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+
+
+def test_many_sequences():
+    """More sequences than the writer keeps in LDS, one row each."""
+    from kernels import allocate_fp4_cache, paged_kv_append_fp4, paged_kv_gather_fp4
+    n, H, D = 1500, 1, 64
+    x = rows_of(n, H, D, torch.float16, 8).cuda()
+    kt = torch.randperm(n, generator=torch.Generator().manual_seed(1)).to(torch.int32)[:, None].cuda()
+    kc = allocate_fp4_cache(n, 2, H, D)
+    ip = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    sp = torch.ones(n, dtype=torch.int32, device="cuda")
+    paged_kv_append_fp4(kc, None, kt, None, x, None, ip, start_pos=sp)
+    got, _ = paged_kv_gather_fp4(kc, None, kt, None, ip, n, sp, dtype=torch.float16)
+    assert torch.equal(got.cpu().double(), R.quantize(x.cpu())[0])
+    assert (kc.codes[:, :, 0] == 0).all()
+
+
+def test_no_rows():
+    from kernels import allocate_fp4_cache, paged_kv_append_fp4, paged_kv_gather_fp4
+    kc = allocate_fp4_cache(2, 16, 2, 64)
+    kt = torch.zeros(3, 2, dtype=torch.int32, device="cuda")
+    ip = torch.zeros(4, dtype=torch.int32, device="cuda")
+    none = torch.empty(0, 2, 64, dtype=torch.bfloat16, device="cuda")
+    paged_kv_append_fp4(kc, None, kt, None, none, None, ip)
+    got, _ = paged_kv_gather_fp4(kc, None, kt, None, ip, 0)
+    assert got.shape == (0, 2, 64) and (kc.codes == 0).all()
+
+
+def test_offsets_past_32_bits():
+    """A pool of more than 2^32 bytes of codes."""
+    from kernels import allocate_fp4_cache, paged_kv_append_fp4, paged_kv_gather_fp4
+    H, D, page, pages = 8, 256, 64, 70000
+    kc = allocate_fp4_cache(pages, page, H, D)
+    x = rows_of(100, H, D, torch.bfloat16, 9).cuda()
+    kt = torch.tensor([[pages - 1, pages - 2]], dtype=torch.int32, device="cuda")
+    ip = indptr([100]).cuda()
+    paged_kv_append_fp4(kc, None, kt, None, x, None, ip)
+    got, _ = paged_kv_gather_fp4(kc, None, kt, None, ip, 100)
+    assert torch.equal(got.cpu().double(), R.quantize(x.cpu())[0])
+    assert not kc.codes[:pages - 2].any()
+
+
+def test_ctypes_path_stream_and_graph():
+    import kernels.fp4_cache as m
+    H, D, page, lens = 4, 128, 16, [3, 40]
+    T = sum(lens)
+    kt, vt, pages = tables(lens, page, 5)
+    k, v = (rows_of(T, H, D, torch.bfloat16, s).cuda() for s in (6, 7))
+    ip, kt, vt = indptr(lens).cuda(), kt.cuda(), vt.cuda()
+    want = [m.allocate_fp4_cache(pages, page, H, D) for _ in range(2)]
+    m.paged_kv_append_fp4(*want, kt, vt, k, v, ip)
+    rows = m.paged_kv_gather_fp4(*want, kt, vt, ip, T)
+    m.USE_EXT = False
+    try:
+        got = [m.allocate_fp4_cache(pages, page, H, D) for _ in range(2)]
+        m.paged_kv_append_fp4(*got, kt, vt, k, v, ip)
+        rows2 = m.paged_kv_gather_fp4(*got, kt, vt, ip, T)
+    finally:
+        m.USE_EXT = True
+    for a, b in zip(got, want):
+        assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+    assert torch.equal(rows[0], rows2[0]) and torch.equal(rows[1], rows2[1])
+    got = [m.allocate_fp4_cache(pages, page, H, D) for _ in range(2)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        m.paged_kv_append_fp4(*got, kt, vt, k, v, ip)
+        held = m.paged_kv_gather_fp4(*got, kt, vt, ip, T)
+    for i in range(3):
+        k.copy_(rows_of(T, H, D, torch.bfloat16, 20 + i))
+        graph.replay()
+        m.paged_kv_append_fp4(*want, kt, vt, k, v, ip)
+        rows = m.paged_kv_gather_fp4(*want, kt, vt, ip, T)
+        torch.cuda.synchronize()
+        assert torch.equal(held[0], rows[0]) and torch.equal(held[1], rows[1])

@@ -17,7 +17,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 CXX = os.environ.get("CXX", "g++")
-SOURCES = [os.path.join(HERE, "csrc", "fa2_fwd.hip")]  # includes every csrc/*.h
+# translation units (compiled in parallel); they include the csrc/*.h
+SOURCES = [os.path.join(HERE, "csrc", n) for n in ("fa2_fwd.hip", "fa2_ops.hip")]
 OUT_DIR = os.path.join(HERE, "kernels")
 OUT = os.path.join(OUT_DIR, "libfa2.so")
 EXT_NAME = "fa2_torch"
@@ -27,8 +28,6 @@ FLAGS = [
     "-O3",
     "-std=c++17",
     "-fPIC",
-    "-shared",
-    "-Wl,-soname,libfa2.so",
     "-I" + os.path.join(ROOT, "include"),
     # packed fp32 VALU ops are kept out of all device code
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
@@ -93,22 +92,46 @@ SAN_HOST_FLAGS = [
 ]
 
 
+def _compile(flags, out_dir, tag, verbose):
+    """Start one hipcc per translation unit; (object, process) of each."""
+    jobs = []
+    for src in SOURCES:
+        obj = os.path.join(out_dir, os.path.splitext(os.path.basename(src))[0] + tag + ".o")
+        cmd = [HIPCC] + flags + ["-c", src, "-o", obj]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        jobs.append((obj, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
+                                           text=True)))
+    return jobs
+
+
+def _link(jobs, flags, out, verbose, what):
+    """Wait for the compilations and link them into ``out``."""
+    logs = [(p.communicate()[0], p.returncode) for _, p in jobs]
+    for log, rc in logs:
+        if rc != 0:
+            raise RuntimeError(f"{what} failed ({rc}):\n{log}")
+    _run([HIPCC] + flags + ["-shared", "-Wl,-soname,libfa2.so"] + [o for o, _ in jobs]
+         + ["-o", out + ".tmp"], verbose, what)
+    os.replace(out + ".tmp", out)
+    for obj, _ in jobs:
+        os.remove(obj)
+
+
 def build(verbose: bool = False, sanitize: bool = False) -> str:
     """Compile libfa2.so and the launch extension; with ``sanitize`` also the
     host-sanitized libfa2.so (in parallel with the regular one)."""
-    tmp = OUT + ".tmp"
+    jobs = _compile(FLAGS, OUT_DIR, "", verbose)
     san = None
     if sanitize:
         os.makedirs(SAN_DIR, exist_ok=True)
-        san_cmd = [HIPCC] + FLAGS + SAN_HOST_FLAGS + SOURCES + ["-o", SAN_OUT + ".tmp"]
-        if verbose:
-            print(" ".join(san_cmd), flush=True)
-        san = subprocess.Popen(san_cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+        san = _compile(FLAGS + SAN_HOST_FLAGS, SAN_DIR, "_san", verbose)
     try:
-        _run([HIPCC] + FLAGS + SOURCES + ["-o", tmp], verbose, "hipcc")
-        os.replace(tmp, OUT)
-    finally:
-        log = san.communicate()[0] if san is not None else ""
+        _link(jobs, FLAGS, OUT, verbose, "hipcc")
+    except RuntimeError:
+        for _, p in san or ():
+            p.communicate()
+        raise
     # Neither of these is needed at run time (the wrapper falls back to the C
     # ABI through ctypes; the sanitizer test skips without its library), so a
     # failure is reported and the build goes on.
@@ -117,11 +140,10 @@ def build(verbose: bool = False, sanitize: bool = False) -> str:
     except Exception as e:  # noqa: BLE001 - missing torch headers, compiler errors
         print(f"warning: launch extension not built: {e}", file=sys.stderr, flush=True)
     if san is not None:
-        if san.returncode != 0:
-            print(f"warning: sanitized host build failed ({san.returncode}):\n{log}",
-                  file=sys.stderr, flush=True)
-        else:
-            os.replace(SAN_OUT + ".tmp", SAN_OUT)
+        try:
+            _link(san, FLAGS + SAN_HOST_FLAGS, SAN_OUT, verbose, "hipcc (sanitized host)")
+        except RuntimeError as e:
+            print(f"warning: sanitized host build failed: {e}", file=sys.stderr, flush=True)
     return OUT
 
 

@@ -31,6 +31,10 @@ namespace fa2 {
 // Sequences one lane of the locating wave adds up at most.
 constexpr int kWalkMaxPer = 1024;
 
+// MODE of kernels whose paged lengths are capped at a.kv_len, what a row of
+// the block table can hold.
+constexpr int kModePagedCapped = 3;
+
 // One piece of a unit for this workgroup.
 struct DecPiece {
   Work w;
@@ -46,6 +50,7 @@ __device__ __forceinline__ int walk_len(const KArgs& a, int b) {
   if constexpr (MODE == FA2_LAYOUT_DENSE) n = a.kv_len;
   else if constexpr (MODE == FA2_LAYOUT_RAGGED) n = a.kv_indptr[b + 1] - a.kv_indptr[b];
   else n = a.kv_indptr[b];
+  if constexpr (MODE == kModePagedCapped) n = min(n, a.kv_len);
   return n > 0 ? n : 0;
 }
 
@@ -82,6 +87,7 @@ __device__ __forceinline__ Work packed_work(const KArgs& a, int b, int kvh, int 
     w.k_base = kvh * a.k_sh;
     w.v_base = kvh * a.v_sh;
   }
+  if constexpr (MODE == kModePagedCapped) w.Lk = min(w.Lk, a.kv_len);
   if (w.Lk < 0) w.Lk = 0;
   w.off = a.mask == FA2_MASK_CAUSAL_BOTTOM_RIGHT ? w.Lk - a.pack_m : 0;
   return w;

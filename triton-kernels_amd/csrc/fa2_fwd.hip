@@ -15,9 +15,8 @@
 #include <algorithm>
 #include <atomic>
 #include <mutex>
-#include <random>
 
-#include "fa2_device.h"
+#include "fa2_host.h"
 #include "fa2_kernel_lds.h"
 #include "fa2_kernel_pp.h"
 #include "fa2_kernel_short.h"
@@ -104,30 +103,6 @@ constexpr int64_t kWholeF32 = 2, kWholeShortF32 = 4;
 // byte offset of the kXcds claim counters after the work list's item count
 // (within the 256 bytes reserved there; a cache line of their own)
 constexpr size_t kClaimOffset = 128;
-
-constexpr int kMaxDevices = 64;
-std::once_flag g_cu_once[kMaxDevices];
-int g_cu_count[kMaxDevices];
-
-int cu_count_current_device() {
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kMaxDevices) return 256;
-  std::call_once(g_cu_once[dev], [dev] {
-    int n = 0;
-    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0)
-      n = 256;
-    g_cu_count[dev] = n;
-  });
-  return g_cu_count[dev];
-}
-
-int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
-int elt_bytes(int dtype) { return dtype == FA2_DTYPE_F32 ? 4 : 2; }
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-bool stride_ok(int64_t s, int eb) { return ((s * eb) & 15) == 0; }
 
 // Head dims the reference kernels take (a power of two that tl.dot accepts).
 bool head_dim_ok(int64_t d) { return d == 16 || d == 32 || d == 64 || d == 128 || d == 256; }
@@ -908,20 +883,6 @@ int workspace_size(const fa2_params* p, size_t* bytes, bool packed, bool least =
 
 // allow_conv = false: fp32 tensors keep the register-staged kernel (no
 // fp16 copies in the workspace; fa2_fwd_noalloc when they do not fit)
-// Tag of one call's merge words (KArgs::merge_tag): a process-wide counter
-// from a random start, skipping the values a cleared or all-ones word holds.
-uint64_t next_merge_tag() {
-  constexpr uint64_t kMask = (uint64_t(1) << kMergeTagBits) - 1;
-  static std::atomic<uint64_t> next{[] {
-    std::random_device rd;
-    return (static_cast<uint64_t>(rd()) << 32) ^ rd();
-  }()};
-  for (;;) {
-    const uint64_t t = next.fetch_add(1, std::memory_order_relaxed) & kMask;
-    if (t != 0 && t != kMask) return t;
-  }
-}
-
 int run(const fa2_params* p, void* stream, bool packed, bool allow_conv = true,
         bool allow_bal = true) {
   int s = packed ? validate_decode(p) : validate(p);

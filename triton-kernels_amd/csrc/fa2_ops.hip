@@ -1,0 +1,428 @@
+// fa2_ops.hip - C ABI and launch logic of the operators around the attention
+// (declared in include/fa2_ops.h).
+#include "fa2_ops.h"
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "fa2_host.h"
+#include "fa2_fp4_rows.h"
+#include "fa2_kernel_decode_fp4.h"
+#include "fa2_norm_rope.h"
+
+namespace fa2 {
+namespace {
+
+constexpr int64_t kLim = INT32_MAX / 2;  // 32-bit counters inside the kernels
+
+int launched() { return hipGetLastError() == hipSuccess ? FA2_OK : FA2_ERR_HIP; }
+
+int log2_exact(int64_t n) {  // -1: not a power of two
+  for (int s = 0; s < 31; ++s)
+    if ((int64_t(1) << s) == n) return s;
+  return -1;
+}
+
+// ---- norms and rotation ------------------------------------------------------
+
+int validate_norm_rope(const fa2_norm_rope_params* p) {
+  if (!p) return FA2_ERR_NULL_POINTER;
+  if (p->dtype < FA2_DTYPE_F16 || p->dtype > FA2_DTYPE_F32) return FA2_ERR_BAD_DTYPE;
+  if (p->weight_dtype != p->dtype && p->weight_dtype != FA2_DTYPE_F32) return FA2_ERR_BAD_DTYPE;
+  const int64_t d = p->head_dim;
+  if (d != 16 && d != 32 && d != 64 && d != 128 && d != 256) return FA2_ERR_HEAD_DIM;
+  if (p->tokens < 0 || p->q_heads < 0 || p->kv_heads < 0 || p->positions < 0 ||
+      p->rotary_dim < 0 || p->rotary_dim > d || p->rotary_dim % 16 || p->rope_stride < 0 ||
+      !(p->eps >= 0.f))
+    return FA2_ERR_BAD_SHAPE;
+  if (p->tokens > 0 && (p->q_rows <= 0 || p->k_rows <= 0)) return FA2_ERR_BAD_SHAPE;
+  if (p->tokens > kLim || p->q_heads > 65536 || p->kv_heads > 65536 || p->positions > kLim ||
+      p->q_rows > kLim || p->k_rows > kLim)
+    return FA2_ERR_TOO_LARGE;
+  const int eb = elt_bytes(p->dtype);
+  const int64_t strides[] = {p->q_sb,  p->q_sh,  p->q_ss,  p->k_sb,  p->k_sh,  p->k_ss,
+                             p->qo_sb, p->qo_sh, p->qo_ss, p->ko_sb, p->ko_sh, p->ko_ss};
+  for (int64_t s : strides)
+    if (!stride_ok(s, eb)) return FA2_ERR_ALIGNMENT;
+  if (p->rope_stride % 4) return FA2_ERR_ALIGNMENT;
+  return FA2_OK;
+}
+
+template <int DT, int D>
+void launch_norm_rope(const NormRopeArgs& a, int u, uint32_t grid, hipStream_t st) {
+  if (u == 4)
+    hipLaunchKernelGGL((fa2_norm_rope_kernel<DT, D, 4>), dim3(grid), dim3(kNrThreads), 0, st, a);
+  else
+    hipLaunchKernelGGL((fa2_norm_rope_kernel<DT, D, 1>), dim3(grid), dim3(kNrThreads), 0, st, a);
+}
+
+template <int DT>
+void launch_norm_rope_dim(int64_t d, const NormRopeArgs& a, int u, uint32_t grid, hipStream_t st) {
+  switch (d) {
+    case 16: return launch_norm_rope<DT, 16>(a, u, grid, st);
+    case 32: return launch_norm_rope<DT, 32>(a, u, grid, st);
+    case 64: return launch_norm_rope<DT, 64>(a, u, grid, st);
+    case 128: return launch_norm_rope<DT, 128>(a, u, grid, st);
+    default: return launch_norm_rope<DT, 256>(a, u, grid, st);
+  }
+}
+
+// ---- the 4-bit cache -----------------------------------------------------------
+
+bool fp4_dim_ok(int64_t d) { return d == 64 || d == 128 || d == 256; }
+
+// (the attention reads two scales of a row at once at head_dim 256)
+bool fp4_scales_ok(const uint8_t* s, int64_t d) {
+  return d < 256 || reinterpret_cast<uintptr_t>(s) % 2 == 0;
+}
+
+int validate_rows(const fa2_fp4_rows_params* p) {
+  if (!p) return FA2_ERR_NULL_POINTER;
+  if (p->dtype < FA2_DTYPE_F16 || p->dtype > FA2_DTYPE_F32) return FA2_ERR_BAD_DTYPE;
+  if (!fp4_dim_ok(p->head_dim)) return FA2_ERR_HEAD_DIM;
+  if (p->batch < 0 || p->kv_heads <= 0 || p->num_rows < 0 || p->page_size <= 0 ||
+      p->num_pages < 0 || p->table_width < 0 || p->k_table_stride < 0 || p->v_table_stride < 0)
+    return FA2_ERR_BAD_SHAPE;
+  if (p->batch > kLim || p->num_rows > kLim || p->page_size > kLim || p->num_pages > kLim ||
+      p->table_width > kLim || p->kv_heads * (p->head_dim / 8) > kLim)
+    return FA2_ERR_TOO_LARGE;
+  const int eb = elt_bytes(p->dtype);
+  const int64_t strides[] = {p->k_ts, p->k_hs, p->v_ts, p->v_hs};
+  for (int64_t s : strides)
+    if (!stride_ok(s, eb)) return FA2_ERR_ALIGNMENT;
+  return FA2_OK;
+}
+
+int fp4_rows(const fa2_fp4_rows_params* p, void* stream, bool append) {
+  int s = validate_rows(p);
+  if (s != FA2_OK) return s;
+  if (p->batch == 0 || p->num_rows == 0) return FA2_OK;
+  const bool has_v = p->v || p->v_codes || p->v_scales || p->v_block_table;
+  if (!p->k || !p->k_codes || !p->k_scales || !p->indptr || !p->k_block_table ||
+      (has_v && (!p->v || !p->v_codes || !p->v_scales || !p->v_block_table)))
+    return FA2_ERR_NULL_POINTER;
+  if (!aligned16(p->k) || !aligned16(p->k_codes) ||
+      (has_v && (!aligned16(p->v) || !aligned16(p->v_codes))))
+    return FA2_ERR_ALIGNMENT;
+  const int64_t eb = elt_bytes(p->dtype);
+  Fp4RowsArgs a{};
+  a.x[0] = static_cast<char*>(p->k);
+  a.x[1] = static_cast<char*>(p->v);
+  a.codes[0] = p->k_codes;
+  a.codes[1] = p->v_codes;
+  a.scales[0] = p->k_scales;
+  a.scales[1] = p->v_scales;
+  a.table[0] = p->k_block_table;
+  a.table[1] = p->v_block_table;
+  a.table_stride[0] = p->k_table_stride;
+  a.table_stride[1] = p->v_table_stride;
+  a.ts[0] = p->k_ts * eb;
+  a.hs[0] = p->k_hs * eb;
+  a.ts[1] = p->v_ts * eb;
+  a.hs[1] = p->v_hs * eb;
+  a.indptr = p->indptr;
+  a.start = p->start_pos;
+  a.batch = static_cast<int32_t>(p->batch);
+  a.heads = static_cast<int32_t>(p->kv_heads);
+  a.words = static_cast<int32_t>(p->kv_heads * (p->head_dim / 8));
+  a.word_shift = log2_exact(p->head_dim / 8);
+  a.num_rows = static_cast<int32_t>(p->num_rows);
+  a.page_size = static_cast<int32_t>(p->page_size);
+  a.page_shift = log2_exact(p->page_size);
+  a.num_pages = static_cast<int32_t>(p->num_pages);
+  a.table_width = static_cast<int32_t>(p->table_width);
+  a.has_v = has_v ? 1 : 0;
+  a.block_rows = std::min(std::max(kF4Pieces / a.words, 1), kF4Rows);
+  const dim3 grid(static_cast<uint32_t>(cdiv(p->num_rows, a.block_rows)));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  auto go = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    if (append)
+      hipLaunchKernelGGL((fa2_fp4_append_kernel<DT>), grid, dim3(kF4Threads), 0, st, a);
+    else
+      hipLaunchKernelGGL((fa2_fp4_gather_kernel<DT>), grid, dim3(kF4Threads), 0, st, a);
+  };
+  if (p->dtype == FA2_DTYPE_F16) go(std::integral_constant<int, FA2_DTYPE_F16>{});
+  else if (p->dtype == FA2_DTYPE_BF16) go(std::integral_constant<int, FA2_DTYPE_BF16>{});
+  else go(std::integral_constant<int, FA2_DTYPE_F32>{});
+  return launched();
+}
+
+// The balanced walk's costs, in KV tiles of 64 keys (see fa2_decode_walk.h)
+constexpr int64_t kD4MinTiles = 4;
+constexpr int64_t kD4GridTiles = 2;
+constexpr int64_t kD4Whole = 24, kD4Short = 12;
+
+struct Fp4Plan {
+  int64_t rows;        // of a unit: Hq / Hkv * q_len
+  int rb;              // 16-row blocks of a q-block
+  int64_t part_rows;
+  int64_t streams, segs, whole;
+  size_t off_ml, off_o, total;
+};
+
+int validate_fp4_decode(const fa2_fp4_decode_params* p) {
+  if (!p) return FA2_ERR_NULL_POINTER;
+  if (p->dtype != FA2_DTYPE_F16 && p->dtype != FA2_DTYPE_BF16) return FA2_ERR_BAD_DTYPE;
+  if (p->mask != FA2_MASK_NONE && p->mask != FA2_MASK_CAUSAL_BOTTOM_RIGHT) return FA2_ERR_BAD_MASK;
+  if (!fp4_dim_ok(p->head_dim)) return FA2_ERR_HEAD_DIM;
+  if (p->batch < 0 || p->q_heads <= 0 || p->kv_heads <= 0 || p->q_len < 0 ||
+      p->q_heads % p->kv_heads)
+    return FA2_ERR_BAD_SHAPE;
+  if (p->page_size <= 0 || p->num_pages < 0 || p->table_width < 0 || p->k_table_stride < 0 ||
+      p->v_table_stride < 0)
+    return FA2_ERR_PAGED_ARGS;
+  if (p->batch > 64 * kWalkMaxPer || p->q_heads > 65536 || p->q_len > kLim ||
+      p->page_size > kLim || p->num_pages > kLim || p->table_width > kLim)
+    return FA2_ERR_TOO_LARGE;
+  // a page's bytes and the keys of a table row in 31 bits
+  if (p->page_size > kLim / (p->kv_heads * (p->head_dim / 2)) ||
+      (p->table_width > 0 && p->page_size > kLim / p->table_width))
+    return FA2_ERR_TOO_LARGE;
+  const int64_t strides[] = {p->q_sb, p->q_sh, p->q_ss, p->o_sb, p->o_sh, p->o_ss};
+  for (int64_t s : strides)
+    if (!stride_ok(s, 2)) return FA2_ERR_ALIGNMENT;
+  if (p->q_heads / p->kv_heads > 1 &&
+      (p->q_sh != p->q_len * p->q_ss || p->o_sh != p->q_len * p->o_ss))
+    return FA2_ERR_Q_LAYOUT;
+  return FA2_OK;
+}
+
+int fp4_plan(const fa2_fp4_decode_params* p, Fp4Plan* pl) {
+  pl->rows = p->q_heads / p->kv_heads * p->q_len;
+  if (pl->rows > kLim) return FA2_ERR_TOO_LARGE;
+  // q-blocks of 16 rows, or of 32 where the accumulators leave room for the tiles
+  // in flight
+  pl->rb = pl->rows <= 16 || p->head_dim == 256 ? 1 : 2;
+  const int64_t nqb = cdiv(pl->rows, 16 * pl->rb);
+  pl->part_rows = std::min<int64_t>(pl->rows, 16 * pl->rb);
+  pl->streams = p->kv_heads * nqb;
+  const int64_t cus = cu_count_current_device();
+  const int64_t tiles = std::max<int64_t>(cdiv(p->table_width * p->page_size, kBN), 1);
+  const int64_t total = tiles * p->batch;  // (at most: lengths are on the device)
+  pl->segs = std::min(std::max<int64_t>(1, cus / pl->streams), cdiv(total, kD4GridTiles));
+  const int64_t part_bytes = 2 * pl->streams * pl->segs * pl->part_rows * p->head_dim * 4;
+  if (total >= (int64_t(1) << 30) || part_bytes >= (int64_t(1) << 31) ||
+      pl->streams * p->batch > kLim)
+    return FA2_ERR_TOO_LARGE;
+  const int64_t grid = pl->streams * pl->segs;
+  const int64_t idle = std::max<int64_t>(0, grid - pl->streams * p->batch);
+  pl->whole = std::max(kD4Whole / 2, kD4Whole * idle / grid);
+  const size_t slots = static_cast<size_t>(2 * grid);
+  size_t off = static_cast<size_t>(pl->streams * p->batch) * sizeof(uint64_t);
+  off = (off + 255) & ~size_t(255);
+  pl->off_ml = off;
+  off += slots * pl->part_rows * 2 * sizeof(float);
+  off = (off + 255) & ~size_t(255);
+  pl->off_o = off;
+  off += slots * pl->part_rows * p->head_dim * sizeof(float);
+  pl->total = off;
+  return FA2_OK;
+}
+
+bool fp4_empty(const fa2_fp4_decode_params* p) { return p->batch == 0 || p->q_len == 0; }
+
+template <int DT, int D>
+void launch_fp4_decode(const Fp4Args& a, int rb, bool even, uint32_t grid, hipStream_t st) {
+  auto go = [&](auto r, auto e) {
+    constexpr int RB = decltype(r)::value;
+    constexpr int kRing = D == 64 ? 6 : D == 128 ? (RB == 1 ? 4 : 3) : 2;
+    hipLaunchKernelGGL((fa2_decode_fp4_kernel<DT, D, RB, kRing, decltype(e)::value>), dim3(grid),
+                       dim3(kD4Threads), 0, st, a);
+  };
+  using One = std::integral_constant<int, 1>;
+  if (rb == 1 && even) go(One{}, std::true_type{});
+  else if (rb == 1) go(One{}, std::false_type{});
+  if constexpr (D <= 128) {
+    using Two = std::integral_constant<int, 2>;
+    if (rb == 2 && even) go(Two{}, std::true_type{});
+    else if (rb == 2) go(Two{}, std::false_type{});
+  }
+}
+
+template <int DT>
+void launch_fp4_decode_dim(int64_t d, const Fp4Args& a, int rb, bool even, uint32_t grid,
+                           hipStream_t st) {
+  if (d == 64) launch_fp4_decode<DT, 64>(a, rb, even, grid, st);
+  else if (d == 128) launch_fp4_decode<DT, 128>(a, rb, even, grid, st);
+  else launch_fp4_decode<DT, 256>(a, rb, even, grid, st);
+}
+
+}  // namespace
+}  // namespace fa2
+
+using namespace fa2;
+
+extern "C" size_t fa2_ops_params_size(int which) {
+  switch (which) {
+    case 0: return sizeof(fa2_norm_rope_params);
+    case 1: return sizeof(fa2_fp4_rows_params);
+    case 2: return sizeof(fa2_fp4_decode_params);
+    default: return 0;
+  }
+}
+
+extern "C" int fa2_norm_rope(const fa2_norm_rope_params* p, void* stream) {
+  int s = validate_norm_rope(p);
+  if (s != FA2_OK) return s;
+  if (p->tokens == 0 || p->q_heads + p->kv_heads == 0) return FA2_OK;
+  if ((p->q_heads && (!p->q || !p->q_out || !p->q_weight)) ||
+      (p->kv_heads && (!p->k || !p->k_out || !p->k_weight)) || !p->position ||
+      (p->rotary_dim && p->positions && !p->rope))
+    return FA2_ERR_NULL_POINTER;
+  const void* ptrs[] = {p->q, p->k, p->q_out, p->k_out, p->q_weight, p->k_weight, p->rope};
+  for (const void* x : ptrs)
+    if (!aligned16(x)) return FA2_ERR_ALIGNMENT;
+  const int eb = elt_bytes(p->dtype);
+  const int64_t lanes = p->head_dim * eb / 32;
+  // Four heads of a token per lane group (their loads in flight together, the
+  // table's row and the weights read once) where that still gives every CU work
+  // for its four SIMDs, else one.
+  const int64_t u = p->tokens * (cdiv(p->q_heads, 4) + cdiv(p->kv_heads, 4)) * lanes >=
+                            int64_t(cu_count_current_device()) * 4 * 64
+                        ? 4
+                        : 1;
+  NormRopeArgs a{};
+  a.x[0] = static_cast<const char*>(p->q);
+  a.x[1] = static_cast<const char*>(p->k);
+  a.y[0] = static_cast<char*>(p->q_out);
+  a.y[1] = static_cast<char*>(p->k_out);
+  a.w[0] = static_cast<const char*>(p->q_weight);
+  a.w[1] = static_cast<const char*>(p->k_weight);
+  a.rope = p->rope;
+  a.pos = p->position;
+  a.sb[0] = p->q_sb * eb; a.sh[0] = p->q_sh * eb; a.ss[0] = p->q_ss * eb;
+  a.sb[1] = p->k_sb * eb; a.sh[1] = p->k_sh * eb; a.ss[1] = p->k_ss * eb;
+  a.ob[0] = p->qo_sb * eb; a.oh[0] = p->qo_sh * eb; a.os[0] = p->qo_ss * eb;
+  a.ob[1] = p->ko_sb * eb; a.oh[1] = p->ko_sh * eb; a.os[1] = p->ko_ss * eb;
+  a.rope_stride = p->rope_stride;
+  a.heads[0] = static_cast<int32_t>(p->q_heads);
+  a.heads[1] = static_cast<int32_t>(p->kv_heads);
+  a.rows[0] = static_cast<int32_t>(p->q_rows);
+  a.rows[1] = static_cast<int32_t>(p->k_rows);
+  a.blocks[0] = static_cast<int32_t>(cdiv(p->q_heads, u));
+  a.blocks[1] = static_cast<int32_t>(cdiv(p->kv_heads, u));
+  const int64_t units = p->tokens * (a.blocks[0] + a.blocks[1]);
+  if (units * lanes > kLim) return FA2_ERR_TOO_LARGE;
+  a.units = static_cast<int32_t>(units);
+  a.positions = static_cast<int32_t>(p->positions);
+  a.rot = static_cast<int32_t>(p->rotary_dim);
+  a.inter = p->interleaved ? 1 : 0;
+  a.pos64 = p->position_64 ? 1 : 0;
+  a.w32 = p->weight_dtype == FA2_DTYPE_F32 ? 1 : 0;
+  a.eps = p->eps;
+  const uint32_t grid = static_cast<uint32_t>(cdiv(units * lanes, kNrThreads));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  switch (p->dtype) {
+    case FA2_DTYPE_F16:
+      launch_norm_rope_dim<FA2_DTYPE_F16>(p->head_dim, a, static_cast<int>(u), grid, st);
+      break;
+    case FA2_DTYPE_BF16:
+      launch_norm_rope_dim<FA2_DTYPE_BF16>(p->head_dim, a, static_cast<int>(u), grid, st);
+      break;
+    default:
+      launch_norm_rope_dim<FA2_DTYPE_F32>(p->head_dim, a, static_cast<int>(u), grid, st);
+  }
+  return launched();
+}
+
+extern "C" int fa2_fp4_append(const fa2_fp4_rows_params* p, void* stream) {
+  return fp4_rows(p, stream, true);
+}
+
+extern "C" int fa2_fp4_gather(const fa2_fp4_rows_params* p, void* stream) {
+  return fp4_rows(p, stream, false);
+}
+
+extern "C" int fa2_fp4_decode_workspace_size(const fa2_fp4_decode_params* p, size_t* bytes) {
+  if (!bytes) return FA2_ERR_NULL_POINTER;
+  int s = validate_fp4_decode(p);
+  if (s != FA2_OK) return s;
+  *bytes = 0;
+  if (fp4_empty(p)) return FA2_OK;
+  Fp4Plan pl{};
+  s = fp4_plan(p, &pl);
+  if (s == FA2_OK) *bytes = pl.total;
+  return s;
+}
+
+extern "C" int fa2_fp4_decode(const fa2_fp4_decode_params* p, void* stream) {
+  int s = validate_fp4_decode(p);
+  if (s != FA2_OK) return s;
+  if (fp4_empty(p)) return FA2_OK;
+  if (!p->q || !p->o || !p->k_codes || !p->k_scales || !p->v_codes || !p->v_scales)
+    return FA2_ERR_NULL_POINTER;
+  if (!p->kv_lens || !p->k_block_table || !p->v_block_table || p->num_pages == 0)
+    return FA2_ERR_PAGED_ARGS;
+  const void* ptrs[] = {p->q, p->o, p->k_codes, p->v_codes};
+  for (const void* x : ptrs)
+    if (!aligned16(x)) return FA2_ERR_ALIGNMENT;
+  if (!fp4_scales_ok(p->k_scales, p->head_dim) || !fp4_scales_ok(p->v_scales, p->head_dim))
+    return FA2_ERR_ALIGNMENT;
+  Fp4Plan pl{};
+  s = fp4_plan(p, &pl);
+  if (s != FA2_OK) return s;
+  if (!p->workspace || p->workspace_bytes < pl.total) return FA2_ERR_WORKSPACE;
+
+  Fp4Args fa{};
+  KArgs& a = fa.a;
+  a.q = p->q;
+  a.k = p->k_codes;
+  a.v = p->v_codes;
+  a.o = p->o;
+  a.kv_indptr = p->kv_lens;
+  a.k_table = p->k_block_table;
+  a.v_table = p->v_block_table;
+  a.q_sb = p->q_sb; a.q_sh = p->q_sh; a.q_ss = p->q_ss;
+  a.o_sb = p->o_sb; a.o_sh = p->o_sh; a.o_ss = p->o_ss;
+  a.k_table_stride = p->k_table_stride;
+  a.v_table_stride = p->v_table_stride;
+  a.batch = static_cast<int32_t>(p->batch);
+  a.hq = static_cast<int32_t>(p->q_heads);
+  a.hkv = static_cast<int32_t>(p->kv_heads);
+  a.q_len = static_cast<int32_t>(pl.rows);
+  a.kv_len = static_cast<int32_t>(p->table_width * p->page_size);
+  a.page_size = static_cast<int32_t>(p->page_size);
+  a.page_shift = log2_exact(p->page_size);
+  a.mask = p->mask;
+  a.num_splits = 1;
+  a.scale_log2 = p->softmax_scale * 1.4426950408889634f;
+  char* ws = static_cast<char*>(p->workspace);
+  a.merge_ctr = reinterpret_cast<uint64_t*>(ws);
+  try {
+    a.merge_tag = next_merge_tag();
+  } catch (...) {  // (no random device: no tag, no call)
+    return FA2_ERR_HIP;
+  }
+  a.part_ml = reinterpret_cast<float*>(ws + pl.off_ml);
+  a.part_o = reinterpret_cast<float*>(ws + pl.off_o);
+  a.part_rows = static_cast<int32_t>(pl.part_rows);
+  a.walk_streams = static_cast<int32_t>(pl.streams);
+  a.walk_segs = static_cast<int32_t>(pl.segs);
+  a.walk_min = kD4MinTiles;
+  a.walk_whole = static_cast<int32_t>(pl.whole);
+  a.walk_short = kD4Short;
+  const int64_t grid = pl.streams * pl.segs;
+  a.walk_dj = static_cast<int32_t>(pl.segs);
+  a.walk_ds = 0;
+  a.walk_rounds = static_cast<int32_t>(cdiv(pl.streams * p->batch, grid));
+  a.pack_m = static_cast<int32_t>(p->q_len);
+  a.dv = static_cast<int32_t>(p->head_dim);
+  fa.ks = p->k_scales;
+  fa.vs = p->v_scales;
+  fa.num_pages = static_cast<int32_t>(p->num_pages);
+  fa.table_width = static_cast<int32_t>(p->table_width);
+  const int64_t d = p->head_dim;
+  fa.head_codes = static_cast<uint32_t>(p->page_size * (d / 2));
+  fa.head_scales = static_cast<uint32_t>(p->page_size * (d / 32));
+  fa.page_codes = static_cast<uint32_t>(p->kv_heads * p->page_size * (d / 2));
+  fa.page_scales = static_cast<uint32_t>(p->kv_heads * p->page_size * (d / 32));
+  const bool even = p->page_size % 16 == 0;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (p->dtype == FA2_DTYPE_F16)
+    launch_fp4_decode_dim<FA2_DTYPE_F16>(d, fa, pl.rb, even, static_cast<uint32_t>(grid), st);
+  else
+    launch_fp4_decode_dim<FA2_DTYPE_BF16>(d, fa, pl.rb, even, static_cast<uint32_t>(grid), st);
+  return launched();
+}

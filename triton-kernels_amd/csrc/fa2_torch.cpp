@@ -15,6 +15,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include "fa2.h"
+#include "fa2_ops.h"
 
 namespace {
 
@@ -291,10 +292,191 @@ int64_t append(const at::Tensor& kc, const c10::optional<at::Tensor>& vc, const 
   return fa2_kv_append(&p, st);
 }
 
+// ---- operators around the attention (include/fa2_ops.h) ----------------------
+
+// A small operand (weights, table) contiguous from a 16-byte boundary.
+at::Tensor packed(const at::Tensor& t) {
+  if (t.is_contiguous() && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) return t;
+  return t.clone(at::MemoryFormat::Contiguous);
+}
+
+// Rows as the kernels take them.  (A contiguous tensor off a 16-byte boundary is
+// copied too, which contiguous() would not do.)
+at::Tensor ready(const at::Tensor& t) {
+  return rows_ok(t) ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+// qk_norm_rope after the Python wrapper's checks; (status, q, k).
+std::tuple<int64_t, at::Tensor, at::Tensor> norm_rope(at::Tensor q, at::Tensor k, at::Tensor qw,
+                                                      at::Tensor kw, at::Tensor rope,
+                                                      at::Tensor positions, double eps,
+                                                      bool interleaved) {
+  const at::Device dev = q.device();
+  const c10::DeviceGuard guard(dev);
+  q = ready(q);
+  k = ready(k);
+  qw = packed(qw);
+  kw = packed(kw);
+  rope = packed(rope);
+  positions = positions.contiguous();
+  at::Tensor qo = at::empty(q.sizes(), q.options());
+  at::Tensor ko = at::empty(k.sizes(), k.options());
+  fa2_norm_rope_params p;
+  std::memset(&p, 0, sizeof(p));
+  p.dtype = dtype_code(q.scalar_type());
+  p.weight_dtype = dtype_code(qw.scalar_type());
+  p.interleaved = interleaved ? 1 : 0;
+  p.eps = static_cast<float>(eps);
+  p.tokens = positions.numel();
+  p.q_heads = q.size(1);
+  p.kv_heads = k.size(1);
+  p.head_dim = q.size(-1);
+  p.rotary_dim = rope.size(1);
+  p.positions = rope.size(0);
+  p.rope_stride = rope.size(1);
+  p.q_rows = q.dim() == 4 ? q.size(2) : p.tokens;
+  p.k_rows = k.dim() == 4 ? k.size(2) : p.tokens;
+  strides3(q, p.q_sb, p.q_sh, p.q_ss);
+  strides3(k, p.k_sb, p.k_sh, p.k_ss);
+  strides3(qo, p.qo_sb, p.qo_sh, p.qo_ss);
+  strides3(ko, p.ko_sb, p.ko_sh, p.ko_ss);
+  p.q = q.data_ptr();
+  p.k = k.data_ptr();
+  p.q_out = qo.data_ptr();
+  p.k_out = ko.data_ptr();
+  p.q_weight = qw.data_ptr();
+  p.k_weight = kw.data_ptr();
+  p.rope = rope.data_ptr<float>();
+  p.position = positions.data_ptr();
+  p.position_64 = positions.scalar_type() == at::kLong ? 1 : 0;
+  const hipStream_t st = c10::hip::getCurrentHIPStream(dev.index()).stream();
+  return {fa2_norm_rope(&p, st), qo, ko};
+}
+
+// paged_kv_append_fp4 and paged_kv_gather_fp4 after the Python wrappers' checks;
+// the status.
+int64_t fp4_rows(bool append, const at::Tensor& kc, const at::Tensor& ks,
+                 const c10::optional<at::Tensor>& vc, const c10::optional<at::Tensor>& vs,
+                 const at::Tensor& k_table, const c10::optional<at::Tensor>& v_table, at::Tensor k,
+                 c10::optional<at::Tensor> v, const at::Tensor& indptr,
+                 const c10::optional<at::Tensor>& start_pos) {
+  const at::Device dev = kc.device();
+  const c10::DeviceGuard guard(dev);
+  if (append) {  // (the gathered tensors are contiguous and aligned)
+    k = ready(k);
+    if (v) v = ready(*v);
+  }
+  const at::Tensor ip = index32(indptr, dev);
+  const at::Tensor kt = table32(k_table, dev);
+  at::Tensor sp, vt;
+  fa2_fp4_rows_params p;
+  std::memset(&p, 0, sizeof(p));
+  p.dtype = dtype_code(k.scalar_type());
+  p.batch = indptr.numel() - 1;
+  p.kv_heads = kc.size(1);
+  p.head_dim = k.size(2);
+  p.num_rows = k.size(0);
+  p.page_size = kc.size(2);
+  p.num_pages = kc.size(0);
+  p.table_width = kt.size(1);
+  p.k_table_stride = kt.stride(0);
+  p.k_ts = k.stride(0);
+  p.k_hs = k.stride(1);
+  p.k = k.data_ptr();
+  p.k_codes = kc.data_ptr<uint8_t>();
+  p.k_scales = ks.data_ptr<uint8_t>();
+  p.indptr = ip.data_ptr<int32_t>();
+  p.k_block_table = kt.data_ptr<int32_t>();
+  if (start_pos) {
+    sp = index32(*start_pos, dev);
+    p.start_pos = sp.data_ptr<int32_t>();
+  }
+  if (vc) {
+    vt = table32(*v_table, dev);
+    p.table_width = std::min(p.table_width, vt.size(1));
+    p.v_table_stride = vt.stride(0);
+    p.v_ts = v->stride(0);
+    p.v_hs = v->stride(1);
+    p.v = v->data_ptr();
+    p.v_codes = vc->data_ptr<uint8_t>();
+    p.v_scales = vs->data_ptr<uint8_t>();
+    p.v_block_table = vt.data_ptr<int32_t>();
+  }
+  const hipStream_t st = c10::hip::getCurrentHIPStream(dev.index()).stream();
+  return append ? fa2_fp4_append(&p, st) : fa2_fp4_gather(&p, st);
+}
+
+// decode_attention_fp4 (q [B,QH,D]) and speculative_decode_attention_fp4 (q
+// [B,QH,M,D]) after the Python wrappers' checks; (status, output).
+std::tuple<int64_t, at::Tensor> fp4_decode(const at::Tensor& q, const at::Tensor& kc,
+                                           const at::Tensor& ks, const at::Tensor& vc,
+                                           const at::Tensor& vs, const at::Tensor& lens,
+                                           const at::Tensor& k_table, const at::Tensor& v_table,
+                                           bool causal) {
+  const at::Device dev = q.device();
+  const c10::DeviceGuard guard(dev);
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  const bool squeeze = q.dim() == 3;
+  at::Tensor q4 = squeeze ? q.unsqueeze(2) : q;
+  const at::Tensor o4 = squeeze ? out.unsqueeze(2) : out;
+  const int64_t M = q4.size(2);
+  if (!run_ok(q4, M)) q4 = q4.clone(at::MemoryFormat::Contiguous);
+  const at::Tensor li = index32(lens, dev);
+  const at::Tensor kt = table32(k_table, dev);
+  const at::Tensor vt = table32(v_table, dev);
+  fa2_fp4_decode_params p;
+  std::memset(&p, 0, sizeof(p));
+  p.dtype = dtype_code(q.scalar_type());
+  p.mask = causal ? FA2_MASK_CAUSAL_BOTTOM_RIGHT : FA2_MASK_NONE;
+  p.batch = q4.size(0);
+  p.q_heads = q4.size(1);
+  p.kv_heads = kc.size(1);
+  p.head_dim = q4.size(3);
+  p.q_len = M;
+  p.page_size = kc.size(2);
+  p.num_pages = kc.size(0);
+  p.table_width = std::min(kt.size(1), vt.size(1));
+  p.k_table_stride = kt.stride(0);
+  p.v_table_stride = vt.stride(0);
+  auto set_strides = [&](const at::Tensor& t, int64_t& sb, int64_t& sh, int64_t& ss) {
+    sb = t.stride(0);
+    sh = t.stride(1);
+    ss = M > 1 ? t.stride(2) : t.stride(1);
+  };
+  set_strides(q4, p.q_sb, p.q_sh, p.q_ss);
+  set_strides(o4, p.o_sb, p.o_sh, p.o_ss);
+  p.q = q4.data_ptr();
+  p.o = out.data_ptr();
+  p.k_codes = kc.data_ptr<uint8_t>();
+  p.k_scales = ks.data_ptr<uint8_t>();
+  p.v_codes = vc.data_ptr<uint8_t>();
+  p.v_scales = vs.data_ptr<uint8_t>();
+  p.kv_lens = li.data_ptr<int32_t>();
+  p.k_block_table = kt.data_ptr<int32_t>();
+  p.v_block_table = vt.data_ptr<int32_t>();
+  p.softmax_scale = static_cast<float>(std::pow(static_cast<double>(p.head_dim), -0.5));
+  size_t ws_bytes = 0;
+  int rc = fa2_fp4_decode_workspace_size(&p, &ws_bytes);
+  if (rc != FA2_OK) return {rc, out};
+  at::Tensor ws;
+  if (ws_bytes) {
+    ws = at::empty({static_cast<int64_t>(ws_bytes)}, q.options().dtype(at::kByte));
+    p.workspace = ws.data_ptr();
+    p.workspace_bytes = ws_bytes;
+  }
+  const hipStream_t st = c10::hip::getCurrentHIPStream(dev.index()).stream();
+  return {fa2_fp4_decode(&p, st), out};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fwd", &fwd, "enqueue fa2_fwd for checked tensors; returns the output");
   m.def("decode", &decode, "enqueue fa2_decode_fwd for checked tensors; the output, or None");
   m.def("append", &append, "enqueue fa2_kv_append for checked tensors; the fa2 status");
+  m.def("norm_rope", &norm_rope, "enqueue fa2_norm_rope for checked tensors; (fa2 status, q, k)");
+  m.def("fp4_rows", &fp4_rows,
+        "enqueue fa2_fp4_append or fa2_fp4_gather for checked tensors; the fa2 status");
+  m.def("fp4_decode", &fp4_decode,
+        "enqueue fa2_fp4_decode for checked tensors; (fa2 status, output)");
 }

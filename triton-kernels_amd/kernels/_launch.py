@@ -38,6 +38,12 @@ def prep(t: torch.Tensor) -> torch.Tensor:
     return t if rows_ok(t) else t.contiguous()
 
 
+def aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` or a contiguous copy whose rows pass :func:`rows_ok` (``prep`` keeps a
+    contiguous tensor off a 16-byte boundary)."""
+    return t if rows_ok(t) else t.clone(memory_format=torch.contiguous_format)
+
+
 def strides(t: torch.Tensor):
     """(batch, head, row) element strides; token-major tensors use (0, head, token)."""
     if t.dim() == 4:
