@@ -10,14 +10,20 @@
 //   * Workgroup = 8 waves, one per CU, over an equal share of the call's KV
 //     tiles (fa2_decode_walk.h).  A wave walks tiles of 32 keys, tile i of
 //     the workgroup's range to wave i % 8, and keeps its own (m, l, O).
-//   * A page's rows of a kv head are contiguous: the 16 rows of a block are one
-//     run of 8 D bytes, which the 64 lanes load straight in the layout of the
-//     MFMA's A operand (lane: row l % 16, D / 4 dims from D / 4 * (l / 16); the
-//     queries take the dims of a k-step in the same order).  kRing tiles per
-//     wave are in flight in registers, across the ends of the pieces.
+//   * A page's rows of a kv head are contiguous.  Direct-to-LDS loads of whole
+//     rows fill a ring of kRing tiles per wave, across the ends of the pieces; a
+//     tile's codes are read into registers at once (they are few) and its slot
+//     filled again, so the whole ring is in flight nearly all the time, from one
+//     copy of the loop.  (Tiles in flight in registers instead need the loop once
+//     per tile in flight: 50 KB of code, whose first execution alone took 6 us.)
 //   * S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32, up to 16 RB rows
-//     of the unit as columns.  V goes through LDS in 16 bits, as its rows
-//     come in and in columns as PV takes them (transpose reads).
+//     of the unit as columns.  A lane expands D / 4 dims of a key of K, in the
+//     layout of the MFMA's A operand (lane: row l % 16, dims D / 4 * (l / 16)
+//     ..; the queries take the dims of a k-step in the same order).  Of V it
+//     expands D / 16 dims of the 8 keys that its P^T fragment has, and pairs them
+//     by key with v_perm: block i of O^T is dim i of every 16 lanes.  (V back
+//     through LDS in 16 bits, for transpose reads, took two thirds of the LDS
+//     time, and that 75 % of a tile's.)
 //   * P goes to the MFMA as the sum of two 16-bit values, high and low part, so
 //     that the weights carry 16 to 22 bits: the MFMAs have the time (a CU's
 //     share of the HBM rate is one tile of 4.3 KB in 440 cycles, of which 24
@@ -35,9 +41,13 @@ namespace fa2 {
 constexpr int kD4Waves = 8;
 constexpr int kD4Threads = 64 * kD4Waves;
 constexpr int kD4Tile = 32;    // keys of a wave's tile
-constexpr int kD4Table = 512;  // block-table entries of a window (K and V each)
 
 typedef __attribute__((address_space(3))) f32x4 lds_f32x4_t;
+typedef __attribute__((address_space(3))) f32x2 lds_f32x2_t;
+typedef __attribute__((address_space(3))) u32x2 lds_u32x2_t;
+typedef __attribute__((address_space(3))) uint32_t lds_u32_t;
+typedef __attribute__((address_space(3))) uint16_t lds_u16_t;
+typedef __attribute__((address_space(3))) uint8_t lds_u8_t;
 
 struct Fp4Args {
   KArgs a;  // a.k, a.v: the codes; a.kv_len: keys a row of the tables can hold
@@ -76,6 +86,17 @@ __device__ __forceinline__ u32x4 fp4_values(uint32_t w, uint32_t sb) {
         __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 3))};
 }
 
+// Values 2 B and 2 B + 1 of a code word, at the scale with the float's bits `f`.
+template <bool BF, int B>
+__device__ __forceinline__ uint32_t fp4_pair(uint32_t w, uint32_t f) {
+  if constexpr (BF)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(
+                                            w, __builtin_bit_cast(float, f), B));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(
+                                            w, __builtin_bit_cast(float, f), B));
+}
+
 // fp32 of the low / high half of a packed pair
 template <bool BF>
 __device__ __forceinline__ f32x2 unpack2(uint32_t w) {
@@ -86,57 +107,83 @@ __device__ __forceinline__ f32x2 unpack2(uint32_t w) {
     return __builtin_convertvector(__builtin_bit_cast(f16x2, w), f32x2);
 }
 
-// A block of 16 keys' codes in one lane: D / 32 words, and its scale byte(s).
-template <int D>
-struct Fp4Block {
-  uint32_t w[D / 32];
-  uint32_t s;
-};
-
-template <int D>
-__device__ __forceinline__ void fp4_load(Fp4Block<D>& b, const uint8_t* codes,
-                                         const uint8_t* scales, uint64_t coff, uint64_t soff,
-                                         uint32_t cl, uint32_t sl) {
-  const uint8_t* c = codes + coff;
-  const uint8_t* s = scales + soff;
-  if constexpr (D == 64) {
-    const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(c + cl));
-    b.w[0] = x[0];
-    b.w[1] = x[1];
-  } else {
-#pragma unroll
-    for (int i = 0; i < D / 128; ++i) {
-      const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(c + cl) + i);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) b.w[4 * i + j] = x[j];
-    }
-  }
-  if constexpr (D == 256)
-    b.s = *reinterpret_cast<const uint16_t*>(s + sl);
-  else
-    b.s = s[sl];
+// Direct-to-LDS loads, lane i to lds + 16 i (or 4 i), from per-lane addresses; wait
+// states as dma_buffer_x4.
+__device__ __forceinline__ void fp4_dma16(const void* p, uint32_t lds) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt"
+               :
+               : "v"(p), "{m0}"(__builtin_amdgcn_readfirstlane(static_cast<int>(lds))));
+}
+// From a uniform base and a 32-bit offset per lane (readlane, then the load).
+__device__ __forceinline__ void fp4_dma16_base(uint64_t base, uint32_t off, uint32_t lds) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1 nt"
+               :
+               : "v"(off), "s"(base),
+                 "{m0}"(__builtin_amdgcn_readfirstlane(static_cast<int>(lds))));
+}
+__device__ __forceinline__ void fp4_dma4(const void* p, uint32_t lds) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off"
+               :
+               : "v"(p), "{m0}"(__builtin_amdgcn_readfirstlane(static_cast<int>(lds))));
 }
 
-// EVEN: page_size is a multiple of 16, so the 16 keys of a block lie in one
-// page: its place is computed on the scalar unit.
-template <int DT, int D, int RB, int RING, bool EVEN>
-__global__ __launch_bounds__(kD4Threads, 1) void fa2_decode_fp4_kernel(Fp4Args fa) {
+__device__ __forceinline__ void fp4_dma2(const void* p, uint32_t lds) {  // into a word each
+  asm volatile("s_nop 0\n\tglobal_load_lds_ushort %0, off"
+               :
+               : "v"(p), "{m0}"(__builtin_amdgcn_readfirstlane(static_cast<int>(lds))));
+}
+
+// Geometry at head dim D with 16 RB rows.
+template <int D, int RB>
+struct Fp4Geo {
+  static constexpr int kPerCu = 1;  // workgroups per CU
+  static constexpr int kRow = D / 2;                  // bytes of a row of codes
+  static constexpr int kNC = kRow / 16;               // its 16-byte chunks
+  static constexpr int kCode = kD4Tile * kRow;        // a tile's codes of K (or V)
+  static constexpr int kLoads = kCode / 1024;         // ... and their loads
+  static constexpr int kScale = D == 256 ? 256 : 128; // LDS bytes of its scales
+  static constexpr int kScaleRow = D == 256 ? 8 : 4;
+  static constexpr int kScaleLoads = D == 256 ? 2 : 1;  // (K and V in one up to 128)
+  static constexpr int kTile = 2 * kCode + 2 * kScale;
+  static constexpr int kInFlight = 2 * kLoads + kScaleLoads;  // loads of a tile
+  static constexpr int kNI = D / 16;                  // dims of V of a lane, blocks of O^T
+  static constexpr int kPD = 64;                      // dims merged at a time
+  static constexpr int kPH = D / kPD;                 // phases
+  static constexpr int kRP = 16 / kNI;                // accumulator rows of a lane per phase
+  static constexpr int kPitch = (kPD + 4) * 4;        // merge rows
+  static constexpr int kStage = 16 * kPitch;          // a wave's merge bytes
+  static constexpr int kTable = 256;                  // block-table entries of a window
+  static constexpr int kRing = D == 64 ? 5 : D == 128 ? 3 : 1;
+  // chunk c of row r lies at chunk c ^ ksw(r): 8 lanes reading a chunk of 8 rows
+  // hit distinct banks
+  static __device__ __forceinline__ int ksw(int r) {
+    return D == 64 ? (r >> 3) & 1 : D == 128 ? (r >> 2) & 3 : (r >> 1) & 7;
+  }
+  // Row p of a block of V in LDS is key vkey(p) of it: the four lane groups read
+  // keys four apart, and so four rows side by side.
+  static __device__ __forceinline__ int vkey(int p) { return (p & 16) + ((p & 15) >> 2) + 4 * (p & 3); }
+  // The dim of O that value sd of merge phase h is.  (Value r of block i in lane group
+  // g is dim D / 4 * g + kNI * r + i; a phase takes kRP rows of each.)
+  static __device__ __forceinline__ int dim(int h, int sd) {
+    return (sd >> 4) * (D / 4) + 16 * h + (sd & 15);
+  }
+};
+
+template <int DT, int D, int RB>
+__global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_decode_fp4_kernel(
+    Fp4Args fa) {
+  using G = Fp4Geo<D, RB>;
   constexpr bool BF = Elt<DT>::kBF;
   constexpr int MODE = kModePagedCapped;
-  constexpr int DJ = D / 32;        // S k-steps = code words of a lane = V chunks of a lane
-  constexpr int DB = D / 16;        // 16-dim blocks of O^T
-  constexpr int kRow = D * 2;       // bytes of a V row in LDS
-  constexpr int kVBytes = kD4Tile * kRow;
-  constexpr int kPitch = (D + 4) * 4;  // merge rows
-  constexpr int kMrg = kD4Waves * 16 * kPitch;
-  constexpr int kLds0 = kD4Waves * kVBytes > kMrg ? kD4Waves * kVBytes : kMrg;
-  constexpr int kLds =
-      kLds0 > kMergePieceBytes<kD4Threads> ? kLds0 : kMergePieceBytes<kD4Threads>;
+  constexpr int DJ = D / 32;        // S k-steps = code words of a lane
   constexpr int kStep = kD4Tile * kD4Waves;
+  constexpr int kSub = D == 256 ? 2 : 1;  // scales of a lane's dims
+  static_assert(kD4Waves * G::kStage >= kMergePieceBytes<kD4Threads>, "merge area");
 
-  __shared__ __attribute__((aligned(1024))) char lds[kLds];
+  __shared__ __attribute__((aligned(1024))) char tiles[kD4Waves * G::kRing * G::kTile];
+  __shared__ __attribute__((aligned(128))) char stage[kD4Waves * G::kStage];
   __shared__ float mrg_ml[kD4Waves][16][2];
-  __shared__ int tab[2][2][kD4Table];
+  __shared__ int tab[2][2][G::kTable];
   __shared__ DecSegment seg_sh;
   __shared__ int merge_flag;
 
@@ -171,7 +218,7 @@ __global__ __launch_bounds__(kD4Threads, 1) void fa2_decode_fp4_kernel(Fp4Args f
     v.ka = ka;
     v.kb = v.kend;
     v.page0 = page_of(ka);
-    const int64_t lim = (static_cast<int64_t>(v.page0) + kD4Table) * a.page_size;
+    const int64_t lim = (static_cast<int64_t>(v.page0) + G::kTable) * a.page_size;
     if (lim < v.kend) {  // whole tiles, so that every window starts at one
       const int n = (static_cast<int>(lim) - ka) / kD4Tile * kD4Tile;
       v.kb = ka + max(n, kD4Tile);
@@ -212,61 +259,145 @@ __global__ __launch_bounds__(kD4Threads, 1) void fa2_decode_fp4_kernel(Fp4Args f
   int buf = 0;
 
   // ---- loads ---------------------------------------------------------------
-  struct Tile {
-    Fp4Block<D> k[2], v[2];
-  };
-  Tile ring[RING];
   const uint8_t* kc = static_cast<const uint8_t*>(a.k);
   const uint8_t* vc = static_cast<const uint8_t*>(a.v);
-  const uint32_t gdim = g * (D / 8);         // this lane's bytes of a row ...
-  const uint32_t gscale = (g * (D / 4)) / 32;  // ... and first scale
-  const uint32_t cl = l16 * (D / 2) + gdim;
-  const uint32_t sl = l16 * (D / 32) + gscale;
   const uint32_t hc = (stream % a.hkv) * fa.head_codes, hs = (stream % a.hkv) * fa.head_scales;
-  struct Source {  // the window that loads are for
-    int ka, kb, page0, tb;
+  const uint32_t ring = lds_addr_of(tiles) + wave * (G::kRing * G::kTile);
+  int wp = 0;   // ring bytes at which the next tile goes in
+  int rp = 0;   // ... and the oldest one lies
+  int fly = 0;  // tiles issued and not yet read
+  auto advance = [&]() {
+    wp = wp + G::kTile == G::kRing * G::kTile ? 0 : wp + G::kTile;
+    ++fly;
   };
-  auto source = [](const Window& v, int tb) { return Source{v.ka, v.kb, v.page0, tb}; };
-  // The tile of v at key n.  Keys past the window are its last block's or
-  // last key's (their weights are zero); a window without keys reads page 0.
-  auto issue = [&](Tile& t, const Source& v, int n) {
-    const int top = max(v.kb - 1, v.ka);
-    const int tb = v.tb;
+  // Page and row in it of key nk of a window.
+  auto place = [&](int nk, int page0, int tb, int which, uint32_t& off) {
+    int lp;
+    if (a.page_shift >= 0) {
+      lp = nk >> a.page_shift;
+      off = nk & (a.page_size - 1);
+    } else {
+      lp = nk / a.page_size;
+      off = nk - lp * a.page_size;
+    }
+    return static_cast<uint32_t>(tab[tb][which][lp - page0]);
+  };
+  auto codes_at = [&](int v, uint32_t pg, uint32_t off) {
+    return (v ? vc : kc) + (uint64_t(pg) * fa.page_codes + (hc + off));
+  };
+  auto scales_at = [&](int v, uint32_t pg, uint32_t off) {
+    return (v ? fa.vs : fa.ks) + (uint64_t(pg) * fa.page_scales + (hs + off));
+  };
+  auto load_scales = [&](const uint8_t* p, uint32_t lds) {
+    if constexpr (D == 64)
+      fp4_dma2(p, lds);
+    else
+      fp4_dma4(p, lds);
+  };
+  // The tile at key n < kb of a window, whole rows; a lane's scales are a word: of a
+  // key (of half of it at D = 256), lanes below 32 K's, the others V's up to D =
+  // 128.  issue_rows: any page size, an address per lane and load; keys past the
+  // window are its last one (their weights are zero).
+  auto issue_rows = [&](int kb, int page0, int tb, int n) {
+    const uint32_t dst = ring + wp;
+    uint32_t off;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      if constexpr (EVEN) {
-        // (16-aligned: ka is a multiple of 32, and so is every tile's start)
-        const int nb = min(n + 16 * x, v.ka + ((top - v.ka) & ~15));
-        const int lp = page_of(nb);
-        const uint32_t off = nb - lp * a.page_size;
-        const int slot = v.ka < v.kb ? lp - v.page0 : 0;
-        const uint32_t pk = __builtin_amdgcn_readfirstlane(v.ka < v.kb ? tab[tb][0][slot] : 0);
-        const uint32_t pv = __builtin_amdgcn_readfirstlane(v.ka < v.kb ? tab[tb][1][slot] : 0);
-        const uint32_t oc = hc + off * (D / 2), os = hs + off * (D / 32);
-        fp4_load<D>(t.k[x], kc, fa.ks, uint64_t(pk) * fa.page_codes + oc,
-                    uint64_t(pk) * fa.page_scales + os, cl, sl);
-        fp4_load<D>(t.v[x], vc, fa.vs, uint64_t(pv) * fa.page_codes + oc,
-                    uint64_t(pv) * fa.page_scales + os, cl, sl);
-      } else {
-        const int nk = min(n + 16 * x + l16, top);
-        const int lp = page_of(nk);
-        const uint32_t off = nk - lp * a.page_size;
-        const int slot = v.ka < v.kb ? lp - v.page0 : 0;
-        const uint32_t pk = v.ka < v.kb ? tab[tb][0][slot] : 0;
-        const uint32_t pv = v.ka < v.kb ? tab[tb][1][slot] : 0;
-        const uint32_t oc = hc + off * (D / 2) + gdim, os = hs + off * (D / 32) + gscale;
-        fp4_load<D>(t.k[x], kc, fa.ks, uint64_t(pk) * fa.page_codes + oc,
-                    uint64_t(pk) * fa.page_scales + os, 0, 0);
-        fp4_load<D>(t.v[x], vc, fa.vs, uint64_t(pv) * fa.page_codes + oc,
-                    uint64_t(pv) * fa.page_scales + os, 0, 0);
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+      for (int i = 0; i < G::kLoads; ++i) {
+        const int r = (i * 64 + lane) / G::kNC;
+        const uint32_t pg = place(min(n + (v ? G::vkey(r) : r), kb - 1), page0, tb, v, off);
+        const int c = (lane % G::kNC) ^ (v ? 0 : G::ksw(r));
+        fp4_dma16(codes_at(v, pg, off * G::kRow + c * 16), dst + v * G::kCode + i * 1024);
+      }
+#pragma unroll
+    for (int i = 0; i < G::kScaleLoads; ++i) {
+      const int v = D == 256 ? i : lane >> 5;
+      const int r = D == 256 ? lane >> 1 : lane & 31;
+      const uint32_t pg = place(min(n + r, kb - 1), page0, tb, v, off);
+      load_scales(scales_at(v, pg, off * (D / 32) + (D == 256 ? 4 * (lane & 1) : 0)),
+                  dst + 2 * G::kCode + i * 256);
+    }
+    advance();
+  };
+  // issue_blocks: page_size a multiple of 16.  The 16 keys of a block are one run
+  // of memory: 16 lanes look up a block each (K's two, V's two), and a load takes
+  // its base from theirs.  (Blocks past the window are its last one, rows past
+  // it in a block what its page holds.)
+  // this lane's place in load i of a block (of both, at D = 64) of K or V
+  auto run = [&](int v, int i) -> uint32_t {
+    const int r = i * (64 / G::kNC) + lane / G::kNC;
+    return (v ? G::vkey(r) : r) * G::kRow + ((lane % G::kNC) ^ (v ? 0 : G::ksw(r))) * 16;
+  };
+  uint32_t run_k[G::kLoads > 1 ? G::kLoads / 2 : 1], run_v[G::kLoads > 1 ? G::kLoads / 2 : 1];
+#pragma unroll
+  for (int i = 0; i < (G::kLoads > 1 ? G::kLoads / 2 : 1); ++i) {
+    run_k[i] = run(0, i);
+    run_v[i] = run(1, i);
+  }
+  auto issue_blocks = [&](int kb, int page0, int tb, int n) {
+    const uint32_t dst = ring + wp;
+    const int top = (kb - 1) & ~15;  // (a window starts at a multiple of 32)
+    uint32_t off;
+    const uint32_t pg = place(min(n + 16 * (g & 1), top), page0, tb, g >> 1, off);
+    if constexpr (D == 64) {  // a load takes both blocks
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        uint32_t o2;
+        const uint32_t p2 = place(min(n + 16 * (lane >> 5), top), page0, tb, v, o2);
+        fp4_dma16(codes_at(v, p2, (o2 - 16 * (lane >> 5)) * G::kRow + (v ? run_v[0] : run_k[0])),
+                  dst + v * G::kCode);
+      }
+    } else {
+      const uint64_t at = reinterpret_cast<uint64_t>(codes_at(g >> 1, pg, off * G::kRow));
+      const int lo = static_cast<int>(at), hi = static_cast<int>(at >> 32);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const uint64_t base =
+            (static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(hi, 16 * b)))
+             << 32) |
+            static_cast<uint32_t>(__builtin_amdgcn_readlane(lo, 16 * b));
+#pragma unroll
+        for (int i = 0; i < G::kLoads / 2; ++i)
+          fp4_dma16_base(base, b < 2 ? run_k[i] : run_v[i],
+                         dst + b * (G::kCode / 2) + i * 1024);
       }
     }
+    if constexpr (D == 256) {
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        const int x = lane >> 5;
+        const uint32_t p2 = place(min(n + 16 * x, top), page0, tb, v, off);
+        load_scales(scales_at(v, p2, off * (D / 32) + 4 * (lane & 31)),
+                    dst + 2 * G::kCode + v * 256);
+      }
+    } else {
+      load_scales(scales_at(g >> 1, pg, (off + l16) * (D / 32)), dst + 2 * G::kCode);
+    }
+    advance();
+  };
+  const bool blocks = a.page_size % 16 == 0;
+  // the next tile of this wave, in this window or the next one
+  int ic = 0, jn = 0;  // its keys
+  auto issue_next = [&]() {
+    const bool here = ic < cur.kb;
+    if (!here && !(has_next && jn < nxt.kb)) return;
+    const int n = here ? ic : jn;
+    ic += here ? kStep : 0;
+    jn += here ? 0 : kStep;
+    const int kb = here ? cur.kb : nxt.kb, p0 = here ? cur.page0 : nxt.page0;
+    const int tb = here ? buf : buf ^ 1;
+    if (blocks)
+      issue_blocks(kb, p0, tb, n);
+    else
+      issue_rows(kb, p0, tb, n);
   };
 
   // ---- state ---------------------------------------------------------------
   u32x4 q[RB][DJ];
   float m[RB], l[RB];
-  f32x4 o[RB][DB];
+  f32x4 o[RB][G::kNI];
+  uint32_t nans[RB];  // NaN blocks of V that a row sees, by the lane's scales
   int q0 = 0, rows = 0;
   // Q^T (B operand): lane row l16, the dims of its group in k-step order
   auto load_q = [&](const Window& v) {
@@ -285,20 +416,91 @@ __global__ __launch_bounds__(kD4Threads, 1) void fa2_decode_fp4_kernel(Fp4Args f
       }
       m[rb] = -INFINITY;
       l[rb] = 0.f;
+      nans[rb] = 0;
 #pragma unroll
-      for (int d = 0; d < DB; ++d) o[rb][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < G::kNI; ++i) o[rb][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
+    // A wait that the compiler sees: with Q in flight at the head of the tile
+    // loop, its first use there would wait for the tiles loaded after it.
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   };
 
-  // V in LDS: row r, 32-byte chunk pair p at p ^ vsw(r), so that the 8 rows that 32
-  // lanes of a transpose read hit distinct banks
-  auto vsw = [](int r) { return D >= 128 ? r & 7 : (r >> 1) & 3; };
-  const uint32_t vbuf = lds_addr_of(lds) + wave * kVBytes;
-  const int vr = 4 * g + (l16 >> 2);
-  const uint32_t voff = vr * kRow + vsw(vr) * 32 + (l16 & 3) * 8;
+  // places in a tile: this lane's dims of V (rows from there: kRow apart by 4), its
+  // scales (of 4 keys, one word each) and the byte in them
+  const uint32_t vat = G::kCode + g * G::kRow + l16 * (D / 32);
+  const uint32_t vsat = 2 * G::kCode + G::kScale + 4 * g * G::kScaleRow +
+                        (D == 256 ? 4 * (l16 >> 3) : 0);
+  const uint32_t vbyte = D == 64 ? l16 >> 3 : D == 128 ? l16 >> 2 : (l16 >> 1) & 3;
+  const uint32_t vrot = (8 * vbyte + 9) & 31;  // ... turned to a float's exponent
 
-  auto compute = [&](const Tile& t, int n0, int kb, int full, const int (&last)[RB]) {
+  // The oldest tile of the ring, at key n0; kb: the window's end, full: no key
+  // below it is hidden from any row, last: the last key that the lane's rows see.
+  auto compute = [&](int n0, int kb, int full, const int (&last)[RB]) {
     const bool edge = n0 + kD4Tile > full;
+    // its loads are performed: those of up to fly - 1 tiles after it may not be
+    if (fly >= 4 && G::kRing >= 4)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * G::kInFlight) : "memory");
+    else if (fly == 3 && G::kRing >= 3)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * G::kInFlight) : "memory");
+    else if (fly == 2)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(G::kInFlight) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    constexpr int kVW = D == 256 ? 2 : 1;  // words of V of a lane and key
+    uint32_t kw[2][DJ], ks[2], vw[8][kVW], vs[8];
+    const uint32_t src = ring + rp;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int r = 16 * x + l16;
+      const uint32_t row = src + r * G::kRow;
+      if constexpr (D == 64) {
+        const u32x2 y =
+            *(const lds_u32x2_t*)lds_ptr(row + ((g >> 1) ^ G::ksw(r)) * 16 + (g & 1) * 8);
+        kw[x][0] = y[0];
+        kw[x][1] = y[1];
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 128; ++i) {
+          const u32x4 y =
+              *(const lds_u32x4_t*)lds_ptr(row + ((g * (D / 128) + i) ^ G::ksw(r)) * 16);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) kw[x][4 * i + j] = y[j];
+        }
+      }
+      const uint32_t at = src + 2 * G::kCode + r * G::kScaleRow + g * (D / 4) / 32;
+      if constexpr (D == 256)
+        ks[x] = *(const lds_u16_t*)lds_ptr(at);
+      else
+        ks[x] = *(const lds_u8_t*)lds_ptr(at);
+      // V: keys 16 x + 4 g ..+3, as the P^T fragment has them
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t va = src + vat + (16 * x + 4 * k) * G::kRow;
+        if constexpr (D == 64) {
+          vw[4 * x + k][0] = *(const lds_u16_t*)lds_ptr(va);
+        } else if constexpr (D == 128) {
+          vw[4 * x + k][0] = *(const lds_u32_t*)lds_ptr(va);
+        } else {
+          const u32x2 y = *(const lds_u32x2_t*)lds_ptr(va);
+          vw[4 * x + k][0] = y[0];
+          vw[4 * x + k][1] = y[1];
+        }
+      }
+      const uint32_t sa = src + vsat + 16 * x * G::kScaleRow;
+      if constexpr (D == 256) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) vs[4 * x + k] = *(const lds_u32_t*)lds_ptr(sa + 8 * k);
+      } else {
+        const u32x4 y = *(const lds_u32x4_t*)lds_ptr(sa);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) vs[4 * x + k] = y[k];
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot is free
+    rp = rp + G::kTile == G::kRing * G::kTile ? 0 : rp + G::kTile;
+    --fly;
+    issue_next();
+
     f32x4 s[RB][2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -306,10 +508,44 @@ __global__ __launch_bounds__(kD4Threads, 1) void fa2_decode_fp4_kernel(Fp4Args f
       for (int rb = 0; rb < RB; ++rb) s[rb][x] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < DJ; ++j) {
-        const uint32_t sb = D == 256 ? (j < DJ / 2 ? t.k[x].s & 255u : t.k[x].s >> 8) : t.k[x].s;
-        const u32x4 kf = fp4_values<BF>(t.k[x].w[j], sb);
+        const uint32_t sb = D == 256 ? (j < DJ / 2 ? ks[x] & 255u : ks[x] >> 8) : ks[x];
+        const u32x4 kf = fp4_values<BF>(kw[x][j], sb);
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) s[rb][x] = mma16x32<BF>(kf, q[rb][j], s[rb][x]);
+      }
+    }
+    // scales of V as floats: the byte in the place of the exponent
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      vs[k] = __builtin_amdgcn_alignbit(vs[k], vs[k], vrot) & 0x7F800000u;
+    // Keys past the end hold anything: zeros.  A block of V that is NaN must
+    // not reach the rows that do not see its key (0 * NaN): where drafts may be
+    // hidden, zeros, and NaN at the end (nans).
+    if (edge) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int key = n0 + 16 * (k >> 2) + (k & 3);  // of lane group 0
+        const bool in = key + 4 * g < kb;
+        const bool bad = in && causal && vs[k] == 0x7F800000u;
+        const uint64_t at = __ballot(bad);
+        if (at) {
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+            for (int gk = 0; gk < 4; ++gk)
+#pragma unroll
+              for (int u = 0; u < kSub; ++u) {
+                // a lane that has the scale of this lane's dims of O
+                const int of = D == 64 ? 8 * (g >> 1) : D == 128 ? 4 * g : 4 * g + 2 * u;
+                if (key + 4 * gk <= last[rb])
+                  nans[rb] |= static_cast<uint32_t>((at >> (16 * gk + of)) & 1) << u;
+              }
+        }
+        if (bad || !in) {
+          vs[k] = 0x3F800000u;
+#pragma unroll
+          for (int j = 0; j < kVW; ++j) vw[k][j] = 0u;
+        }
       }
     }
     u32x4 ph[RB], pl[RB];
@@ -335,7 +571,7 @@ __global__ __launch_bounds__(kD4Threads, 1) void fa2_decode_fp4_kernel(Fp4Args f
         m[rb] = mn;
         l[rb] *= alpha;
 #pragma unroll
-        for (int d = 0; d < DB; ++d) o[rb][d] *= alpha;
+        for (int i = 0; i < G::kNI; ++i) o[rb][i] *= alpha;
       }
       // (the difference is taken before the scale: no score is too large for it)
       const float mu = m[rb] == -INFINITY ? 0.f : m[rb];
@@ -347,88 +583,43 @@ __global__ __launch_bounds__(kD4Threads, 1) void fa2_decode_fp4_kernel(Fp4Args f
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        ph[rb][r] = pack2<BF>(e[2 * r], e[2 * r + 1]);
-        const uint32_t hw = ph[rb][r];
+        const uint32_t hw = pack2<BF>(e[2 * r], e[2 * r + 1]);
         const f32x2 h = unpack2<BF>(hw);
+        ph[rb][r] = hw;
         pl[rb][r] = pack2<BF>(e[2 * r] - h[0], e[2 * r + 1] - h[1]);
       }
     }
-    // V: 16 bits, to LDS.  Keys past the end hold anything: zeros instead.  A
-    // block that is NaN must not reach the rows that do not see its key (0 *
-    // NaN): where drafts may be hidden, zeros, and NaN afterwards (nan_keys).
-    constexpr int kSub = D == 256 ? 2 : 1;  // scales of a lane
-    uint64_t nan_at[2][kSub] = {};
-    bool nan_keys = false;
+    // O^T: dims 2 t and 2 t + 1 of each lane's, 8 keys each
+    auto pair_step = [&](auto tc) {
+      constexpr int t = decltype(tc)::value;
+      uint32_t c[8];
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int r = 16 * x + l16;
-      uint32_t vw[DJ], vs = t.v[x].s;
+      for (int k = 0; k < 8; ++k) c[k] = fp4_pair<BF, t & 3>(vw[k][t >> 2], vs[k]);
+      u32x4 va, vb;
 #pragma unroll
-      for (int j = 0; j < DJ; ++j) vw[j] = t.v[x].w[j];
-      if (edge) {
-        const bool in = n0 + r < kb;
-        bool drop[kSub];
-#pragma unroll
-        for (int u = 0; u < kSub; ++u) {
-          const bool bad = in && causal && ((vs >> (8 * u)) & 255u) == 255u;
-          nan_at[x][u] = __ballot(bad);
-          nan_keys = nan_keys || nan_at[x][u] != 0;
-          drop[u] = bad || !in;
-          if (drop[u]) vs = (vs & ~(255u << (8 * u))) | (127u << (8 * u));
-        }
-#pragma unroll
-        for (int j = 0; j < DJ; ++j)
-          if (drop[j * kSub / DJ]) vw[j] = 0u;
+      for (int k = 0; k < 4; ++k) {
+        va[k] = __builtin_amdgcn_perm(c[2 * k + 1], c[2 * k], 0x05040100u);
+        vb[k] = __builtin_amdgcn_perm(c[2 * k + 1], c[2 * k], 0x07060302u);
       }
 #pragma unroll
-      for (int j = 0; j < DJ; ++j) {
-        const uint32_t sb = D == 256 ? (j < DJ / 2 ? vs & 255u : vs >> 8) : vs;
-        const int c = g * DJ + j;
-        *(lds_u32x4_t*)lds_ptr(vbuf + r * kRow + (((c >> 1) ^ vsw(r)) * 32) + (c & 1) * 16) =
-            fp4_values<BF>(vw[j], sb);
+      for (int rb = 0; rb < RB; ++rb) {
+        o[rb][2 * t] = mma16x32<BF>(va, pl[rb], o[rb][2 * t]);
+        o[rb][2 * t + 1] = mma16x32<BF>(vb, pl[rb], o[rb][2 * t + 1]);
+        o[rb][2 * t] = mma16x32<BF>(va, ph[rb], o[rb][2 * t]);
+        o[rb][2 * t + 1] = mma16x32<BF>(vb, ph[rb], o[rb][2 * t + 1]);
       }
+    };
+    pair_step(std::integral_constant<int, 0>{});
+    pair_step(std::integral_constant<int, 1>{});
+    if constexpr (D >= 128) {
+      pair_step(std::integral_constant<int, 2>{});
+      pair_step(std::integral_constant<int, 3>{});
     }
-    asm volatile("" ::: "memory");  // (a wave's LDS operations are performed in order)
-    constexpr int kH = DB / 2;  // half of the V^T fragments are read before their MFMAs
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      u32x4 vf[kH];
-#pragma unroll
-      for (int d = 0; d < kH; ++d) {
-        const uint32_t va = vbuf + (voff ^ (32u * (h * kH + d)));
-        const u32x2 lo = __builtin_bit_cast(
-            u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)lds_ptr(va)));
-        const u32x2 hi = __builtin_bit_cast(
-            u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)lds_ptr(va + 16 * kRow)));
-        vf[d] = (u32x4){lo[0], lo[1], hi[0], hi[1]};
-      }
-#pragma unroll
-      for (int d = 0; d < kH; ++d)
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          o[rb][h * kH + d] = mma16x32<BF>(vf[d], pl[rb], o[rb][h * kH + d]);
-          o[rb][h * kH + d] = mma16x32<BF>(vf[d], ph[rb], o[rb][h * kH + d]);
-        }
-    }
-    asm volatile("" ::: "memory");
-    if (nan_keys) {
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll 1
-          for (int k = 0; k < 16; ++k) {
-            if (n0 + 16 * x + k > last[rb]) break;
-#pragma unroll
-            for (int d = 0; d < DB; ++d) {
-              // the lane group and scale that hold dims 16 d ..+15
-              const int gg = d * 4 / DB, u = kSub == 1 ? 0 : (d / 2) & 1;
-              if ((nan_at[x][u] >> (16 * gg + k)) & 1) {
-                const float nan = __builtin_nanf("");
-                o[rb][d] = (f32x4){nan, nan, nan, nan};
-              }
-            }
-          }
+    if constexpr (D == 256) {
+      pair_step(std::integral_constant<int, 4>{});
+      pair_step(std::integral_constant<int, 5>{});
+      pair_step(std::integral_constant<int, 6>{});
+      pair_step(std::integral_constant<int, 7>{});
     }
   };
 
@@ -437,8 +628,13 @@ __global__ __launch_bounds__(kD4Threads, 1) void fa2_decode_fp4_kernel(Fp4Args f
   // This wave's first tile of a window: the tiles of consecutive windows go
   // round the waves without a gap, so that none gets more than its share.
   int turn = wave;
-#pragma unroll
-  for (int i = 0; i < RING; ++i) issue(ring[i], source(cur, 0), cur.ka + turn * kD4Tile + i * kStep);
+  auto turn_after = [&](const Window& v) {
+    return (turn - (v.kb - v.ka + kD4Tile - 1) / kD4Tile) & (kD4Waves - 1);
+  };
+  ic = cur.ka + turn * kD4Tile;
+  if (has_next) jn = nxt.ka + turn_after(cur) * kD4Tile;
+#pragma unroll 1
+  for (int i = 0; i < G::kRing; ++i) issue_next();
 
   for (;;) {
     const Work& w = cur.p.w;
@@ -446,43 +642,36 @@ __global__ __launch_bounds__(kD4Threads, 1) void fa2_decode_fp4_kernel(Fp4Args f
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb)
       last[rb] = causal ? min(cur.kb - 1, w.off + diag_row(a, q0 + 16 * rb + l16)) : cur.kb - 1;
-    // no key below this one is hidden from any row
     const int full = causal ? min(cur.kb, w.off + 1) : cur.kb;
-    const int turn_next = (turn - (cur.kb - cur.ka + kD4Tile - 1) / kD4Tile) & (kD4Waves - 1);
-
-    // Rounds of RING tiles; a round's slots are loaded again with the next
-    // round's tiles, or the next window's first ones, as they are used.
-    for (int n0 = cur.ka + turn * kD4Tile;;) {
-      const bool more = n0 + RING * kStep < cur.kb;
-      const bool here = more || !has_next;
-      const int nx = here ? n0 + RING * kStep : nxt.ka + turn_next * kD4Tile;
-      const Source src = here ? source(cur, buf) : source(nxt, buf ^ 1);
-#pragma unroll
-      for (int i = 0; i < RING; ++i) {
-        if (n0 + i * kStep < cur.kb) compute(ring[i], n0 + i * kStep, cur.kb, full, last);
-        issue(ring[i], src, nx + i * kStep);
-      }
-      if (!more) break;
-      n0 += RING * kStep;
-    }
-    turn = turn_next;
+    for (int n0 = cur.ka + turn * kD4Tile; n0 < cur.kb; n0 += kStep)
+      compute(n0, cur.kb, full, last);
+    turn = turn_after(cur);
 
     if (cur.kb >= cur.kend) {
-      // ---- the piece's end: merge the waves' states, 16 rows at a time --------
+      // ---- the piece's end: merge the waves' states, kPD dims at a time -------
       const DecPiece& p = cur.p;
       const int64_t slot = p.np == 1 ? 0 : walk_slot(a, sg.C, p.us, stream, p.mine);
       const uint32_t pr = static_cast<uint32_t>(a.part_rows);
       const __amdgpu_buffer_rsrc_t rm = make_rsrc_uniform(a.part_ml + slot * pr * 2, pr * 8);
       const __amdgpu_buffer_rsrc_t ro = make_rsrc_uniform(a.part_o + slot * pr * D, pr * D * 4);
-      const uint32_t area = lds_addr_of(lds);
+      const uint32_t area = lds_addr_of(stage);
+      constexpr int kTPR = G::kPD / 2;  // threads of a row, two dims each
+      const int lr = tid / kTPR, sd = (tid % kTPR) * 2;
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
         if (16 * rb >= rows) break;
+        if (__any(nans[rb])) {
+          const float nan = __builtin_nanf("");
+#pragma unroll
+          for (int i = 0; i < G::kNI; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)  // (two scales at D = 256: dims 64 g + 16 r + i)
+              if ((nans[rb] >> (D == 256 ? r >> 1 : 0)) & 1) o[rb][i][r] = nan;
+        }
         float lw = l[rb];
         lw += __shfl_xor(lw, 16);
         lw += __shfl_xor(lw, 32);
         const float mw = m[rb] * a.scale_log2;  // (-inf stays -inf)
-        if (rb > 0) __syncthreads();  // the rows before are read
         if (g == 0) {
           mrg_ml[wave][l16][0] = mw;
           mrg_ml[wave][l16][1] = lw;
@@ -492,51 +681,58 @@ __global__ __launch_bounds__(kD4Threads, 1) void fa2_decode_fp4_kernel(Fp4Args f
 #pragma unroll
         for (int x = 0; x < kD4Waves; ++x) mg = fmaxf(mg, mrg_ml[x][l16][0]);
         const float f = fast_exp2(mw - (mg == -INFINITY ? 0.f : mg));
-        const uint32_t po = area + (wave * 16 + l16) * kPitch + 16 * g;
-#pragma unroll
-        for (int d = 0; d < DB; ++d) *(lds_f32x4_t*)lds_ptr(po + 64 * d) = o[rb][d] * f;
-        __syncthreads();
-        constexpr int kTPR = D / 4;
-        constexpr int kRP = kD4Threads / kTPR;
-        const int col = (tid % kTPR) * 4;
-        for (int lr = tid / kTPR; lr < 16; lr += kRP) {
-          const int r = 16 * rb + lr;
-          if (r >= rows) continue;
-          float mt = -INFINITY;
+        // of the row that this thread adds up
+        float mt = -INFINITY, lt = 0.f;
+        if (lr < 16) {
 #pragma unroll
           for (int x = 0; x < kD4Waves; ++x) mt = fmaxf(mt, mrg_ml[x][lr][0]);
           const float mu = mt == -INFINITY ? 0.f : mt;
-          float lt = 0.f;
-          f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int x = 0; x < kD4Waves; ++x) {
+          for (int x = 0; x < kD4Waves; ++x)
             lt += mrg_ml[x][lr][1] * fast_exp2(mrg_ml[x][lr][0] - mu);
-            acc += *(const lds_f32x4_t*)lds_ptr(area + (x * 16 + lr) * kPitch + col * 4);
-          }
-          if (p.np == 1) {  // 0/0 -> NaN for a row with no key, as the 16-bit kernels
-            const float inv = 1.f / lt;
-            *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.o) + w.o_base +
-                                      static_cast<int64_t>(q0 + r) * a.o_ss + col) =
-                (u32x2){pack2<BF>(acc[0] * inv, acc[1] * inv),
-                        pack2<BF>(acc[2] * inv, acc[3] * inv)};
-          } else {
-            if (col == 0)
-              __builtin_amdgcn_raw_buffer_store_b64(
-                  (u32x2){__builtin_bit_cast(uint32_t, mt), __builtin_bit_cast(uint32_t, lt)}, rm,
-                  r * 8, 0, kCpolSc1);
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc), ro,
-                                                   (r * D + col) * 4, 0, kCpolSc1);
-          }
         }
+        const int r = 16 * rb + lr;
+        const float inv = 1.f / lt;  // 0/0 -> NaN for a row with no key, as the 16-bit kernels
+#pragma unroll
+        for (int h = 0; h < G::kPH; ++h) {
+          const uint32_t po = area + (wave * 16 + l16) * G::kPitch + 64 * g;
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            f32x4 y;
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              y[u] = o[rb][(e + u) % G::kNI][h * G::kRP + (e + u) / G::kNI] * f;
+            *(lds_f32x4_t*)lds_ptr(po + 4 * e) = y;
+          }
+          __syncthreads();
+          if (lr < 16 && r < rows) {
+            f32x2 acc = (f32x2){0.f, 0.f};
+#pragma unroll
+            for (int x = 0; x < kD4Waves; ++x)
+              acc += *(const lds_f32x2_t*)lds_ptr(area + (x * 16 + lr) * G::kPitch + sd * 4);
+            const int dim = G::dim(h, sd);
+            if (p.np == 1)
+              *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) + w.o_base +
+                                           static_cast<int64_t>(q0 + r) * a.o_ss + dim) =
+                  pack2<BF>(acc[0] * inv, acc[1] * inv);
+            else
+              __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, acc), ro,
+                                                    (r * D + dim) * 4, 0, kCpolSc1);
+          }
+          __syncthreads();
+        }
+        if (p.np > 1 && lr < 16 && r < rows && sd == 0)
+          __builtin_amdgcn_raw_buffer_store_b64(
+              (u32x2){__builtin_bit_cast(uint32_t, mt), __builtin_bit_cast(uint32_t, lt)}, rm,
+              r * 8, 0, kCpolSc1);
       }
-      __syncthreads();  // (also where the unit has no rows in this block)
       if (p.np > 1) {
         merge_publish();
         __syncthreads();
         if (merge_count(a, p.unit, p.np, &merge_flag))
           merge_pieces<DT, D, kD4Threads, 16 * RB>(
               a, [&](int s) { return walk_slot(a, sg.C, p.us, stream, s); }, p.np, rows, w.o_base,
-              q0, lds);
+              q0, stage);
       }
       if (has_next) load_q(nxt);
     }
@@ -545,8 +741,15 @@ __global__ __launch_bounds__(kD4Threads, 1) void fa2_decode_fp4_kernel(Fp4Args f
     cur = nxt;
     buf ^= 1;
     has_next = next_window(cur, nxt);
-    if (has_next) load_table(nxt, buf ^ 1);
-    __syncthreads();  // the table (read at this window's end) is in LDS
+    ic = jn;
+    if (has_next) {
+      load_table(nxt, buf ^ 1);
+      jn = nxt.ka + turn_after(cur) * kD4Tile;
+    }
+    __syncthreads();  // the table is in LDS
+    // (windows of few tiles leave the ring with room)
+#pragma unroll 1
+    while (fly < G::kRing && (ic < cur.kb || (has_next && jn < nxt.kb))) issue_next();
   }
 }
 

@@ -72,11 +72,6 @@ void launch_norm_rope_dim(int64_t d, const NormRopeArgs& a, int u, uint32_t grid
 
 bool fp4_dim_ok(int64_t d) { return d == 64 || d == 128 || d == 256; }
 
-// (the attention reads two scales of a row at once at head_dim 256)
-bool fp4_scales_ok(const uint8_t* s, int64_t d) {
-  return d < 256 || reinterpret_cast<uintptr_t>(s) % 2 == 0;
-}
-
 int validate_rows(const fa2_fp4_rows_params* p) {
   if (!p) return FA2_ERR_NULL_POINTER;
   if (p->dtype < FA2_DTYPE_F16 || p->dtype > FA2_DTYPE_F32) return FA2_ERR_BAD_DTYPE;
@@ -198,10 +193,10 @@ int fp4_plan(const fa2_fp4_decode_params* p, Fp4Plan* pl) {
   const int64_t nqb = cdiv(pl->rows, 16 * pl->rb);
   pl->part_rows = std::min<int64_t>(pl->rows, 16 * pl->rb);
   pl->streams = p->kv_heads * nqb;
-  const int64_t cus = cu_count_current_device();
+  const int64_t wgs = cu_count_current_device();
   const int64_t tiles = std::max<int64_t>(cdiv(p->table_width * p->page_size, kBN), 1);
   const int64_t total = tiles * p->batch;  // (at most: lengths are on the device)
-  pl->segs = std::min(std::max<int64_t>(1, cus / pl->streams), cdiv(total, kD4GridTiles));
+  pl->segs = std::min(std::max<int64_t>(1, wgs / pl->streams), cdiv(total, kD4GridTiles));
   const int64_t part_bytes = 2 * pl->streams * pl->segs * pl->part_rows * p->head_dim * 4;
   if (total >= (int64_t(1) << 30) || part_bytes >= (int64_t(1) << 31) ||
       pl->streams * p->batch > kLim)
@@ -224,29 +219,19 @@ int fp4_plan(const fa2_fp4_decode_params* p, Fp4Plan* pl) {
 bool fp4_empty(const fa2_fp4_decode_params* p) { return p->batch == 0 || p->q_len == 0; }
 
 template <int DT, int D>
-void launch_fp4_decode(const Fp4Args& a, int rb, bool even, uint32_t grid, hipStream_t st) {
-  auto go = [&](auto r, auto e) {
-    constexpr int RB = decltype(r)::value;
-    constexpr int kRing = D == 64 ? 6 : D == 128 ? (RB == 1 ? 4 : 3) : 2;
-    hipLaunchKernelGGL((fa2_decode_fp4_kernel<DT, D, RB, kRing, decltype(e)::value>), dim3(grid),
-                       dim3(kD4Threads), 0, st, a);
-  };
-  using One = std::integral_constant<int, 1>;
-  if (rb == 1 && even) go(One{}, std::true_type{});
-  else if (rb == 1) go(One{}, std::false_type{});
-  if constexpr (D <= 128) {
-    using Two = std::integral_constant<int, 2>;
-    if (rb == 2 && even) go(Two{}, std::true_type{});
-    else if (rb == 2) go(Two{}, std::false_type{});
-  }
+void launch_fp4_decode(const Fp4Args& a, int rb, uint32_t grid, hipStream_t st) {
+  if (rb == 1)
+    hipLaunchKernelGGL((fa2_decode_fp4_kernel<DT, D, 1>), dim3(grid), dim3(kD4Threads), 0, st, a);
+  if constexpr (D <= 128)
+    if (rb == 2)
+      hipLaunchKernelGGL((fa2_decode_fp4_kernel<DT, D, 2>), dim3(grid), dim3(kD4Threads), 0, st, a);
 }
 
 template <int DT>
-void launch_fp4_decode_dim(int64_t d, const Fp4Args& a, int rb, bool even, uint32_t grid,
-                           hipStream_t st) {
-  if (d == 64) launch_fp4_decode<DT, 64>(a, rb, even, grid, st);
-  else if (d == 128) launch_fp4_decode<DT, 128>(a, rb, even, grid, st);
-  else launch_fp4_decode<DT, 256>(a, rb, even, grid, st);
+void launch_fp4_decode_dim(int64_t d, const Fp4Args& a, int rb, uint32_t grid, hipStream_t st) {
+  if (d == 64) launch_fp4_decode<DT, 64>(a, rb, grid, st);
+  else if (d == 128) launch_fp4_decode<DT, 128>(a, rb, grid, st);
+  else launch_fp4_decode<DT, 256>(a, rb, grid, st);
 }
 
 }  // namespace
@@ -358,8 +343,8 @@ extern "C" int fa2_fp4_decode(const fa2_fp4_decode_params* p, void* stream) {
   const void* ptrs[] = {p->q, p->o, p->k_codes, p->v_codes};
   for (const void* x : ptrs)
     if (!aligned16(x)) return FA2_ERR_ALIGNMENT;
-  if (!fp4_scales_ok(p->k_scales, p->head_dim) || !fp4_scales_ok(p->v_scales, p->head_dim))
-    return FA2_ERR_ALIGNMENT;
+  for (const uint8_t* x : {p->k_scales, p->v_scales})  // (read in words)
+    if (reinterpret_cast<uintptr_t>(x) % 4) return FA2_ERR_ALIGNMENT;
   Fp4Plan pl{};
   s = fp4_plan(p, &pl);
   if (s != FA2_OK) return s;
@@ -418,11 +403,10 @@ extern "C" int fa2_fp4_decode(const fa2_fp4_decode_params* p, void* stream) {
   fa.head_scales = static_cast<uint32_t>(p->page_size * (d / 32));
   fa.page_codes = static_cast<uint32_t>(p->kv_heads * p->page_size * (d / 2));
   fa.page_scales = static_cast<uint32_t>(p->kv_heads * p->page_size * (d / 32));
-  const bool even = p->page_size % 16 == 0;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (p->dtype == FA2_DTYPE_F16)
-    launch_fp4_decode_dim<FA2_DTYPE_F16>(d, fa, pl.rb, even, static_cast<uint32_t>(grid), st);
+    launch_fp4_decode_dim<FA2_DTYPE_F16>(d, fa, pl.rb, static_cast<uint32_t>(grid), st);
   else
-    launch_fp4_decode_dim<FA2_DTYPE_BF16>(d, fa, pl.rb, even, static_cast<uint32_t>(grid), st);
+    launch_fp4_decode_dim<FA2_DTYPE_BF16>(d, fa, pl.rb, static_cast<uint32_t>(grid), st);
   return launched();
 }
