@@ -1050,35 +1050,38 @@ __device__ __forceinline__ void merge_publish() {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-__device__ __forceinline__ bool merge_count(const KArgs& a, int unit, int S, int* flag) {
-  if (threadIdx.x == 0) {
-    uint64_t* c = a.merge_ctr + unit;
-    const uint64_t tag = a.merge_tag;
-    // The first arrival replaces whatever the word held by (tag, 1); the
-    // others add.  (A compare-and-swap per arrival retries once for every
-    // other arrival: 63 pieces of one unit took 190 us to count.)
-    uint64_t old = __hip_atomic_load(c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    uint64_t cnt;
-    for (;;) {
-      if ((old >> kMergeCountBits) == tag) {
-        cnt = __hip_atomic_fetch_add(c, uint64_t(1), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) &
-              ((uint64_t(1) << kMergeCountBits) - 1);
-        break;
-      }
-      if (__hip_atomic_compare_exchange_strong(c, &old, (tag << kMergeCountBits) | 1,
-                                               __ATOMIC_RELAXED, __ATOMIC_RELAXED,
-                                               __HIP_MEMORY_SCOPE_AGENT)) {
-        cnt = 0;
-        break;
-      }
+// By one thread: counts a split of `unit`; whether it completed the count.
+__device__ __forceinline__ bool merge_arrive(const KArgs& a, int unit, int S) {
+  uint64_t* c = a.merge_ctr + unit;
+  const uint64_t tag = a.merge_tag;
+  // The first arrival replaces whatever the word held by (tag, 1); the
+  // others add.  (A compare-and-swap per arrival retries once for every
+  // other arrival: 63 pieces of one unit took 190 us to count.)
+  uint64_t old = __hip_atomic_load(c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  uint64_t cnt;
+  for (;;) {
+    if ((old >> kMergeCountBits) == tag) {
+      cnt = __hip_atomic_fetch_add(c, uint64_t(1), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) &
+            ((uint64_t(1) << kMergeCountBits) - 1);
+      break;
     }
-    const bool last = static_cast<int>(cnt) + 1 == S;
-    // the next launch with this tag (a graph replay) starts from zero; no
-    // split of this launch adds to the word after the last one
-    if (last)
-      __hip_atomic_store(c, tag << kMergeCountBits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    *static_cast<volatile int*>(flag) = last ? 1 : 0;
+    if (__hip_atomic_compare_exchange_strong(c, &old, (tag << kMergeCountBits) | 1,
+                                             __ATOMIC_RELAXED, __ATOMIC_RELAXED,
+                                             __HIP_MEMORY_SCOPE_AGENT)) {
+      cnt = 0;
+      break;
+    }
   }
+  const bool last = static_cast<int>(cnt) + 1 == S;
+  // the next launch with this tag (a graph replay) starts from zero; no
+  // split of this launch adds to the word after the last one
+  if (last)
+    __hip_atomic_store(c, tag << kMergeCountBits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return last;
+}
+
+__device__ __forceinline__ bool merge_count(const KArgs& a, int unit, int S, int* flag) {
+  if (threadIdx.x == 0) *static_cast<volatile int*>(flag) = merge_arrive(a, unit, S) ? 1 : 0;
   __syncthreads();
   // (the partials are read after this, at device scope: the count that made
   // this split the last was taken after every split's stores were performed)

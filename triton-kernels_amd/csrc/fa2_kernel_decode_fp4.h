@@ -151,7 +151,7 @@ struct Fp4Geo {
   static constexpr int kPH = D / kPD;                 // phases
   static constexpr int kRP = 16 / kNI;                // accumulator rows of a lane per phase
   static constexpr int kPitch = (kPD + 4) * 4;        // merge rows
-  static constexpr int kStage = 16 * kPitch;          // a wave's merge bytes
+  static constexpr int kStage = 16 * kPitch;          // a wave's merge area
   static constexpr int kTable = 256;                  // block-table entries of a window
   static constexpr int kRing = D == 64 ? 5 : D == 128 ? 3 : 1;
   // chunk c of row r lies at chunk c ^ ksw(r): 8 lanes reading a chunk of 8 rows
@@ -182,10 +182,10 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
 
   __shared__ __attribute__((aligned(1024))) char tiles[kD4Waves * G::kRing * G::kTile];
   __shared__ __attribute__((aligned(128))) char stage[kD4Waves * G::kStage];
-  __shared__ float mrg_ml[kD4Waves][16][2];
+  __shared__ float mrg_ml[2][kD4Waves][16][2];
   __shared__ int tab[2][2][G::kTable];
-  __shared__ DecSegment seg_sh;
-  __shared__ int merge_flag;
+  __shared__ DecSegment seg_sh[kD4Waves];
+  __shared__ int merge_flag[2];
 
   const KArgs& a = fa.a;
   const int tid = threadIdx.x;
@@ -197,21 +197,55 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
   const int stream = static_cast<int>(blockIdx.x) % a.walk_streams;
   const int seg_k = static_cast<int>(blockIdx.x) / a.walk_streams;
 
-  if (wave == 0) walk_locate<MODE>(a, seg_k, &seg_sh);
-  __syncthreads();
-  DecSegment sg;
-  sg.j = __builtin_amdgcn_readfirstlane(seg_sh.j);
-  sg.us = __builtin_amdgcn_readfirstlane(seg_sh.us);
-  sg.s0 = __builtin_amdgcn_readfirstlane(seg_sh.s0);
-  sg.s1 = __builtin_amdgcn_readfirstlane(seg_sh.s1);
-  sg.C = __builtin_amdgcn_readfirstlane(seg_sh.C);
+  // This workgroup's units: all of one kv head and q-block.
+  const int kvh = stream % a.hkv, qblk = stream / a.hkv;
+  const int head0 = kvh * (a.hq / a.hkv);
+  const int q0 = qblk * (16 * RB), rows = min(a.q_len - q0, 16 * RB);
 
-  // A window: keys [ka, kb) of a piece, all of it unless its block-table
-  // entries exceed the LDS table.
+  // The segment, found by each wave for itself (no barrier); a batch of up to 64
+  // keeps its lengths in the lanes.
+  const int lens = lane < a.batch ? walk_len<MODE>(a, lane) : 0;
+  walk_locate<MODE>(a, seg_k, &seg_sh[wave]);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  DecSegment sg;
+  sg.j = __builtin_amdgcn_readfirstlane(seg_sh[wave].j);
+  sg.us = __builtin_amdgcn_readfirstlane(seg_sh[wave].us);
+  sg.s0 = __builtin_amdgcn_readfirstlane(seg_sh[wave].s0);
+  sg.s1 = __builtin_amdgcn_readfirstlane(seg_sh[wave].s1);
+  sg.C = __builtin_amdgcn_readfirstlane(seg_sh[wave].C);
+
+  // A piece (DecPiece without what is the same for all of the workgroup's), and a
+  // window of it: keys [ka, kb), all of it unless its block-table entries exceed
+  // the LDS table.
   struct Window {
-    DecPiece p;
-    int ka, kb, kend;  // kend: the piece's end
-    int page0;         // first logical page
+    int b, us, W, Lk;   // sequence, the unit's start in the stream, weight, length
+    int np, mine;       // pieces of the unit, this one's index
+    int ka, kb, kend;   // kend: the piece's end
+    int page0;          // first logical page
+  };
+  // The piece of sequence j's unit, from us in the stream (as walk_piece).
+  auto piece_at = [&](Window& v, int j, int us) -> bool {
+    const bool whole = sg.C == 0;
+    if (j >= a.batch || (!whole && us >= sg.s1)) return false;
+    v.b = j;
+    v.us = us;
+    v.Lk = a.batch <= 64 ? __builtin_amdgcn_readlane(lens, j) : walk_len<MODE>(a, j);
+    v.W = walk_weight(v.Lk);
+    v.np = 1;
+    v.mine = 0;
+    v.ka = 0;
+    v.kend = v.Lk;
+    if (!whole) {
+      // (segment k starts at k C: only its ends can lie in other segments' units)
+      const int kf = us >= sg.s0 ? seg_k : us / sg.C;
+      const int kl = us + v.W <= sg.s1 ? seg_k : (us + v.W - 1) / sg.C;
+      v.np = kl - kf + 1;
+      v.mine = seg_k - kf;
+      v.ka = max(sg.s0 - us, 0) * kBN;
+      v.kend = min(min(us + v.W, sg.s1) - us, (v.Lk + kBN - 1) / kBN) * kBN;
+      v.kend = min(v.kend, v.Lk);
+    }
+    return true;
   };
   auto page_of = [&](int n) { return a.page_shift >= 0 ? n >> a.page_shift : n / a.page_size; };
   auto window_at = [&](Window& v, int ka) {
@@ -225,9 +259,8 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
     }
   };
   auto first_window = [&](Window& v, int j, int us) -> bool {
-    if (!walk_piece<MODE>(a, sg, stream, seg_k, j, us, v.p)) return false;
-    v.kend = min((v.p.t0 + v.p.T) * kBN, v.p.w.Lk);
-    window_at(v, v.p.t0 * kBN);
+    if (!piece_at(v, j, us)) return false;
+    window_at(v, v.ka);
     return true;
   };
   auto next_window = [&](const Window& c, Window& v) -> bool {
@@ -236,32 +269,33 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
       window_at(v, c.kb);
       return true;
     }
-    return first_window(v, walk_next(a, sg, c.p.w.b), c.p.us + c.p.W);
+    return first_window(v, walk_next(a, sg, c.b), c.us + c.W);
   };
-  // entries of the window's pages, clamped into the pool
-  auto load_table = [&](const Window& v, int buf) {
-    if (v.ka >= v.kb) return;
-    const int last = page_of(v.kb - 1);
-    for (int i = tid; i <= last - v.page0; i += kD4Threads) {
-      const int col = min(v.page0 + i, fa.table_width - 1);
-      const int pk = a.k_table[v.p.w.b * a.k_table_stride + col];
-      const int pv = a.v_table[v.p.w.b * a.v_table_stride + col];
-      tab[buf][0][i] = min(max(pk, 0), fa.num_pages - 1);
-      tab[buf][1][i] = min(max(pv, 0), fa.num_pages - 1);
-    }
+  // Entries of a window's pages, clamped into the pool: one per thread, K's by the
+  // first half of the workgroup; loaded, then put into LDS.
+  static_assert(2 * G::kTable <= kD4Threads, "one entry per thread");
+  const int half = wave / (kD4Waves / 2), slot_t = tid % (kD4Threads / 2);
+  auto fetch_entry = [&](const Window& v) -> int {
+    if (v.ka >= v.kb || slot_t > page_of(v.kb - 1) - v.page0) return 0;
+    const int col = min(v.page0 + slot_t, fa.table_width - 1);
+    return half ? a.v_table[v.b * a.v_table_stride + col]
+                : a.k_table[v.b * a.k_table_stride + col];
+  };
+  auto put_entry = [&](int e, int buf) {
+    if (slot_t < G::kTable) tab[buf][half][slot_t] = min(max(e, 0), fa.num_pages - 1);
   };
 
   Window cur, nxt;
   if (!first_window(cur, sg.j, sg.us)) return;
   bool has_next = next_window(cur, nxt);
-  load_table(cur, 0);
-  if (has_next) load_table(nxt, 1);
+  const int entry0 = fetch_entry(cur);
+  const int entry1 = has_next ? fetch_entry(nxt) : 0;
   int buf = 0;
 
   // ---- loads ---------------------------------------------------------------
   const uint8_t* kc = static_cast<const uint8_t*>(a.k);
   const uint8_t* vc = static_cast<const uint8_t*>(a.v);
-  const uint32_t hc = (stream % a.hkv) * fa.head_codes, hs = (stream % a.hkv) * fa.head_scales;
+  const uint32_t hc = kvh * fa.head_codes, hs = kvh * fa.head_scales;
   const uint32_t ring = lds_addr_of(tiles) + wave * (G::kRing * G::kTile);
   int wp = 0;   // ring bytes at which the next tile goes in
   int rp = 0;   // ... and the oldest one lies
@@ -398,32 +432,34 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
   float m[RB], l[RB];
   f32x4 o[RB][G::kNI];
   uint32_t nans[RB];  // NaN blocks of V that a row sees, by the lane's scales
-  int q0 = 0, rows = 0;
   // Q^T (B operand): lane row l16, the dims of its group in k-step order
-  auto load_q = [&](const Window& v) {
-    q0 = v.p.w.qblk * (16 * RB);
-    rows = min(v.p.w.Lq - q0, 16 * RB);
+  auto fetch_q = [&](const Window& v, u32x4 (&x)[RB][DJ]) {
+    const int64_t base = v.b * a.q_sb + head0 * a.q_sh + q0 * a.q_ss;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       const int r = 16 * rb + l16;
 #pragma unroll
       for (int j = 0; j < DJ; ++j) {
-        q[rb][j] = (u32x4){0u, 0u, 0u, 0u};
+        x[rb][j] = (u32x4){0u, 0u, 0u, 0u};
         if (r < rows)
-          q[rb][j] = *reinterpret_cast<const u32x4*>(
-              static_cast<const uint16_t*>(a.q) + v.p.w.q_base +
-              static_cast<int64_t>(q0 + r) * a.q_ss + g * (D / 4) + 8 * j);
+          x[rb][j] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + base +
+                                                     r * a.q_ss + g * (D / 4) + 8 * j);
       }
+    }
+  };
+  auto reset = [&]() {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
       m[rb] = -INFINITY;
       l[rb] = 0.f;
       nans[rb] = 0;
 #pragma unroll
       for (int i = 0; i < G::kNI; ++i) o[rb][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
-    // A wait that the compiler sees: with Q in flight at the head of the tile
-    // loop, its first use there would wait for the tiles loaded after it.
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   };
+  // A wait that the compiler sees: with a value of its own in flight at the head of
+  // the tile loop, the first use there would wait for the tiles loaded after it.
+  auto settle = [] { __builtin_amdgcn_s_waitcnt(0x0F70); };  // vmcnt(0)
 
   // places in a tile: this lane's dims of V (rows from there: kRow apart by 4), its
   // scales (of 4 keys, one word each) and the byte in them
@@ -623,8 +659,106 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
     }
   };
 
-  load_q(cur);
+  constexpr bool kAhead = RB * DJ <= 4;  // the next piece's Q is loaded ahead
+  u32x4 qn[RB][kAhead ? DJ : 1];
+  fetch_q(cur, q);
+  if constexpr (kAhead)
+    if (has_next) fetch_q(nxt, qn);
+  reset();
+  put_entry(entry0, 0);
+  put_entry(entry1, 1);
+  settle();
   __syncthreads();  // the tables are in LDS
+
+  // ---- pieces' ends ----------------------------------------------------------
+  // The waves' states meet in LDS: wave x's row r, kPD dims, at area + x * ws + r *
+  // kPitch, its maximum (log2 units) and sum in mrg_ml[mi]; added up in wave
+  // order and written, to the output or to the piece's part slot.
+  auto put_state = [&](auto rbc, auto hc_, uint32_t at) {  // phase h of this lane's row
+    constexpr int rb = decltype(rbc)::value, h = decltype(hc_)::value;
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      f32x4 y;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) y[u] = o[rb][(e + u) % G::kNI][h * G::kRP + (e + u) / G::kNI];
+      *(lds_f32x4_t*)lds_ptr(at + 64 * g + 4 * e) = y;
+    }
+  };
+  auto put_stats = [&](auto rbc, int mi) {
+    constexpr int rb = decltype(rbc)::value;
+    if (__any(nans[rb])) {
+      const float nan = __builtin_nanf("");
+#pragma unroll
+      for (int i = 0; i < G::kNI; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)  // (two scales at D = 256: dims 64 g + 16 r + i)
+          if ((nans[rb] >> (D == 256 ? r >> 1 : 0)) & 1) o[rb][i][r] = nan;
+    }
+    l[rb] += __shfl_xor(l[rb], 16);
+    l[rb] += __shfl_xor(l[rb], 32);
+    if (g == 0) {
+      mrg_ml[mi][wave][l16][0] = m[rb] * a.scale_log2;  // (-inf stays -inf)
+      mrg_ml[mi][wave][l16][1] = l[rb];
+    }
+  };
+  // Rows r0 .. r0 + n - 1 of a piece: phase h0, or with `phases` > 1 all of them, each
+  // with 16 / phases rows of its own.
+  auto add_up = [&](int b, int np, int us, int mine, uint32_t area, uint32_t ws, int mi, int r0,
+                    int n, int h0, int phases) {
+    const int64_t slot = np == 1 ? 0 : walk_slot(a, sg.C, us, stream, mine);
+    const uint32_t pr = static_cast<uint32_t>(a.part_rows);
+    const __amdgpu_buffer_rsrc_t rm = make_rsrc_uniform(a.part_ml + slot * pr * 2, pr * 8);
+    const __amdgpu_buffer_rsrc_t ro = make_rsrc_uniform(a.part_o + slot * pr * D, pr * D * 4);
+    uint16_t* out = static_cast<uint16_t*>(a.o) + (b * a.o_sb + head0 * a.o_sh + q0 * a.o_ss);
+    const int sd = (tid % 32) * 2;  // 32 threads a row, two dims each
+    for (int it = tid / 32; it < n * phases; it += kD4Threads / 32) {
+      const int h = phases > 1 ? it % G::kPH : h0;
+      const int lr = phases > 1 ? it / G::kPH : it;
+      float mt = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < kD4Waves; ++x) mt = fmaxf(mt, mrg_ml[mi][x][lr][0]);
+      const float mu = mt == -INFINITY ? 0.f : mt;
+      float lt = 0.f;
+      f32x2 acc = (f32x2){0.f, 0.f};
+      const uint32_t at =
+          area + sd * 4 + ((phases > 1 ? h * (16 / G::kPH) : 0) + lr) * G::kPitch;
+#pragma unroll
+      for (int x = 0; x < kD4Waves; ++x) {
+        const float f = fast_exp2(mrg_ml[mi][x][lr][0] - mu);
+        lt += f * mrg_ml[mi][x][lr][1];
+        acc += f * *(const lds_f32x2_t*)lds_ptr(at + x * ws);
+      }
+      const int r = r0 + lr;
+      const int dim = G::dim(h, sd);
+      if (np == 1) {
+        const float inv = 1.f / lt;  // 0/0 -> NaN for a row with no key, as in 16 bits
+        *reinterpret_cast<uint32_t*>(out + r * a.o_ss + dim) =
+            pack2<BF>(acc[0] * inv, acc[1] * inv);
+      } else {
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, acc), ro,
+                                              (r * D + dim) * 4, 0, kCpolSc1);
+        if (h == 0 && sd == 0)
+          __builtin_amdgcn_raw_buffer_store_b64(
+              (u32x2){__builtin_bit_cast(uint32_t, mt), __builtin_bit_cast(uint32_t, lt)}, rm,
+              r * 8, 0, kCpolSc1);
+      }
+    }
+  };
+  // A state that fits one area is left there, and the wave goes on to the next
+  // piece without a barrier; the piece is added up when the next but one ends,
+  // or with the last one, whose states lie in the ring.
+  const bool fits = RB == 1 && rows <= 16 / G::kPH;
+  const uint32_t area0 = lds_addr_of(stage), area1 = lds_addr_of(tiles);
+  constexpr uint32_t kWs0 = G::kStage, kWs1 = G::kRing * G::kTile;
+  static_assert(kWs1 >= G::kStage, "a wave's state in its ring");
+  struct Left {
+    int b, np, us, mine;
+  };
+  Left left = {0, 0, 0, 0};  // (np 0: none)
+  // Cut units are counted when the workgroup is done: it has two at most, one
+  // from each end of its segment.
+  Left cut[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+
   // This wave's first tile of a window: the tiles of consecutive windows go
   // round the waves without a gap, so that none gets more than its share.
   int turn = wave;
@@ -637,119 +771,128 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
   for (int i = 0; i < G::kRing; ++i) issue_next();
 
   for (;;) {
-    const Work& w = cur.p.w;
+    const int off = cur.Lk - a.pack_m;
     int last[RB];  // last visible key of this lane's rows
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb)
-      last[rb] = causal ? min(cur.kb - 1, w.off + diag_row(a, q0 + 16 * rb + l16)) : cur.kb - 1;
-    const int full = causal ? min(cur.kb, w.off + 1) : cur.kb;
-    for (int n0 = cur.ka + turn * kD4Tile; n0 < cur.kb; n0 += kStep)
+      last[rb] = causal ? min(cur.kb - 1, off + diag_row(a, q0 + 16 * rb + l16)) : cur.kb - 1;
+    const int full = causal ? min(cur.kb, off + 1) : cur.kb;
+    for (int n0 = cur.ka + turn * kD4Tile; n0 < cur.kb; n0 += kStep) {
+      // The two waves of a SIMD (i and i + 4) take turns in going first: left to
+      // itself, the older one finishes its share early and the other is alone.
+      if (((n0 / kStep) ^ (wave >> 2)) & 1)
+        __builtin_amdgcn_s_setprio(1);
+      else
+        __builtin_amdgcn_s_setprio(0);
       compute(n0, cur.kb, full, last);
+    }
     turn = turn_after(cur);
 
-    if (cur.kb >= cur.kend) {
-      // ---- the piece's end: merge the waves' states, kPD dims at a time -------
-      const DecPiece& p = cur.p;
-      const int64_t slot = p.np == 1 ? 0 : walk_slot(a, sg.C, p.us, stream, p.mine);
-      const uint32_t pr = static_cast<uint32_t>(a.part_rows);
-      const __amdgpu_buffer_rsrc_t rm = make_rsrc_uniform(a.part_ml + slot * pr * 2, pr * 8);
-      const __amdgpu_buffer_rsrc_t ro = make_rsrc_uniform(a.part_o + slot * pr * D, pr * D * 4);
-      const uint32_t area = lds_addr_of(stage);
-      constexpr int kTPR = G::kPD / 2;  // threads of a row, two dims each
-      const int lr = tid / kTPR, sd = (tid % kTPR) * 2;
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        if (16 * rb >= rows) break;
-        if (__any(nans[rb])) {
-          const float nan = __builtin_nanf("");
-#pragma unroll
-          for (int i = 0; i < G::kNI; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)  // (two scales at D = 256: dims 64 g + 16 r + i)
-              if ((nans[rb] >> (D == 256 ? r >> 1 : 0)) & 1) o[rb][i][r] = nan;
-        }
-        float lw = l[rb];
-        lw += __shfl_xor(lw, 16);
-        lw += __shfl_xor(lw, 32);
-        const float mw = m[rb] * a.scale_log2;  // (-inf stays -inf)
-        if (g == 0) {
-          mrg_ml[wave][l16][0] = mw;
-          mrg_ml[wave][l16][1] = lw;
-        }
-        __syncthreads();
-        float mg = -INFINITY;
-#pragma unroll
-        for (int x = 0; x < kD4Waves; ++x) mg = fmaxf(mg, mrg_ml[x][l16][0]);
-        const float f = fast_exp2(mw - (mg == -INFINITY ? 0.f : mg));
-        // of the row that this thread adds up
-        float mt = -INFINITY, lt = 0.f;
-        if (lr < 16) {
-#pragma unroll
-          for (int x = 0; x < kD4Waves; ++x) mt = fmaxf(mt, mrg_ml[x][lr][0]);
-          const float mu = mt == -INFINITY ? 0.f : mt;
-#pragma unroll
-          for (int x = 0; x < kD4Waves; ++x)
-            lt += mrg_ml[x][lr][1] * fast_exp2(mrg_ml[x][lr][0] - mu);
-        }
-        const int r = 16 * rb + lr;
-        const float inv = 1.f / lt;  // 0/0 -> NaN for a row with no key, as the 16-bit kernels
-#pragma unroll
-        for (int h = 0; h < G::kPH; ++h) {
-          const uint32_t po = area + (wave * 16 + l16) * G::kPitch + 64 * g;
-#pragma unroll
-          for (int e = 0; e < 16; e += 4) {
-            f32x4 y;
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-              y[u] = o[rb][(e + u) % G::kNI][h * G::kRP + (e + u) / G::kNI] * f;
-            *(lds_f32x4_t*)lds_ptr(po + 4 * e) = y;
-          }
-          __syncthreads();
-          if (lr < 16 && r < rows) {
-            f32x2 acc = (f32x2){0.f, 0.f};
-#pragma unroll
-            for (int x = 0; x < kD4Waves; ++x)
-              acc += *(const lds_f32x2_t*)lds_ptr(area + (x * 16 + lr) * G::kPitch + sd * 4);
-            const int dim = G::dim(h, sd);
-            if (p.np == 1)
-              *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) + w.o_base +
-                                           static_cast<int64_t>(q0 + r) * a.o_ss + dim) =
-                  pack2<BF>(acc[0] * inv, acc[1] * inv);
-            else
-              __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, acc), ro,
-                                                    (r * D + dim) * 4, 0, kCpolSc1);
-          }
-          __syncthreads();
-        }
-        if (p.np > 1 && lr < 16 && r < rows && sd == 0)
-          __builtin_amdgcn_raw_buffer_store_b64(
-              (u32x2){__builtin_bit_cast(uint32_t, mt), __builtin_bit_cast(uint32_t, lt)}, rm,
-              r * 8, 0, kCpolSc1);
+    const bool piece_end = cur.kb >= cur.kend;
+    if (piece_end) {
+      if (cur.np > 1) {
+        cut[1] = cut[0];
+        cut[0] = Left{cur.b, cur.np, cur.us, cur.mine};
       }
-      if (p.np > 1) {
-        merge_publish();
-        __syncthreads();
-        if (merge_count(a, p.unit, p.np, &merge_flag))
-          merge_pieces<DT, D, kD4Threads, 16 * RB>(
-              a, [&](int s) { return walk_slot(a, sg.C, p.us, stream, s); }, p.np, rows, w.o_base,
-              q0, stage);
+      using Zero = std::integral_constant<int, 0>;
+      if (fits) {
+        if (has_next && left.np) {
+          __syncthreads();
+          add_up(left.b, left.np, left.us, left.mine, area0, kWs0, 0, 0, rows, 0, G::kPH);
+          __syncthreads();
+          left.np = 0;
+        }
+        put_stats(Zero{}, has_next ? 0 : 1);
+        if (l16 < rows) {
+          const uint32_t at = (has_next ? area0 + wave * kWs0 : area1 + wave * kWs1) +
+                              l16 * G::kPitch;
+          put_state(Zero{}, Zero{}, at);
+          if constexpr (G::kPH > 1)
+            put_state(Zero{}, std::integral_constant<int, 1>{}, at + 16 / G::kPH * G::kPitch);
+          if constexpr (G::kPH > 2) {
+            put_state(Zero{}, std::integral_constant<int, 2>{}, at + 32 / G::kPH * G::kPitch);
+            put_state(Zero{}, std::integral_constant<int, 3>{}, at + 48 / G::kPH * G::kPitch);
+          }
+        }
+        if (has_next) left = Left{cur.b, cur.np, cur.us, cur.mine};
+      } else {
+        auto merge16 = [&](auto rbc) {
+          constexpr int rb = decltype(rbc)::value;
+          if (16 * rb >= rows) return;
+          const int n = min(rows - 16 * rb, 16);
+          put_stats(rbc, 0);
+          auto phase = [&](auto h) {
+            put_state(rbc, h, area0 + wave * kWs0 + l16 * G::kPitch);
+            __syncthreads();
+            add_up(cur.b, cur.np, cur.us, cur.mine, area0, kWs0, 0, 16 * rb, n,
+                   decltype(h)::value, 1);
+            __syncthreads();
+          };
+          phase(Zero{});
+          if constexpr (G::kPH > 1) phase(std::integral_constant<int, 1>{});
+          if constexpr (G::kPH > 2) {
+            phase(std::integral_constant<int, 2>{});
+            phase(std::integral_constant<int, 3>{});
+          }
+        };
+        merge16(Zero{});
+        if constexpr (RB > 1) merge16(std::integral_constant<int, 1>{});
       }
-      if (has_next) load_q(nxt);
     }
-    if (!has_next) return;
-    __syncthreads();  // the finished window's table and the merge area are free
+    if (!has_next) break;
+    if (piece_end) {
+      if constexpr (kAhead) {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+          for (int j = 0; j < DJ; ++j) q[rb][j] = qn[rb][j];
+      } else {
+        fetch_q(nxt, q);
+      }
+      reset();
+    }
     cur = nxt;
     buf ^= 1;
     has_next = next_window(cur, nxt);
     ic = jn;
     if (has_next) {
-      load_table(nxt, buf ^ 1);
       jn = nxt.ka + turn_after(cur) * kD4Tile;
+      const int e = fetch_entry(nxt);
+      if constexpr (kAhead)
+        if (nxt.ka == 0 || nxt.b != cur.b) fetch_q(nxt, qn);
+      __syncthreads();  // the finished window's table is free
+      put_entry(e, buf ^ 1);
+      settle();
+      __syncthreads();  // the table is in LDS
+    } else if (!kAhead) {
+      settle();
     }
-    __syncthreads();  // the table is in LDS
     // (windows of few tiles leave the ring with room)
 #pragma unroll 1
     while (fly < G::kRing && (ic < cur.kb || (has_next && jn < nxt.kb))) issue_next();
+  }
+  if (fits) {
+    __syncthreads();
+    if (left.np)
+      add_up(left.b, left.np, left.us, left.mine, area0, kWs0, 0, 0, rows, 0, G::kPH);
+    add_up(cur.b, cur.np, cur.us, cur.mine, area1, kWs1, 1, 0, rows, 0, G::kPH);
+  }
+  if (cut[0].np == 0) return;
+  merge_publish();
+  __syncthreads();
+  // one wave counts each; the last of a unit's pieces merges them
+  if (tid == 0) merge_flag[0] = merge_arrive(a, cut[0].b * a.walk_streams + stream, cut[0].np);
+  if (tid == 64 && cut[1].np)
+    merge_flag[1] = merge_arrive(a, cut[1].b * a.walk_streams + stream, cut[1].np);
+  __syncthreads();
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) {
+    const Left c = i ? cut[1] : cut[0];
+    if (c.np == 0 || *static_cast<volatile int*>(&merge_flag[i]) == 0) continue;
+    if (i) __syncthreads();
+    merge_pieces<DT, D, kD4Threads, 16 * RB>(
+        a, [&](int s) { return walk_slot(a, sg.C, c.us, stream, s); }, c.np, rows,
+        c.b * a.o_sb + head0 * a.o_sh, q0, stage);
   }
 }
 
