@@ -1050,14 +1050,19 @@ __device__ __forceinline__ void merge_publish() {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-// By one thread: counts a split of `unit`; whether it completed the count.
-__device__ __forceinline__ bool merge_arrive(const KArgs& a, int unit, int S) {
+// The word of `unit`, as it is now.
+__device__ __forceinline__ uint64_t merge_word(const KArgs& a, int unit) {
+  return __hip_atomic_load(a.merge_ctr + unit, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// By one thread: counts a split of `unit`, whose word was `old` at some time of this
+// launch; whether it completed the count.
+__device__ __forceinline__ bool merge_arrive(const KArgs& a, int unit, int S, uint64_t old) {
   uint64_t* c = a.merge_ctr + unit;
   const uint64_t tag = a.merge_tag;
   // The first arrival replaces whatever the word held by (tag, 1); the
   // others add.  (A compare-and-swap per arrival retries once for every
   // other arrival: 63 pieces of one unit took 190 us to count.)
-  uint64_t old = __hip_atomic_load(c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   uint64_t cnt;
   for (;;) {
     if ((old >> kMergeCountBits) == tag) {
@@ -1081,7 +1086,7 @@ __device__ __forceinline__ bool merge_arrive(const KArgs& a, int unit, int S) {
 }
 
 __device__ __forceinline__ bool merge_count(const KArgs& a, int unit, int S, int* flag) {
-  if (threadIdx.x == 0) *static_cast<volatile int*>(flag) = merge_arrive(a, unit, S) ? 1 : 0;
+  if (threadIdx.x == 0) *static_cast<volatile int*>(flag) = merge_arrive(a, unit, S, merge_word(a, unit)) ? 1 : 0;
   __syncthreads();
   // (the partials are read after this, at device scope: the count that made
   // this split the last was taken after every split's stores were performed)

@@ -151,9 +151,13 @@ struct Fp4Geo {
   static constexpr int kPH = D / kPD;                 // phases
   static constexpr int kRP = 16 / kNI;                // accumulator rows of a lane per phase
   static constexpr int kPitch = (kPD + 4) * 4;        // merge rows
-  static constexpr int kStage = 16 * kPitch;          // a wave's merge area
+  static constexpr int kSP = D == 128 ? 2 : 1;        // phases of 16 rows that a wave's area holds
+  static constexpr int kStage = 16 * kSP * kPitch;
+  static constexpr int kAllRows = 16 * kSP / kPH;     // rows of which it holds all phases
   static constexpr int kTable = 256;                  // block-table entries of a window
-  static constexpr int kRing = D == 64 ? 5 : D == 128 ? 3 : 1;
+  // Two tiles in flight per wave are enough: D64, 16 x 8200 keys, 8 drafts 35.1 / 34.2 / 33.6
+  // us at 5 / 3 / 2; D128, 16 x 16000-32768 keys 49.3 / 47.1 / 46.4 at 3 / 2 / 1.
+  static constexpr int kRing = D == 256 ? 1 : 2;
   // chunk c of row r lies at chunk c ^ ksw(r): 8 lanes reading a chunk of 8 rows
   // hit distinct banks
   static __device__ __forceinline__ int ksw(int r) {
@@ -168,6 +172,19 @@ struct Fp4Geo {
     return (sd >> 4) * (D / 4) + 16 * h + (sd & 15);
   }
 };
+
+// Sum (or maximum, of numbers >= 0) over the lanes up to each, on the VALU.
+template <bool MAX>
+__device__ __forceinline__ int wave_scan(int x) {
+  auto join = [](int a, int b) { return MAX ? max(a, b) : a + b; };
+  x = join(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false));  // row_shr 1, 2, 4, 8
+  x = join(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false));
+  x = join(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false));
+  x = join(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false));
+  x = join(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false));  // row_bcast 15, 31
+  x = join(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false));
+  return x;
+}
 
 template <int DT, int D, int RB>
 __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_decode_fp4_kernel(
@@ -202,17 +219,36 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
   const int head0 = kvh * (a.hq / a.hkv);
   const int q0 = qblk * (16 * RB), rows = min(a.q_len - q0, 16 * RB);
 
-  // The segment, found by each wave for itself (no barrier); a batch of up to 64
-  // keeps its lengths in the lanes.
-  const int lens = lane < a.batch ? walk_len<MODE>(a, lane) : 0;
-  walk_locate<MODE>(a, seg_k, &seg_sh[wave]);
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  // The segment, found by each wave for itself (no barrier).  A batch of up to 64
+  // keeps its lengths in the lanes (walk_locate's rule, on one length per lane).
+  const bool in_lanes = a.batch <= 64;
+  const int lens = in_lanes && lane < a.batch ? walk_len<MODE>(a, lane) : 0;
   DecSegment sg;
-  sg.j = __builtin_amdgcn_readfirstlane(seg_sh[wave].j);
-  sg.us = __builtin_amdgcn_readfirstlane(seg_sh[wave].us);
-  sg.s0 = __builtin_amdgcn_readfirstlane(seg_sh[wave].s0);
-  sg.s1 = __builtin_amdgcn_readfirstlane(seg_sh[wave].s1);
-  sg.C = __builtin_amdgcn_readfirstlane(seg_sh[wave].C);
+  if (in_lanes) {
+    const int W = lane < a.batch ? walk_weight(lens) : 0;
+    const int incl = wave_scan<false>(W);
+    const int total = __builtin_amdgcn_readlane(incl, 63);
+    const int longest = __builtin_amdgcn_readlane(wave_scan<true>(W), 63);
+    const int C = max((total + a.walk_segs - 1) / a.walk_segs, a.walk_min);
+    sg = DecSegment{seg_k, 0, 0, 0, 0};
+    if (longest > a.walk_short && !walk_keep_whole(a, longest, C, a.walk_whole)) {
+      const int s0 = min(seg_k * C, total);
+      const uint64_t at = __ballot(incl - W <= s0 && s0 < incl);
+      sg = DecSegment{a.batch, total, total, total, C};
+      if (at) {
+        const int j = __builtin_ctzll(at);
+        sg = DecSegment{j, __builtin_amdgcn_readlane(incl - W, j), s0, min(s0 + C, total), C};
+      }
+    }
+  } else {
+    walk_locate<MODE>(a, seg_k, &seg_sh[wave]);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    sg.j = __builtin_amdgcn_readfirstlane(seg_sh[wave].j);
+    sg.us = __builtin_amdgcn_readfirstlane(seg_sh[wave].us);
+    sg.s0 = __builtin_amdgcn_readfirstlane(seg_sh[wave].s0);
+    sg.s1 = __builtin_amdgcn_readfirstlane(seg_sh[wave].s1);
+    sg.C = __builtin_amdgcn_readfirstlane(seg_sh[wave].C);
+  }
 
   // A piece (DecPiece without what is the same for all of the workgroup's), and a
   // window of it: keys [ka, kb), all of it unless its block-table entries exceed
@@ -229,7 +265,7 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
     if (j >= a.batch || (!whole && us >= sg.s1)) return false;
     v.b = j;
     v.us = us;
-    v.Lk = a.batch <= 64 ? __builtin_amdgcn_readlane(lens, j) : walk_len<MODE>(a, j);
+    v.Lk = in_lanes ? __builtin_amdgcn_readlane(lens, j) : walk_len<MODE>(a, j);
     v.W = walk_weight(v.Lk);
     v.np = 1;
     v.mine = 0;
@@ -701,27 +737,26 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
       mrg_ml[mi][wave][l16][1] = l[rb];
     }
   };
-  // Rows r0 .. r0 + n - 1 of a piece: phase h0, or with `phases` > 1 all of them, each
-  // with 16 / phases rows of its own.
+  // Rows r0 .. r0 + n - 1 of a piece, phases h0 .. h0 + nh - 1, rg rows of an area each.
   auto add_up = [&](int b, int np, int us, int mine, uint32_t area, uint32_t ws, int mi, int r0,
-                    int n, int h0, int phases) {
+                    int n, int h0, int nh, int rg) {
     const int64_t slot = np == 1 ? 0 : walk_slot(a, sg.C, us, stream, mine);
     const uint32_t pr = static_cast<uint32_t>(a.part_rows);
     const __amdgpu_buffer_rsrc_t rm = make_rsrc_uniform(a.part_ml + slot * pr * 2, pr * 8);
     const __amdgpu_buffer_rsrc_t ro = make_rsrc_uniform(a.part_o + slot * pr * D, pr * D * 4);
     uint16_t* out = static_cast<uint16_t*>(a.o) + (b * a.o_sb + head0 * a.o_sh + q0 * a.o_ss);
     const int sd = (tid % 32) * 2;  // 32 threads a row, two dims each
-    for (int it = tid / 32; it < n * phases; it += kD4Threads / 32) {
-      const int h = phases > 1 ? it % G::kPH : h0;
-      const int lr = phases > 1 ? it / G::kPH : it;
+    for (int it = tid / 32; it < n * nh; it += kD4Threads / 32) {
+      const int hh = nh == G::kPH ? it % G::kPH : it % G::kSP;
+      const int lr = nh == G::kPH ? it / G::kPH : it / G::kSP;
+      const int h = h0 + hh;
       float mt = -INFINITY;
 #pragma unroll
       for (int x = 0; x < kD4Waves; ++x) mt = fmaxf(mt, mrg_ml[mi][x][lr][0]);
       const float mu = mt == -INFINITY ? 0.f : mt;
       float lt = 0.f;
       f32x2 acc = (f32x2){0.f, 0.f};
-      const uint32_t at =
-          area + sd * 4 + ((phases > 1 ? h * (16 / G::kPH) : 0) + lr) * G::kPitch;
+      const uint32_t at = area + sd * 4 + (hh * rg + lr) * G::kPitch;
 #pragma unroll
       for (int x = 0; x < kD4Waves; ++x) {
         const float f = fast_exp2(mrg_ml[mi][x][lr][0] - mu);
@@ -747,7 +782,7 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
   // A state that fits one area is left there, and the wave goes on to the next
   // piece without a barrier; the piece is added up when the next but one ends,
   // or with the last one, whose states lie in the ring.
-  const bool fits = RB == 1 && rows <= 16 / G::kPH;
+  const bool fits = RB == 1 && rows <= G::kAllRows;
   const uint32_t area0 = lds_addr_of(stage), area1 = lds_addr_of(tiles);
   constexpr uint32_t kWs0 = G::kStage, kWs1 = G::kRing * G::kTile;
   static_assert(kWs1 >= G::kStage, "a wave's state in its ring");
@@ -798,7 +833,8 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
       if (fits) {
         if (has_next && left.np) {
           __syncthreads();
-          add_up(left.b, left.np, left.us, left.mine, area0, kWs0, 0, 0, rows, 0, G::kPH);
+          add_up(left.b, left.np, left.us, left.mine, area0, kWs0, 0, 0, rows, 0, G::kPH,
+             G::kAllRows);
           __syncthreads();
           left.np = 0;
         }
@@ -808,10 +844,10 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
                               l16 * G::kPitch;
           put_state(Zero{}, Zero{}, at);
           if constexpr (G::kPH > 1)
-            put_state(Zero{}, std::integral_constant<int, 1>{}, at + 16 / G::kPH * G::kPitch);
+            put_state(Zero{}, std::integral_constant<int, 1>{}, at + G::kAllRows * G::kPitch);
           if constexpr (G::kPH > 2) {
-            put_state(Zero{}, std::integral_constant<int, 2>{}, at + 32 / G::kPH * G::kPitch);
-            put_state(Zero{}, std::integral_constant<int, 3>{}, at + 48 / G::kPH * G::kPitch);
+            put_state(Zero{}, std::integral_constant<int, 2>{}, at + 2 * G::kAllRows * G::kPitch);
+            put_state(Zero{}, std::integral_constant<int, 3>{}, at + 3 * G::kAllRows * G::kPitch);
           }
         }
         if (has_next) left = Left{cur.b, cur.np, cur.us, cur.mine};
@@ -821,18 +857,21 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
           if (16 * rb >= rows) return;
           const int n = min(rows - 16 * rb, 16);
           put_stats(rbc, 0);
-          auto phase = [&](auto h) {
-            put_state(rbc, h, area0 + wave * kWs0 + l16 * G::kPitch);
+          auto phases = [&](auto h) {  // as many as an area holds
+            constexpr int H = decltype(h)::value;
+            const uint32_t at = area0 + wave * kWs0 + l16 * G::kPitch;
+            put_state(rbc, h, at);
+            if constexpr (G::kSP > 1)
+              put_state(rbc, std::integral_constant<int, H + 1>{}, at + 16 * G::kPitch);
             __syncthreads();
-            add_up(cur.b, cur.np, cur.us, cur.mine, area0, kWs0, 0, 16 * rb, n,
-                   decltype(h)::value, 1);
+            add_up(cur.b, cur.np, cur.us, cur.mine, area0, kWs0, 0, 16 * rb, n, H, G::kSP, 16);
             __syncthreads();
           };
-          phase(Zero{});
-          if constexpr (G::kPH > 1) phase(std::integral_constant<int, 1>{});
-          if constexpr (G::kPH > 2) {
-            phase(std::integral_constant<int, 2>{});
-            phase(std::integral_constant<int, 3>{});
+          phases(Zero{});
+          if constexpr (D == 256) {
+            phases(std::integral_constant<int, 1>{});
+            phases(std::integral_constant<int, 2>{});
+            phases(std::integral_constant<int, 3>{});
           }
         };
         merge16(Zero{});
@@ -871,19 +910,25 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
 #pragma unroll 1
     while (fly < G::kRing && (ic < cur.kb || (has_next && jn < nxt.kb))) issue_next();
   }
+  // the words that count the cut units, read ahead of the count
+  uint64_t word = 0;
+  if ((tid == 0 && cut[0].np) || (tid == 64 && cut[1].np))
+    word = merge_word(a, cut[tid ? 1 : 0].b * a.walk_streams + stream);
   if (fits) {
     __syncthreads();
     if (left.np)
-      add_up(left.b, left.np, left.us, left.mine, area0, kWs0, 0, 0, rows, 0, G::kPH);
-    add_up(cur.b, cur.np, cur.us, cur.mine, area1, kWs1, 1, 0, rows, 0, G::kPH);
+      add_up(left.b, left.np, left.us, left.mine, area0, kWs0, 0, 0, rows, 0, G::kPH,
+             G::kAllRows);
+    add_up(cur.b, cur.np, cur.us, cur.mine, area1, kWs1, 1, 0, rows, 0, G::kPH, G::kAllRows);
   }
   if (cut[0].np == 0) return;
   merge_publish();
   __syncthreads();
   // one wave counts each; the last of a unit's pieces merges them
-  if (tid == 0) merge_flag[0] = merge_arrive(a, cut[0].b * a.walk_streams + stream, cut[0].np);
+  if (tid == 0)
+    merge_flag[0] = merge_arrive(a, cut[0].b * a.walk_streams + stream, cut[0].np, word);
   if (tid == 64 && cut[1].np)
-    merge_flag[1] = merge_arrive(a, cut[1].b * a.walk_streams + stream, cut[1].np);
+    merge_flag[1] = merge_arrive(a, cut[1].b * a.walk_streams + stream, cut[1].np, word);
   __syncthreads();
 #pragma unroll 1
   for (int i = 0; i < 2; ++i) {
