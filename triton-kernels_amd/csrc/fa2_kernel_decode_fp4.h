@@ -868,10 +868,10 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
             __syncthreads();
           };
           phases(Zero{});
-          if constexpr (D == 256) {
-            phases(std::integral_constant<int, 1>{});
-            phases(std::integral_constant<int, 2>{});
-            phases(std::integral_constant<int, 3>{});
+          if constexpr (G::kPH > G::kSP) phases(std::integral_constant<int, G::kSP>{});
+          if constexpr (G::kPH > 2 * G::kSP) {
+            phases(std::integral_constant<int, 2 * G::kSP>{});
+            phases(std::integral_constant<int, 3 * G::kSP>{});
           }
         };
         merge16(Zero{});
