@@ -128,7 +128,8 @@ int fp4_rows(const fa2_fp4_rows_params* p, void* stream, bool append) {
   a.num_pages = static_cast<int32_t>(p->num_pages);
   a.table_width = static_cast<int32_t>(p->table_width);
   a.has_v = has_v ? 1 : 0;
-  a.block_rows = std::min(std::max(kF4Pieces / a.words, 1), kF4Rows);
+  a.rows_at_once = std::max(kF4Threads / a.words, 1);
+  a.block_rows = 4 * a.rows_at_once;
   const dim3 grid(static_cast<uint32_t>(cdiv(p->num_rows, a.block_rows)));
   hipStream_t st = static_cast<hipStream_t>(stream);
   auto go = [&](auto dt) {
@@ -262,8 +263,8 @@ extern "C" int fa2_norm_rope(const fa2_norm_rope_params* p, void* stream) {
   const int eb = elt_bytes(p->dtype);
   const int64_t lanes = p->head_dim * eb / 32;
   // Four heads of a token per lane group (their loads in flight together, the
-  // table's row and the weights read once) where that still gives every CU work
-  // for its four SIMDs, else one.
+  // table's row and the weights read once) where that still gives every CU a
+  // wave for each of its four SIMDs, else one.
   const int64_t u = p->tokens * (cdiv(p->q_heads, 4) + cdiv(p->kv_heads, 4)) * lanes >=
                             int64_t(cu_count_current_device()) * 4 * 64
                         ? 4

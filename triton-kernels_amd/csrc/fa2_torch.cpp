@@ -306,11 +306,41 @@ at::Tensor ready(const at::Tensor& t) {
   return rows_ok(t) ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
-// qk_norm_rope after the Python wrapper's checks; (status, q, k).
+// The functions below make the checks of the Python wrappers themselves (the
+// chain of attribute reads there costs 2 to 4 us per call) and return kRefused for
+// arguments that do not pass: the wrapper then runs its own and raises.
+constexpr int64_t kRefused = -1;
+
+bool real_type(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16 || t == at::kFloat; }
+
+// T of [T, H, D], or B * M of [B, H, M, D]
+int64_t tokens_of(const at::Tensor& t) { return t.dim() == 3 ? t.size(0) : t.size(0) * t.size(2); }
+
+bool norm_rope_ok(const at::Tensor& q, const at::Tensor& k, const at::Tensor& qw,
+                  const at::Tensor& kw, const at::Tensor& rope, const at::Tensor& positions,
+                  double eps) {
+  const at::Device dev = q.device();
+  if (!q.is_cuda() || k.device() != dev || qw.device() != dev || kw.device() != dev ||
+      rope.device() != dev || positions.device() != dev)
+    return false;
+  if ((q.dim() != 3 && q.dim() != 4) || (k.dim() != 3 && k.dim() != 4)) return false;
+  const auto dt = q.scalar_type();
+  const int64_t D = q.size(-1);
+  return real_type(dt) && k.scalar_type() == dt && k.size(-1) == D &&
+         tokens_of(k) == tokens_of(q) && qw.dim() == 1 && kw.dim() == 1 && qw.size(0) == D &&
+         kw.size(0) == D && qw.scalar_type() == kw.scalar_type() &&
+         (qw.scalar_type() == dt || qw.scalar_type() == at::kFloat) &&
+         (positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong) &&
+         positions.numel() == tokens_of(q) && rope.scalar_type() == at::kFloat &&
+         rope.dim() == 2 && rope.size(1) <= D && rope.size(1) % 16 == 0 && eps >= 0;
+}
+
+// qk_norm_rope; (status, q, k).
 std::tuple<int64_t, at::Tensor, at::Tensor> norm_rope(at::Tensor q, at::Tensor k, at::Tensor qw,
                                                       at::Tensor kw, at::Tensor rope,
                                                       at::Tensor positions, double eps,
                                                       bool interleaved) {
+  if (!norm_rope_ok(q, k, qw, kw, rope, positions, eps)) return {kRefused, q, k};
   const at::Device dev = q.device();
   const c10::DeviceGuard guard(dev);
   q = ready(q);
@@ -353,13 +383,45 @@ std::tuple<int64_t, at::Tensor, at::Tensor> norm_rope(at::Tensor q, at::Tensor k
   return {fa2_norm_rope(&p, st), qo, ko};
 }
 
-// paged_kv_append_fp4 and paged_kv_gather_fp4 after the Python wrappers' checks;
-// the status.
-int64_t fp4_rows(bool append, const at::Tensor& kc, const at::Tensor& ks,
-                 const c10::optional<at::Tensor>& vc, const c10::optional<at::Tensor>& vs,
-                 const at::Tensor& k_table, const c10::optional<at::Tensor>& v_table, at::Tensor k,
-                 c10::optional<at::Tensor> v, const at::Tensor& indptr,
-                 const c10::optional<at::Tensor>& start_pos) {
+using OptTensor = c10::optional<at::Tensor>;
+
+// A cache's codes and scales (fp4_cache.check_cache)
+bool cache_ok(const at::Tensor& c, const at::Tensor& s, const at::Device& dev) {
+  if (c.device() != dev || s.device() != dev || c.scalar_type() != at::kByte ||
+      s.scalar_type() != at::kByte || c.dim() != 4 || s.dim() != 4 || !c.is_contiguous() ||
+      !s.is_contiguous() || c.numel() == 0)
+    return false;
+  const int64_t D = c.size(3) * 2;
+  return (D == 64 || D == 128 || D == 256) && s.size(0) == c.size(0) && s.size(1) == c.size(1) &&
+         s.size(2) == c.size(2) && s.size(3) == D / 32;
+}
+
+// The arguments that the writer and the reader share; k and v: the rows.
+bool rows_args_ok(const at::Tensor& kc, const at::Tensor& ks, const OptTensor& vc,
+                  const OptTensor& vs, const at::Tensor& k_table, const OptTensor& v_table,
+                  const at::Tensor& k, const OptTensor& v, const at::Tensor& indptr,
+                  const OptTensor& start_pos) {
+  const at::Device dev = kc.device();
+  if (!kc.is_cuda() || !cache_ok(kc, ks, dev) || k_table.device() != dev ||
+      indptr.device() != dev || k.device() != dev)
+    return false;
+  const int64_t B = indptr.numel() - 1;
+  if (B < 0 || k_table.dim() != 2 || k_table.size(0) < B ||
+      (start_pos && start_pos->numel() < B) || !real_type(k.scalar_type()) || k.dim() != 3 ||
+      k.size(1) != kc.size(1) || k.size(2) != kc.size(3) * 2)
+    return false;
+  if (vc.has_value() != v.has_value() || vc.has_value() != vs.has_value() ||
+      vc.has_value() != v_table.has_value())
+    return false;
+  return !vc || (cache_ok(*vc, *vs, dev) && vc->sizes() == kc.sizes() &&
+                 v_table->dim() == 2 && v_table->size(0) >= B && v->device() == dev &&
+                 v->scalar_type() == k.scalar_type() && v->sizes() == k.sizes());
+}
+
+int64_t fp4_rows(bool append, const at::Tensor& kc, const at::Tensor& ks, const OptTensor& vc,
+                 const OptTensor& vs, const at::Tensor& k_table, const OptTensor& v_table,
+                 at::Tensor k, OptTensor v, const at::Tensor& indptr, const OptTensor& start_pos) {
+  if (!rows_args_ok(kc, ks, vc, vs, k_table, v_table, k, v, indptr, start_pos)) return kRefused;
   const at::Device dev = kc.device();
   const c10::DeviceGuard guard(dev);
   if (append) {  // (the gathered tensors are contiguous and aligned)
@@ -406,14 +468,53 @@ int64_t fp4_rows(bool append, const at::Tensor& kc, const at::Tensor& ks,
   return append ? fa2_fp4_append(&p, st) : fa2_fp4_gather(&p, st);
 }
 
+// paged_kv_append_fp4: writes the rows; the status.
+int64_t fp4_append(const at::Tensor& kc, const at::Tensor& ks, const OptTensor& vc,
+                   const OptTensor& vs, const at::Tensor& k_table, const OptTensor& v_table,
+                   const at::Tensor& k, const OptTensor& v, const at::Tensor& indptr,
+                   const OptTensor& start_pos) {
+  return fp4_rows(true, kc, ks, vc, vs, k_table, v_table, k, v, indptr, start_pos);
+}
+
+// paged_kv_gather_fp4 into new tensors of type `like`'s; (status, k, v).
+std::tuple<int64_t, at::Tensor, OptTensor> fp4_gather(
+    const at::Tensor& kc, const at::Tensor& ks, const OptTensor& vc, const OptTensor& vs,
+    const at::Tensor& k_table, const OptTensor& v_table, int64_t num_rows, at::ScalarType dtype,
+    const at::Tensor& indptr, const OptTensor& start_pos) {
+  if (num_rows < 0 || kc.dim() != 4 || !real_type(dtype)) return {kRefused, kc, vc};
+  const auto opts = kc.options().dtype(dtype);
+  const int64_t H = kc.size(1), D = kc.size(3) * 2;
+  at::Tensor k = at::empty({num_rows, H, D}, opts);
+  OptTensor v;
+  if (vc) v = at::empty({num_rows, H, D}, opts);
+  return {fp4_rows(false, kc, ks, vc, vs, k_table, v_table, k, v, indptr, start_pos), k, v};
+}
+
+// ... into given ones; the status.
+int64_t fp4_gather_into(const at::Tensor& kc, const at::Tensor& ks, const OptTensor& vc,
+                        const OptTensor& vs, const at::Tensor& k_table, const OptTensor& v_table,
+                        const at::Tensor& k, const OptTensor& v, const at::Tensor& indptr,
+                        const OptTensor& start_pos) {
+  return fp4_rows(false, kc, ks, vc, vs, k_table, v_table, k, v, indptr, start_pos);
+}
+
 // decode_attention_fp4 (q [B,QH,D]) and speculative_decode_attention_fp4 (q
-// [B,QH,M,D]) after the Python wrappers' checks; (status, output).
+// [B,QH,M,D]): `dims` is q's; (status, output).
 std::tuple<int64_t, at::Tensor> fp4_decode(const at::Tensor& q, const at::Tensor& kc,
                                            const at::Tensor& ks, const at::Tensor& vc,
                                            const at::Tensor& vs, const at::Tensor& lens,
                                            const at::Tensor& k_table, const at::Tensor& v_table,
-                                           bool causal) {
+                                           bool causal, int64_t dims) {
   const at::Device dev = q.device();
+  const auto dt = q.scalar_type();
+  if (!q.is_cuda() || q.dim() != dims || (dims == 4 && q.size(2) > 16) || kc.dim() != 4 ||
+      (dt != at::kHalf && dt != at::kBFloat16) || !cache_ok(kc, ks, dev) ||
+      !cache_ok(vc, vs, dev) || vc.sizes() != kc.sizes() || q.size(-1) != kc.size(3) * 2 ||
+      q.size(1) == 0 || q.size(1) % kc.size(1) != 0 || lens.device() != dev ||
+      k_table.device() != dev || v_table.device() != dev || lens.numel() < q.size(0) ||
+      k_table.dim() != 2 || v_table.dim() != 2 || k_table.size(0) < q.size(0) ||
+      v_table.size(0) < q.size(0))
+    return {kRefused, q};
   const c10::DeviceGuard guard(dev);
   at::Tensor out = at::empty(q.sizes(), q.options());
   const bool squeeze = q.dim() == 3;
@@ -474,9 +575,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fwd", &fwd, "enqueue fa2_fwd for checked tensors; returns the output");
   m.def("decode", &decode, "enqueue fa2_decode_fwd for checked tensors; the output, or None");
   m.def("append", &append, "enqueue fa2_kv_append for checked tensors; the fa2 status");
-  m.def("norm_rope", &norm_rope, "enqueue fa2_norm_rope for checked tensors; (fa2 status, q, k)");
-  m.def("fp4_rows", &fp4_rows,
-        "enqueue fa2_fp4_append or fa2_fp4_gather for checked tensors; the fa2 status");
+  m.def("norm_rope", &norm_rope, "enqueue fa2_norm_rope; (fa2 status, -1: bad arguments, q, k)");
+  m.def("fp4_append", &fp4_append, "enqueue fa2_fp4_append; the fa2 status, -1: bad arguments");
+  m.def("fp4_gather", &fp4_gather, "enqueue fa2_fp4_gather; (fa2 status or -1, k, v)");
+  m.def("fp4_gather_into", &fp4_gather_into, "enqueue fa2_fp4_gather; the fa2 status or -1");
   m.def("fp4_decode", &fp4_decode,
-        "enqueue fa2_fp4_decode for checked tensors; (fa2 status, output)");
+        "enqueue fa2_fp4_decode; (fa2 status or -1, output)");
 }

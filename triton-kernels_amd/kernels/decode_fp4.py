@@ -41,10 +41,8 @@ def decode_attention_fp4(
     v_block_table: torch.Tensor,
 ) -> torch.Tensor:
     """See the module docstring."""
-    if q.dim() != 3:
-        raise ValueError("decode_attention_fp4: q must be [B, QH, D]")
     return _decode("decode_attention_fp4", q, k_cache, v_cache, kv_indptr, k_block_table,
-                   v_block_table, False)
+                   v_block_table, False, 3)
 
 
 def speculative_decode_attention_fp4(
@@ -58,14 +56,23 @@ def speculative_decode_attention_fp4(
     v_block_table: torch.Tensor,
 ) -> torch.Tensor:
     """See the module docstring."""
-    if q.dim() != 4:
-        raise ValueError("speculative_decode_attention_fp4: q must be [B, QH, M, D]")
-    assert q.shape[2] <= 16, "Speculative decode is intended for small draft lengths (M <= 16)."
     return _decode("speculative_decode_attention_fp4", q, k_cache, v_cache, kv_indptr,
-                   k_block_table, v_block_table, bool(causal))
+                   k_block_table, v_block_table, bool(causal), 4)
 
 
-def _decode(name, q, k_cache, v_cache, lens, k_table, v_table, causal):
+def _decode(name, q, k_cache, v_cache, lens, k_table, v_table, causal, dims):
+    x = ext() if USE_EXT else None
+    if x is not None and v_cache is not None:
+        rc, out = x.fp4_decode(q, *k_cache, *v_cache, lens, k_table, v_table, causal, dims)
+        if rc == 0:
+            return out
+        if rc > 0:
+            raise _ops.OpsError(name, rc)
+    # (the extension makes these checks itself and leaves the errors to them)
+    if q.dim() != dims:
+        raise ValueError(f"{name}: q must be {'[B, QH, D]' if dims == 3 else '[B, QH, M, D]'}")
+    if dims == 4:
+        assert q.shape[2] <= 16, "Speculative decode is intended for small draft lengths (M <= 16)."
     if v_cache is None:
         raise ValueError(f"{name}: v_cache is missing")
     kc, ks, vc, vs = check_cache(name, k_cache, v_cache)
@@ -79,13 +86,9 @@ def _decode(name, q, k_cache, v_cache, lens, k_table, v_table, causal):
         raise ValueError(f"{name}: q's head_dim {D} is not the cache's ({kc.shape[3] * 2})")
     if QH == 0 or QH % KVH != 0:
         raise ValueError(f"{name}: q_heads ({QH}) must be a multiple of kv_heads ({KVH})")
-    if lens.numel() < B or k_table.shape[0] < B or v_table.shape[0] < B:
+    if (lens.numel() < B or k_table.dim() != 2 or v_table.dim() != 2 or k_table.shape[0] < B
+            or v_table.shape[0] < B):
         raise ValueError(f"{name}: kv_indptr and the block tables need {B} rows")
-    x = ext() if USE_EXT else None
-    if x is not None:
-        rc, out = x.fp4_decode(q, kc, ks, vc, vs, lens, k_table, v_table, causal)
-        _ops.check(name, rc)
-        return out
     return _run(name, q, kc, ks, vc, vs, lens, k_table, v_table, causal)
 
 

@@ -95,7 +95,8 @@ def _check_rows(name, kc, vc, k_table, v_table, indptr, start_pos):
     if (v_table is None) == has_v:
         raise ValueError(f"{name}: pass the V arguments together")
     B = indptr.numel() - 1
-    if B < 0 or k_table.shape[0] < B or (has_v and v_table.shape[0] < B):
+    if B < 0 or k_table.dim() != 2 or k_table.shape[0] < B or (
+            has_v and (v_table.dim() != 2 or v_table.shape[0] < B)):
         raise ValueError(f"{name}: the block tables need one row per sequence")
     if start_pos is not None and start_pos.numel() < B:
         raise ValueError(f"{name}: start_pos needs one entry per sequence")
@@ -123,6 +124,15 @@ def paged_kv_append_fp4(
     the cache, are not written; no two rows of a call may share a place.
     """
     name = "paged_kv_append_fp4"
+    x = ext() if USE_EXT else None
+    if x is not None:
+        rc = x.fp4_append(*k_cache, *(v_cache if v_cache is not None else (None, None)),
+                          k_block_table, v_block_table, k_new, v_new, new_indptr, start_pos)
+        if rc == 0:
+            return
+        if rc > 0:
+            raise _ops.OpsError(name, rc)
+    # (the extension makes these checks itself and leaves the errors to them)
     kc, ks, vc, vs = check_cache(name, k_cache, v_cache)
     if (v_new is None) != (vc is None):
         raise ValueError(f"{name}: pass the V arguments together")
@@ -136,11 +146,6 @@ def paged_kv_append_fp4(
         raise ValueError(f"{name}: new rows must be [T, {H}, {D}]")
     if v_new is not None and (v_new.shape != k_new.shape or v_new.dtype != k_new.dtype):
         raise ValueError(f"{name}: k_new and v_new must have equal shapes and dtypes")
-    x = ext() if USE_EXT else None
-    if x is not None:
-        _ops.check(name, x.fp4_rows(True, kc, ks, vc, vs, k_block_table, v_block_table, k_new,
-                                    v_new, new_indptr, start_pos))
-        return
     k_new = aligned(k_new)
     v_new = aligned(v_new) if v_new is not None else None
     _rows(name, "fa2_fp4_append", kc, ks, vc, vs, k_block_table, v_block_table, k_new, v_new,
@@ -171,6 +176,15 @@ def paged_kv_gather_fp4(
     and ``v_block_table`` may both be ``None``: then v is ``None``.
     """
     name = "paged_kv_gather_fp4"
+    x = ext() if USE_EXT else None
+    if x is not None and out is None:
+        rc, k, v = x.fp4_gather(*k_cache, *(v_cache if v_cache is not None else (None, None)),
+                                k_block_table, v_block_table, num_rows, dtype, indptr, start_pos)
+        if rc == 0:
+            return k, v
+        if rc > 0:
+            raise _ops.OpsError(name, rc)
+    # (the extension makes these checks itself and leaves the errors to them)
     kc, ks, vc, vs = check_cache(name, k_cache, v_cache)
     B = _check_rows(name, kc, vc, k_block_table, v_block_table, indptr, start_pos)
     shape = (int(num_rows), kc.shape[1], kc.shape[3] * 2)
@@ -191,10 +205,9 @@ def paged_kv_gather_fp4(
                 raise TypeError(f"{name}: out must be float16, bfloat16 or float32, k and v alike")
             if t.shape != shape or not t.is_contiguous() or t.data_ptr() % 16:
                 raise ValueError(f"{name}: out must be contiguous {list(shape)} tensors")
-    x = ext() if USE_EXT else None
     if x is not None:
-        _ops.check(name, x.fp4_rows(False, kc, ks, vc, vs, k_block_table, v_block_table, k, v,
-                                    indptr, start_pos))
+        _ops.check(name, x.fp4_gather_into(kc, ks, vc, vs, k_block_table, v_block_table, k, v,
+                                           indptr, start_pos))
     else:
         _rows(name, "fa2_fp4_gather", kc, ks, vc, vs, k_block_table, v_block_table, k, v, indptr,
               start_pos, B)

@@ -66,6 +66,15 @@ def qk_norm_rope(
     ``positions``: T integers (int32 or int64, any shape), a token's row of the
     table; a token whose position is outside ``[0, P)`` becomes NaN.
     """
+    x = ext() if USE_EXT else None
+    if x is not None:
+        rc, q_out, k_out = x.norm_rope(q, k, q_weight, k_weight, rope_table, positions, eps,
+                                       interleaved)
+        if rc == 0:
+            return q_out, k_out
+        if rc > 0:
+            raise _ops.OpsError(_NAME, rc)
+    # (the extension makes these checks itself and leaves the errors to them)
     assert q.dtype == k.dtype, "Tensors must have the same dtype"
     assert (q.device == k.device == q_weight.device == k_weight.device == rope_table.device
             == positions.device), "Tensors must be on the same device"
@@ -93,13 +102,6 @@ def qk_norm_rope(
         raise ValueError(f"{_NAME}: rotary_dim {R} must be a multiple of 16, at most {D}")
     if not eps >= 0:
         raise ValueError(f"{_NAME}: eps must not be negative")
-    x = ext() if USE_EXT else None
-    if x is not None:
-        rc, q_out, k_out = x.norm_rope(q, k, q_weight, k_weight, rope_table, positions, float(eps),
-                                       bool(interleaved))
-        _ops.check(_NAME, rc)
-        return q_out, k_out
-
     q, k = aligned(q), aligned(k)
     q_weight, k_weight, rope_table = (
         t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(
