@@ -173,6 +173,12 @@ struct Fp4Geo {
   }
 };
 
+// The value of lane l ^ 8 (a rotation by 8 within each 16 lanes).
+__device__ __forceinline__ float half_swap(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x128,
+                                                               0xF, 0xF, true));
+}
+
 // Sum (or maximum, of numbers >= 0) over the lanes up to each, on the VALU.
 template <bool MAX>
 __device__ __forceinline__ int wave_scan(int x) {
@@ -186,7 +192,11 @@ __device__ __forceinline__ int wave_scan(int x) {
   return x;
 }
 
-template <int DT, int D, int RB>
+// HALF: up to 8 rows, which take the 16 columns twice: columns 0-7 go with the first
+// 16 keys of a tile and 8-15 with the others, so a lane has 4 scores per tile
+// instead of 8, half of them of no row.  The halves are states of their own, joined
+// at a piece's end.
+template <int DT, int D, int RB, bool HALF>
 __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_decode_fp4_kernel(
     Fp4Args fa) {
   using G = Fp4Geo<D, RB>;
@@ -196,6 +206,8 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
   constexpr int kStep = kD4Tile * kD4Waves;
   constexpr int kSub = D == 256 ? 2 : 1;  // scales of a lane's dims
   static_assert(kD4Waves * G::kStage >= kMergePieceBytes<kD4Threads>, "merge area");
+  static_assert(!HALF || RB == 1, "HALF");
+  constexpr int NX = HALF ? 1 : 2;  // 16-key blocks that a lane's scores are from
 
   __shared__ __attribute__((aligned(1024))) char tiles[kD4Waves * G::kRing * G::kTile];
   __shared__ __attribute__((aligned(128))) char stage[kD4Waves * G::kStage];
@@ -210,6 +222,8 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15;
   const int g = lane >> 4;
+  const int lrow = HALF ? l16 & 7 : l16;  // this lane's row (of each 16)
+  const bool second = HALF && l16 >= 8;
   const bool causal = a.mask != FA2_MASK_NONE;
   const int stream = static_cast<int>(blockIdx.x) % a.walk_streams;
   const int seg_k = static_cast<int>(blockIdx.x) / a.walk_streams;
@@ -473,7 +487,7 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
     const int64_t base = v.b * a.q_sb + head0 * a.q_sh + q0 * a.q_ss;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      const int r = 16 * rb + l16;
+      const int r = 16 * rb + lrow;
 #pragma unroll
       for (int j = 0; j < DJ; ++j) {
         x[rb][j] = (u32x4){0u, 0u, 0u, 0u};
@@ -623,16 +637,22 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
     u32x4 ph[RB], pl[RB];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
+      if constexpr (HALF) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[rb][0][r] = second ? s[rb][1][r] : s[rb][0][r];
+      }
       if (edge) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+        for (int x = 0; x < NX; ++x)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            s[rb][x][r] = n0 + 16 * x + 4 * g + r <= last[rb] ? s[rb][x][r] : -INFINITY;
+          for (int r = 0; r < 4; ++r) {
+            const int key = n0 + (HALF ? (second ? 16 : 0) : 16 * x) + 4 * g + r;
+            s[rb][x][r] = key <= last[rb] ? s[rb][x][r] : -INFINITY;
+          }
       }
       float mx = -INFINITY;
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
+      for (int x = 0; x < NX; ++x)
 #pragma unroll
         for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[rb][x][r]);
       if (__any((mx - m[rb]) * a.scale_log2 > kRescaleThreshold)) {
@@ -647,18 +667,29 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
       }
       // (the difference is taken before the scale: no score is too large for it)
       const float mu = m[rb] == -INFINITY ? 0.f : m[rb];
-      float e[8];
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        e[r] = fast_exp2((s[rb][r >> 2][r & 3] - mu) * a.scale_log2);
-        l[rb] += e[r];
-      }
+      for (int x = 0; x < NX; ++x) {
+        float e[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const uint32_t hw = pack2<BF>(e[2 * r], e[2 * r + 1]);
-        const f32x2 h = unpack2<BF>(hw);
-        ph[rb][r] = hw;
-        pl[rb][r] = pack2<BF>(e[2 * r] - h[0], e[2 * r + 1] - h[1]);
+        for (int r = 0; r < 4; ++r) {
+          e[r] = fast_exp2((s[rb][x][r] - mu) * a.scale_log2);
+          l[rb] += e[r];
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint32_t hw = pack2<BF>(e[2 * r], e[2 * r + 1]);
+          const f32x2 h = unpack2<BF>(hw);
+          const uint32_t lw = pack2<BF>(e[2 * r] - h[0], e[2 * r + 1] - h[1]);
+          if constexpr (HALF) {  // the other block's keys: zero
+            ph[rb][r] = second ? 0u : hw;
+            pl[rb][r] = second ? 0u : lw;
+            ph[rb][2 + r] = second ? hw : 0u;
+            pl[rb][2 + r] = second ? lw : 0u;
+          } else {
+            ph[rb][2 * x + r] = hw;
+            pl[rb][2 * x + r] = lw;
+          }
+        }
       }
     }
     // O^T: dims 2 t and 2 t + 1 of each lane's, 8 keys each
@@ -732,6 +763,21 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
     }
     l[rb] += __shfl_xor(l[rb], 16);
     l[rb] += __shfl_xor(l[rb], 32);
+    if constexpr (HALF) {  // both halves get their sum
+      const float mo = half_swap(m[rb]);
+      const float mn = fmaxf(m[rb], mo);
+      const float f = fast_exp2((m[rb] - (mn == -INFINITY ? 0.f : mn)) * a.scale_log2);
+      m[rb] = mn;
+      const float lf = l[rb] * f;
+      l[rb] = lf + half_swap(lf);
+#pragma unroll
+      for (int i = 0; i < G::kNI; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float y = o[rb][i][r] * f;
+          o[rb][i][r] = y + half_swap(y);
+        }
+    }
     if (g == 0) {
       mrg_ml[mi][wave][l16][0] = m[rb] * a.scale_log2;  // (-inf stays -inf)
       mrg_ml[mi][wave][l16][1] = l[rb];
@@ -810,7 +856,7 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
     int last[RB];  // last visible key of this lane's rows
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb)
-      last[rb] = causal ? min(cur.kb - 1, off + diag_row(a, q0 + 16 * rb + l16)) : cur.kb - 1;
+      last[rb] = causal ? min(cur.kb - 1, off + diag_row(a, q0 + 16 * rb + lrow)) : cur.kb - 1;
     const int full = causal ? min(cur.kb, off + 1) : cur.kb;
     for (int n0 = cur.ka + turn * kD4Tile; n0 < cur.kb; n0 += kStep) {
       // The two waves of a SIMD (i and i + 4) take turns in going first: left to

@@ -221,11 +221,17 @@ bool fp4_empty(const fa2_fp4_decode_params* p) { return p->batch == 0 || p->q_le
 
 template <int DT, int D>
 void launch_fp4_decode(const Fp4Args& a, int rb, uint32_t grid, hipStream_t st) {
-  if (rb == 1)
-    hipLaunchKernelGGL((fa2_decode_fp4_kernel<DT, D, 1>), dim3(grid), dim3(kD4Threads), 0, st, a);
+  // (up to 8 rows take the 16 columns twice)
+  if (rb == 1 && a.a.q_len <= 8)
+    hipLaunchKernelGGL((fa2_decode_fp4_kernel<DT, D, 1, true>), dim3(grid), dim3(kD4Threads), 0,
+                       st, a);
+  else if (rb == 1)
+    hipLaunchKernelGGL((fa2_decode_fp4_kernel<DT, D, 1, false>), dim3(grid), dim3(kD4Threads), 0,
+                       st, a);
   if constexpr (D <= 128)
     if (rb == 2)
-      hipLaunchKernelGGL((fa2_decode_fp4_kernel<DT, D, 2>), dim3(grid), dim3(kD4Threads), 0, st, a);
+      hipLaunchKernelGGL((fa2_decode_fp4_kernel<DT, D, 2, false>), dim3(grid), dim3(kD4Threads), 0,
+                         st, a);
 }
 
 template <int DT>
