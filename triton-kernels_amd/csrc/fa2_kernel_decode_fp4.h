@@ -11,11 +11,14 @@
 //     tiles (fa2_decode_walk.h).  A wave walks tiles of 32 keys, tile i of
 //     the workgroup's range to wave i % 8, and keeps its own (m, l, O).
 //   * A page's rows of a kv head are contiguous.  Direct-to-LDS loads of whole
-//     rows fill a ring of kRing tiles per wave, across the ends of the pieces; a
-//     tile's codes are read into registers at once (they are few) and its slot
-//     filled again, so the whole ring is in flight nearly all the time, from one
-//     copy of the loop.  (Tiles in flight in registers instead need the loop once
-//     per tile in flight: 50 KB of code, whose first execution alone took 6 us.)
+//     rows bring a tile per wave, across the ends of the pieces; its codes are
+//     read into registers at once (they are few) and the next tile is on its way
+//     while it is computed.  (Tiles in flight in registers instead need the loop
+//     once per tile: 50 KB of code.  More tiles in flight in LDS gain nothing: the
+//     first burst takes the longer, D128 49.3 / 47.1 / 46.4 us at 3 / 2 / 1 for 16 x
+//     16000-32768 keys, and each wait has to count them.)
+//   * What bounds the loop is its instructions: with all keys in one page, in L2, the
+//     calls take 10 % less.  So the tile loop has next to no branches in its way.
 //   * S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32, up to 16 RB rows
 //     of the unit as columns.  A lane expands D / 4 dims of a key of K, in the
 //     layout of the MFMA's A operand (lane: row l % 16, dims D / 4 * (l / 16)
@@ -56,6 +59,7 @@ struct Fp4Args {
   int32_t num_pages, table_width;
   uint32_t page_codes, page_scales;  // bytes of a page, and of its rows of one head
   uint32_t head_codes, head_scales;
+  uint32_t page_mul, page_sh;  // n / page_size = (2 n * page_mul) >> 32 >> page_sh
 };
 
 template <bool BF>
@@ -133,10 +137,9 @@ __device__ __forceinline__ void fp4_dma2(const void* p, uint32_t lds) {  // into
                : "v"(p), "{m0}"(__builtin_amdgcn_readfirstlane(static_cast<int>(lds))));
 }
 
-// Geometry at head dim D with 16 RB rows.
-template <int D, int RB>
+// Geometry at head dim D.
+template <int D>
 struct Fp4Geo {
-  static constexpr int kPerCu = 1;  // workgroups per CU
   static constexpr int kRow = D / 2;                  // bytes of a row of codes
   static constexpr int kNC = kRow / 16;               // its 16-byte chunks
   static constexpr int kCode = kD4Tile * kRow;        // a tile's codes of K (or V)
@@ -145,19 +148,14 @@ struct Fp4Geo {
   static constexpr int kScaleRow = D == 256 ? 8 : 4;
   static constexpr int kScaleLoads = D == 256 ? 2 : 1;  // (K and V in one up to 128)
   static constexpr int kTile = 2 * kCode + 2 * kScale;
-  static constexpr int kInFlight = 2 * kLoads + kScaleLoads;  // loads of a tile
   static constexpr int kNI = D / 16;                  // dims of V of a lane, blocks of O^T
   static constexpr int kPD = 64;                      // dims merged at a time
   static constexpr int kPH = D / kPD;                 // phases
   static constexpr int kRP = 16 / kNI;                // accumulator rows of a lane per phase
   static constexpr int kPitch = (kPD + 4) * 4;        // merge rows
-  static constexpr int kSP = D == 128 ? 2 : 1;        // phases of 16 rows that a wave's area holds
-  static constexpr int kStage = 16 * kSP * kPitch;
-  static constexpr int kAllRows = 16 * kSP / kPH;     // rows of which it holds all phases
+  static constexpr int kStage = 16 * kPitch;          // a wave's merge area: a phase of 16 rows
+  static constexpr int kAllRows = 16 / kPH;           // ... or all phases of so many
   static constexpr int kTable = 256;                  // block-table entries of a window
-  // Two tiles in flight per wave are enough: D64, 16 x 8200 keys, 8 drafts 35.1 / 34.2 / 33.6
-  // us at 5 / 3 / 2; D128, 16 x 16000-32768 keys 49.3 / 47.1 / 46.4 at 3 / 2 / 1.
-  static constexpr int kRing = D == 256 ? 1 : 2;
   // chunk c of row r lies at chunk c ^ ksw(r): 8 lanes reading a chunk of 8 rows
   // hit distinct banks
   static __device__ __forceinline__ int ksw(int r) {
@@ -196,10 +194,10 @@ __device__ __forceinline__ int wave_scan(int x) {
 // 16 keys of a tile and 8-15 with the others, so a lane has 4 scores per tile
 // instead of 8, half of them of no row.  The halves are states of their own, joined
 // at a piece's end.
-template <int DT, int D, int RB, bool HALF>
-__global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_decode_fp4_kernel(
+template <int DT, int D, int RB, bool HALF, bool BLOCKS>
+__global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
     Fp4Args fa) {
-  using G = Fp4Geo<D, RB>;
+  using G = Fp4Geo<D>;
   constexpr bool BF = Elt<DT>::kBF;
   constexpr int MODE = kModePagedCapped;
   constexpr int DJ = D / 32;        // S k-steps = code words of a lane
@@ -209,10 +207,10 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
   static_assert(!HALF || RB == 1, "HALF");
   constexpr int NX = HALF ? 1 : 2;  // 16-key blocks that a lane's scores are from
 
-  __shared__ __attribute__((aligned(1024))) char tiles[kD4Waves * G::kRing * G::kTile];
-  __shared__ __attribute__((aligned(128))) char stage[kD4Waves * G::kStage];
+  __shared__ __attribute__((aligned(1024))) char tiles[kD4Waves * G::kTile];
+  __shared__ __attribute__((aligned(128))) char stage[2 * kD4Waves * G::kStage];
   __shared__ float mrg_ml[2][kD4Waves][16][2];
-  __shared__ int tab[2][2][G::kTable];
+  __shared__ int tab[3][2][G::kTable];
   __shared__ DecSegment seg_sh[kD4Waves];
   __shared__ int merge_flag[2];
 
@@ -297,7 +295,10 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
     }
     return true;
   };
-  auto page_of = [&](int n) { return a.page_shift >= 0 ? n >> a.page_shift : n / a.page_size; };
+  // n / page_size for n < 2^30 (fa2_fp4_decode)
+  auto page_of = [&](int n) {
+    return static_cast<int>(__umulhi(2u * static_cast<uint32_t>(n), fa.page_mul) >> fa.page_sh);
+  };
   auto window_at = [&](Window& v, int ka) {
     v.ka = ka;
     v.kb = v.kend;
@@ -338,32 +339,25 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
   Window cur, nxt;
   if (!first_window(cur, sg.j, sg.us)) return;
   bool has_next = next_window(cur, nxt);
+  // Block-table entries are in LDS for this window (tab[buf]) and the next one, and on
+  // their way for the one after.
+  Window nn;
+  bool has_nn = has_next && next_window(nxt, nn);
   const int entry0 = fetch_entry(cur);
   const int entry1 = has_next ? fetch_entry(nxt) : 0;
+  int entry = has_nn ? fetch_entry(nn) : 0;
   int buf = 0;
+  auto buf_after = [&](int n) { return buf + n >= 3 ? buf + n - 3 : buf + n; };
 
   // ---- loads ---------------------------------------------------------------
   const uint8_t* kc = static_cast<const uint8_t*>(a.k);
   const uint8_t* vc = static_cast<const uint8_t*>(a.v);
   const uint32_t hc = kvh * fa.head_codes, hs = kvh * fa.head_scales;
-  const uint32_t ring = lds_addr_of(tiles) + wave * (G::kRing * G::kTile);
-  int wp = 0;   // ring bytes at which the next tile goes in
-  int rp = 0;   // ... and the oldest one lies
-  int fly = 0;  // tiles issued and not yet read
-  auto advance = [&]() {
-    wp = wp + G::kTile == G::kRing * G::kTile ? 0 : wp + G::kTile;
-    ++fly;
-  };
+  const uint32_t src = lds_addr_of(tiles) + wave * G::kTile;  // this wave's tile
   // Page and row in it of key nk of a window.
   auto place = [&](int nk, int page0, int tb, int which, uint32_t& off) {
-    int lp;
-    if (a.page_shift >= 0) {
-      lp = nk >> a.page_shift;
-      off = nk & (a.page_size - 1);
-    } else {
-      lp = nk / a.page_size;
-      off = nk - lp * a.page_size;
-    }
+    const int lp = page_of(nk);
+    off = nk - lp * a.page_size;
     return static_cast<uint32_t>(tab[tb][which][lp - page0]);
   };
   auto codes_at = [&](int v, uint32_t pg, uint32_t off) {
@@ -383,7 +377,6 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
   // 128.  issue_rows: any page size, an address per lane and load; keys past the
   // window are its last one (their weights are zero).
   auto issue_rows = [&](int kb, int page0, int tb, int n) {
-    const uint32_t dst = ring + wp;
     uint32_t off;
 #pragma unroll
     for (int v = 0; v < 2; ++v)
@@ -392,7 +385,7 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
         const int r = (i * 64 + lane) / G::kNC;
         const uint32_t pg = place(min(n + (v ? G::vkey(r) : r), kb - 1), page0, tb, v, off);
         const int c = (lane % G::kNC) ^ (v ? 0 : G::ksw(r));
-        fp4_dma16(codes_at(v, pg, off * G::kRow + c * 16), dst + v * G::kCode + i * 1024);
+        fp4_dma16(codes_at(v, pg, off * G::kRow + c * 16), src + v * G::kCode + i * 1024);
       }
 #pragma unroll
     for (int i = 0; i < G::kScaleLoads; ++i) {
@@ -400,9 +393,8 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
       const int r = D == 256 ? lane >> 1 : lane & 31;
       const uint32_t pg = place(min(n + r, kb - 1), page0, tb, v, off);
       load_scales(scales_at(v, pg, off * (D / 32) + (D == 256 ? 4 * (lane & 1) : 0)),
-                  dst + 2 * G::kCode + i * 256);
+                  src + 2 * G::kCode + i * 256);
     }
-    advance();
   };
   // issue_blocks: page_size a multiple of 16.  The 16 keys of a block are one run
   // of memory: 16 lanes look up a block each (K's two, V's two), and a load takes
@@ -420,7 +412,6 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
     run_v[i] = run(1, i);
   }
   auto issue_blocks = [&](int kb, int page0, int tb, int n) {
-    const uint32_t dst = ring + wp;
     const int top = (kb - 1) & ~15;  // (a window starts at a multiple of 32)
     uint32_t off;
     const uint32_t pg = place(min(n + 16 * (g & 1), top), page0, tb, g >> 1, off);
@@ -430,7 +421,7 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
         uint32_t o2;
         const uint32_t p2 = place(min(n + 16 * (lane >> 5), top), page0, tb, v, o2);
         fp4_dma16(codes_at(v, p2, (o2 - 16 * (lane >> 5)) * G::kRow + (v ? run_v[0] : run_k[0])),
-                  dst + v * G::kCode);
+                  src + v * G::kCode);
       }
     } else {
       const uint64_t at = reinterpret_cast<uint64_t>(codes_at(g >> 1, pg, off * G::kRow));
@@ -444,7 +435,7 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
 #pragma unroll
         for (int i = 0; i < G::kLoads / 2; ++i)
           fp4_dma16_base(base, b < 2 ? run_k[i] : run_v[i],
-                         dst + b * (G::kCode / 2) + i * 1024);
+                         src + b * (G::kCode / 2) + i * 1024);
       }
     }
     if constexpr (D == 256) {
@@ -453,28 +444,28 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
         const int x = lane >> 5;
         const uint32_t p2 = place(min(n + 16 * x, top), page0, tb, v, off);
         load_scales(scales_at(v, p2, off * (D / 32) + 4 * (lane & 31)),
-                    dst + 2 * G::kCode + v * 256);
+                    src + 2 * G::kCode + v * 256);
       }
     } else {
-      load_scales(scales_at(g >> 1, pg, (off + l16) * (D / 32)), dst + 2 * G::kCode);
+      load_scales(scales_at(g >> 1, pg, (off + l16) * (D / 32)), src + 2 * G::kCode);
     }
-    advance();
   };
-  const bool blocks = a.page_size % 16 == 0;
-  // the next tile of this wave, in this window or the next one
-  int ic = 0, jn = 0;  // its keys
+  // The next tile of this wave, in this window or the next one, where there is one.
+  int ic = 0, jn = 0;  // its key in either
+  bool fly = false;    // whether a tile is on its way
   auto issue_next = [&]() {
     const bool here = ic < cur.kb;
-    if (!here && !(has_next && jn < nxt.kb)) return;
-    const int n = here ? ic : jn;
-    ic += here ? kStep : 0;
-    jn += here ? 0 : kStep;
-    const int kb = here ? cur.kb : nxt.kb, p0 = here ? cur.page0 : nxt.page0;
-    const int tb = here ? buf : buf ^ 1;
-    if (blocks)
-      issue_blocks(kb, p0, tb, n);
-    else
-      issue_rows(kb, p0, tb, n);
+    fly = here || (has_next && jn < nxt.kb);
+    if (__builtin_expect(fly, 1)) {
+      const int n = here ? ic : jn, kb = here ? cur.kb : nxt.kb;
+      const int p0 = here ? cur.page0 : nxt.page0, tb = here ? buf : buf_after(1);
+      ic += here ? kStep : 0;
+      jn += here ? 0 : kStep;
+      if constexpr (BLOCKS)
+        issue_blocks(kb, p0, tb, n);
+      else
+        issue_rows(kb, p0, tb, n);
+    }
   };
 
   // ---- state ---------------------------------------------------------------
@@ -523,18 +514,9 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
   // below it is hidden from any row, last: the last key that the lane's rows see.
   auto compute = [&](int n0, int kb, int full, const int (&last)[RB]) {
     const bool edge = n0 + kD4Tile > full;
-    // its loads are performed: those of up to fly - 1 tiles after it may not be
-    if (fly >= 4 && G::kRing >= 4)
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * G::kInFlight) : "memory");
-    else if (fly == 3 && G::kRing >= 3)
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * G::kInFlight) : "memory");
-    else if (fly == 2)
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(G::kInFlight) : "memory");
-    else
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     constexpr int kVW = D == 256 ? 2 : 1;  // words of V of a lane and key
     uint32_t kw[2][DJ], ks[2], vw[8][kVW], vs[8];
-    const uint32_t src = ring + rp;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       const int r = 16 * x + l16;
@@ -582,9 +564,7 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
         for (int k = 0; k < 4; ++k) vs[4 * x + k] = y[k];
       }
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot is free
-    rp = rp + G::kTile == G::kRing * G::kTile ? 0 : rp + G::kTile;
-    --fly;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile is read
     issue_next();
 
     f32x4 s[RB][2];
@@ -607,7 +587,7 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
     // Keys past the end hold anything: zeros.  A block of V that is NaN must
     // not reach the rows that do not see its key (0 * NaN): where drafts may be
     // hidden, zeros, and NaN at the end (nans).
-    if (edge) {
+    if (__builtin_expect(edge, 0)) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const int key = n0 + 16 * (k >> 2) + (k & 3);  // of lane group 0
@@ -641,7 +621,7 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[rb][0][r] = second ? s[rb][1][r] : s[rb][0][r];
       }
-      if (edge) {
+      if (__builtin_expect(edge, 0)) {
 #pragma unroll
         for (int x = 0; x < NX; ++x)
 #pragma unroll
@@ -655,7 +635,7 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
       for (int x = 0; x < NX; ++x)
 #pragma unroll
         for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[rb][x][r]);
-      if (__any((mx - m[rb]) * a.scale_log2 > kRescaleThreshold)) {
+      if (__builtin_expect(__any((mx - m[rb]) * a.scale_log2 > kRescaleThreshold), 0)) {
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         const float mn = fmaxf(m[rb], mx);
@@ -726,7 +706,7 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
     }
   };
 
-  constexpr bool kAhead = RB * DJ <= 4;  // the next piece's Q is loaded ahead
+  constexpr bool kAhead = D <= 128;  // the next piece's Q is loaded ahead
   u32x4 qn[RB][kAhead ? DJ : 1];
   fetch_q(cur, q);
   if constexpr (kAhead)
@@ -784,8 +764,8 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
     }
   };
   // Rows r0 .. r0 + n - 1 of a piece, phases h0 .. h0 + nh - 1, rg rows of an area each.
-  auto add_up = [&](int b, int np, int us, int mine, uint32_t area, uint32_t ws, int mi, int r0,
-                    int n, int h0, int nh, int rg) {
+  auto add_up = [&](int b, int np, int us, int mine, uint32_t area, int mi, int r0, int n, int h0, int nh) {
+    const int rg = nh > 1 ? G::kAllRows : 16;  // rows of an area's phase
     const int64_t slot = np == 1 ? 0 : walk_slot(a, sg.C, us, stream, mine);
     const uint32_t pr = static_cast<uint32_t>(a.part_rows);
     const __amdgpu_buffer_rsrc_t rm = make_rsrc_uniform(a.part_ml + slot * pr * 2, pr * 8);
@@ -793,8 +773,8 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
     uint16_t* out = static_cast<uint16_t*>(a.o) + (b * a.o_sb + head0 * a.o_sh + q0 * a.o_ss);
     const int sd = (tid % 32) * 2;  // 32 threads a row, two dims each
     for (int it = tid / 32; it < n * nh; it += kD4Threads / 32) {
-      const int hh = nh == G::kPH ? it % G::kPH : it % G::kSP;
-      const int lr = nh == G::kPH ? it / G::kPH : it / G::kSP;
+      const int hh = nh > 1 ? it % G::kPH : 0;
+      const int lr = nh > 1 ? it / G::kPH : it;
       const int h = h0 + hh;
       float mt = -INFINITY;
 #pragma unroll
@@ -807,7 +787,7 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
       for (int x = 0; x < kD4Waves; ++x) {
         const float f = fast_exp2(mrg_ml[mi][x][lr][0] - mu);
         lt += f * mrg_ml[mi][x][lr][1];
-        acc += f * *(const lds_f32x2_t*)lds_ptr(at + x * ws);
+        acc += f * *(const lds_f32x2_t*)lds_ptr(at + x * G::kStage);
       }
       const int r = r0 + lr;
       const int dim = G::dim(h, sd);
@@ -825,17 +805,17 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
       }
     }
   };
-  // A state that fits one area is left there, and the wave goes on to the next
-  // piece without a barrier; the piece is added up when the next but one ends,
-  // or with the last one, whose states lie in the ring.
+  // A state that fits one area is left there, in the two areas by turns, and added
+  // up behind the next barrier: that of the next but one window's table, or the
+  // last one.  So a workgroup of two pieces, as most are, has none before its end.
   const bool fits = RB == 1 && rows <= G::kAllRows;
-  const uint32_t area0 = lds_addr_of(stage), area1 = lds_addr_of(tiles);
-  constexpr uint32_t kWs0 = G::kStage, kWs1 = G::kRing * G::kTile;
-  static_assert(kWs1 >= G::kStage, "a wave's state in its ring");
+  const uint32_t area0 = lds_addr_of(stage), area1 = area0 + kD4Waves * G::kStage;
   struct Left {
     int b, np, us, mine;
   };
   Left left = {0, 0, 0, 0};  // (np 0: none)
+  int which = 0;             // the area that the next state goes to
+  bool added = false;
   // Cut units are counted when the workgroup is done: it has two at most, one
   // from each end of its segment.
   Left cut[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
@@ -848,8 +828,7 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
   };
   ic = cur.ka + turn * kD4Tile;
   if (has_next) jn = nxt.ka + turn_after(cur) * kD4Tile;
-#pragma unroll 1
-  for (int i = 0; i < G::kRing; ++i) issue_next();
+  issue_next();
 
   for (;;) {
     const int off = cur.Lk - a.pack_m;
@@ -877,17 +856,10 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
       }
       using Zero = std::integral_constant<int, 0>;
       if (fits) {
-        if (has_next && left.np) {
-          __syncthreads();
-          add_up(left.b, left.np, left.us, left.mine, area0, kWs0, 0, 0, rows, 0, G::kPH,
-             G::kAllRows);
-          __syncthreads();
-          left.np = 0;
-        }
-        put_stats(Zero{}, has_next ? 0 : 1);
+        if (!has_next && added) __syncthreads();  // the area may still be read
+        put_stats(Zero{}, which);
         if (l16 < rows) {
-          const uint32_t at = (has_next ? area0 + wave * kWs0 : area1 + wave * kWs1) +
-                              l16 * G::kPitch;
+          const uint32_t at = (which ? area1 : area0) + wave * G::kStage + l16 * G::kPitch;
           put_state(Zero{}, Zero{}, at);
           if constexpr (G::kPH > 1)
             put_state(Zero{}, std::integral_constant<int, 1>{}, at + G::kAllRows * G::kPitch);
@@ -897,28 +869,26 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
           }
         }
         if (has_next) left = Left{cur.b, cur.np, cur.us, cur.mine};
-      } else {
+        which ^= 1;
+      } else {  // two phases at a time, one in each area
         auto merge16 = [&](auto rbc) {
           constexpr int rb = decltype(rbc)::value;
           if (16 * rb >= rows) return;
           const int n = min(rows - 16 * rb, 16);
           put_stats(rbc, 0);
-          auto phases = [&](auto h) {  // as many as an area holds
+          auto phases = [&](auto h) {
             constexpr int H = decltype(h)::value;
-            const uint32_t at = area0 + wave * kWs0 + l16 * G::kPitch;
-            put_state(rbc, h, at);
-            if constexpr (G::kSP > 1)
-              put_state(rbc, std::integral_constant<int, H + 1>{}, at + 16 * G::kPitch);
+            const uint32_t at = wave * G::kStage + l16 * G::kPitch;
+            put_state(rbc, h, area0 + at);
+            if constexpr (G::kPH > 1) put_state(rbc, std::integral_constant<int, H + 1>{}, area1 + at);
             __syncthreads();
-            add_up(cur.b, cur.np, cur.us, cur.mine, area0, kWs0, 0, 16 * rb, n, H, G::kSP, 16);
+#pragma unroll 1
+            for (int u = 0; u < (G::kPH > 1 ? 2 : 1); ++u)
+              add_up(cur.b, cur.np, cur.us, cur.mine, u ? area1 : area0, 0, 16 * rb, n, H + u, 1);
             __syncthreads();
           };
           phases(Zero{});
-          if constexpr (G::kPH > G::kSP) phases(std::integral_constant<int, G::kSP>{});
-          if constexpr (G::kPH > 2 * G::kSP) {
-            phases(std::integral_constant<int, 2 * G::kSP>{});
-            phases(std::integral_constant<int, 3 * G::kSP>{});
-          }
+          if constexpr (G::kPH > 2) phases(std::integral_constant<int, 2>{});
         };
         merge16(Zero{});
         if constexpr (RB > 1) merge16(std::integral_constant<int, 1>{});
@@ -937,24 +907,29 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
       reset();
     }
     cur = nxt;
-    buf ^= 1;
-    has_next = next_window(cur, nxt);
+    nxt = nn;
+    has_next = has_nn;
+    buf = buf_after(1);
     ic = jn;
     if (has_next) {
       jn = nxt.ka + turn_after(cur) * kD4Tile;
-      const int e = fetch_entry(nxt);
+      // (its place was the table of the window before the one that ended, which no
+      // wave reads since the last barrier)
+      put_entry(entry, buf_after(1));
+      __syncthreads();
+      if (left.np) {
+        add_up(left.b, left.np, left.us, left.mine, which ? area0 : area1, which ^ 1, 0, rows, 0,
+               G::kPH);
+        left.np = 0;
+        added = true;
+      }
+      has_nn = next_window(nxt, nn);
+      entry = has_nn ? fetch_entry(nn) : 0;
       if constexpr (kAhead)
-        if (nxt.ka == 0 || nxt.b != cur.b) fetch_q(nxt, qn);
-      __syncthreads();  // the finished window's table is free
-      put_entry(e, buf ^ 1);
-      settle();
-      __syncthreads();  // the table is in LDS
-    } else if (!kAhead) {
-      settle();
+        if (nxt.b != cur.b) fetch_q(nxt, qn);
     }
-    // (windows of few tiles leave the ring with room)
-#pragma unroll 1
-    while (fly < G::kRing && (ic < cur.kb || (has_next && jn < nxt.kb))) issue_next();
+    if constexpr (!kAhead) settle();
+    if (!fly) issue_next();  // (this wave had no tile in the window before)
   }
   // the words that count the cut units, read ahead of the count
   uint64_t word = 0;
@@ -962,10 +937,13 @@ __global__ __launch_bounds__(kD4Threads, (2 * Fp4Geo<D, RB>::kPerCu)) void fa2_d
     word = merge_word(a, cut[tid ? 1 : 0].b * a.walk_streams + stream);
   if (fits) {
     __syncthreads();
-    if (left.np)
-      add_up(left.b, left.np, left.us, left.mine, area0, kWs0, 0, 0, rows, 0, G::kPH,
-             G::kAllRows);
-    add_up(cur.b, cur.np, cur.us, cur.mine, area1, kWs1, 1, 0, rows, 0, G::kPH, G::kAllRows);
+    // (the last state went to area which ^ 1, one left before it to the other)
+#pragma unroll 1
+    for (int u = left.np ? 0 : 1; u < 2; ++u) {
+      const Left p = u ? Left{cur.b, cur.np, cur.us, cur.mine} : left;
+      const int mi = u ? which ^ 1 : which;
+      add_up(p.b, p.np, p.us, p.mine, mi ? area1 : area0, mi, 0, rows, 0, G::kPH);
+    }
   }
   if (cut[0].np == 0) return;
   merge_publish();

@@ -219,26 +219,37 @@ int fp4_plan(const fa2_fp4_decode_params* p, Fp4Plan* pl) {
 
 bool fp4_empty(const fa2_fp4_decode_params* p) { return p->batch == 0 || p->q_len == 0; }
 
-template <int DT, int D>
+template <int DT, int D, bool BLOCKS>
 void launch_fp4_decode(const Fp4Args& a, int rb, uint32_t grid, hipStream_t st) {
-  // (up to 8 rows take the 16 columns twice)
-  if (rb == 1 && a.a.q_len <= 8)
-    hipLaunchKernelGGL((fa2_decode_fp4_kernel<DT, D, 1, true>), dim3(grid), dim3(kD4Threads), 0,
-                       st, a);
-  else if (rb == 1)
-    hipLaunchKernelGGL((fa2_decode_fp4_kernel<DT, D, 1, false>), dim3(grid), dim3(kD4Threads), 0,
-                       st, a);
-  if constexpr (D <= 128)
+  const dim3 block(kD4Threads);
+  // (up to 8 rows take the 16 columns twice; at D = 256 registers do not reach)
+  const bool half = D <= 128 && rb == 1 && a.a.q_len <= 8;
+  if (rb == 1 && !half)
+    hipLaunchKernelGGL((fa2_decode_fp4_kernel<DT, D, 1, false, BLOCKS>), dim3(grid), block, 0, st,
+                       a);
+  if constexpr (D <= 128) {
+    if (half)
+      hipLaunchKernelGGL((fa2_decode_fp4_kernel<DT, D, 1, true, BLOCKS>), dim3(grid), block, 0, st,
+                         a);
     if (rb == 2)
-      hipLaunchKernelGGL((fa2_decode_fp4_kernel<DT, D, 2, false>), dim3(grid), dim3(kD4Threads), 0,
-                         st, a);
+      hipLaunchKernelGGL((fa2_decode_fp4_kernel<DT, D, 2, false, BLOCKS>), dim3(grid), block, 0, st,
+                         a);
+  }
+}
+
+template <int DT, int D>
+void launch_fp4_decode_pages(const Fp4Args& a, int rb, uint32_t grid, hipStream_t st) {
+  if (a.a.page_size % 16 == 0)
+    launch_fp4_decode<DT, D, true>(a, rb, grid, st);
+  else
+    launch_fp4_decode<DT, D, false>(a, rb, grid, st);
 }
 
 template <int DT>
 void launch_fp4_decode_dim(int64_t d, const Fp4Args& a, int rb, uint32_t grid, hipStream_t st) {
-  if (d == 64) launch_fp4_decode<DT, 64>(a, rb, grid, st);
-  else if (d == 128) launch_fp4_decode<DT, 128>(a, rb, grid, st);
-  else launch_fp4_decode<DT, 256>(a, rb, grid, st);
+  if (d == 64) launch_fp4_decode_pages<DT, 64>(a, rb, grid, st);
+  else if (d == 128) launch_fp4_decode_pages<DT, 128>(a, rb, grid, st);
+  else launch_fp4_decode_pages<DT, 256>(a, rb, grid, st);
 }
 
 }  // namespace
@@ -376,7 +387,6 @@ extern "C" int fa2_fp4_decode(const fa2_fp4_decode_params* p, void* stream) {
   a.q_len = static_cast<int32_t>(pl.rows);
   a.kv_len = static_cast<int32_t>(p->table_width * p->page_size);
   a.page_size = static_cast<int32_t>(p->page_size);
-  a.page_shift = log2_exact(p->page_size);
   a.mask = p->mask;
   a.num_splits = 1;
   a.scale_log2 = p->softmax_scale * 1.4426950408889634f;
@@ -410,6 +420,14 @@ extern "C" int fa2_fp4_decode(const fa2_fp4_decode_params* p, void* stream) {
   fa.head_scales = static_cast<uint32_t>(p->page_size * (d / 32));
   fa.page_codes = static_cast<uint32_t>(p->kv_heads * p->page_size * (d / 2));
   fa.page_scales = static_cast<uint32_t>(p->kv_heads * p->page_size * (d / 32));
+  // n / page_size for n < 2^30 as (2 n * page_mul) >> 32 >> page_sh, with page_sh =
+  // floor(log2 page_size) and page_mul = ceil(2^(31 + page_sh) / page_size): page_mul
+  // is off by less than 1, the quotient by less than n / 2^(31 + page_sh), which is
+  // under 1 / page_size since 2^page_sh > page_size / 2
+  int sh = 0;
+  while ((int64_t(2) << sh) <= p->page_size) ++sh;
+  fa.page_sh = static_cast<uint32_t>(sh);
+  fa.page_mul = static_cast<uint32_t>(cdiv(int64_t(1) << (31 + sh), p->page_size));
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (p->dtype == FA2_DTYPE_F16)
     launch_fp4_decode_dim<FA2_DTYPE_F16>(d, fa, pl.rb, static_cast<uint32_t>(grid), st);
