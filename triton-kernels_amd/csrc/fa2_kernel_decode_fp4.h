@@ -177,6 +177,24 @@ __device__ __forceinline__ float half_swap(float x) {
                                                                0xF, 0xF, true));
 }
 
+// x of the lane and of lane ^ 16 (or ^ 32), in the same order in both.
+template <int X>
+__device__ __forceinline__ f32x2 lane_pair(float x) {
+  const int w = __builtin_bit_cast(int, x);
+  u32x2 y;
+  if constexpr (X == 16)
+    y = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(w, w, false, false));
+  else
+    y = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(w, w, false, false));
+  return __builtin_bit_cast(f32x2, y);
+}
+template <bool MAX>
+__device__ __forceinline__ float over_groups(float x) {  // the four lanes l % 16
+  const f32x2 y = lane_pair<16>(x);
+  const f32x2 z = lane_pair<32>(MAX ? fmaxf(y[0], y[1]) : y[0] + y[1]);
+  return MAX ? fmaxf(z[0], z[1]) : z[0] + z[1];
+}
+
 // Sum (or maximum, of numbers >= 0) over the lanes up to each, on the VALU.
 template <bool MAX>
 __device__ __forceinline__ int wave_scan(int x) {
@@ -209,7 +227,7 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
 
   __shared__ __attribute__((aligned(1024))) char tiles[kD4Waves * G::kTile];
   __shared__ __attribute__((aligned(128))) char stage[2 * kD4Waves * G::kStage];
-  __shared__ float mrg_ml[2][kD4Waves][16][2];
+  __shared__ __attribute__((aligned(8))) float mrg_ml[2][kD4Waves][16][2];
   __shared__ int tab[3][2][G::kTable];
   __shared__ DecSegment seg_sh[kD4Waves];
   __shared__ int merge_flag[2];
@@ -336,16 +354,12 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
     if (slot_t < G::kTable) tab[buf][half][slot_t] = min(max(e, 0), fa.num_pages - 1);
   };
 
-  Window cur, nxt;
-  if (!first_window(cur, sg.j, sg.us)) return;
-  bool has_next = next_window(cur, nxt);
   // Block-table entries are in LDS for this window (tab[buf]) and the next one, and on
   // their way for the one after.
-  Window nn;
-  bool has_nn = has_next && next_window(nxt, nn);
+  Window cur, nxt, nn;
+  bool has_next = false, has_nn = false;
+  if (!first_window(cur, sg.j, sg.us)) return;
   const int entry0 = fetch_entry(cur);
-  const int entry1 = has_next ? fetch_entry(nxt) : 0;
-  int entry = has_nn ? fetch_entry(nn) : 0;
   int buf = 0;
   auto buf_after = [&](int n) { return buf + n >= 3 ? buf + n - 3 : buf + n; };
 
@@ -636,8 +650,7 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
 #pragma unroll
         for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[rb][x][r]);
       if (__builtin_expect(__any((mx - m[rb]) * a.scale_log2 > kRescaleThreshold), 0)) {
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        mx = over_groups<true>(mx);
         const float mn = fmaxf(m[rb], mx);
         const float alpha = fast_exp2((m[rb] - (mn == -INFINITY ? 0.f : mn)) * a.scale_log2);
         m[rb] = mn;
@@ -709,12 +722,13 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
   constexpr bool kAhead = D <= 128;  // the next piece's Q is loaded ahead
   u32x4 qn[RB][kAhead ? DJ : 1];
   fetch_q(cur, q);
+  has_next = next_window(cur, nxt);  // (while the first entries are on their way)
+  const int entry1 = has_next ? fetch_entry(nxt) : 0;
   if constexpr (kAhead)
     if (has_next) fetch_q(nxt, qn);
   reset();
   put_entry(entry0, 0);
   put_entry(entry1, 1);
-  settle();
   __syncthreads();  // the tables are in LDS
 
   // ---- pieces' ends ----------------------------------------------------------
@@ -741,8 +755,7 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
         for (int r = 0; r < 4; ++r)  // (two scales at D = 256: dims 64 g + 16 r + i)
           if ((nans[rb] >> (D == 256 ? r >> 1 : 0)) & 1) o[rb][i][r] = nan;
     }
-    l[rb] += __shfl_xor(l[rb], 16);
-    l[rb] += __shfl_xor(l[rb], 32);
+    l[rb] = over_groups<false>(l[rb]);
     if constexpr (HALF) {  // both halves get their sum
       const float mo = half_swap(m[rb]);
       const float mn = fmaxf(m[rb], mo);
@@ -763,45 +776,53 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
       mrg_ml[mi][wave][l16][1] = l[rb];
     }
   };
-  // Rows r0 .. r0 + n - 1 of a piece, phases h0 .. h0 + nh - 1, rg rows of an area each.
-  auto add_up = [&](int b, int np, int us, int mine, uint32_t area, int mi, int r0, int n, int h0, int nh) {
-    const int rg = nh > 1 ? G::kAllRows : 16;  // rows of an area's phase
-    const int64_t slot = np == 1 ? 0 : walk_slot(a, sg.C, us, stream, mine);
-    const uint32_t pr = static_cast<uint32_t>(a.part_rows);
-    const __amdgpu_buffer_rsrc_t rm = make_rsrc_uniform(a.part_ml + slot * pr * 2, pr * 8);
-    const __amdgpu_buffer_rsrc_t ro = make_rsrc_uniform(a.part_o + slot * pr * D, pr * D * 4);
-    uint16_t* out = static_cast<uint16_t*>(a.o) + (b * a.o_sb + head0 * a.o_sh + q0 * a.o_ss);
-    const int sd = (tid % 32) * 2;  // 32 threads a row, two dims each
-    for (int it = tid / 32; it < n * nh; it += kD4Threads / 32) {
-      const int hh = nh > 1 ? it % G::kPH : 0;
-      const int lr = nh > 1 ? it / G::kPH : it;
-      const int h = h0 + hh;
+  struct Left {  // what is left of a piece (np 0: nothing)
+    int b, np, us, mine;
+  };
+  // Rows r0 .. r0 + n - 1 of a piece, phases h0 .. h0 + nh - 1: phase h0 + i of row r
+  // lies i * step + r * kPitch into the area.
+  auto add_up = [&](const Left& p, uint32_t area, int mi, int r0, int n, int h0, int nh, int step) {
+    const int sd = (tid % 16) * 4;  // 16 threads a row and phase, four dims each
+    for (int it = tid / 16; it < n * nh; it += kD4Threads / 16) {
+      const int hh = nh == 1 ? 0 : it % nh, lr = nh == 1 ? it : it / nh;
+      const uint32_t at = area + hh * step + lr * G::kPitch + sd * 4;
+      f32x2 ml[kD4Waves];
+#pragma unroll
+      for (int w = 0; w < kD4Waves; ++w)
+        ml[w] = *reinterpret_cast<const f32x2*>(mrg_ml[mi][w][lr]);
       float mt = -INFINITY;
 #pragma unroll
-      for (int x = 0; x < kD4Waves; ++x) mt = fmaxf(mt, mrg_ml[mi][x][lr][0]);
+      for (int w = 0; w < kD4Waves; ++w) mt = fmaxf(mt, ml[w][0]);
       const float mu = mt == -INFINITY ? 0.f : mt;
       float lt = 0.f;
-      f32x2 acc = (f32x2){0.f, 0.f};
-      const uint32_t at = area + sd * 4 + (hh * rg + lr) * G::kPitch;
+      f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int x = 0; x < kD4Waves; ++x) {
-        const float f = fast_exp2(mrg_ml[mi][x][lr][0] - mu);
-        lt += f * mrg_ml[mi][x][lr][1];
-        acc += f * *(const lds_f32x2_t*)lds_ptr(at + x * G::kStage);
+      for (int w = 0; w < kD4Waves; ++w) {
+        const float f = fast_exp2(ml[w][0] - mu);
+        lt += f * ml[w][1];
+        acc += f * *(const lds_f32x4_t*)lds_ptr(at + w * G::kStage);
       }
       const int r = r0 + lr;
-      const int dim = G::dim(h, sd);
-      if (np == 1) {
-        const float inv = 1.f / lt;  // 0/0 -> NaN for a row with no key, as in 16 bits
-        *reinterpret_cast<uint32_t*>(out + r * a.o_ss + dim) =
-            pack2<BF>(acc[0] * inv, acc[1] * inv);
+      const int dim = G::dim(h0 + hh, sd);
+      if (p.np == 1) {
+        // (0/0 -> NaN for a row with no key, as in 16 bits; otherwise lt >= 2^-8)
+        const float inv = __builtin_amdgcn_rcpf(lt);
+        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.o) + p.b * a.o_sb + head0 * a.o_sh +
+                                  (q0 + r) * a.o_ss + dim) =
+            (u32x2){pack2<BF>(acc[0] * inv, acc[1] * inv), pack2<BF>(acc[2] * inv, acc[3] * inv)};
       } else {
-        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, acc), ro,
-                                              (r * D + dim) * 4, 0, kCpolSc1);
-        if (h == 0 && sd == 0)
+        // the slot of this workgroup's piece (walk_slot)
+        const int64_t slot =
+            (static_cast<int64_t>(seg_k) * a.walk_streams + stream) * 2 +
+            (p.mine == 0 && p.us != sg.s0);
+        const uint32_t pr = static_cast<uint32_t>(a.part_rows);
+        __builtin_amdgcn_raw_buffer_store_b128(
+            __builtin_bit_cast(u32x4, acc),
+            make_rsrc_uniform(a.part_o + slot * pr * D, pr * D * 4), (r * D + dim) * 4, 0, kCpolSc1);
+        if (h0 + hh == 0 && sd == 0)
           __builtin_amdgcn_raw_buffer_store_b64(
-              (u32x2){__builtin_bit_cast(uint32_t, mt), __builtin_bit_cast(uint32_t, lt)}, rm,
-              r * 8, 0, kCpolSc1);
+              (u32x2){__builtin_bit_cast(uint32_t, mt), __builtin_bit_cast(uint32_t, lt)},
+              make_rsrc_uniform(a.part_ml + slot * pr * 2, pr * 8), r * 8, 0, kCpolSc1);
       }
     }
   };
@@ -810,10 +831,7 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
   // last one.  So a workgroup of two pieces, as most are, has none before its end.
   const bool fits = RB == 1 && rows <= G::kAllRows;
   const uint32_t area0 = lds_addr_of(stage), area1 = area0 + kD4Waves * G::kStage;
-  struct Left {
-    int b, np, us, mine;
-  };
-  Left left = {0, 0, 0, 0};  // (np 0: none)
+  Left left = {0, 0, 0, 0};
   int which = 0;             // the area that the next state goes to
   bool added = false;
   // Cut units are counted when the workgroup is done: it has two at most, one
@@ -829,6 +847,9 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
   ic = cur.ka + turn * kD4Tile;
   if (has_next) jn = nxt.ka + turn_after(cur) * kD4Tile;
   issue_next();
+  has_nn = has_next && next_window(nxt, nn);  // (while the first tile is on its way)
+  int entry = has_nn ? fetch_entry(nn) : 0;
+  settle();
 
   for (;;) {
     const int off = cur.Lk - a.pack_m;
@@ -882,9 +903,8 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
             put_state(rbc, h, area0 + at);
             if constexpr (G::kPH > 1) put_state(rbc, std::integral_constant<int, H + 1>{}, area1 + at);
             __syncthreads();
-#pragma unroll 1
-            for (int u = 0; u < (G::kPH > 1 ? 2 : 1); ++u)
-              add_up(cur.b, cur.np, cur.us, cur.mine, u ? area1 : area0, 0, 16 * rb, n, H + u, 1);
+            add_up(Left{cur.b, cur.np, cur.us, cur.mine}, area0, 0, 16 * rb, n, H,
+                   G::kPH > 1 ? 2 : 1, area1 - area0);
             __syncthreads();
           };
           phases(Zero{});
@@ -918,8 +938,8 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
       put_entry(entry, buf_after(1));
       __syncthreads();
       if (left.np) {
-        add_up(left.b, left.np, left.us, left.mine, which ? area0 : area1, which ^ 1, 0, rows, 0,
-               G::kPH);
+        add_up(left, which ? area0 : area1, which ^ 1, 0, rows, 0, G::kPH,
+               G::kAllRows * G::kPitch);
         left.np = 0;
         added = true;
       }
@@ -942,7 +962,7 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
     for (int u = left.np ? 0 : 1; u < 2; ++u) {
       const Left p = u ? Left{cur.b, cur.np, cur.us, cur.mine} : left;
       const int mi = u ? which ^ 1 : which;
-      add_up(p.b, p.np, p.us, p.mine, mi ? area1 : area0, mi, 0, rows, 0, G::kPH);
+      add_up(p, mi ? area1 : area0, mi, 0, rows, 0, G::kPH, G::kAllRows * G::kPitch);
     }
   }
   if (cut[0].np == 0) return;
