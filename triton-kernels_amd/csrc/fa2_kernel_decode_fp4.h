@@ -223,6 +223,7 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
   constexpr int kSub = D == 256 ? 2 : 1;  // scales of a lane's dims
   static_assert(kD4Waves * G::kStage >= kMergePieceBytes<kD4Threads>, "merge area");
   static_assert(!HALF || RB == 1, "HALF");
+  constexpr int kAlign = RB == 1 ? 8 : 12, kGap = RB == 1 ? 5 : 8;
   constexpr int NX = HALF ? 1 : 2;  // 16-key blocks that a lane's scores are from
 
   __shared__ __attribute__((aligned(1024))) char tiles[kD4Waves * G::kTile];
@@ -254,20 +255,47 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
   const bool in_lanes = a.batch <= 64;
   const int lens = in_lanes && lane < a.batch ? walk_len<MODE>(a, lane) : 0;
   DecSegment sg;
+  int room = 0;  // what a unit takes of the stream (in_lanes)
+  int gap = 0;
   if (in_lanes) {
     const int W = lane < a.batch ? walk_weight(lens) : 0;
-    const int incl = wave_scan<false>(W);
-    const int total = __builtin_amdgcn_readlane(incl, 63);
+    int total = __builtin_amdgcn_readlane(wave_scan<false>(W), 63);
     const int longest = __builtin_amdgcn_readlane(wave_scan<true>(W), 63);
-    const int C = max((total + a.walk_segs - 1) / a.walk_segs, a.walk_min);
+    int C = max((total + a.walk_segs - 1) / a.walk_segs, a.walk_min);
     sg = DecSegment{seg_k, 0, 0, 0, 0};
     if (longest > a.walk_short && !walk_keep_whole(a, longest, C, a.walk_whole)) {
+      int incl = 0;
+      bool fit = false;
+      if (a.batch <= a.walk_segs) {
+        for (int c = C; c <= C + kAlign && !fit; c += kAlign / 2) {
+          const float inv = __builtin_amdgcn_rcpf(static_cast<float>(c));
+          int n = static_cast<int>(static_cast<float>(W) * inv);
+          n += n * c < W;
+          n -= (n - 1) * c >= W && n > 0;
+          incl = wave_scan<false>(n);
+          fit = __builtin_amdgcn_readlane(incl, 63) <= a.walk_segs;
+          if (fit) {
+            C = c;
+            incl *= c;
+            room = n * c;
+          }
+        }
+      }
+      if (!fit) {
+        gap = kGap;
+        room = W ? W + kGap : 0;
+        incl = wave_scan<false>(room);
+        total = __builtin_amdgcn_readlane(incl, 63);
+        C = max((total + a.walk_segs - 1) / a.walk_segs, a.walk_min);
+      }
+      total = __builtin_amdgcn_readlane(incl, 63);
       const int s0 = min(seg_k * C, total);
-      const uint64_t at = __ballot(incl - W <= s0 && s0 < incl);
+      const uint64_t at = __ballot(incl - room <= s0 && s0 < incl);
       sg = DecSegment{a.batch, total, total, total, C};
       if (at) {
         const int j = __builtin_ctzll(at);
-        sg = DecSegment{j, __builtin_amdgcn_readlane(incl - W, j), s0, min(s0 + C, total), C};
+        sg = DecSegment{j, __builtin_amdgcn_readlane(incl - room, j) + gap, s0,
+                        min(s0 + C, total), C};
       }
     }
   } else {
@@ -284,7 +312,7 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
   // window of it: keys [ka, kb), all of it unless its block-table entries exceed
   // the LDS table.
   struct Window {
-    int b, us, W, Lk;   // sequence, the unit's start in the stream, weight, length
+    int b, us, W, room, Lk;   // sequence, the unit's start in the stream, weight, length
     int np, mine;       // pieces of the unit, this one's index
     int ka, kb, kend;   // kend: the piece's end
     int page0;          // first logical page
@@ -297,6 +325,7 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
     v.us = us;
     v.Lk = in_lanes ? __builtin_amdgcn_readlane(lens, j) : walk_len<MODE>(a, j);
     v.W = walk_weight(v.Lk);
+    v.room = in_lanes ? __builtin_amdgcn_readlane(room, j) : v.W;
     v.np = 1;
     v.mine = 0;
     v.ka = 0;
@@ -338,7 +367,7 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
       window_at(v, c.kb);
       return true;
     }
-    return first_window(v, walk_next(a, sg, c.b), c.us + c.W);
+    return first_window(v, walk_next(a, sg, c.b), c.us + c.room);
   };
   // Entries of a window's pages, clamped into the pool: one per thread, K's by the
   // first half of the workgroup; loaded, then put into LDS.
