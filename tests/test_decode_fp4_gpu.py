@@ -120,6 +120,40 @@ def test_long(dtype, D, QH, KVH, M, page, lens):
     c.check(c.call())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("QH,KVH,M", [(24, 1, 0), (16, 4, 5), (8, 2, 8), (24, 1, 4), (34, 2, 1)])
+@pytest.mark.parametrize("page", [16, 5])
+def test_wide_tables(dtype, D, QH, KVH, M, page):
+    """More than 16 rows where the tables could hold many keys (q-blocks of 32 up to
+    D128), and the same with tables of just the pages (q-blocks of 16)."""
+    c = Case([0, 1, 33, 2000, M, 130, 1100], QH, KVH, D, M, dtype, page, 23, causal=bool(M))
+    c.check(c.call())
+    width = -(-(1 << 20) // (page * KVH))  # 7 * 2^14 tiles of 64 keys and more
+    wide = [torch.full((7, width), -1, dtype=torch.int32) for _ in range(2)]
+    for w, t in zip(wide, c.tables):
+        w[:, :t.shape[1]] = t
+    c.check(c.call(k_block_table=wide[0].cuda(), v_block_table=wide[1].cuda()))
+
+
+@pytest.mark.parametrize("D,KVH,page,lens", [
+    (128, 16, 16, [60 + 59 * (i * 7 % 50) for i in range(50)]),     # several units a workgroup
+    (128, 1, 16, [2900 if i % 9 == 0 else 40 + i for i in range(70)]),  # more than 64 sequences
+    (64, 16, 48, [2900 if i % 9 == 0 else 40 + i for i in range(66)]),
+    (128, 2, 48, [5000, 100, 2047]),
+    (256, 8, 16, [3000 if i % 5 == 0 else 7 * i for i in range(33)]),
+    (64, 8, 16, [1030] * 16),                                       # equal units
+    (128, 1, 16, [1030 + i for i in range(64)]),
+])
+def test_shares(D, KVH, page, lens):
+    """Workgroups with several units and units with several workgroups."""
+    c = Case(lens, 2 * KVH, KVH, D, 0, torch.bfloat16, page, 24)
+    out = c.call().cpu().unsqueeze(2)
+    for b in range(0, len(lens), 3):
+        want, tol = R.attention(c.q[b], *c.values(b), False)
+        R.within(out[b], want, tol)
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_windows_inside_a_piece(D):
     """Units stay whole and span several windows of the LDS block table."""
@@ -210,6 +244,52 @@ def test_strides_and_index_types():
                               **{n: d[n] for n in ("kv_indptr", "k_block_table",
                                                    "v_block_table")})
     assert torch.equal(one[:, :, 0], sq)
+
+
+@pytest.mark.parametrize("drafts", [False, True])
+@pytest.mark.parametrize("bad", ["dims", "dtype", "head_dim", "heads", "lens", "rows", "v", "codes",
+                                 "pages", "scales", "device", "drafts"])
+def test_refusals(drafts, bad):
+    """Each is refused on the host, with and without the extension."""
+    import kernels.decode_fp4 as m
+    c = Case([40, 3], 4, 2, 128, 3 if drafts else 0, torch.float16, 16, 25)
+    d = c.dev()
+    q, k, v = d.pop("q"), d.pop("k_cache"), d.pop("v_cache")
+    if bad == "dims":
+        q = q[0]
+    elif bad == "dtype":
+        q = q.float()
+    elif bad == "head_dim":
+        q = q[..., :64]
+    elif bad == "heads":
+        q = q[:, :3]
+    elif bad == "lens":
+        d["kv_indptr"] = d["kv_indptr"][:1]
+    elif bad == "rows":
+        d["v_block_table"] = d["v_block_table"][:1]
+    elif bad == "v":
+        v = None
+    elif bad == "codes":
+        v = (v[0].float(), v[1])
+    elif bad == "pages":
+        v = (v[0][1:], v[1][1:])
+    elif bad == "scales":
+        k = (k[0], k[1][..., :3])
+    elif bad == "device":
+        d["kv_indptr"] = d["kv_indptr"].cpu()
+    elif not drafts:
+        q = q.unsqueeze(2)
+    else:
+        q = q[:, :, :1].expand(-1, -1, 17, -1)
+    call = m.speculative_decode_attention_fp4 if drafts else m.decode_attention_fp4
+    for use in (True, False):
+        m.USE_EXT = use
+        try:
+            with pytest.raises((ValueError, TypeError, AssertionError, RuntimeError)):
+                call(q, k, v, **d)
+        finally:
+            m.USE_EXT = True
+    torch.cuda.synchronize()
 
 
 def test_empty_batch():

@@ -154,7 +154,6 @@ struct Fp4Geo {
   static constexpr int kRP = 16 / kNI;                // accumulator rows of a lane per phase
   static constexpr int kPitch = (kPD + 4) * 4;        // merge rows
   static constexpr int kStage = 16 * kPitch;          // a wave's merge area: a phase of 16 rows
-  static constexpr int kAllRows = 16 / kPH;           // ... or all phases of so many
   static constexpr int kTable = 256;                  // block-table entries of a window
   // chunk c of row r lies at chunk c ^ ksw(r): 8 lanes reading a chunk of 8 rows
   // hit distinct banks
@@ -170,12 +169,6 @@ struct Fp4Geo {
     return (sd >> 4) * (D / 4) + 16 * h + (sd & 15);
   }
 };
-
-// The value of lane l ^ 8 (a rotation by 8 within each 16 lanes).
-__device__ __forceinline__ float half_swap(float x) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x128,
-                                                               0xF, 0xF, true));
-}
 
 // x of the lane and of lane ^ 16 (or ^ 32), in the same order in both.
 template <int X>
@@ -208,11 +201,7 @@ __device__ __forceinline__ int wave_scan(int x) {
   return x;
 }
 
-// HALF: up to 8 rows, which take the 16 columns twice: columns 0-7 go with the first
-// 16 keys of a tile and 8-15 with the others, so a lane has 4 scores per tile
-// instead of 8, half of them of no row.  The halves are states of their own, joined
-// at a piece's end.
-template <int DT, int D, int RB, bool HALF, bool BLOCKS>
+template <int DT, int D, int RB, bool BLOCKS>
 __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
     Fp4Args fa) {
   using G = Fp4Geo<D>;
@@ -222,13 +211,11 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
   constexpr int kStep = kD4Tile * kD4Waves;
   constexpr int kSub = D == 256 ? 2 : 1;  // scales of a lane's dims
   static_assert(kD4Waves * G::kStage >= kMergePieceBytes<kD4Threads>, "merge area");
-  static_assert(!HALF || RB == 1, "HALF");
   constexpr int kAlign = RB == 1 ? 8 : 12, kGap = RB == 1 ? 5 : 8;
-  constexpr int NX = HALF ? 1 : 2;  // 16-key blocks that a lane's scores are from
 
   __shared__ __attribute__((aligned(1024))) char tiles[kD4Waves * G::kTile];
   __shared__ __attribute__((aligned(128))) char stage[2 * kD4Waves * G::kStage];
-  __shared__ __attribute__((aligned(8))) float mrg_ml[2][kD4Waves][16][2];
+  __shared__ __attribute__((aligned(8))) float mrg_ml[kD4Waves][16][2];
   __shared__ int tab[3][2][G::kTable];
   __shared__ DecSegment seg_sh[kD4Waves];
   __shared__ int merge_flag[2];
@@ -239,8 +226,6 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15;
   const int g = lane >> 4;
-  const int lrow = HALF ? l16 & 7 : l16;  // this lane's row (of each 16)
-  const bool second = HALF && l16 >= 8;
   const bool causal = a.mask != FA2_MASK_NONE;
   const int stream = static_cast<int>(blockIdx.x) % a.walk_streams;
   const int seg_k = static_cast<int>(blockIdx.x) / a.walk_streams;
@@ -521,7 +506,7 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
     const int64_t base = v.b * a.q_sb + head0 * a.q_sh + q0 * a.q_ss;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      const int r = 16 * rb + lrow;
+      const int r = 16 * rb + l16;
 #pragma unroll
       for (int j = 0; j < DJ; ++j) {
         x[rb][j] = (u32x4){0u, 0u, 0u, 0u};
@@ -660,22 +645,18 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
     u32x4 ph[RB], pl[RB];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      if constexpr (HALF) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[rb][0][r] = second ? s[rb][1][r] : s[rb][0][r];
-      }
       if (__builtin_expect(edge, 0)) {
 #pragma unroll
-        for (int x = 0; x < NX; ++x)
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int key = n0 + (HALF ? (second ? 16 : 0) : 16 * x) + 4 * g + r;
+            const int key = n0 + 16 * x + 4 * g + r;
             s[rb][x][r] = key <= last[rb] ? s[rb][x][r] : -INFINITY;
           }
       }
       float mx = -INFINITY;
 #pragma unroll
-      for (int x = 0; x < NX; ++x)
+      for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[rb][x][r]);
       if (__builtin_expect(__any((mx - m[rb]) * a.scale_log2 > kRescaleThreshold), 0)) {
@@ -690,7 +671,7 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
       // (the difference is taken before the scale: no score is too large for it)
       const float mu = m[rb] == -INFINITY ? 0.f : m[rb];
 #pragma unroll
-      for (int x = 0; x < NX; ++x) {
+      for (int x = 0; x < 2; ++x) {
         float e[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -702,15 +683,8 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
           const uint32_t hw = pack2<BF>(e[2 * r], e[2 * r + 1]);
           const f32x2 h = unpack2<BF>(hw);
           const uint32_t lw = pack2<BF>(e[2 * r] - h[0], e[2 * r + 1] - h[1]);
-          if constexpr (HALF) {  // the other block's keys: zero
-            ph[rb][r] = second ? 0u : hw;
-            pl[rb][r] = second ? 0u : lw;
-            ph[rb][2 + r] = second ? hw : 0u;
-            pl[rb][2 + r] = second ? lw : 0u;
-          } else {
-            ph[rb][2 * x + r] = hw;
-            pl[rb][2 * x + r] = lw;
-          }
+          ph[rb][2 * x + r] = hw;
+          pl[rb][2 * x + r] = lw;
         }
       }
     }
@@ -762,7 +736,7 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
 
   // ---- pieces' ends ----------------------------------------------------------
   // The waves' states meet in LDS: wave x's row r, kPD dims, at area + x * ws + r *
-  // kPitch, its maximum (log2 units) and sum in mrg_ml[mi]; added up in wave
+  // kPitch, its maximum (log2 units) and sum in mrg_ml; added up in wave
   // order and written, to the output or to the piece's part slot.
   auto put_state = [&](auto rbc, auto hc_, uint32_t at) {  // phase h of this lane's row
     constexpr int rb = decltype(rbc)::value, h = decltype(hc_)::value;
@@ -774,7 +748,7 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
       *(lds_f32x4_t*)lds_ptr(at + 64 * g + 4 * e) = y;
     }
   };
-  auto put_stats = [&](auto rbc, int mi) {
+  auto put_stats = [&](auto rbc) {
     constexpr int rb = decltype(rbc)::value;
     if (__any(nans[rb])) {
       const float nan = __builtin_nanf("");
@@ -785,87 +759,84 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
           if ((nans[rb] >> (D == 256 ? r >> 1 : 0)) & 1) o[rb][i][r] = nan;
     }
     l[rb] = over_groups<false>(l[rb]);
-    if constexpr (HALF) {  // both halves get their sum
-      const float mo = half_swap(m[rb]);
-      const float mn = fmaxf(m[rb], mo);
-      const float f = fast_exp2((m[rb] - (mn == -INFINITY ? 0.f : mn)) * a.scale_log2);
-      m[rb] = mn;
-      const float lf = l[rb] * f;
-      l[rb] = lf + half_swap(lf);
-#pragma unroll
-      for (int i = 0; i < G::kNI; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float y = o[rb][i][r] * f;
-          o[rb][i][r] = y + half_swap(y);
-        }
-    }
     if (g == 0) {
-      mrg_ml[mi][wave][l16][0] = m[rb] * a.scale_log2;  // (-inf stays -inf)
-      mrg_ml[mi][wave][l16][1] = l[rb];
+      mrg_ml[wave][l16][0] = m[rb] * a.scale_log2;  // (-inf stays -inf)
+      mrg_ml[wave][l16][1] = l[rb];
     }
   };
-  struct Left {  // what is left of a piece (np 0: nothing)
+  struct Cut {  // a piece of a cut unit (np 0: none)
     int b, np, us, mine;
   };
-  // Rows r0 .. r0 + n - 1 of a piece, phases h0 .. h0 + nh - 1: phase h0 + i of row r
-  // lies i * step + r * kPitch into the area.
-  auto add_up = [&](const Left& p, uint32_t area, int mi, int r0, int n, int h0, int nh, int step) {
+  // 16 rows from 16 rb on of the piece cur, n of them, phases H and H + 1, one in each area
+  const uint32_t area0 = lds_addr_of(stage), area1 = area0 + kD4Waves * G::kStage;
+  constexpr int kTwo = G::kPH > 1 ? 2 : 1;
+  bool dirty = false;  // the areas may still be read
+  auto add_up = [&](int r0, int n, int h0) {
     const int sd = (tid % 16) * 4;  // 16 threads a row and phase, four dims each
-    for (int it = tid / 16; it < n * nh; it += kD4Threads / 16) {
-      const int hh = nh == 1 ? 0 : it % nh, lr = nh == 1 ? it : it / nh;
-      const uint32_t at = area + hh * step + lr * G::kPitch + sd * 4;
-      f32x2 ml[kD4Waves];
+    const int it = tid / 16, hh = it % kTwo, lr = it / kTwo;
+    if (lr >= n) return;
+    const uint32_t at = (hh ? area1 : area0) + lr * G::kPitch + sd * 4;
+    f32x2 ml[kD4Waves];
 #pragma unroll
-      for (int w = 0; w < kD4Waves; ++w)
-        ml[w] = *reinterpret_cast<const f32x2*>(mrg_ml[mi][w][lr]);
-      float mt = -INFINITY;
+    for (int w = 0; w < kD4Waves; ++w) ml[w] = *reinterpret_cast<const f32x2*>(mrg_ml[w][lr]);
+    float mt = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kD4Waves; ++w) mt = fmaxf(mt, ml[w][0]);
-      const float mu = mt == -INFINITY ? 0.f : mt;
-      float lt = 0.f;
-      f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int w = 0; w < kD4Waves; ++w) mt = fmaxf(mt, ml[w][0]);
+    const float mu = mt == -INFINITY ? 0.f : mt;
+    float lt = 0.f;
+    f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int w = 0; w < kD4Waves; ++w) {
-        const float f = fast_exp2(ml[w][0] - mu);
-        lt += f * ml[w][1];
-        acc += f * *(const lds_f32x4_t*)lds_ptr(at + w * G::kStage);
-      }
-      const int r = r0 + lr;
-      const int dim = G::dim(h0 + hh, sd);
-      if (p.np == 1) {
-        // (0/0 -> NaN for a row with no key, as in 16 bits; otherwise lt >= 2^-8)
-        const float inv = __builtin_amdgcn_rcpf(lt);
-        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.o) + p.b * a.o_sb + head0 * a.o_sh +
-                                  (q0 + r) * a.o_ss + dim) =
-            (u32x2){pack2<BF>(acc[0] * inv, acc[1] * inv), pack2<BF>(acc[2] * inv, acc[3] * inv)};
-      } else {
-        // the slot of this workgroup's piece (walk_slot)
-        const int64_t slot =
-            (static_cast<int64_t>(seg_k) * a.walk_streams + stream) * 2 +
-            (p.mine == 0 && p.us != sg.s0);
-        const uint32_t pr = static_cast<uint32_t>(a.part_rows);
-        __builtin_amdgcn_raw_buffer_store_b128(
-            __builtin_bit_cast(u32x4, acc),
-            make_rsrc_uniform(a.part_o + slot * pr * D, pr * D * 4), (r * D + dim) * 4, 0, kCpolSc1);
-        if (h0 + hh == 0 && sd == 0)
-          __builtin_amdgcn_raw_buffer_store_b64(
-              (u32x2){__builtin_bit_cast(uint32_t, mt), __builtin_bit_cast(uint32_t, lt)},
-              make_rsrc_uniform(a.part_ml + slot * pr * 2, pr * 8), r * 8, 0, kCpolSc1);
-      }
+    for (int w = 0; w < kD4Waves; ++w) {
+      const float f = fast_exp2(ml[w][0] - mu);
+      lt += f * ml[w][1];
+      acc += f * *(const lds_f32x4_t*)lds_ptr(at + w * G::kStage);
+    }
+    const int r = r0 + lr;
+    const int dim = G::dim(h0 + hh, sd);
+    if (cur.np == 1) {
+      // (0/0 -> NaN for a row with no key, as in 16 bits; otherwise lt >= 2^-8)
+      const float inv = __builtin_amdgcn_rcpf(lt);
+      *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.o) + cur.b * a.o_sb + head0 * a.o_sh +
+                                (q0 + r) * a.o_ss + dim) =
+          (u32x2){pack2<BF>(acc[0] * inv, acc[1] * inv), pack2<BF>(acc[2] * inv, acc[3] * inv)};
+    } else {
+      // the slot of this workgroup's piece (walk_slot, without its division)
+      const int64_t slot = (static_cast<int64_t>(seg_k) * a.walk_streams + stream) * 2 +
+                           (cur.mine == 0 && cur.us != sg.s0);
+      const uint32_t pr = static_cast<uint32_t>(a.part_rows);
+      __builtin_amdgcn_raw_buffer_store_b128(
+          __builtin_bit_cast(u32x4, acc),
+          make_rsrc_uniform(a.part_o + slot * pr * D, pr * D * 4), (r * D + dim) * 4, 0, kCpolSc1);
+      if (h0 + hh == 0 && sd == 0)
+        __builtin_amdgcn_raw_buffer_store_b64(
+            (u32x2){__builtin_bit_cast(uint32_t, mt), __builtin_bit_cast(uint32_t, lt)},
+            make_rsrc_uniform(a.part_ml + slot * pr * 2, pr * 8), r * 8, 0, kCpolSc1);
     }
   };
-  // A state that fits one area is left there, in the two areas by turns, and added
-  // up behind the next barrier: that of the next but one window's table, or the
-  // last one.  So a workgroup of two pieces, as most are, has none before its end.
-  const bool fits = RB == 1 && rows <= G::kAllRows;
-  const uint32_t area0 = lds_addr_of(stage), area1 = area0 + kD4Waves * G::kStage;
-  Left left = {0, 0, 0, 0};
-  int which = 0;             // the area that the next state goes to
-  bool added = false;
+  static_assert(kD4Threads / 16 >= 16 * kTwo, "one pass");
+  auto merge16 = [&](auto rbc) {
+    constexpr int rb = decltype(rbc)::value;
+    if (16 * rb >= rows) return;
+    const int n = min(rows - 16 * rb, 16);
+    auto phases = [&](auto h) {
+      constexpr int H = decltype(h)::value;
+      if (dirty) __syncthreads();
+      if constexpr (H == 0) put_stats(rbc);
+      if (l16 < n) {
+        const uint32_t at = wave * G::kStage + l16 * G::kPitch;
+        put_state(rbc, h, area0 + at);
+        if constexpr (G::kPH > 1) put_state(rbc, std::integral_constant<int, H + 1>{}, area1 + at);
+      }
+      __syncthreads();
+      add_up(16 * rb, n, H);
+      dirty = true;
+    };
+    phases(std::integral_constant<int, 0>{});
+    if constexpr (G::kPH > 2) phases(std::integral_constant<int, 2>{});
+  };
   // Cut units are counted when the workgroup is done: it has two at most, one
   // from each end of its segment.
-  Left cut[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  Cut cut[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 
   // This wave's first tile of a window: the tiles of consecutive windows go
   // round the waves without a gap, so that none gets more than its share.
@@ -885,63 +856,20 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
     int last[RB];  // last visible key of this lane's rows
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb)
-      last[rb] = causal ? min(cur.kb - 1, off + diag_row(a, q0 + 16 * rb + lrow)) : cur.kb - 1;
+      last[rb] = causal ? min(cur.kb - 1, off + diag_row(a, q0 + 16 * rb + l16)) : cur.kb - 1;
     const int full = causal ? min(cur.kb, off + 1) : cur.kb;
-    for (int n0 = cur.ka + turn * kD4Tile; n0 < cur.kb; n0 += kStep) {
-      // The two waves of a SIMD (i and i + 4) take turns in going first: left to
-      // itself, the older one finishes its share early and the other is alone.
-      if (((n0 / kStep) ^ (wave >> 2)) & 1)
-        __builtin_amdgcn_s_setprio(1);
-      else
-        __builtin_amdgcn_s_setprio(0);
+    for (int n0 = cur.ka + turn * kD4Tile; n0 < cur.kb; n0 += kStep)
       compute(n0, cur.kb, full, last);
-    }
     turn = turn_after(cur);
 
     const bool piece_end = cur.kb >= cur.kend;
     if (piece_end) {
       if (cur.np > 1) {
         cut[1] = cut[0];
-        cut[0] = Left{cur.b, cur.np, cur.us, cur.mine};
+        cut[0] = Cut{cur.b, cur.np, cur.us, cur.mine};
       }
-      using Zero = std::integral_constant<int, 0>;
-      if (fits) {
-        if (!has_next && added) __syncthreads();  // the area may still be read
-        put_stats(Zero{}, which);
-        if (l16 < rows) {
-          const uint32_t at = (which ? area1 : area0) + wave * G::kStage + l16 * G::kPitch;
-          put_state(Zero{}, Zero{}, at);
-          if constexpr (G::kPH > 1)
-            put_state(Zero{}, std::integral_constant<int, 1>{}, at + G::kAllRows * G::kPitch);
-          if constexpr (G::kPH > 2) {
-            put_state(Zero{}, std::integral_constant<int, 2>{}, at + 2 * G::kAllRows * G::kPitch);
-            put_state(Zero{}, std::integral_constant<int, 3>{}, at + 3 * G::kAllRows * G::kPitch);
-          }
-        }
-        if (has_next) left = Left{cur.b, cur.np, cur.us, cur.mine};
-        which ^= 1;
-      } else {  // two phases at a time, one in each area
-        auto merge16 = [&](auto rbc) {
-          constexpr int rb = decltype(rbc)::value;
-          if (16 * rb >= rows) return;
-          const int n = min(rows - 16 * rb, 16);
-          put_stats(rbc, 0);
-          auto phases = [&](auto h) {
-            constexpr int H = decltype(h)::value;
-            const uint32_t at = wave * G::kStage + l16 * G::kPitch;
-            put_state(rbc, h, area0 + at);
-            if constexpr (G::kPH > 1) put_state(rbc, std::integral_constant<int, H + 1>{}, area1 + at);
-            __syncthreads();
-            add_up(Left{cur.b, cur.np, cur.us, cur.mine}, area0, 0, 16 * rb, n, H,
-                   G::kPH > 1 ? 2 : 1, area1 - area0);
-            __syncthreads();
-          };
-          phases(Zero{});
-          if constexpr (G::kPH > 2) phases(std::integral_constant<int, 2>{});
-        };
-        merge16(Zero{});
-        if constexpr (RB > 1) merge16(std::integral_constant<int, 1>{});
-      }
+      merge16(std::integral_constant<int, 0>{});
+      if constexpr (RB > 1) merge16(std::integral_constant<int, 1>{});
     }
     if (!has_next) break;
     if (piece_end) {
@@ -966,12 +894,7 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
       // wave reads since the last barrier)
       put_entry(entry, buf_after(1));
       __syncthreads();
-      if (left.np) {
-        add_up(left, which ? area0 : area1, which ^ 1, 0, rows, 0, G::kPH,
-               G::kAllRows * G::kPitch);
-        left.np = 0;
-        added = true;
-      }
+      dirty = false;
       has_nn = next_window(nxt, nn);
       entry = has_nn ? fetch_entry(nn) : 0;
       if constexpr (kAhead)
@@ -984,16 +907,6 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
   uint64_t word = 0;
   if ((tid == 0 && cut[0].np) || (tid == 64 && cut[1].np))
     word = merge_word(a, cut[tid ? 1 : 0].b * a.walk_streams + stream);
-  if (fits) {
-    __syncthreads();
-    // (the last state went to area which ^ 1, one left before it to the other)
-#pragma unroll 1
-    for (int u = left.np ? 0 : 1; u < 2; ++u) {
-      const Left p = u ? Left{cur.b, cur.np, cur.us, cur.mine} : left;
-      const int mi = u ? which ^ 1 : which;
-      add_up(p, mi ? area1 : area0, mi, 0, rows, 0, G::kPH, G::kAllRows * G::kPitch);
-    }
-  }
   if (cut[0].np == 0) return;
   merge_publish();
   __syncthreads();
@@ -1005,7 +918,7 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
   __syncthreads();
 #pragma unroll 1
   for (int i = 0; i < 2; ++i) {
-    const Left c = i ? cut[1] : cut[0];
+    const Cut c = i ? cut[1] : cut[0];
     if (c.np == 0 || *static_cast<volatile int*>(&merge_flag[i]) == 0) continue;
     if (i) __syncthreads();
     merge_pieces<DT, D, kD4Threads, 16 * RB>(

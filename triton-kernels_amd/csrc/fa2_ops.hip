@@ -148,6 +148,7 @@ int fp4_rows(const fa2_fp4_rows_params* p, void* stream, bool append) {
 // The balanced walk's costs, in KV tiles of 64 keys (see fa2_decode_walk.h)
 constexpr int64_t kD4MinTiles = 4;
 constexpr int64_t kD4GridTiles = 2;
+constexpr int64_t kD4Wide = 24;
 constexpr int64_t kD4Whole = 24, kD4Short = 12;
 
 struct Fp4Plan {
@@ -188,19 +189,23 @@ int validate_fp4_decode(const fa2_fp4_decode_params* p) {
 int fp4_plan(const fa2_fp4_decode_params* p, Fp4Plan* pl) {
   pl->rows = p->q_heads / p->kv_heads * p->q_len;
   if (pl->rows > kLim) return FA2_ERR_TOO_LARGE;
-  // q-blocks of 16 rows, or of 32 where the accumulators leave room for the tiles
-  // in flight
-  pl->rb = pl->rows <= 16 || p->head_dim == 256 ? 1 : 2;
-  const int64_t nqb = cdiv(pl->rows, 16 * pl->rb);
-  pl->part_rows = std::min<int64_t>(pl->rows, 16 * pl->rb);
-  pl->streams = p->kv_heads * nqb;
   const int64_t wgs = cu_count_current_device();
   const int64_t tiles = std::max<int64_t>(cdiv(p->table_width * p->page_size, kBN), 1);
   const int64_t total = tiles * p->batch;  // (at most: lengths are on the device)
+  if (total >= (int64_t(1) << 30)) return FA2_ERR_TOO_LARGE;
+  // More than 16 rows: q-blocks of 32 share K and V, q-blocks of 16 have less to add up
+  // and twice the units to fill the card with.  32 where the tables hold kD4Wide tiles per
+  // workgroup (D = 256 has no registers for it): 20 rows x 8 kv heads of D128, 16 / 32
+  // rows a block, 11 / 15 us for 4 x 1000 keys, 17 / 21 for 16 x 2048 (16 tiles), 40 /
+  // 37 for 32 x 1000-3000 (47), 54 / 48 for 16 x 8192 (64).
+  const bool wide = p->head_dim <= 128 && pl->rows > 16 && total * p->kv_heads > kD4Wide * wgs;
+  pl->rb = wide ? 2 : 1;
+  const int64_t nqb = cdiv(pl->rows, 16 * pl->rb);
+  pl->part_rows = std::min<int64_t>(pl->rows, 16 * pl->rb);
+  pl->streams = p->kv_heads * nqb;
   pl->segs = std::min(std::max<int64_t>(1, wgs / pl->streams), cdiv(total, kD4GridTiles));
   const int64_t part_bytes = 2 * pl->streams * pl->segs * pl->part_rows * p->head_dim * 4;
-  if (total >= (int64_t(1) << 30) || part_bytes >= (int64_t(1) << 31) ||
-      pl->streams * p->batch > kLim)
+  if (part_bytes >= (int64_t(1) << 31) || pl->streams * p->batch > kLim)
     return FA2_ERR_TOO_LARGE;
   const int64_t grid = pl->streams * pl->segs;
   const int64_t idle = std::max<int64_t>(0, grid - pl->streams * p->batch);
@@ -222,19 +227,13 @@ bool fp4_empty(const fa2_fp4_decode_params* p) { return p->batch == 0 || p->q_le
 template <int DT, int D, bool BLOCKS>
 void launch_fp4_decode(const Fp4Args& a, int rb, uint32_t grid, hipStream_t st) {
   const dim3 block(kD4Threads);
-  // (up to 8 rows take the 16 columns twice; at D = 256 registers do not reach)
-  const bool half = D <= 128 && rb == 1 && a.a.q_len <= 8;
-  if (rb == 1 && !half)
-    hipLaunchKernelGGL((fa2_decode_fp4_kernel<DT, D, 1, false, BLOCKS>), dim3(grid), block, 0, st,
-                       a);
   if constexpr (D <= 128) {
-    if (half)
-      hipLaunchKernelGGL((fa2_decode_fp4_kernel<DT, D, 1, true, BLOCKS>), dim3(grid), block, 0, st,
-                         a);
-    if (rb == 2)
-      hipLaunchKernelGGL((fa2_decode_fp4_kernel<DT, D, 2, false, BLOCKS>), dim3(grid), block, 0, st,
-                         a);
+    if (rb == 2) {
+      hipLaunchKernelGGL((fa2_decode_fp4_kernel<DT, D, 2, BLOCKS>), dim3(grid), block, 0, st, a);
+      return;
+    }
   }
+  hipLaunchKernelGGL((fa2_decode_fp4_kernel<DT, D, 1, BLOCKS>), dim3(grid), block, 0, st, a);
 }
 
 template <int DT, int D>
