@@ -66,11 +66,12 @@ int fa2_norm_rope(const fa2_norm_rope_params* p, void* stream);
  *
  * codes  uint8 [num_pages, kv_heads, page_size, head_dim / 2]
  * scales uint8 [num_pages, kv_heads, page_size, head_dim / 32]
- * both contiguous, the scales from a 4-byte boundary; head_dim 64, 128 or 256.  Value d of a row is nibble d % 2 (0:
- * low) of byte d / 2, an E2M1 number (sign, two exponent bits, one mantissa bit: 0
- * .5 1 1.5 2 3 4 6), times 2^(scale - 127) of its block d / 32; scale 255 is
- * NaN.  (OCP MX FP4 with blocks of 32.)  Logical row n of sequence b is row n %
- * page_size of page table[b][n / page_size].
+ * both contiguous, the scales from a 4-byte boundary; head_dim 64, 128 or 256; a
+ * page's codes less than 2^30 bytes.  Value d of a row is nibble d % 2 (0: low) of byte
+ * d / 2, an E2M1 number (sign, two exponent bits, one mantissa bit: 0 .5 1 1.5 2 3 4
+ * 6), times 2^(scale - 127) of its block d / 32; scale 255 is NaN.  (OCP MX FP4
+ * with blocks of 32.)  Logical row n of sequence b is row n % page_size of page
+ * table[b][n / page_size].
  *
  * The writer gives a block the least power of two at which its largest value is
  * at most 6 after rounding, kept between 2^-23 and 2^13 for fp16 rows and 2^-100

@@ -89,6 +89,14 @@ def test_rows_refusals(entry, kw, code):
     assert rows(entry, **kw) == code
 
 
+@pytest.mark.parametrize("entry", ["fa2_fp4_append", "fa2_fp4_gather"])
+@pytest.mark.parametrize("kw", [dict(page_size=2 ** 23), dict(kv_heads=2 ** 25),
+                                dict(kv_heads=2 ** 62), dict(kv_heads=2 ** 14, page_size=2 ** 11)])
+def test_rows_pages_past_31_bits(entry, kw):
+    """Offsets inside a page are 32-bit: larger pages are refused."""
+    assert rows(entry, **kw) == 13
+
+
 def test_rows_nothing_to_do():
     assert rows(batch=0) == 0 and rows(num_rows=0) == 0
     assert _ops.lib().fa2_fp4_append(None, None) == 1

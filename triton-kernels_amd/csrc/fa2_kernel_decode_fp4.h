@@ -8,17 +8,15 @@
 // of them per instruction at full rate, scale included: the kernel computes what
 // the 16-bit decode kernel computes on the cache's values.
 //   * Workgroup = 8 waves, one per CU, over an equal share of the call's KV
-//     tiles (fa2_decode_walk.h).  A wave walks tiles of 32 keys, tile i of
-//     the workgroup's range to wave i % 8, and keeps its own (m, l, O).
+//     tiles (fa2_decode_walk.h; kernel comment below).  A wave walks tiles of 32
+//     keys, tile i of the workgroup's range to wave i % 8, and keeps its own (m, l,
+//     O); they are added up in LDS at a piece's end.
 //   * A page's rows of a kv head are contiguous.  Direct-to-LDS loads of whole
 //     rows bring a tile per wave, across the ends of the pieces; its codes are
 //     read into registers at once (they are few) and the next tile is on its way
 //     while it is computed.  (Tiles in flight in registers instead need the loop
-//     once per tile: 50 KB of code.  More tiles in flight in LDS gain nothing: the
-//     first burst takes the longer, D128 49.3 / 47.1 / 46.4 us at 3 / 2 / 1 for 16 x
-//     16000-32768 keys, and each wait has to count them.)
-//   * What bounds the loop is its instructions: with all keys in one page, in L2, the
-//     calls take 10 % less.  So the tile loop has next to no branches in its way.
+//     once per tile: 50 KB of code.  More tiles in flight in LDS gain nothing: 49.3
+//     / 47.1 / 46.4 us at 3 / 2 / 1 for 16 x 16000-32768 keys of 4 heads of D128.)
 //   * S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32, up to 16 RB rows
 //     of the unit as columns.  A lane expands D / 4 dims of a key of K, in the
 //     layout of the MFMA's A operand (lane: row l % 16, dims D / 4 * (l / 16)
@@ -28,12 +26,17 @@
 //     through LDS in 16 bits, for transpose reads, took two thirds of the LDS
 //     time, and that 75 % of a tile's.)
 //   * P goes to the MFMA as the sum of two 16-bit values, high and low part, so
-//     that the weights carry 16 to 22 bits: the MFMAs have the time (a CU's
-//     share of the HBM rate is one tile of 4.3 KB in 440 cycles, of which 24
-//     MFMAs on four SIMDs take 100), and the output is then off by its own
-//     rounding alone.
+//     that the weights carry 16 to 22 bits and the output is off by its own rounding
+//     alone; the low parts cost 5 % of a long call.
 //   * Running maxima and sums in fp32, raised only when a score passes the
 //     maximum by 2^8, as in the 16-bit kernels.
+// Measured on MI355X, us (and the cache's bytes per s): 64 sequences of 512-8192 keys,
+// 32 / 8 heads of D128, 66 (4.6 TB/s); 16 of 16000-32768, 32 / 4 heads, 45 (4.6); 16 of
+// 8200 with 8 drafts, 8 / 8 heads of D64, 27 (2.7); 33 of 100-4096 with 5 drafts, 16 / 4
+// heads, 21 (1.6); 4 of 1023, 10.5.  The 16-bit decode reads 6.1 TB/s.  The long calls are
+// bound by the loop's instructions as much as by memory (10 % less with every page in
+// L2); the short ones by what a workgroup does once: 3 us until its first tile is
+// there, about 2 us per change of units, 4 us to count and merge cut units.
 #pragma once
 
 #include "fa2_decode_walk.h"
@@ -201,6 +204,19 @@ __device__ __forceinline__ int wave_scan(int x) {
   return x;
 }
 
+// The walk here, for batches of up to 64 sequences (their lengths are in the lanes; longer
+// batches take the walk as it is):
+//   * Units start at segments where that makes segments at most kAlign tiles longer:
+//     then a workgroup has one piece.
+//   * Otherwise a unit takes kGap tiles of room in its stream besides its own, what a
+//     change of units costs, so that workgroups with several have fewer tiles.
+// Neither / the second alone / both, us: 33 x 100-4096 keys with 5 drafts of 16 / 4 heads
+// 32.8 / 25.2 / 21.4; 16 x 4096-8192 of 32 / 2 heads 22.8 / 21.5 / 17.5; 16 x 8200 with 8
+// drafts of 8 / 8 heads of D64 30.5 / 27.6 / 27.2.  kAlign 4 to 16 and kGap 3 to 8 are within 2 %
+// for 16 rows; for 32 rows (8, 6), (12, 8), (16, 8), (24, 4) take 22.2, 21.3, 22.0, 23.8.
+//
+// BLOCKS: pages of whole blocks of 16 rows, whose addresses are found once per block
+// instead of once per row: 64 x 512-8192 keys in pages of 16 take 71 us, 75.5 without.
 template <int DT, int D, int RB, bool BLOCKS>
 __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
     Fp4Args fa) {
@@ -211,7 +227,7 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
   constexpr int kStep = kD4Tile * kD4Waves;
   constexpr int kSub = D == 256 ? 2 : 1;  // scales of a lane's dims
   static_assert(kD4Waves * G::kStage >= kMergePieceBytes<kD4Threads>, "merge area");
-  constexpr int kAlign = RB == 1 ? 8 : 12, kGap = RB == 1 ? 5 : 8;
+  constexpr int kAlign = RB == 1 ? 8 : 12, kGap = RB == 1 ? 5 : 8;  // tiles
 
   __shared__ __attribute__((aligned(1024))) char tiles[kD4Waves * G::kTile];
   __shared__ __attribute__((aligned(128))) char stage[2 * kD4Waves * G::kStage];
@@ -240,8 +256,8 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
   const bool in_lanes = a.batch <= 64;
   const int lens = in_lanes && lane < a.batch ? walk_len<MODE>(a, lane) : 0;
   DecSegment sg;
-  int room = 0;  // what a unit takes of the stream (in_lanes)
-  int gap = 0;
+  int room = 0;  // in_lanes: what the lane's unit takes of its stream (0: no unit)
+  int gap = 0;   // ... and of that, ahead of its tiles
   if (in_lanes) {
     const int W = lane < a.batch ? walk_weight(lens) : 0;
     int total = __builtin_amdgcn_readlane(wave_scan<false>(W), 63);
@@ -253,6 +269,7 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
       bool fit = false;
       if (a.batch <= a.walk_segs) {
         for (int c = C; c <= C + kAlign && !fit; c += kAlign / 2) {
+          // n = ceil(W / c): a first guess off by one at most, put right
           const float inv = __builtin_amdgcn_rcpf(static_cast<float>(c));
           int n = static_cast<int>(static_cast<float>(W) * inv);
           n += n * c < W;
@@ -297,7 +314,8 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
   // window of it: keys [ka, kb), all of it unless its block-table entries exceed
   // the LDS table.
   struct Window {
-    int b, us, W, room, Lk;   // sequence, the unit's start in the stream, weight, length
+    // sequence, its tiles' start in the stream and number, its room, its length
+    int b, us, W, room, Lk;
     int np, mine;       // pieces of the unit, this one's index
     int ka, kb, kend;   // kend: the piece's end
     int page0;          // first logical page
@@ -538,7 +556,7 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
   const uint32_t vbyte = D == 64 ? l16 >> 3 : D == 128 ? l16 >> 2 : (l16 >> 1) & 3;
   const uint32_t vrot = (8 * vbyte + 9) & 31;  // ... turned to a float's exponent
 
-  // The oldest tile of the ring, at key n0; kb: the window's end, full: no key
+  // This wave's tile, at key n0; kb: the window's end, full: no key
   // below it is hidden from any row, last: the last key that the lane's rows see.
   auto compute = [&](int n0, int kb, int full, const int (&last)[RB]) {
     const bool edge = n0 + kD4Tile > full;
@@ -858,8 +876,16 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
     for (int rb = 0; rb < RB; ++rb)
       last[rb] = causal ? min(cur.kb - 1, off + diag_row(a, q0 + 16 * rb + l16)) : cur.kb - 1;
     const int full = causal ? min(cur.kb, off + 1) : cur.kb;
-    for (int n0 = cur.ka + turn * kD4Tile; n0 < cur.kb; n0 += kStep)
+    for (int n0 = cur.ka + turn * kD4Tile; n0 < cur.kb; n0 += kStep) {
+      // The two waves of a SIMD (i and i + 4) take turns in going first: left to
+      // itself, the older one finishes its share early and the other is alone (4 x
+      // 300-600 keys 7.8 -> 7.5 us, 16 x 8200 with drafts 27.7 -> 27.3).
+      if (((n0 / kStep) ^ (wave >> 2)) & 1)
+        __builtin_amdgcn_s_setprio(1);
+      else
+        __builtin_amdgcn_s_setprio(0);
       compute(n0, cur.kb, full, last);
+    }
     turn = turn_after(cur);
 
     const bool piece_end = cur.kb >= cur.kend;

@@ -80,7 +80,8 @@ int validate_rows(const fa2_fp4_rows_params* p) {
       p->num_pages < 0 || p->table_width < 0 || p->k_table_stride < 0 || p->v_table_stride < 0)
     return FA2_ERR_BAD_SHAPE;
   if (p->batch > kLim || p->num_rows > kLim || p->page_size > kLim || p->num_pages > kLim ||
-      p->table_width > kLim || p->kv_heads * (p->head_dim / 8) > kLim)
+      p->table_width > kLim || p->kv_heads > kLim / (p->head_dim / 2) ||
+      p->page_size > kLim / (p->kv_heads * (p->head_dim / 2)))  // (a page's bytes: 31 bits)
     return FA2_ERR_TOO_LARGE;
   const int eb = elt_bytes(p->dtype);
   const int64_t strides[] = {p->k_ts, p->k_hs, p->v_ts, p->v_hs};
@@ -145,11 +146,18 @@ int fp4_rows(const fa2_fp4_rows_params* p, void* stream, bool append) {
   return launched();
 }
 
-// The balanced walk's costs, in KV tiles of 64 keys (see fa2_decode_walk.h)
+// The balanced walk's costs, in KV tiles of 64 keys (fa2_decode_walk.h).  A segment of
+// cut units has kD4MinTiles at least (2 instead of 4: 1 x 1023 keys of 8 kv heads 11.0 /
+// 11.3 us, 4 x 1023 12.3 / 11.7); the grid has a workgroup per kD4GridTiles at most (2 or
+// 4: the same).  Units stay whole where that costs at most kD4Whole tiles, in proportion
+// to the CUs that whole units leave idle and half of it at least, or they have kD4Short
+// at most.  Whole / cut (with 8 and 4 in their place), us, 8 kv heads of D128: 1 x 1023 keys 10.3
+// / 11.3, 8 x 700 9.4 / 11.5, 16 x 500-1000 10.8 / 13.2, 16 x 1500 13.2 / 14.5, 32 x
+// 1000-2000 17.2 / 17.8, 8 x 1500 12.9 / 12.3.
 constexpr int64_t kD4MinTiles = 4;
 constexpr int64_t kD4GridTiles = 2;
-constexpr int64_t kD4Wide = 24;
 constexpr int64_t kD4Whole = 24, kD4Short = 12;
+constexpr int64_t kD4Wide = 24;  // (fp4_plan)
 
 struct Fp4Plan {
   int64_t rows;        // of a unit: Hq / Hkv * q_len
