@@ -202,11 +202,14 @@ int fp4_plan(const fa2_fp4_decode_params* p, Fp4Plan* pl) {
   const int64_t total = tiles * p->batch;  // (at most: lengths are on the device)
   if (total >= (int64_t(1) << 30)) return FA2_ERR_TOO_LARGE;
   // More than 16 rows: q-blocks of 32 share K and V, q-blocks of 16 have less to add up
-  // and twice the units to fill the card with.  32 where the tables hold kD4Wide tiles per
-  // workgroup (D = 256 has no registers for it): 20 rows x 8 kv heads of D128, 16 / 32
-  // rows a block, 11 / 15 us for 4 x 1000 keys, 17 / 21 for 16 x 2048 (16 tiles), 40 /
-  // 37 for 32 x 1000-3000 (47), 54 / 48 for 16 x 8192 (64).
-  const bool wide = p->head_dim <= 128 && pl->rows > 16 && total * p->kv_heads > kD4Wide * wgs;
+  // (D = 256 has no registers for 32).  16 where every unit of them still has a workgroup
+  // and the tables hold kD4Wide tiles per workgroup at most.  20 rows of D128, q-blocks
+  // of 16 / 32, us: 8 kv heads, 4 x 1000 keys 11 / 15, 16 x 2048 (256 units, 16 tiles) 17 /
+  // 21, 16 x 8192 (64 tiles) 54 / 48, 32 x 1000-3000 (512 units) 40 / 37; 4 kv heads, 33 x
+  // 100-2000 (264 units, 17 tiles) 22 / 19.
+  const bool wide = p->head_dim <= 128 && pl->rows > 16 &&
+                    (p->batch * p->kv_heads * cdiv(pl->rows, 16) > wgs ||
+                     total * p->kv_heads > kD4Wide * wgs);
   pl->rb = wide ? 2 : 1;
   const int64_t nqb = cdiv(pl->rows, 16 * pl->rb);
   pl->part_rows = std::min<int64_t>(pl->rows, 16 * pl->rb);
