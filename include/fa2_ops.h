@@ -132,7 +132,7 @@ typedef struct fa2_fp4_decode_params {
   const int32_t* v_block_table;
   float softmax_scale;
   int32_t reserved0;
-  void* workspace;          /* any prior content; one per call in flight        */
+  void* workspace;          /* 16-byte aligned, any prior content; one per call in flight */
   size_t workspace_bytes;
 } fa2_fp4_decode_params;
 

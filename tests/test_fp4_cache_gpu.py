@@ -252,3 +252,91 @@ def test_ctypes_path_stream_and_graph():
         rows = m.paged_kv_gather_fp4(*want, kt, vt, ip, T)
         torch.cuda.synchronize()
         assert torch.equal(held[0], rows[0]) and torch.equal(held[1], rows[1])
+
+
+@pytest.mark.parametrize("bad", ["codes", "scales", "ctype", "contiguous", "v", "v_table", "v_rows",
+                                 "tables", "start", "rtype", "rows", "mixed", "device", "count"])
+def test_refusals(bad):
+    """The same error with and without the extension, before any launch."""
+    import kernels.fp4_cache as m
+    H, D, page, lens = 2, 64, 16, [3, 20]
+    T = sum(lens)
+    kt, vt, pages = tables(lens, page, 5)
+    kt, vt, ip = kt.cuda(), vt.cuda(), indptr(lens).cuda()
+    k, v = (rows_of(T, H, D, torch.bfloat16, s).cuda() for s in (6, 7))
+    kc, vc = (m.allocate_fp4_cache(pages, page, H, D) for _ in range(2))
+    sp, count, gather = torch.zeros(2, dtype=torch.int32, device="cuda"), T, True
+    if bad == "codes":
+        vc = m.allocate_fp4_cache(pages, page, H, 128)
+    elif bad == "scales":
+        kc = (kc.codes, kc.scales[..., :1].contiguous())
+    elif bad == "ctype":
+        kc = (kc.codes.char(), kc.scales)
+    elif bad == "contiguous":
+        kc = (kc.codes.transpose(1, 2), kc.scales.transpose(1, 2))
+    elif bad == "v":
+        vc = None
+    elif bad == "v_table":
+        vt = None
+    elif bad == "v_rows":
+        v, gather = None, False
+    elif bad == "tables":
+        kt = kt[:1]
+    elif bad == "start":
+        sp = sp[:1]
+    elif bad == "rtype":
+        k, v, gather = k.double(), v.double(), False
+    elif bad == "rows":
+        k, v, gather = k[:, :1], v[:, :1], False
+    elif bad == "mixed":
+        v, gather = v.float(), False
+    elif bad == "device":
+        ip = ip.cpu()
+    else:
+        count = -1
+    calls = [lambda: m.paged_kv_gather_fp4(kc, vc, kt, vt, ip, count, sp)] if gather else []
+    if bad != "count":
+        calls.append(lambda: m.paged_kv_append_fp4(kc, vc, kt, vt, k, v, ip, sp))
+    for call in calls:
+        seen = []
+        for use in (True, False):
+            m.USE_EXT = use
+            try:
+                with pytest.raises((ValueError, TypeError, AssertionError)) as e:
+                    call()
+                seen.append((e.type, str(e.value)))
+            finally:
+                m.USE_EXT = True
+        assert seen[0] == seen[1]
+    torch.cuda.synchronize()
+
+
+def test_gather_into_tensors():
+    """Into given tensors; rows that no sequence holds stay as they were, and tensors
+    that do not fit are refused."""
+    import kernels.fp4_cache as m
+    H, D, page, lens = 3, 64, 16, [5, 0, 33]
+    T, ahead, behind = sum(lens), 2, 3
+    kt, vt, pages = tables(lens, page, 5)
+    kt, vt, ip = kt.cuda(), vt.cuda(), indptr(lens).cuda()
+    k, v = (rows_of(T, H, D, torch.float16, s).cuda() for s in (6, 7))
+    kc, vc = (m.allocate_fp4_cache(pages, page, H, D) for _ in range(2))
+    m.paged_kv_append_fp4(kc, vc, kt, vt, k, v, ip)
+    n = ahead + T + behind
+    for use in (True, False):
+        m.USE_EXT = use
+        try:
+            out = tuple(torch.full((n, H, D), 7.0, dtype=torch.float16, device="cuda")
+                        for _ in range(2))
+            got = m.paged_kv_gather_fp4(kc, vc, kt, vt, ip + ahead, n, out=out)
+            assert got[0] is out[0] and got[1] is out[1]
+            for x, rows in zip(got, (k, v)):
+                assert (x[:ahead] == 7).all() and (x[ahead + T:] == 7).all()
+                assert torch.equal(x[ahead:ahead + T].cpu().double(), R.quantize(rows.cpu())[0])
+            for bad in ((out[0][:-1], out[1]), (out[0], out[1].float()), (out[0], None),
+                        (out[0].transpose(0, 1).contiguous().transpose(0, 1), out[1]),
+                        (out[0].int(), out[1].int()), (out[0].cpu(), out[1])):
+                with pytest.raises((ValueError, TypeError, AssertionError)):
+                    m.paged_kv_gather_fp4(kc, vc, kt, vt, ip + ahead, n, out=bad)
+        finally:
+            m.USE_EXT = True

@@ -162,3 +162,59 @@ def test_table_of_far_positions():
         a = p * 10000.0 ** (-2 * i / 64)
         assert abs(t[p, i].item() - math.cos(a)) <= 2 ** -24 + 1e-9
         assert abs(t[p, 32 + i].item() - math.sin(a)) <= 2 ** -24 + 1e-9
+
+
+@pytest.mark.parametrize("bad", ["dtype", "mixed", "dim", "dims", "tokens", "weight", "wtype",
+                                 "wmixed", "positions", "ptype", "table", "ttype", "wide", "odd",
+                                 "eps", "device"])
+def test_refusals(bad):
+    """The same error with and without the extension, before any launch."""
+    import kernels.norm_rope as m
+    q, k, qw, kw, _ = data(6, 4, 2, 64, torch.float16, 31)
+    q, k, qw, kw = (t.cuda() for t in (q, k, qw, kw))
+    table = m.build_rope_table(16, 64, device="cuda")
+    pos = torch.arange(6, device="cuda")
+    kwargs = {}
+    if bad == "dtype":
+        q, k = q.double(), k.double()
+    elif bad == "mixed":
+        k = k.float()
+    elif bad == "dim":
+        q, k, qw, kw = (t[..., :48] for t in (q, k, qw, kw))
+    elif bad == "dims":
+        q = q[0]
+    elif bad == "tokens":
+        k = k[:5]
+    elif bad == "weight":
+        kw = kw[:32]
+    elif bad == "wtype":
+        qw, kw = qw.bfloat16(), kw.bfloat16()
+    elif bad == "wmixed":
+        kw = kw.float()
+    elif bad == "positions":
+        pos = pos[:5]
+    elif bad == "ptype":
+        pos = pos.short()
+    elif bad == "table":
+        table = table[0]
+    elif bad == "ttype":
+        table = table.half()
+    elif bad == "wide":
+        table = m.build_rope_table(16, 128, device="cuda")
+    elif bad == "odd":
+        table = table[:, :24]
+    elif bad == "eps":
+        kwargs["eps"] = -1e-6
+    else:
+        pos = pos.cpu()
+    seen = []
+    for use in (True, False):
+        m.USE_EXT = use
+        try:
+            with pytest.raises((ValueError, TypeError, AssertionError)) as e:
+                m.qk_norm_rope(q, k, qw, kw, table, pos, **kwargs)
+            seen.append((e.type, str(e.value)))
+        finally:
+            m.USE_EXT = True
+    assert seen[0] == seen[1]
+    torch.cuda.synchronize()

@@ -146,6 +146,11 @@ def test_decode_pointer_refusals(kw, code):
     assert _ops.lib().fa2_fp4_decode(ctypes.byref(p), None) == code
 
 
+def test_decode_workspace_off_16_bytes():
+    p = decode_params(workspace=0x1008, workspace_bytes=1 << 30)
+    assert _ops.lib().fa2_fp4_decode(ctypes.byref(p), None) == 7
+
+
 def test_decode_workspace_and_nothing_to_do():
     n = ctypes.c_size_t(0)
     size = lambda p: (_ops.lib().fa2_fp4_decode_workspace_size(ctypes.byref(p), ctypes.byref(n)),

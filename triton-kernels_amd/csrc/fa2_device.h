@@ -1086,7 +1086,8 @@ __device__ __forceinline__ bool merge_arrive(const KArgs& a, int unit, int S, ui
 }
 
 __device__ __forceinline__ bool merge_count(const KArgs& a, int unit, int S, int* flag) {
-  if (threadIdx.x == 0) *static_cast<volatile int*>(flag) = merge_arrive(a, unit, S, merge_word(a, unit)) ? 1 : 0;
+  if (threadIdx.x == 0)
+    *static_cast<volatile int*>(flag) = merge_arrive(a, unit, S, merge_word(a, unit)) ? 1 : 0;
   __syncthreads();
   // (the partials are read after this, at device scope: the count that made
   // this split the last was taken after every split's stores were performed)

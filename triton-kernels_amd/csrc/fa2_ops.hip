@@ -377,6 +377,7 @@ extern "C" int fa2_fp4_decode(const fa2_fp4_decode_params* p, void* stream) {
   s = fp4_plan(p, &pl);
   if (s != FA2_OK) return s;
   if (!p->workspace || p->workspace_bytes < pl.total) return FA2_ERR_WORKSPACE;
+  if (!aligned16(p->workspace)) return FA2_ERR_ALIGNMENT;
 
   Fp4Args fa{};
   KArgs& a = fa.a;

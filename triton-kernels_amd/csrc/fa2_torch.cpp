@@ -326,7 +326,8 @@ bool norm_rope_ok(const at::Tensor& q, const at::Tensor& k, const at::Tensor& qw
   if ((q.dim() != 3 && q.dim() != 4) || (k.dim() != 3 && k.dim() != 4)) return false;
   const auto dt = q.scalar_type();
   const int64_t D = q.size(-1);
-  return real_type(dt) && k.scalar_type() == dt && k.size(-1) == D &&
+  return real_type(dt) && (D == 16 || D == 32 || D == 64 || D == 128 || D == 256) &&
+         k.scalar_type() == dt && k.size(-1) == D &&
          tokens_of(k) == tokens_of(q) && qw.dim() == 1 && kw.dim() == 1 && qw.size(0) == D &&
          kw.size(0) == D && qw.scalar_type() == kw.scalar_type() &&
          (qw.scalar_type() == dt || qw.scalar_type() == at::kFloat) &&
