@@ -340,3 +340,22 @@ def test_gather_into_tensors():
                     m.paged_kv_gather_fp4(kc, vc, kt, vt, ip + ahead, n, out=bad)
         finally:
             m.USE_EXT = True
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gather_past_the_caches(dtype):
+    """More than 2^28 bytes of rows (sequences that share their pages)."""
+    from kernels import allocate_fp4_cache, paged_kv_append_fp4, paged_kv_gather_fp4
+    H, D, page, n = 8, 128, 16, 1001
+    seqs = (1 << 28) // (n * H * D * 2 * dtype.itemsize) + 2
+    kt, vt, pages = tables([n], page, 5)
+    kt, vt = kt.cuda(), vt.cuda()
+    k, v = (rows_of(n, H, D, dtype, s).cuda() for s in (6, 7))
+    kc, vc = (allocate_fp4_cache(pages, page, H, D) for _ in range(2))
+    paged_kv_append_fp4(kc, vc, kt, vt, k, v, indptr([n]).cuda())
+    want = paged_kv_gather_fp4(kc, vc, kt, vt, indptr([n]).cuda(), n, dtype=dtype)
+    assert torch.equal(want[0].cpu().double(), R.quantize(k.cpu())[0])
+    got = paged_kv_gather_fp4(kc, vc, kt.expand(seqs, -1), vt.expand(seqs, -1).contiguous(),
+                              indptr([n] * seqs).cuda(), n * seqs, dtype=dtype)
+    for x, w in zip(got, want):
+        assert torch.equal(x.view(seqs, n, H, D), w.expand(seqs, -1, -1, -1))

@@ -13,15 +13,17 @@
 // Both are copies bound by HBM: rows are touched once in 16 or 32 bits and once
 // in 4.25.  A thread takes 8 values (a code word), four neighbouring lanes a block:
 // its maximum is two quad exchanges.  Rows are located as in fa2_kv_append.h:
-// indptr in LDS, one lane per row; then a thread goes down the rows at a column of
-// its own, four at a time.  The cache's side goes in whole blocks: lane i of a quad
+// indptr and the starts in LDS, one lane per row; a thread takes a column of its own of
+// four rows, which the writer loads before their places are known (64 rows 8.8 -> 8.2 us
+// with the reader after it).  The cache's side goes in whole blocks: lane i of a quad
 // moves the four words of the block in row i, and a 4 x 4 transpose within the quad
 // (DPP) turns them from or into a word of each row.  (A word and a scale byte per
 // lane and row takes three memory instructions for each KB of rows, not 1.5.)
-// Measured on MI355X: 139k rows of 8 heads of D128 bf16 gathered in 178 us that way,
-// 151 this way (5.36 TB/s; a copy of 1 GiB 5.05), 8.6k rows appended in 15.5 / 15.0
-// (3.7 TB/s), 64 rows in 4.8.  Workgroups of four rows per thread; of 8 / 12 / 16: 154 /
-// 162 / 163 us for the first.  The gathered rows are stored non-temporally (211 -> 197).
+// Measured on MI355X, 8 heads of D128 bf16: 139 k rows gathered in 141 us (5.7 TB/s; a copy
+// of 1 GiB 5.05; word by word 178), 10.7 k rows appended in 14.7 and gathered in 12 (3.8 and
+// 4.6 TB/s: one latency after another, all workgroups at once), 64 rows in 5.0 and 4.7.
+// Workgroups of 8 / 12 / 16 rows per thread took 154 / 162 / 163 us for the first instead
+// of 151.  The gathered rows are stored non-temporally (211 -> 197).
 #pragma once
 
 #include "fa2_device.h"
@@ -42,7 +44,7 @@ struct Fp4RowsArgs {
   const int32_t* indptr;
   const int32_t* start;  // may be null: every sequence starts at 0
   int32_t batch, heads, words, num_rows, page_size, page_shift, num_pages, table_width;
-  int32_t block_rows;    // rows per workgroup, <= kF4Rows
+  int32_t block_rows;    // rows per workgroup: 4 * rows_at_once, <= kF4Rows
   int32_t rows_at_once;  // rows that the workgroup's threads cover, one word each
   int32_t word_shift;    // log2 of the code words of a head
   int32_t has_v;
@@ -76,16 +78,31 @@ __device__ __forceinline__ uint32_t quad_lane(uint32_t x) {
 }
 
 // Offset of each of the workgroup's rows in the codes, head 0, in LDS; -1: no such
-// row, -2: the row has no page.
+// row, -2: the row has no page.  `meanwhile` runs while the prefix sums are on their way.
+template <typename F>
 __device__ __forceinline__ void fp4_locate(const Fp4RowsArgs& a, int r0, int64_t (*at)[kF4Rows],
-                                           int* ip_sh) {
+                                           int (*sh)[kF4Indptr + 1], F meanwhile) {
   const int tid = threadIdx.x;
   const bool staged = a.batch <= kF4Indptr;
+  auto start_of = [&](int b) { return a.start && b < a.batch ? a.start[b] : 0; };
+  int ip0 = 0, st0 = 0;
+  if (staged && tid <= a.batch) {
+    ip0 = a.indptr[tid];
+    st0 = start_of(tid);
+  }
+  meanwhile();
   if (staged) {
-    for (int i = tid; i <= a.batch; i += kF4Threads) ip_sh[i] = a.indptr[i];
+    if (tid <= a.batch) {
+      sh[0][tid] = ip0;
+      sh[1][tid] = st0;
+    }
+    for (int i = tid + kF4Threads; i <= a.batch; i += kF4Threads) {
+      sh[0][i] = a.indptr[i];
+      sh[1][i] = start_of(i);
+    }
     __syncthreads();
   }
-  const int* ip = staged ? ip_sh : a.indptr;
+  const int* ip = staged ? sh[0] : a.indptr;
   if (tid < a.block_rows) {
     const int t = r0 + tid;
     int64_t pos[2] = {-1, -1};
@@ -98,7 +115,7 @@ __device__ __forceinline__ void fp4_locate(const Fp4RowsArgs& a, int r0, int64_t
       }
       const int j = t - ip[lo];
       if (j >= 0 && t < ip[lo + 1]) {
-        const int64_t n = (a.start ? a.start[lo] : 0) + static_cast<int64_t>(j);
+        const int64_t n = (staged ? sh[1][lo] : start_of(lo)) + static_cast<int64_t>(j);
         const int64_t lp = a.page_shift >= 0 ? n >> a.page_shift : n / a.page_size;
         const bool in = n >= 0 && lp < a.table_width;
         const int64_t off = n - lp * a.page_size;
@@ -176,69 +193,71 @@ template <int DT>
 __global__ __launch_bounds__(kF4Threads) void fa2_fp4_append_kernel(Fp4RowsArgs a) {
   constexpr int kW = DT == FA2_DTYPE_F32 ? 2 : 1;  // 16-byte loads of 8 values
   __shared__ int64_t at[2][kF4Rows];
-  __shared__ int ip_sh[kF4Indptr + 1];
+  __shared__ int sh[2][kF4Indptr + 1];
   const int r0 = blockIdx.x * a.block_rows;
-  fp4_locate(a, r0, at, ip_sh);
   const int rows = min(a.block_rows, a.num_rows - r0);
-  for (int col0 = 0; col0 < a.words; col0 += kF4Threads) {
-    const Fp4Share s = fp4_share(a, col0);
+  u32x4 in[4][2][kW];
+  Fp4Share s;
+  auto load = [&](int col0) {  // this thread's word of four rows of K and V
+    s = fp4_share(a, col0);
     const int h = s.col >> a.word_shift, w = s.col & ((1 << a.word_shift) - 1);
-    const char* src[2];
 #pragma unroll
-    for (int v = 0; v < 2; ++v)
-      src[v] = a.x[v] + static_cast<int64_t>(r0 + s.first) * a.ts[v] + h * a.hs[v] + w * (16 * kW);
-    // (all threads go round together: the lanes of a quad exchange values)
-    for (int base = 0; base < rows; base += s.step * 4) {
-      u32x4 in[4][2][kW];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int r = base + u * s.step + s.first;
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-#pragma unroll
-          for (int i = 0; i < kW; ++i) in[u][v][i] = (u32x4){0u, 0u, 0u, 0u};
-          if (r < rows && at[v][r] >= 0)
-#pragma unroll
-            for (int i = 0; i < kW; ++i)
-              in[u][v][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src[v]) + i);
-          src[v] += s.step * a.ts[v];
-        }
-      }
-      const int own = base + (threadIdx.x & 3) * s.step + s.first;  // the row this lane writes
+    for (int u = 0; u < 4; ++u) {
+      const int r = u * s.step + s.first;
 #pragma unroll
       for (int v = 0; v < 2; ++v) {
-        uint32_t code[4], scale = 0;
+        const char* src =
+            a.x[v] + static_cast<int64_t>(r0 + r) * a.ts[v] + h * a.hs[v] + w * (16 * kW);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          float x[8];
-          fp4_unpack8<DT>(in[u][v], x);
-          uint32_t top = 0;
+        for (int i = 0; i < kW; ++i) in[u][v][i] = (u32x4){0u, 0u, 0u, 0u};
+        if (r < rows && (v == 0 || a.has_v))
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            top = max(top, __builtin_bit_cast(uint32_t, x[i]) & 0x7FFFFFFFu);
-          top = max(top, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(
-                             0, static_cast<int>(top), 0xB1, 0xF, 0xF, true)));
-          top = max(top, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(
-                             0, static_cast<int>(top), 0x4E, 0xF, 0xF, true)));
-          const uint32_t sb = fp4_scale<DT>(top);
-          const float f = __builtin_bit_cast(float, sb << 23);
-          uint32_t c = 0;
-          c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[0], x[1], f, 0);
-          c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[2], x[3], f, 1);
-          c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[4], x[5], f, 2);
-          c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[6], x[7], f, 3);
-          code[u] = sb == 255 ? 0 : c;
-          scale = (threadIdx.x & 3) == u ? sb : scale;
-        }
-        quad_transpose(code);
-        const int64_t p = own < rows ? at[v][own] : -1;
-        if (p >= 0) {
-          const int64_t c = p + s.code;
-          *reinterpret_cast<u32x4*>(a.codes[v] + c) = (u32x4){code[0], code[1], code[2], code[3]};
-          a.scales[v][c >> 4] = static_cast<uint8_t>(scale);
-        }
+          for (int i = 0; i < kW; ++i)
+            in[u][v][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src) + i);
       }
     }
+  };
+  // (the rows are read whether they have a place or not: their loads need not wait for it)
+  fp4_locate(a, r0, at, sh, [&] { load(0); });
+  for (int col0 = 0;;) {
+    // (all threads go round together: the lanes of a quad exchange values)
+    const int own = (threadIdx.x & 3) * s.step + s.first;  // the row this lane writes
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      uint32_t code[4], scale = 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        float x[8];
+        fp4_unpack8<DT>(in[u][v], x);
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          top = max(top, __builtin_bit_cast(uint32_t, x[i]) & 0x7FFFFFFFu);
+        top = max(top, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(
+                           0, static_cast<int>(top), 0xB1, 0xF, 0xF, true)));
+        top = max(top, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(
+                           0, static_cast<int>(top), 0x4E, 0xF, 0xF, true)));
+        const uint32_t sb = fp4_scale<DT>(top);
+        const float f = __builtin_bit_cast(float, sb << 23);
+        uint32_t c = 0;
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[0], x[1], f, 0);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[2], x[3], f, 1);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[4], x[5], f, 2);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[6], x[7], f, 3);
+        code[u] = sb == 255 ? 0 : c;
+        scale = (threadIdx.x & 3) == u ? sb : scale;
+      }
+      quad_transpose(code);
+      const int64_t p = own < rows ? at[v][own] : -1;
+      if (p >= 0) {
+        const int64_t c = p + s.code;
+        *reinterpret_cast<u32x4*>(a.codes[v] + c) = (u32x4){code[0], code[1], code[2], code[3]};
+        a.scales[v][c >> 4] = static_cast<uint8_t>(scale);
+      }
+    }
+    col0 += kF4Threads;
+    if (col0 >= a.words) break;
+    load(col0);
   }
 }
 
@@ -268,13 +287,15 @@ __device__ __forceinline__ void fp4_expand8(uint32_t w, uint32_t sb, u32x4* r) {
   }
 }
 
-template <int DT>
-__global__ __launch_bounds__(kF4Threads) void fa2_fp4_gather_kernel(Fp4RowsArgs a) {
+// WAVES: at most so many waves per SIMD (fa2_ops.hip has the rule and what it measured).
+template <int DT, int WAVES>
+__global__ __launch_bounds__(kF4Threads) __attribute__((amdgpu_waves_per_eu(1, WAVES))) void
+fa2_fp4_gather_kernel(Fp4RowsArgs a) {
   constexpr int kW = DT == FA2_DTYPE_F32 ? 2 : 1;
   __shared__ int64_t at[2][kF4Rows];
-  __shared__ int ip_sh[kF4Indptr + 1];
+  __shared__ int sh[2][kF4Indptr + 1];
   const int r0 = blockIdx.x * a.block_rows;
-  fp4_locate(a, r0, at, ip_sh);
+  fp4_locate(a, r0, at, sh, [] {});
   const int rows = min(a.block_rows, a.num_rows - r0);
   for (int col0 = 0; col0 < a.words; col0 += kF4Threads) {
     const Fp4Share s = fp4_share(a, col0);
@@ -283,38 +304,36 @@ __global__ __launch_bounds__(kF4Threads) void fa2_fp4_gather_kernel(Fp4RowsArgs 
 #pragma unroll
     for (int v = 0; v < 2; ++v)
       dst[v] = a.x[v] + static_cast<int64_t>(r0 + s.first) * a.ts[v] + h * a.hs[v] + w * (16 * kW);
-    for (int base = 0; base < rows; base += s.step * 4) {
-      const int own = base + (threadIdx.x & 3) * s.step + s.first;  // the row this lane reads
-      uint32_t code[2][4], scale[2];
+    const int own = (threadIdx.x & 3) * s.step + s.first;  // the row this lane reads
+    uint32_t code[2][4], scale[2];
 #pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        const int64_t p = own < rows ? at[v][own] : -1;
-        u32x4 x = (u32x4){0u, 0u, 0u, 0u};  // (no page: zeros)
-        scale[v] = 127;
-        if (p >= 0) {
-          const int64_t c = p + s.code;
-          x = *reinterpret_cast<const u32x4*>(a.codes[v] + c);
-          scale[v] = a.scales[v][c >> 4];
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) code[v][i] = x[i];
+    for (int v = 0; v < 2; ++v) {
+      const int64_t p = own < rows ? at[v][own] : -1;
+      u32x4 x = (u32x4){0u, 0u, 0u, 0u};  // (no page: zeros)
+      scale[v] = 127;
+      if (p >= 0) {
+        const int64_t c = p + s.code;
+        x = *reinterpret_cast<const u32x4*>(a.codes[v] + c);
+        scale[v] = a.scales[v][c >> 4];
       }
 #pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        quad_transpose(code[v]);
-        const uint32_t sb[4] = {quad_lane<0>(scale[v]), quad_lane<1>(scale[v]),
-                                quad_lane<2>(scale[v]), quad_lane<3>(scale[v])};
+      for (int i = 0; i < 4; ++i) code[v][i] = x[i];
+    }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int r = base + u * s.step + s.first;
-          u32x4 x[kW];
-          fp4_expand8<DT>(code[v][u], sb[u], x);
-          if (r < rows && at[v][r] != -1 && (v == 0 || a.has_v))
+    for (int v = 0; v < 2; ++v) {
+      quad_transpose(code[v]);
+      const uint32_t sb[4] = {quad_lane<0>(scale[v]), quad_lane<1>(scale[v]),
+                              quad_lane<2>(scale[v]), quad_lane<3>(scale[v])};
 #pragma unroll
-            for (int i = 0; i < kW; ++i)
-              __builtin_nontemporal_store(x[i], reinterpret_cast<u32x4*>(dst[v]) + i);
-          dst[v] += s.step * a.ts[v];
-        }
+      for (int u = 0; u < 4; ++u) {
+        const int r = u * s.step + s.first;
+        u32x4 x[kW];
+        fp4_expand8<DT>(code[v][u], sb[u], x);
+        if (r < rows && at[v][r] != -1 && (v == 0 || a.has_v))
+#pragma unroll
+          for (int i = 0; i < kW; ++i)
+            __builtin_nontemporal_store(x[i], reinterpret_cast<u32x4*>(dst[v]) + i);
+        dst[v] += s.step * a.ts[v];
       }
     }
   }
