@@ -122,7 +122,8 @@ def test_long(dtype, D, QH, KVH, M, page, lens):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("D", [64, 128, 256])
-@pytest.mark.parametrize("QH,KVH,M", [(24, 1, 0), (16, 4, 5), (8, 2, 8), (24, 1, 4), (34, 2, 1)])
+@pytest.mark.parametrize("QH,KVH,M", [(24, 1, 0), (16, 4, 5), (8, 2, 8), (24, 1, 4), (34, 2, 1),
+                                       (40, 1, 16)])
 @pytest.mark.parametrize("page", [16, 5])
 def test_wide_tables(dtype, D, QH, KVH, M, page):
     """More than 16 rows where the tables could hold many keys (q-blocks of 32 up to
@@ -144,6 +145,7 @@ def test_wide_tables(dtype, D, QH, KVH, M, page):
     (256, 8, 16, [3000 if i % 5 == 0 else 7 * i for i in range(33)]),
     (64, 8, 16, [1030] * 16),                                       # equal units
     (128, 1, 16, [1030 + i for i in range(64)]),
+    (64, 300, 16, [200, 1, 77, 640]),                               # more heads than CUs
 ])
 def test_shares(D, KVH, page, lens):
     """Workgroups with several units and units with several workgroups."""
