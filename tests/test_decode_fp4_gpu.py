@@ -462,3 +462,29 @@ def test_serving_steps(dtype, M):
         size = torch.stack([vs[b].abs().amax((0, 2))[i // (QH // KVH)] for i in range(QH)])
         R.within(out[t:t + n].transpose(0, 1), want, tol + 2 * h * size[:, None, None])
         t += n
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("M", [0, 3])
+@pytest.mark.parametrize("quanta", [2.49, 16.49, 100.4])
+def test_small_weights(dtype, D, M, quanta):
+    """Weights far below the largest count in full: every wave's first tile has a key
+    that takes nearly all of the softmax and whose value is zero, so the output is
+    the sum of weights of ``quanta`` * 2^-24 of the largest (2^-24: the least that fp16
+    holds).  All terms are positive: A of fp4_ref's bound is the output."""
+    QH, KVH, n = 4, 2, 768
+    c = Case([n, n - 5], QH, KVH, D, M, dtype, 16, 26, causal=bool(M))
+    lead = math.log(2.0 ** 24 / quanta)  # of the score, over zeros
+    # a key of D values 3: its score is 3 * sqrt(D) * the query's value
+    c.q = torch.full((2, QH, max(M, 1), D), lead / (3 * D ** 0.5)).to(dtype)
+    for i, (codes, scales) in enumerate(c.caches):
+        codes[:] = 0 if i == 0 else 0x22                        # K 0, V 1
+        scales[:] = 127
+        for b in range(2):
+            for j in range(8):
+                pg = c.tables[i][b, 32 * j // 16].item()
+                codes[pg, :, 0] = 0x55 if i == 0 else 0         # K 3, V 0
+    out = c.call()
+    c.check(out)
+    assert (out > 0).all()

@@ -25,11 +25,15 @@
 //     by key with v_perm: block i of O^T is dim i of every 16 lanes.  (V back
 //     through LDS in 16 bits, for transpose reads, took two thirds of the LDS
 //     time, and that 75 % of a tile's.)
-//   * P goes to the MFMA as the sum of two 16-bit values, high and low part, so
-//     that the weights carry 16 to 22 bits and the output is off by its own rounding
-//     alone; the low parts cost 5 % of a long call.
+//   * P goes to the MFMA as the sum of two 16-bit values, high and low part, which costs 5
+//     % of a long call.  bf16: 16 bits of a weight, off by 2^-18 of it, so that 0.22 % of
+//     the outputs of 64 sequences of 512-8192 keys round the other way than the exact
+//     ones (0.04 % with exact weights); a third part, which makes them exact, takes
+//     64.1 us for 60.9 there, 22.2 for 20.7 with 20 rows.  fp16: 22 bits, and weights from
+//     2^11 down (kLift), so that one of 2^-25 of a wave's largest still has 11 and none is
+//     off by more than 2^-36 of that (from 1 down, 2^-20 is off by up to 3 %).
 //   * Running maxima and sums in fp32, raised only when a score passes the
-//     maximum by 2^8, as in the 16-bit kernels.
+//     maximum by 2^8 (bf16, as in the 16-bit kernels) or 2^4.
 // Measured on MI355X, us (and the cache's bytes per s): 64 sequences of 512-8192 keys,
 // 32 / 8 heads of D128, 66 (4.6 TB/s); 16 of 16000-32768, 32 / 4 heads, 45 (4.6); 16 of
 // 8200 with 8 drafts, 8 / 8 heads of D64, 27 (2.7); 33 of 100-4096 with 5 drafts, 16 / 4
@@ -227,6 +231,8 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
   constexpr int kStep = kD4Tile * kD4Waves;
   constexpr int kSub = D == 256 ? 2 : 1;  // scales of a lane's dims
   static_assert(kD4Waves * G::kStage >= kMergePieceBytes<kD4Threads>, "merge area");
+  // fp16 weights are at most 2^kRaise * 2^kLift = 2^15
+  constexpr float kRaise = BF ? kRescaleThreshold : 4.f, kLift = BF ? 0.f : 11.f;
   constexpr int kAlign = RB == 1 ? 8 : 12, kGap = RB == 1 ? 5 : 8;  // tiles
 
   __shared__ __attribute__((aligned(1024))) char tiles[kD4Waves * G::kTile];
@@ -677,7 +683,7 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
       for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[rb][x][r]);
-      if (__builtin_expect(__any((mx - m[rb]) * a.scale_log2 > kRescaleThreshold), 0)) {
+      if (__builtin_expect(__any((mx - m[rb]) * a.scale_log2 > kRaise), 0)) {
         mx = over_groups<true>(mx);
         const float mn = fmaxf(m[rb], mx);
         const float alpha = fast_exp2((m[rb] - (mn == -INFINITY ? 0.f : mn)) * a.scale_log2);
@@ -693,7 +699,8 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
         float e[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          e[r] = fast_exp2((s[rb][x][r] - mu) * a.scale_log2);
+          const float y = s[rb][x][r] - mu;
+          e[r] = fast_exp2(BF ? y * a.scale_log2 : __builtin_fmaf(y, a.scale_log2, kLift));
           l[rb] += e[r];
         }
 #pragma unroll
@@ -812,7 +819,7 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
     const int r = r0 + lr;
     const int dim = G::dim(h0 + hh, sd);
     if (cur.np == 1) {
-      // (0/0 -> NaN for a row with no key, as in 16 bits; otherwise lt >= 2^-8)
+      // (0/0 -> NaN for a row with no key, as in 16 bits; otherwise lt >= 1)
       const float inv = __builtin_amdgcn_rcpf(lt);
       *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.o) + cur.b * a.o_sb + head0 * a.o_sh +
                                 (q0 + r) * a.o_ss + dim) =
