@@ -14,6 +14,8 @@
 
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
+
 #include "fa2.h"
 #include "fa2_ops.h"
 
@@ -34,16 +36,26 @@ bool rows_ok(const at::Tensor& t) {
 
 at::Tensor prep(const at::Tensor& t) { return rows_ok(t) ? t : t.contiguous(); }
 
+// The element stride of dim d as the kernels take it.  torch keeps any stride on a
+// dim of size one and calls the tensor contiguous all the same (one token of a
+// wider row): the layout's own stride then.
+int64_t stride_of(const at::Tensor& t, int64_t d) {
+  if (!t.is_contiguous()) return t.stride(d);
+  int64_t s = 1;
+  for (int64_t i = d + 1; i < t.dim(); ++i) s *= std::max<int64_t>(t.size(i), 1);
+  return s;
+}
+
 // (batch, head, row) element strides; token-major tensors (token, head).
 void strides3(const at::Tensor& t, int64_t& sb, int64_t& sh, int64_t& ss) {
   if (t.dim() == 4) {
-    sb = t.stride(0);
-    sh = t.stride(1);
-    ss = t.stride(2);
+    sb = stride_of(t, 0);
+    sh = stride_of(t, 1);
+    ss = stride_of(t, 2);
   } else {
     sb = 0;
-    sh = t.stride(1);
-    ss = t.stride(0);
+    sh = stride_of(t, 1);
+    ss = stride_of(t, 0);
   }
 }
 
@@ -159,7 +171,7 @@ at::Tensor fwd(at::Tensor q, at::Tensor k, at::Tensor v, int64_t layout, int64_t
 // Rows r = (head in group) * M + m of a kv-head group form one strided run
 // (kernels/decode.py:run_ok), t [B,QH,M,D].
 bool run_ok(const at::Tensor& t, int64_t M) {
-  return rows_ok(t) && (M == 1 || t.stride(1) == M * t.stride(2));
+  return rows_ok(t) && (M == 1 || stride_of(t, 1) == M * stride_of(t, 2));
 }
 
 // decode_attention (q [B,QH,D]) and speculative_decode_attention (q
@@ -220,9 +232,9 @@ c10::optional<at::Tensor> decode(at::Tensor q, at::Tensor k, at::Tensor v, int64
   p.softmax_scale = static_cast<float>(std::pow(static_cast<double>(p.head_dim), -0.5));
   // M = 1: the rows of a unit are its heads, the row stride is the head stride
   auto set_strides = [&](const at::Tensor& t, int64_t& sb, int64_t& sh, int64_t& ss) {
-    sb = t.stride(0);
-    sh = t.stride(1);
-    ss = M > 1 ? t.stride(2) : t.stride(1);
+    sb = stride_of(t, 0);
+    sh = stride_of(t, 1);
+    ss = stride_of(t, M > 1 ? 2 : 1);
   };
   set_strides(q4, p.q_sb, p.q_sh, p.q_ss);
   set_strides(dst, p.o_sb, p.o_sh, p.o_ss);
@@ -269,8 +281,8 @@ int64_t append(const at::Tensor& kc, const c10::optional<at::Tensor>& vc, const 
   p.num_pages = kc.size(0) / page_size;
   p.table_width = kt.size(1);
   p.k_table_stride = kt.stride(0);
-  p.new_ts = kn.stride(0);
-  p.new_hs = kn.stride(1);
+  p.new_ts = stride_of(kn, 0);
+  p.new_hs = stride_of(kn, 1);
   p.cache_ts = kc.stride(0);
   p.cache_hs = kc.stride(1);
   p.k_new = kn.data_ptr();
@@ -443,8 +455,8 @@ int64_t fp4_rows(bool append, const at::Tensor& kc, const at::Tensor& ks, const 
   p.num_pages = kc.size(0);
   p.table_width = kt.size(1);
   p.k_table_stride = kt.stride(0);
-  p.k_ts = k.stride(0);
-  p.k_hs = k.stride(1);
+  p.k_ts = stride_of(k, 0);
+  p.k_hs = stride_of(k, 1);
   p.k = k.data_ptr();
   p.k_codes = kc.data_ptr<uint8_t>();
   p.k_scales = ks.data_ptr<uint8_t>();
@@ -458,8 +470,8 @@ int64_t fp4_rows(bool append, const at::Tensor& kc, const at::Tensor& ks, const 
     vt = table32(*v_table, dev);
     p.table_width = std::min(p.table_width, vt.size(1));
     p.v_table_stride = vt.stride(0);
-    p.v_ts = v->stride(0);
-    p.v_hs = v->stride(1);
+    p.v_ts = stride_of(*v, 0);
+    p.v_hs = stride_of(*v, 1);
     p.v = v->data_ptr();
     p.v_codes = vc->data_ptr<uint8_t>();
     p.v_scales = vs->data_ptr<uint8_t>();
@@ -541,9 +553,9 @@ std::tuple<int64_t, at::Tensor> fp4_decode(const at::Tensor& q, const at::Tensor
   p.k_table_stride = kt.stride(0);
   p.v_table_stride = vt.stride(0);
   auto set_strides = [&](const at::Tensor& t, int64_t& sb, int64_t& sh, int64_t& ss) {
-    sb = t.stride(0);
-    sh = t.stride(1);
-    ss = M > 1 ? t.stride(2) : t.stride(1);
+    sb = stride_of(t, 0);
+    sh = stride_of(t, 1);
+    ss = stride_of(t, M > 1 ? 2 : 1);
   };
   set_strides(q4, p.q_sb, p.q_sh, p.q_ss);
   set_strides(o4, p.o_sb, p.o_sh, p.o_ss);

@@ -44,11 +44,23 @@ def aligned(t: torch.Tensor) -> torch.Tensor:
     return t if rows_ok(t) else t.clone(memory_format=torch.contiguous_format)
 
 
+def stride_of(t: torch.Tensor, d: int) -> int:
+    """The element stride of dim ``d`` as the kernels take it.  torch keeps any stride
+    on a dim of size one and calls the tensor contiguous all the same (one token
+    of a wider row): the layout's own stride then."""
+    if not t.is_contiguous():
+        return t.stride(d)
+    s = 1
+    for n in t.shape[d + 1:]:
+        s *= max(n, 1)
+    return s
+
+
 def strides(t: torch.Tensor):
     """(batch, head, row) element strides; token-major tensors use (0, head, token)."""
     if t.dim() == 4:
-        return t.stride(0), t.stride(1), t.stride(2)
-    return 0, t.stride(1), t.stride(0)
+        return stride_of(t, 0), stride_of(t, 1), stride_of(t, 2)
+    return 0, stride_of(t, 1), stride_of(t, 0)
 
 
 def index_tensor(t: torch.Tensor, device) -> torch.Tensor:

@@ -32,7 +32,8 @@ from __future__ import annotations
 import torch
 
 from . import _fa2
-from ._launch import check_dtype_and_dim, enqueue, ext, index_tensor, prep, rows_ok, table
+from ._launch import (check_dtype_and_dim, enqueue, ext, index_tensor, prep, rows_ok, stride_of,
+                      table)
 
 # The launch goes through the C++ extension when it is built, else through
 # ctypes; both enqueue the same libfa2.so entry point with the same parameters.
@@ -158,10 +159,10 @@ def _run_decode(name, q4, k, v, out4, *, layout, causal, batch, q_heads, kv_head
     # one strided run of rows per kv-head group: row r = head * M + m
     # (M = 1: the rows of a group are its heads, the row stride is the head stride)
     def run_ok(t):
-        return rows_ok(t) and (M == 1 or t.stride(1) == M * t.stride(2))
+        return rows_ok(t) and (M == 1 or stride_of(t, 1) == M * stride_of(t, 2))
 
     def abi_strides(t):
-        return (t.stride(0), t.stride(1), t.stride(2) if M > 1 else t.stride(1))
+        return (stride_of(t, 0), stride_of(t, 1), stride_of(t, 2 if M > 1 else 1))
 
     if not run_ok(q4):
         q4 = q4.contiguous()

@@ -24,7 +24,7 @@ from __future__ import annotations
 import torch
 
 from . import _fa2, _ops
-from ._launch import DTYPES, ext, index_tensor, rows_ok, table
+from ._launch import DTYPES, ext, index_tensor, rows_ok, stride_of, table
 from .fp4_cache import check_cache
 
 # As kernels/decode.py: the C++ extension launches when it is built.
@@ -98,7 +98,7 @@ def _run(name, q, kc, ks, vc, vs, lens, k_table, v_table, causal, workspace=None
     dev = q.device
     q4 = q.unsqueeze(2) if q.dim() == 3 else q
     B, QH, M, D = q4.shape
-    if not rows_ok(q4) or (M > 1 and q4.stride(1) != M * q4.stride(2)):
+    if not rows_ok(q4) or (M > 1 and stride_of(q4, 1) != M * stride_of(q4, 2)):
         q4 = q4.clone(memory_format=torch.contiguous_format)
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     o4 = out.unsqueeze(2) if q.dim() == 3 else out
@@ -111,9 +111,9 @@ def _run(name, q, kc, ks, vc, vs, lens, k_table, v_table, causal, workspace=None
     p.table_width = min(kt.shape[1], vt.shape[1])
     p.k_table_stride, p.v_table_stride = kt.stride(0), vt.stride(0)
     for t, pre in ((q4, "q"), (o4, "o")):
-        setattr(p, pre + "_sb", t.stride(0))
-        setattr(p, pre + "_sh", t.stride(1))
-        setattr(p, pre + "_ss", t.stride(2) if M > 1 else t.stride(1))
+        setattr(p, pre + "_sb", stride_of(t, 0))
+        setattr(p, pre + "_sh", stride_of(t, 1))
+        setattr(p, pre + "_ss", stride_of(t, 2 if M > 1 else 1))
     p.q, p.o = q4.data_ptr(), out.data_ptr()
     p.k_codes, p.k_scales = kc.data_ptr(), ks.data_ptr()
     p.v_codes, p.v_scales = vc.data_ptr(), vs.data_ptr()

@@ -37,7 +37,7 @@ from typing import NamedTuple
 import torch
 
 from . import _ops
-from ._launch import DTYPES, aligned, ext, index_tensor, table
+from ._launch import DTYPES, aligned, ext, index_tensor, stride_of, table
 
 # As kernels/decode.py: the C++ extension launches when it is built.
 USE_EXT = True
@@ -225,7 +225,7 @@ def _rows(name, entry, kc, ks, vc, vs, k_table, v_table, k, v, indptr, start_pos
     p.batch, p.kv_heads, p.head_dim, p.num_rows = B, kc.shape[1], k.shape[2], k.shape[0]
     p.page_size, p.num_pages, p.table_width = kc.shape[2], kc.shape[0], kt.shape[1]
     p.k_table_stride = kt.stride(0)
-    p.k_ts, p.k_hs = k.stride(0), k.stride(1)
+    p.k_ts, p.k_hs = stride_of(k, 0), stride_of(k, 1)
     p.k, p.k_codes, p.k_scales = k.data_ptr(), kc.data_ptr(), ks.data_ptr()
     p.indptr, p.k_block_table = ip.data_ptr(), kt.data_ptr()
     if sp is not None:
@@ -234,7 +234,7 @@ def _rows(name, entry, kc, ks, vc, vs, k_table, v_table, k, v, indptr, start_pos
         vt = table(v_table, dev)
         p.table_width = min(kt.shape[1], vt.shape[1])
         p.v_table_stride = vt.stride(0)
-        p.v_ts, p.v_hs = v.stride(0), v.stride(1)
+        p.v_ts, p.v_hs = stride_of(v, 0), stride_of(v, 1)
         p.v, p.v_codes, p.v_scales = v.data_ptr(), vc.data_ptr(), vs.data_ptr()
         p.v_block_table = vt.data_ptr()
     with torch.cuda.device(dev):

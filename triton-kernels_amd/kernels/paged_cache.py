@@ -26,7 +26,7 @@ from __future__ import annotations
 import torch
 
 from . import _fa2
-from ._launch import DTYPES, ext, index_tensor, table
+from ._launch import DTYPES, ext, index_tensor, stride_of, table
 
 # As kernels/decode.py: the C++ extension launches when it is built.
 USE_EXT = True
@@ -109,7 +109,7 @@ def paged_kv_append(
     p.table_width = kt.shape[1]
     p.k_table_stride = kt.stride(0)
     p.v_table_stride = vt.stride(0) if has_v else 0
-    p.new_ts, p.new_hs = kn.stride(0), kn.stride(1)
+    p.new_ts, p.new_hs = stride_of(kn, 0), stride_of(kn, 1)
     p.cache_ts, p.cache_hs = kc.stride(0), kc.stride(1)
     p.k_new, p.k_cache = kn.data_ptr(), kc.data_ptr()
     p.new_indptr, p.k_block_table = ip.data_ptr(), kt.data_ptr()
