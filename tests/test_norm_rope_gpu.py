@@ -218,3 +218,32 @@ def test_refusals(bad):
             m.USE_EXT = True
     assert seen[0] == seen[1]
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,rot", [(64, 32), (128, 48), (128, 0), (256, 64), (32, 16)])
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("T", [3, 3001])  # (one and four heads per lane group)
+def test_infinities_stay_in_their_place(dtype, D, rot, inter, T):
+    """An infinity makes its own value NaN and the rest of its row zeros; in a rotated
+    pair both are NaN by the formula, in the dims behind them only itself.  A weight
+    that is infinite or NaN touches its own dim alone there."""
+    from kernels import build_rope_table, qk_norm_rope
+    q, k, qw, kw, g = data(T, 5, 2, D, dtype, 7)
+    table = (build_rope_table(5000, rot, device="cuda") if rot
+             else torch.empty(5000, 0, device="cuda"))
+    pos = torch.randint(0, 5000, (T,), generator=g, dtype=torch.int32)
+    q[0, 0, D - 1] = math.inf
+    q[1, 4, rot] = -math.inf
+    q[T - 1, 2, rot + (D - rot) // 2] = math.inf
+    q[2, 1, 0] = math.inf                               # (rotated, where rot > 0)
+    k[T - 1, 1, D - 2] = math.nan                       # all of its row
+    kw[rot + 1], kw[D - 1] = math.inf, math.nan
+    qo, ko = qk_norm_rope(q.cuda(), k.cuda(), qw.cuda(), kw.cuda(), table, pos.cuda(),
+                          interleaved=inter)
+    check(qo, q, qw, table, pos, inter)
+    want, tol = R.norm_rope(k, kw, table.cpu(), pos, inter, 1e-6)
+    # (a value times the infinite weight is infinite in both)
+    ko, inf = ko.cpu().double(), torch.isinf(want)
+    assert torch.equal(ko[inf], want[inf])
+    R.within(torch.where(inf, 0.0, ko), torch.where(inf, 0.0, want), torch.where(inf, 0.0, tol))

@@ -115,7 +115,6 @@ __global__ __launch_bounds__(kNrThreads) void fa2_norm_rope_kernel(NormRopeArgs 
   const int64_t pos = a.pos64 ? static_cast<const int64_t*>(a.pos)[t]
                               : static_cast<const int32_t*>(a.pos)[t];
   float c[E], s[E], w[2 * E];
-  // (no rotation is the one by cos 1, sin 0)
 #pragma unroll
   for (int i = 0; i < E; ++i) {
     c[i] = 1.f;
@@ -170,7 +169,10 @@ __global__ __launch_bounds__(kNrThreads) void fa2_norm_rope_kernel(NormRopeArgs 
     for (int i = 0; i < 2 * E; ++i) v[i] = v[i] * r * w[i];
     // pairs (i, E + i), or neighbours, of the lane's 2 E values
     float z[2 * E];
-    if (a.inter) {
+    if (!rotated) {  // (a rotation by cos 1, sin 0 would spread infinities and NaN)
+#pragma unroll
+      for (int i = 0; i < 2 * E; ++i) z[i] = v[i];
+    } else if (a.inter) {
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         z[2 * i] = v[2 * i] * c[i] - v[2 * i + 1] * s[i];
