@@ -359,3 +359,31 @@ def test_gather_past_the_caches(dtype):
                               indptr([n] * seqs).cuda(), n * seqs, dtype=dtype)
     for x, w in zip(got, want):
         assert torch.equal(x.view(seqs, n, H, D), w.expand(seqs, -1, -1, -1))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_error_bound_of_a_block(dtype):
+    """The error of a block is at most 1/5 of its largest value a, which the step keeps
+    within 3.5 <= a < 7 steps: values from 4 steps up are off by at most one step, which is
+    a / 5 at a = 5 (midway between 4 and 6, it becomes 4) and less elsewhere (a - 4 below 5,
+    1 above); the others by half a step at most, a / 7."""
+    from kernels import allocate_fp4_cache, paged_kv_append_fp4, paged_kv_gather_fp4
+    tops = [3.5, 3.75, 4.0, 4.5, 4.75, 5.0, 5.25, 5.5, 5.75, 6.0, 6.5, 6.75, 6.9375]
+    x = torch.empty(16 * len(tops), 1, 64, dtype=torch.float64)
+    g = torch.Generator().manual_seed(30)
+    for i, a in enumerate(tops):
+        for j in range(16):
+            row = (torch.rand(64, generator=g, dtype=torch.float64) * 2 - 1) * a
+            row[[j, 32 + j]] = torch.tensor([a, -a], dtype=torch.float64)
+            x[16 * i + j, 0] = row * 2.0 ** (j - 8)
+    x = x.to(dtype)
+    n = x.shape[0]
+    kt = torch.arange(-(-n // 16), dtype=torch.int32).cuda()[None]
+    kc, ip = allocate_fp4_cache(kt.shape[1], 16, 1, 64), indptr([n]).cuda()
+    paged_kv_append_fp4(kc, None, kt, None, x.cuda(), None, ip)
+    got, _ = paged_kv_gather_fp4(kc, None, kt, None, ip, n, dtype=dtype)
+    blocks = x.double().unflatten(-1, (-1, 32))
+    err = (got.cpu().double().unflatten(-1, (-1, 32)) - blocks).abs().amax(-1)
+    share = (err / blocks.abs().amax(-1)).view(len(tops), -1)
+    assert (share <= 0.2).all()
+    assert (share[tops.index(5.0)] == 0.2).all()

@@ -21,11 +21,11 @@ readers pay next to nothing for the format and add no rounding of their own.
 * :func:`allocate_fp4_cache` - an empty cache.
 
 Quantisation of a block of 32: the least power of two at which the largest
-value is at most 6 after rounding, each value to the nearest code, ties to even
-(an error of at most 1/7 of the block's largest value).  Powers are kept in
-2 ** -23 ... 2 ** 13 for fp16 rows and 2 ** -100 ... 2 ** 125 for bf16 and fp32
-rows, so that every cached value is exact in the rows' type; past 49152 fp16
-rows saturate.  A block with an infinity or NaN is NaN.
+value is at most 6 after rounding, each value to the nearest code, ties to even.
+Powers are kept in 2 ** -23 ... 2 ** 13 for fp16 rows and 2 ** -100 ... 2 ** 125
+for bf16 and fp32 rows, so that every cached value is exact in the rows' type;
+past 49152 fp16 rows saturate.  Inside that range a value is off by at most 1/5 of
+its block's largest (5 steps become 4).  A block with an infinity or NaN is NaN.
 
 The computation runs in ``libfa2.so`` (include/fa2_ops.h); no fallback.
 """
