@@ -488,3 +488,63 @@ def test_small_weights(dtype, D, M, quanta):
     out = c.call()
     c.check(out)
     assert (out > 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("M", [0, 2])
+@pytest.mark.parametrize("lens", [[100, 333], [5000, 64], [700] * 5])
+def test_one_key_far_above_the_others(dtype, D, M, lens):
+    """Scores at the largest scales, far past the exponent's range.  A key of +-6 with
+    the queries' signs scores 6 sum |q_d|, which with these queries passes every other
+    key by half of that at least (checked), the scores' errors by far less: its
+    weight is one, all others are zero, and the output is its row of V, a number of
+    the type, times (1 + 2 u) at most: that number."""
+    H = 3
+    c = Case(lens, H, H, D, M, dtype, 16, 27)
+    c.q[:, :, 1:] = c.q[:, :, :1] * 0.5  # (drafts of one direction: one key for all)
+    top = 127 + 13 if dtype == torch.float16 else 127 + 60
+    for codes, scales in c.caches:
+        scales[scales != 255] = top
+    at = [n * (i % 3) // 2 if i % 3 < 2 else n - 1 for i, n in enumerate(lens)]
+    codes, scales = c.caches[0]
+    for b, j in enumerate(at):
+        pg = c.tables[0][b, j // 16].item()
+        nib = 7 + 8 * torch.signbit(c.q[b, :, 0]).to(torch.uint8)
+        codes[pg, :, j % 16] = R.pack(nib)
+    out = c.call()
+    out = out.cpu() if M else out.cpu().unsqueeze(2)
+    for b, j in enumerate(at):
+        k, v = c.values(b)
+        s = torch.einsum("hmd,nhd->hmn", c.q[b].double(), k)
+        rest = s.clone()
+        rest[..., j] = -math.inf
+        assert (rest.amax(-1) < 0.5 * s[..., j]).all()
+        assert torch.equal(out[b].double(), v[j].unsqueeze(1).expand_as(out[b]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("which", ["keys", "values", "low keys", "low values"])
+def test_ends_of_the_type_with_ordinary_scores(dtype, D, which):
+    """K or V at the largest or smallest scales with queries that keep the scores
+    ordinary: fp4_ref's bound is tight (checked), outputs near the type's maximum."""
+    lo, hi = (-23, 13) if dtype == torch.float16 else (-100, 120)
+    e = lo if "low" in which else hi
+    c = Case([100, 1033], 4, 2, D, 0, dtype, 16, 28)
+    codes, scales = c.caches["values" in which]
+    scales[scales != 255] = 127 + e
+    if "keys" in which:
+        # (queries of 2^-13 are fp16's small normal numbers, of 2^13 its large ones)
+        shift = -e - 2 if dtype == torch.bfloat16 else max(min(-e - 2, 12), -12)
+        c.q = (c.q.double() * 2.0 ** shift).to(dtype)
+    out = c.call().cpu().unsqueeze(2)
+    for b in range(2):
+        want, tol = R.attention(c.q[b], *c.values(b), False)
+        # The bound is h |o| (2^-8) and a share of A = sum p |v|: 4 (D + 4) u of the largest
+        # score, here under 2^4, so 2^-10 at D = 256.  A is up to sqrt(1033) |o| and more
+        # where signs cancel: 2^-5 in all.  (fp16 at the smallest values: half the type's
+        # least number is all of it.)
+        if which != "low values":
+            assert (tol / want.abs()).median() < 0.1
+        R.within(out[b], want, tol)
