@@ -548,3 +548,14 @@ def test_ends_of_the_type_with_ordinary_scores(dtype, D, which):
         if which != "low values":
             assert (tol / want.abs()).median() < 0.1
         R.within(out[b], want, tol)
+
+
+@pytest.mark.parametrize("D,QH,KVH,M,lens", [
+    (128, 8, 1, 0, [100001]),                    # one context, longer than 2^16 keys
+    (64, 4, 2, 3, [70000, 40000]),
+    (128, 32, 32, 0, [1500, 33, 700]),           # more than 8 heads of K and V
+    (64, 20, 20, 4, [900, 1]),
+])
+def test_longer_contexts_and_more_heads(D, QH, KVH, M, lens):
+    c = Case(lens, QH, KVH, D, M, torch.bfloat16, 16, 29, causal=bool(M))
+    c.check(c.call())

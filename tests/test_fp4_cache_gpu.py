@@ -387,3 +387,62 @@ def test_error_bound_of_a_block(dtype):
     share = (err / blocks.abs().amax(-1)).view(len(tops), -1)
     assert (share <= 0.2).all()
     assert (share[tops.index(5.0)] == 0.2).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,D", [(32, 128), (20, 128), (9, 256), (33, 64), (17, 64), (64, 256)])
+@pytest.mark.parametrize("only_k", [False, True])
+def test_wide_rows(dtype, H, D, only_k):
+    """More code words in a row than the workgroup has threads, and row lengths that
+    leave threads idle; rows that the last workgroup does not fill."""
+    from kernels import allocate_fp4_cache, paged_kv_append_fp4, paged_kv_gather_fp4
+    lens, start, page = [1, 0, 18, 6], [3, 0, 15, 0], 16
+    T = sum(lens) + 1                                       # and a row that is nobody's
+    k, v = rows_of(T, H, D, dtype, 31), rows_of(T, H, D, dtype, 32)
+    kt, vt, pages = tables([a + b for a, b in zip(lens, start)], page, 33)
+    kc, vc = (allocate_fp4_cache(pages, page, H, D) for _ in range(2))
+    ip, sp = indptr(lens).cuda(), torch.tensor(start, dtype=torch.int32).cuda()
+    sides = [(k, kc, kt)] + ([] if only_k else [(v, vc, vt)])
+    args = (kc, None if only_k else vc, kt.cuda(), None if only_k else vt.cuda())
+    paged_kv_append_fp4(*args, k.cuda(), None if only_k else v.cuda(), ip, start_pos=sp)
+    out = [torch.full((T, H, D), 7.0, dtype=dtype, device="cuda") for _ in sides]
+    paged_kv_gather_fp4(*args, ip, T, sp, out=(out[0], None if only_k else out[1]))
+    for (x, cache, table), got in zip(sides, out):
+        val, nib, scale = R.quantize(x)
+        codes, scales = torch.zeros_like(cache.codes.cpu()), torch.zeros_like(cache.scales.cpu())
+        t = 0
+        for b, n in enumerate(lens):
+            for j in range(n):
+                pg, off = place(table, b, start[b] + j, page)
+                codes[pg, :, off], scales[pg, :, off] = R.pack(nib[t]), scale[t]
+                t += 1
+        assert torch.equal(cache.codes.cpu(), codes)
+        assert torch.equal(cache.scales.cpu(), scales)
+        assert torch.equal(got[:-1].cpu().double(), val[:-1])
+        assert (got[-1] == 7.0).all()
+
+
+@pytest.mark.parametrize("n", [255, 256, 257, 300, 512, 513])
+def test_batches_around_the_staged_ones(n):
+    """As many sequences as a workgroup has threads, as its LDS holds, and one more."""
+    from kernels import allocate_fp4_cache, paged_kv_append_fp4, paged_kv_gather_fp4
+    H, D, page = 2, 64, 4
+    g = torch.Generator().manual_seed(n)
+    lens = torch.randint(0, 4, (n,), generator=g).tolist()
+    lens[-1], start = 2, torch.randint(0, 6, (n,), generator=g)
+    T = sum(lens)
+    x = rows_of(T, H, D, torch.bfloat16, 34)
+    kt, _, pages = tables([a + b for a, b in zip(lens, start.tolist())], page, 35)
+    kc = allocate_fp4_cache(pages, page, H, D)
+    ip, sp = indptr(lens).cuda(), start.to(torch.int32).cuda()
+    paged_kv_append_fp4(kc, None, kt.cuda(), None, x.cuda(), None, ip, start_pos=sp)
+    got, _ = paged_kv_gather_fp4(kc, None, kt.cuda(), None, ip, T, sp)
+    val, nib, _ = R.quantize(x)
+    assert torch.equal(got.cpu().double(), val)
+    t, codes = 0, torch.zeros_like(kc.codes.cpu())
+    for b, m in enumerate(lens):
+        for j in range(m):
+            pg, off = place(kt, b, start[b].item() + j, page)
+            codes[pg, :, off] = R.pack(nib[t])
+            t += 1
+    assert torch.equal(kc.codes.cpu(), codes)
