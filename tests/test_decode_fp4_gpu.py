@@ -559,3 +559,59 @@ def test_ends_of_the_type_with_ordinary_scores(dtype, D, which):
 def test_longer_contexts_and_more_heads(D, QH, KVH, M, lens):
     c = Case(lens, QH, KVH, D, M, torch.bfloat16, 16, 29, causal=bool(M))
     c.check(c.call())
+
+
+@pytest.mark.parametrize("drafts", [False, True])
+@pytest.mark.parametrize("bad,kind,text", [
+    ("dims", ValueError, "q must be [B, QH"), ("dtype", TypeError, "unsupported dtype"),
+    ("head_dim", ValueError, "head_dim"), ("heads", ValueError, "multiple of kv_heads"),
+    ("lens", ValueError, "need 2 rows"), ("rows", ValueError, "need 2 rows"),
+    ("v", ValueError, "v_cache is missing"), ("codes", TypeError, "must be uint8"),
+    ("pages", ValueError, "equal shapes"), ("scales", ValueError, "contiguous"),
+    ("device", AssertionError, "same device"), ("aligned", RuntimeError, "status 7"),
+])
+def test_refusals_name_the_cause(drafts, bad, kind, text):
+    """One exception and one message for each cause, with and without the extension."""
+    import kernels.decode_fp4 as m
+    c = Case([40, 3], 4, 2, 128, 3 if drafts else 0, torch.float16, 16, 25)
+    d = c.dev()
+    q, k, v = d.pop("q"), d.pop("k_cache"), d.pop("v_cache")
+    if bad == "dims":
+        q = q[0]
+    elif bad == "dtype":
+        q = q.float()
+    elif bad == "head_dim":
+        q = q[..., :64]
+    elif bad == "heads":
+        q = q[:, :3]
+    elif bad == "lens":
+        d["kv_indptr"] = d["kv_indptr"][:1]
+    elif bad == "rows":
+        d["v_block_table"] = d["v_block_table"][:1]
+    elif bad == "v":
+        v = None
+    elif bad == "codes":
+        v = (v[0].char(), v[1])
+    elif bad == "pages":
+        v = (v[0][1:], v[1][1:])
+    elif bad == "scales":
+        k = (k[0], k[1][..., :3])
+    elif bad == "device":
+        d["kv_indptr"] = d["kv_indptr"].cpu()
+    else:  # codes off a 16-byte boundary
+        n = k[0].numel()
+        k = (torch.zeros(n + 8, dtype=torch.uint8, device="cuda")[8:].view(k[0].shape), k[1])
+    name = "speculative_decode_attention_fp4" if drafts else "decode_attention_fp4"
+    said = []
+    for use in (True, False):
+        m.USE_EXT = use
+        try:
+            with pytest.raises(kind) as e:
+                getattr(m, name)(q, k, v, **d)
+        finally:
+            m.USE_EXT = True
+        assert text in str(e.value)
+        assert kind is AssertionError or str(e.value).startswith(name)
+        said.append((type(e.value), str(e.value)))
+    assert said[0] == said[1]
+    torch.cuda.synchronize()
