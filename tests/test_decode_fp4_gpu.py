@@ -615,3 +615,30 @@ def test_refusals_name_the_cause(drafts, bad, kind, text):
         said.append((type(e.value), str(e.value)))
     assert said[0] == said[1]
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("use_ext", [True, False])
+def test_int64_lengths_past_32_bits(use_ext):
+    """A length of 2^32 and more is past the table and counts as its keys; entries
+    that 32 bits do not hold are clamped into the pool from their own side."""
+    import kernels.decode_fp4 as m
+    c = Case([48, 32], 4, 2, 64, 0, torch.float16, 16, 37)
+    m.USE_EXT = use_ext
+    try:
+        want = c.call()
+        got = c.call(kv_indptr=torch.tensor([2 ** 32 + 5, 32], device="cuda"))
+        assert torch.equal(got, want)
+        last = c.caches[0][0].shape[0] - 1
+        for codes, scales in c.caches:
+            scales[scales == 255] = 126
+        tables = []
+        for t in c.tables:
+            t[1] = torch.tensor([0, last, -1])
+            t64 = t.long()
+            t64[1] = torch.tensor([-2 ** 32 + 3, 2 ** 32 + 1, -1])
+            tables.append(t64.cuda())
+        want = c.call()
+        got = c.call(k_block_table=tables[0], v_block_table=tables[1])
+        assert torch.equal(got[1], want[1])
+    finally:
+        m.USE_EXT = True

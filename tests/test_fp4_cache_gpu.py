@@ -446,3 +446,28 @@ def test_batches_around_the_staged_ones(n):
             codes[pg, :, off] = R.pack(nib[t])
             t += 1
     assert torch.equal(kc.codes.cpu(), codes)
+
+
+@pytest.mark.parametrize("use_ext", [True, False])
+def test_int64_indices_past_32_bits(use_ext):
+    """Entries and positions that 32 bits do not hold are outside, not another page."""
+    import kernels.fp4_cache as m
+    H, D, page = 1, 64, 4
+    x = rows_of(16, H, D, torch.bfloat16, 36).cuda()
+    far = 2 ** 32
+    kt = torch.tensor([[far, 1], [-2 ** 63, 2], [0, -far], [3, far + 3]], device="cuda")
+    sp = torch.tensor([0, 0, 0, far], device="cuda")
+    ip = torch.arange(0, 17, 4, device="cuda")
+    kc = m.allocate_fp4_cache(4, page, H, D)
+    m.USE_EXT = use_ext
+    try:
+        m.paged_kv_append_fp4(kc, None, kt, None, x, None, ip, start_pos=sp)
+        got, _ = m.paged_kv_gather_fp4(kc, None, kt, None, ip, 16, sp)
+    finally:
+        m.USE_EXT = True
+    val, nib, _ = R.quantize(x.cpu())
+    want = torch.zeros_like(kc.codes.cpu())
+    want[0] = R.pack(nib)[8:12].transpose(0, 1)  # sequence 2 alone has a page
+    assert torch.equal(kc.codes.cpu(), want)
+    assert torch.equal(got[8:12].cpu().double(), val[8:12])
+    assert not got[:8].any() and not got[12:].any()

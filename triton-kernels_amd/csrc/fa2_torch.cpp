@@ -398,6 +398,18 @@ std::tuple<int64_t, at::Tensor, at::Tensor> norm_rope(at::Tensor q, at::Tensor k
 
 using OptTensor = c10::optional<at::Tensor>;
 
+// Indices of the 4-bit cache's calls.  What is outside a pool or past a table must stay
+// so in 32 bits: int64 values saturate (a table entry of 2^32 is not page 0).
+at::Tensor in_32_bits(const at::Tensor& t) {
+  return t.scalar_type() == at::kLong ? t.clamp(INT32_MIN, INT32_MAX) : t;
+}
+at::Tensor fp4_index(const at::Tensor& t, const at::Device& dev) {
+  return index32(in_32_bits(t), dev);
+}
+at::Tensor fp4_table(const at::Tensor& t, const at::Device& dev) {
+  return table32(in_32_bits(t), dev);
+}
+
 // A cache's codes and scales (fp4_cache.check_cache)
 bool cache_ok(const at::Tensor& c, const at::Tensor& s, const at::Device& dev) {
   if (c.device() != dev || s.device() != dev || c.scalar_type() != at::kByte ||
@@ -441,8 +453,8 @@ int64_t fp4_rows(bool append, const at::Tensor& kc, const at::Tensor& ks, const 
     k = ready(k);
     if (v) v = ready(*v);
   }
-  const at::Tensor ip = index32(indptr, dev);
-  const at::Tensor kt = table32(k_table, dev);
+  const at::Tensor ip = fp4_index(indptr, dev);
+  const at::Tensor kt = fp4_table(k_table, dev);
   at::Tensor sp, vt;
   fa2_fp4_rows_params p;
   std::memset(&p, 0, sizeof(p));
@@ -463,11 +475,11 @@ int64_t fp4_rows(bool append, const at::Tensor& kc, const at::Tensor& ks, const 
   p.indptr = ip.data_ptr<int32_t>();
   p.k_block_table = kt.data_ptr<int32_t>();
   if (start_pos) {
-    sp = index32(*start_pos, dev);
+    sp = fp4_index(*start_pos, dev);
     p.start_pos = sp.data_ptr<int32_t>();
   }
   if (vc) {
-    vt = table32(*v_table, dev);
+    vt = fp4_table(*v_table, dev);
     p.table_width = std::min(p.table_width, vt.size(1));
     p.v_table_stride = vt.stride(0);
     p.v_ts = stride_of(*v, 0);
@@ -535,9 +547,9 @@ std::tuple<int64_t, at::Tensor> fp4_decode(const at::Tensor& q, const at::Tensor
   const at::Tensor o4 = squeeze ? out.unsqueeze(2) : out;
   const int64_t M = q4.size(2);
   if (!run_ok(q4, M)) q4 = q4.clone(at::MemoryFormat::Contiguous);
-  const at::Tensor li = index32(lens, dev);
-  const at::Tensor kt = table32(k_table, dev);
-  const at::Tensor vt = table32(v_table, dev);
+  const at::Tensor li = fp4_index(lens, dev);
+  const at::Tensor kt = fp4_table(k_table, dev);
+  const at::Tensor vt = fp4_table(v_table, dev);
   fa2_fp4_decode_params p;
   std::memset(&p, 0, sizeof(p));
   p.dtype = dtype_code(q.scalar_type());

@@ -75,6 +75,12 @@ def table(t: torch.Tensor, device) -> torch.Tensor:
     return t
 
 
+def in_32_bits(t: torch.Tensor) -> torch.Tensor:
+    """``t`` for a conversion to int32 that saturates: what is outside a pool or past a
+    table stays so (a table entry of 2 ** 32 is not page 0)."""
+    return t.clamp(-2 ** 31, 2 ** 31 - 1) if t.dtype == torch.int64 else t
+
+
 _EXT = None
 _EXT_ERROR = None
 

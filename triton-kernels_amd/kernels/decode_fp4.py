@@ -24,7 +24,7 @@ from __future__ import annotations
 import torch
 
 from . import _fa2, _ops
-from ._launch import DTYPES, ext, index_tensor, rows_ok, stride_of, table
+from ._launch import DTYPES, ext, in_32_bits, index_tensor, rows_ok, stride_of, table
 from .fp4_cache import check_cache
 
 # As kernels/decode.py: the C++ extension launches when it is built.
@@ -102,7 +102,8 @@ def _run(name, q, kc, ks, vc, vs, lens, k_table, v_table, causal, workspace=None
         q4 = q4.clone(memory_format=torch.contiguous_format)
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     o4 = out.unsqueeze(2) if q.dim() == 3 else out
-    li, kt, vt = index_tensor(lens, dev), table(k_table, dev), table(v_table, dev)
+    li = index_tensor(in_32_bits(lens), dev)
+    kt, vt = table(in_32_bits(k_table), dev), table(in_32_bits(v_table), dev)
     p = _ops.Fp4DecodeParams()
     p.dtype = DTYPES[q.dtype]
     p.mask = _fa2.MASK_BOTTOM_RIGHT if causal else _fa2.MASK_NONE

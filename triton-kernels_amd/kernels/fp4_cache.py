@@ -37,7 +37,7 @@ from typing import NamedTuple
 import torch
 
 from . import _ops
-from ._launch import DTYPES, aligned, ext, index_tensor, stride_of, table
+from ._launch import DTYPES, aligned, ext, in_32_bits, index_tensor, stride_of, table
 
 # As kernels/decode.py: the C++ extension launches when it is built.
 USE_EXT = True
@@ -217,9 +217,9 @@ def paged_kv_gather_fp4(
 def _rows(name, entry, kc, ks, vc, vs, k_table, v_table, k, v, indptr, start_pos, B):
     """The ctypes launch of the writer and the reader."""
     dev = kc.device
-    ip = index_tensor(indptr, dev)
-    sp = index_tensor(start_pos, dev) if start_pos is not None else None
-    kt = table(k_table, dev)
+    ip = index_tensor(in_32_bits(indptr), dev)
+    sp = index_tensor(in_32_bits(start_pos), dev) if start_pos is not None else None
+    kt = table(in_32_bits(k_table), dev)
     p = _ops.Fp4RowsParams()
     p.dtype = DTYPES[k.dtype]
     p.batch, p.kv_heads, p.head_dim, p.num_rows = B, kc.shape[1], k.shape[2], k.shape[0]
@@ -231,7 +231,7 @@ def _rows(name, entry, kc, ks, vc, vs, k_table, v_table, k, v, indptr, start_pos
     if sp is not None:
         p.start_pos = sp.data_ptr()
     if vc is not None:
-        vt = table(v_table, dev)
+        vt = table(in_32_bits(v_table), dev)
         p.table_width = min(kt.shape[1], vt.shape[1])
         p.v_table_stride = vt.stride(0)
         p.v_ts, p.v_hs = stride_of(v, 0), stride_of(v, 1)
