@@ -471,3 +471,25 @@ def test_int64_indices_past_32_bits(use_ext):
     assert torch.equal(kc.codes.cpu(), want)
     assert torch.equal(got[8:12].cpu().double(), val[8:12])
     assert not got[:8].any() and not got[12:].any()
+
+
+@pytest.mark.parametrize("written", [torch.bfloat16, torch.float32])
+def test_gather_in_fp16_of_other_rows(written):
+    """Every scale that bf16 and fp32 rows give, read in fp16: the values rounded to
+    nearest, to fp16's small numbers and zero below its range and infinity past it."""
+    from kernels import allocate_fp4_cache, paged_kv_append_fp4, paged_kv_gather_fp4
+    e = torch.arange(-101, 120, dtype=torch.float64)
+    x = torch.empty(len(e), 1, 64, dtype=torch.float64)
+    x[:, 0] = torch.tensor([0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.5] * 8, dtype=torch.float64)
+    x = (x * torch.exp2(e)[:, None, None]).to(written)
+    n = len(e)
+    kt = torch.arange(-(-n // 16), dtype=torch.int32).cuda()[None]
+    kc, ip = allocate_fp4_cache(kt.shape[1], 16, 1, 64), indptr([n]).cuda()
+    paged_kv_append_fp4(kc, None, kt, None, x.cuda(), None, ip)
+    val = R.quantize(x)[0]
+    for to in DTYPES:
+        got, _ = paged_kv_gather_fp4(kc, None, kt, None, ip, n, dtype=to)
+        assert torch.equal(got.cpu(), val.to(to)), to
+        out = torch.empty(n, 1, 64, dtype=to, device="cuda")
+        paged_kv_gather_fp4(kc, None, kt, None, ip, n, out=(out, None))  # (out's type)
+        assert torch.equal(out, got)

@@ -164,7 +164,10 @@ def paged_kv_gather_fp4(
     dtype: torch.dtype = torch.bfloat16,
     out=None,
 ):
-    """Rows of the caches in ``dtype``: (k, v) ``[num_rows, KVH, D]`` each, exact.
+    """Rows of the caches in ``dtype``: (k, v) ``[num_rows, KVH, D]`` each; exact in the
+    type of the rows that were written, in bf16 for fp16 rows too, and in fp32.  (fp16
+    rounds what bf16 or fp32 rows left outside 2 ** -24 ... 65504: to its own small
+    numbers, zero or infinity.)
 
     Row ``indptr[b] + j`` is logical row ``start_pos[b] + j`` (``None``: from 0) of
     sequence b; with ``indptr`` as ``kv_indptr`` the result is the ragged K/V of
@@ -172,8 +175,9 @@ def paged_kv_gather_fp4(
     that nothing waits for the device.  Rows past the table width or with a table
     entry outside the cache are zeros; rows that no sequence holds are left as
     they are in ``out`` (a pair of contiguous ``[num_rows, KVH, D]`` tensors,
-    returned; ``None``: new ones, in which such rows hold anything).  ``v_cache``
-    and ``v_block_table`` may both be ``None``: then v is ``None``.
+    returned, whose type stands in ``dtype``'s place; ``None``: new ones, in which
+    such rows hold anything).  ``v_cache`` and ``v_block_table`` may both be ``None``:
+    then v is ``None``.
     """
     name = "paged_kv_gather_fp4"
     x = ext() if USE_EXT else None
