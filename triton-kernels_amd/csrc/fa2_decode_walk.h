@@ -31,8 +31,8 @@ namespace fa2 {
 // Sequences one lane of the locating wave adds up at most.
 constexpr int kWalkMaxPer = 1024;
 
-// MODE of kernels whose paged lengths are capped at a.kv_len, what a row of
-// the block table can hold.
+// MODE of walk_len and walk_locate for paged lengths that are capped at a.kv_len, what
+// a row of the block table can hold.
 constexpr int kModePagedCapped = 3;
 
 // One piece of a unit for this workgroup.
@@ -62,6 +62,7 @@ __device__ __forceinline__ int walk_weight(int Lk) {
 // The Work of packed-head unit (sequence b, kv head kvh, q-block qblk).
 template <int MODE>
 __device__ __forceinline__ Work packed_work(const KArgs& a, int b, int kvh, int qblk) {
+  static_assert(MODE != kModePagedCapped, "lengths are not capped here");
   Work w;
   w.valid = true;
   w.b = b;
@@ -87,7 +88,6 @@ __device__ __forceinline__ Work packed_work(const KArgs& a, int b, int kvh, int 
     w.k_base = kvh * a.k_sh;
     w.v_base = kvh * a.v_sh;
   }
-  if constexpr (MODE == kModePagedCapped) w.Lk = min(w.Lk, a.kv_len);
   if (w.Lk < 0) w.Lk = 0;
   w.off = a.mask == FA2_MASK_CAUSAL_BOTTOM_RIGHT ? w.Lk - a.pack_m : 0;
   return w;
