@@ -26,7 +26,7 @@
 // of 151.  The gathered rows are stored non-temporally (211 -> 197).
 #pragma once
 
-#include "fa2_device.h"
+#include "fa2_values.h"
 
 namespace fa2 {
 
@@ -146,30 +146,6 @@ __device__ __forceinline__ uint32_t fp4_scale(uint32_t bits) {
   return static_cast<uint32_t>(min(max(e, lo), hi));
 }
 
-template <int DT>
-__device__ __forceinline__ void fp4_unpack8(const u32x4* r, float* x) {
-  if constexpr (DT == FA2_DTYPE_F32) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t w = r[i / 4][i % 4];
-      x[i] = __builtin_bit_cast(float, w);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t w = r[0][i];
-      if constexpr (DT == FA2_DTYPE_BF16) {
-        x[2 * i] = __builtin_bit_cast(float, w << 16);
-        x[2 * i + 1] = __builtin_bit_cast(float, w & 0xFFFF0000u);
-      } else {
-        const f32x2 f = __builtin_convertvector(__builtin_bit_cast(f16x2, w), f32x2);
-        x[2 * i] = f[0];
-        x[2 * i + 1] = f[1];
-      }
-    }
-  }
-}
-
 // This thread's words: column `col` of rows `first`, first + step, ...; columns
 // cols ... further where a row has more words than the workgroup threads.
 struct Fp4Share {
@@ -228,7 +204,8 @@ __global__ __launch_bounds__(kF4Threads) void fa2_fp4_append_kernel(Fp4RowsArgs 
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         float x[8];
-        fp4_unpack8<DT>(in[u][v], x);
+#pragma unroll
+        for (int i = 0; i < kW; ++i) unpack16<DT>(in[u][v][i], x + 8 / kW * i);
         uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -264,20 +241,10 @@ __global__ __launch_bounds__(kF4Threads) void fa2_fp4_append_kernel(Fp4RowsArgs 
 // The 8 values of a code word in DT at 2^(sb - 127)
 template <int DT>
 __device__ __forceinline__ void fp4_expand8(uint32_t w, uint32_t sb, u32x4* r) {
-  const float f = __builtin_bit_cast(float, sb << 23);
-  if constexpr (DT == FA2_DTYPE_BF16) {
-    r[0] = (u32x4){
-        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 0)),
-        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 1)),
-        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 2)),
-        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 3))};
-  } else if constexpr (DT == FA2_DTYPE_F16) {
-    r[0] = (u32x4){
-        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 0)),
-        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 1)),
-        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 2)),
-        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 3))};
+  if constexpr (DT != FA2_DTYPE_F32) {
+    r[0] = fp4_values<DT == FA2_DTYPE_BF16>(w, sb);
   } else {
+    const float f = __builtin_bit_cast(float, sb << 23);
     const f32x2 x0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, f, 0);
     const f32x2 x1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, f, 1);
     const f32x2 x2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, f, 2);

@@ -45,6 +45,7 @@
 
 #include "fa2_decode_walk.h"
 #include "fa2_kernel_lds.h"
+#include "fa2_values.h"
 
 namespace fa2 {
 
@@ -77,24 +78,6 @@ __device__ __forceinline__ f32x4 mma16x32(u32x4 a, u32x4 b, f32x4 c) {
   else
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-
-// The 8 values of a code word at the scale with E8M0 byte `sb` (255: NaN).
-template <bool BF>
-__device__ __forceinline__ u32x4 fp4_values(uint32_t w, uint32_t sb) {
-  const float f = __builtin_bit_cast(float, sb << 23);
-  if constexpr (BF)
-    return (u32x4){
-        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 0)),
-        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 1)),
-        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 2)),
-        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 3))};
-  else
-    return (u32x4){
-        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 0)),
-        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 1)),
-        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 2)),
-        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 3))};
 }
 
 // Values 2 B and 2 B + 1 of a code word, at the scale with the float's bits `f`.

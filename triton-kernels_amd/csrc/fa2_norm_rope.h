@@ -18,7 +18,7 @@
 // smaller 3.2 and 5.1.
 #pragma once
 
-#include "fa2_device.h"
+#include "fa2_values.h"
 
 namespace fa2 {
 
@@ -40,44 +40,6 @@ struct NormRopeArgs {
   int32_t pos64;
   float eps;
 };
-
-// 16 bytes of values as fp32
-template <int DT>
-__device__ __forceinline__ void nr_unpack(u32x4 r, float* x) {
-  if constexpr (DT == FA2_DTYPE_F32) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t w = r[i];
-      x[i] = __builtin_bit_cast(float, w);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t w = r[i];
-      if constexpr (DT == FA2_DTYPE_BF16) {
-        x[2 * i] = __builtin_bit_cast(float, w << 16);
-        x[2 * i + 1] = __builtin_bit_cast(float, w & 0xFFFF0000u);
-      } else {
-        const f32x2 f = __builtin_convertvector(__builtin_bit_cast(f16x2, w), f32x2);
-        x[2 * i] = f[0];
-        x[2 * i + 1] = f[1];
-      }
-    }
-  }
-}
-
-template <int DT>
-__device__ __forceinline__ u32x4 nr_pack(const float* x) {
-  u32x4 r;
-  if constexpr (DT == FA2_DTYPE_F32) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(uint32_t, x[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = pack2<DT == FA2_DTYPE_BF16>(x[2 * i], x[2 * i + 1]);
-  }
-  return r;
-}
 
 template <int DT, int D, int U>
 __global__ __launch_bounds__(kNrThreads) void fa2_norm_rope_kernel(NormRopeArgs a) {
@@ -148,16 +110,16 @@ __global__ __launch_bounds__(kNrThreads) void fa2_norm_rope_kernel(NormRopeArgs 
       }
     }
   } else {
-    nr_unpack<DT>(*reinterpret_cast<const u32x4*>(wp + c0 * 16), w);
-    nr_unpack<DT>(*reinterpret_cast<const u32x4*>(wp + c1 * 16), w + E);
+    unpack16<DT>(*reinterpret_cast<const u32x4*>(wp + c0 * 16), w);
+    unpack16<DT>(*reinterpret_cast<const u32x4*>(wp + c1 * 16), w + E);
   }
 
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     if (h0 + u >= heads) break;
     float v[2 * E];
-    nr_unpack<DT>(in[u][0], v);
-    nr_unpack<DT>(in[u][1], v + E);
+    unpack16<DT>(in[u][0], v);
+    unpack16<DT>(in[u][1], v + E);
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < 2 * E; ++i) ss = __builtin_fmaf(v[i], v[i], ss);
@@ -189,11 +151,11 @@ __global__ __launch_bounds__(kNrThreads) void fa2_norm_rope_kernel(NormRopeArgs 
     u32x4* o0 = reinterpret_cast<u32x4*>(o + c0 * 16);
     u32x4* o1 = reinterpret_cast<u32x4*>(o + c1 * 16);
     if constexpr (U > 1) {  // many rows: past the caches
-      __builtin_nontemporal_store(nr_pack<DT>(z), o0);
-      __builtin_nontemporal_store(nr_pack<DT>(z + E), o1);
+      __builtin_nontemporal_store(pack16<DT>(z), o0);
+      __builtin_nontemporal_store(pack16<DT>(z + E), o1);
     } else {
-      *o0 = nr_pack<DT>(z);
-      *o1 = nr_pack<DT>(z + E);
+      *o0 = pack16<DT>(z);
+      *o1 = pack16<DT>(z + E);
     }
   }
 }
