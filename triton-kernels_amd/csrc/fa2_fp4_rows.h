@@ -23,7 +23,10 @@
 // of 1 GiB 5.05; word by word 178), 10.7 k rows appended in 14.7 and gathered in 12 (3.8 and
 // 4.6 TB/s: one latency after another, all workgroups at once), 64 rows in 5.0 and 4.7.
 // Workgroups of 8 / 12 / 16 rows per thread took 154 / 162 / 163 us for the first instead
-// of 151.  The gathered rows are stored non-temporally (211 -> 197).
+// of 151.  Gathered rows of 16 bits are stored non-temporally (139 k rows 157.5 -> 139.6 us; with
+// attention of 16 queries per sequence after it 372 -> 375, which would rather find them
+// in the caches: 17 k rows 53.5 -> 54.5, 2 k rows and 64 queries 30.4 -> 33.3), fp32 rows
+// through the caches (139 k rows 558 -> 285).
 #pragma once
 
 #include "fa2_values.h"
@@ -299,7 +302,15 @@ fa2_fp4_gather_kernel(Fp4RowsArgs a) {
         if (r < rows && at[v][r] != -1 && (v == 0 || a.has_v))
 #pragma unroll
           for (int i = 0; i < kW; ++i)
-            __builtin_nontemporal_store(x[i], reinterpret_cast<u32x4*>(dst[v]) + i);
+          {
+            // fp32: a lane's 32 bytes leave as two stores, which past the caches would
+            // be half lines each
+            u32x4* d = reinterpret_cast<u32x4*>(dst[v]) + i;
+            if constexpr (kW == 1)
+              __builtin_nontemporal_store(x[i], d);
+            else
+              *d = x[i];
+          }
         dst[v] += s.step * a.ts[v];
       }
     }
