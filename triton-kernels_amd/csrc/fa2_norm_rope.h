@@ -12,10 +12,9 @@
 // rotation needs no exchange between lanes, and either order of pairs takes
 // the same E cosines and sines.  A lane group takes U heads of a token: their
 // loads are in flight together, the table's row and the weights are read once.
-// Measured on MI355X, 32 + 8 heads of D128 bf16, us per call: 64 tokens 3.2, 512
-// 4.9, 2048 10.4 (4.1 TB/s), 8192 34.6 (4.97 TB/s; a copy of 1 GiB 5.05).  With
-// cached stores for the larger calls 12.0 and 37.5, with non-temporal ones for the
-// smaller 3.2 and 5.1.
+// Measured on MI355X, 32 + 8 heads of D128 bf16, us: 64 tokens 4.0 and 512 5.7 (kernel
+// traces; the calls are bound by the host), 2048 9.3 (4.6 TB/s), 8192 34.0 (5.05 TB/s; a
+// copy of 1 GiB 5.05), calls back to back; fp32 8192 57.3 (5.9 TB/s).
 #pragma once
 
 #include "fa2_values.h"
@@ -41,7 +40,9 @@ struct NormRopeArgs {
   float eps;
 };
 
-template <int DT, int D, int U>
+// PAST: stores past the caches, all dims rotated in pairs (i, i + D / 2) (fa2_ops.hip has the
+// rule and what it measured).
+template <int DT, int D, int U, bool PAST>
 __global__ __launch_bounds__(kNrThreads) void fa2_norm_rope_kernel(NormRopeArgs a) {
   constexpr int E = DT == FA2_DTYPE_F32 ? 4 : 8;
   constexpr int kLanes = D / (2 * E);  // of a row
@@ -62,9 +63,9 @@ __global__ __launch_bounds__(kNrThreads) void fa2_norm_rope_kernel(NormRopeArgs 
 
   // this lane's chunks, and its first pair
   const int nrot = a.rot / (2 * E);
-  const bool rotated = lane < nrot;
-  const int c0 = rotated && !a.inter ? lane : 2 * lane;
-  const int c1 = rotated && !a.inter ? lane + nrot : 2 * lane + 1;
+  const bool rotated = PAST || lane < nrot, inter = !PAST && a.inter;
+  const int c0 = rotated && !inter ? lane : 2 * lane;
+  const int c1 = rotated && !inter ? lane + nrot : 2 * lane + 1;
 
   u32x4 in[U][2];
 #pragma unroll
@@ -134,7 +135,7 @@ __global__ __launch_bounds__(kNrThreads) void fa2_norm_rope_kernel(NormRopeArgs 
     if (!rotated) {  // (a rotation by cos 1, sin 0 would spread infinities and NaN)
 #pragma unroll
       for (int i = 0; i < 2 * E; ++i) z[i] = v[i];
-    } else if (a.inter) {
+    } else if (inter) {
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         z[2 * i] = v[2 * i] * c[i] - v[2 * i + 1] * s[i];
@@ -150,7 +151,7 @@ __global__ __launch_bounds__(kNrThreads) void fa2_norm_rope_kernel(NormRopeArgs 
     char* o = y + u * a.oh[which];
     u32x4* o0 = reinterpret_cast<u32x4*>(o + c0 * 16);
     u32x4* o1 = reinterpret_cast<u32x4*>(o + c1 * 16);
-    if constexpr (U > 1) {  // many rows: past the caches
+    if constexpr (PAST) {
       __builtin_nontemporal_store(pack16<DT>(z), o0);
       __builtin_nontemporal_store(pack16<DT>(z + E), o1);
     } else {

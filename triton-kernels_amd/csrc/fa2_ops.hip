@@ -51,10 +51,19 @@ int validate_norm_rope(const fa2_norm_rope_params* p) {
 
 template <int DT, int D>
 void launch_norm_rope(const NormRopeArgs& a, int u, uint32_t grid, hipStream_t st) {
-  if (u == 4)
-    hipLaunchKernelGGL((fa2_norm_rope_kernel<DT, D, 4>), dim3(grid), dim3(kNrThreads), 0, st, a);
+  const dim3 g(grid), block(kNrThreads);
+  // Stores past the caches where there are many rows of 16 bits and the lanes' chunks are
+  // runs of memory; two chunks side by side per lane (neighbouring pairs, dims that are
+  // not rotated) are half lines there.  Past / through the caches, us, 40 heads of D128: 2048
+  // tokens 9.3 / 11.8, 8192 34.0 / 35.3, with the 4-bit append after it 45.5 / 46.0, but
+  // with attention over sequences of 1024 after it 133.8 / 129.9; 8192 in neighbouring
+  // pairs 46.7 / 38.1, half of the dims rotated 40.8 / 37.7, fp32 59.4 / 57.3.
+  if (u != 4)
+    hipLaunchKernelGGL((fa2_norm_rope_kernel<DT, D, 1, false>), g, block, 0, st, a);
+  else if (DT != FA2_DTYPE_F32 && a.rot == D && !a.inter)
+    hipLaunchKernelGGL((fa2_norm_rope_kernel<DT, D, 4, DT != FA2_DTYPE_F32>), g, block, 0, st, a);
   else
-    hipLaunchKernelGGL((fa2_norm_rope_kernel<DT, D, 1>), dim3(grid), dim3(kNrThreads), 0, st, a);
+    hipLaunchKernelGGL((fa2_norm_rope_kernel<DT, D, 4, false>), g, block, 0, st, a);
 }
 
 template <int DT>
