@@ -14,16 +14,18 @@
 // in 4.25.  A thread takes 8 values (a code word), four neighbouring lanes a block:
 // its maximum is two quad exchanges.  Rows are located as in fa2_kv_append.h:
 // indptr and the starts in LDS, one lane per row; a thread takes a column of its own of
-// four rows, which the writer loads before their places are known (64 rows 8.8 -> 8.2 us
-// with the reader after it).  The cache's side goes in whole blocks: lane i of a quad
+// four rows, which the writer loads before their places are known (64 rows 5.25 -> 4.95
+// us; 10.7 k rows the same).  The cache's side goes in whole blocks: lane i of a quad
 // moves the four words of the block in row i, and a 4 x 4 transpose within the quad
 // (DPP) turns them from or into a word of each row.  (A word and a scale byte per
 // lane and row takes three memory instructions for each KB of rows, not 1.5.)
-// Measured on MI355X, 8 heads of D128 bf16: 139 k rows gathered in 141 us (5.7 TB/s; a copy
-// of 1 GiB 5.05; word by word 178), 10.7 k rows appended in 14.7 and gathered in 12 (3.8 and
-// 4.6 TB/s: one latency after another, all workgroups at once), 64 rows in 5.0 and 4.7.
-// Workgroups of 8 / 12 / 16 rows per thread took 154 / 162 / 163 us for the first instead
-// of 151.  Gathered rows of 16 bits are stored non-temporally (139 k rows 157.5 -> 139.6 us; with
+// Measured on MI355X, 8 heads of D128 bf16: 139 k rows gathered in 139.6 us (5.7 TB/s; a copy
+// of 1 GiB 5.05), calls back to back; by kernel traces, 10.7 k rows appended in 14.8 and
+// gathered in 12.1 (3.8 and 4.6 TB/s: one latency after another, all workgroups at once),
+// 64 rows in 5.0 and 4.8.  fp32: 139 k rows gathered in 285 (4.5 TB/s), 10.7 k appended in 22.
+// At 8 waves per SIMD, where 139 k rows take 152 us, a word at a time took 178 and
+// workgroups of 8 / 12 / 16 rows per thread 154 / 162 / 163.
+// Gathered rows of 16 bits are stored non-temporally (139 k rows 157.5 -> 139.6 us; with
 // attention of 16 queries per sequence after it 372 -> 375, which would rather find them
 // in the caches: 17 k rows 53.5 -> 54.5, 2 k rows and 64 queries 30.4 -> 33.3), fp32 rows
 // through the caches (139 k rows 558 -> 285).

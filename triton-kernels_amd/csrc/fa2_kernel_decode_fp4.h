@@ -15,8 +15,9 @@
 //     rows bring a tile per wave, across the ends of the pieces; its codes are
 //     read into registers at once (they are few) and the next tile is on its way
 //     while it is computed.  (Tiles in flight in registers instead need the loop
-//     once per tile: 50 KB of code.  More tiles in flight in LDS gain nothing: 49.3
-//     / 47.1 / 46.4 us at 3 / 2 / 1 for 16 x 16000-32768 keys of 4 heads of D128.)
+//     once per tile: 50 KB of code.  More tiles in flight in LDS gained nothing in long
+//     calls of an earlier form of this kernel: 49.3 / 47.1 / 46.4 us at 3 / 2 / 1 for 16 x
+//     16000-32768 keys of 4 heads of D128; short calls were not measured.)
 //   * S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32, up to 16 RB rows
 //     of the unit as columns.  A lane expands D / 4 dims of a key of K, in the
 //     layout of the MFMA's A operand (lane: row l % 16, dims D / 4 * (l / 16)
@@ -25,8 +26,8 @@
 //     by key with v_perm: block i of O^T is dim i of every 16 lanes.  (V back
 //     through LDS in 16 bits, for transpose reads, took two thirds of the LDS
 //     time, and that 75 % of a tile's.)
-//   * P goes to the MFMA as the sum of two 16-bit values, high and low part, which costs 5
-//     % of a long call.  bf16: 16 bits of a weight, off by 2^-18 of it, so that 0.22 % of
+//   * P goes to the MFMA as the sum of two 16-bit values, high and low part, which costs
+//     1 to 3.5 % of a long call, 6 % with 20 rows.  bf16: 16 bits of a weight, off by 2^-18 of it, so that 0.22 % of
 //     the outputs of 64 sequences of 512-8192 keys round the other way than the exact
 //     ones (0.04 % with exact weights); a third part, which makes them exact, takes
 //     64.1 us for 60.9 there, 22.2 for 20.7 with 20 rows.  fp16: 22 bits, and weights from
@@ -34,13 +35,15 @@
 //     off by more than 2^-36 of that (from 1 down, 2^-20 is off by up to 3 %).
 //   * Running maxima and sums in fp32, raised only when a score passes the
 //     maximum by 2^8 (bf16, as in the 16-bit kernels) or 2^4.
-// Measured on MI355X, us (and the cache's bytes per s): 64 sequences of 512-8192 keys,
-// 32 / 8 heads of D128, 66 (4.6 TB/s); 16 of 16000-32768, 32 / 4 heads, 45 (4.6); 16 of
-// 8200 with 8 drafts, 8 / 8 heads of D64, 27 (2.7); 33 of 100-4096 with 5 drafts, 16 / 4
-// heads, 21 (1.6); 4 of 1023, 10.5.  The 16-bit decode reads 6.1 TB/s.  The long calls are
-// bound by the loop's instructions as much as by memory (10 % less with every page in
-// L2); the short ones by what a workgroup does once: 3 us until its first tile is
-// there, about 2 us per change of units, 4 us to count and merge cut units.
+// Measured on MI355X, us per call, calls back to back (and the cache's bytes per s; under
+// the profiler the kernel alone takes 2 to 7 % more than such a call): 64 sequences of
+// 512-8192 keys, 32 / 8 heads of D128, 61 (5.0 TB/s), of D64 51.7 (3.1), of D256 109 (5.8);
+// 16 of 16000-32768, 32 / 4 heads, 44 (4.7); 16 of 8200 with 8 drafts, 8 / 8 heads of D64,
+// 25.3 (2.8); 33 of 100-4096 with 5 drafts, 16 / 4 heads, 20.8 (1.6); 4 of 1023, 10.5.  The
+// 16-bit decode reads 6.1 TB/s.  The long calls are bound by the loop's instructions as
+// much as by memory (8 % less with every page in L2, both under the profiler); the
+// short ones by what a workgroup does once: 3 us until its first tile is there, about 2
+// us per change of units, 4 us to count and merge cut units.
 #pragma once
 
 #include "fa2_decode_walk.h"
@@ -198,12 +201,14 @@ __device__ __forceinline__ int wave_scan(int x) {
 //   * Otherwise a unit takes kGap tiles of room in its stream besides its own, what a
 //     change of units costs, so that workgroups with several have fewer tiles.
 // Neither / the second alone / both, us: 33 x 100-4096 keys with 5 drafts of 16 / 4 heads
-// 32.8 / 25.2 / 21.4; 16 x 4096-8192 of 32 / 2 heads 22.8 / 21.5 / 17.5; 16 x 8200 with 8
-// drafts of 8 / 8 heads of D64 30.5 / 27.6 / 27.2.  kAlign 4 to 16 and kGap 3 to 8 are within 2 %
-// for 16 rows; for 32 rows (8, 6), (12, 8), (16, 8), (24, 4) take 22.2, 21.3, 22.0, 23.8.
+// 32.6 / 24.8 / 20.8; 16 x 4096-8192 of 32 / 2 heads 21.4 / 19.9 / 16.0; 16 x 8200 with 8
+// drafts of 8 / 8 heads of D64 28.8 / 25.6 / 25.3.  (kAlign, kGap) of (8, 5), (8, 3), (8, 6), (4,
+// 5), (16, 8), (24, 4) take 16.0, 16.0, 16.0, 16.6, 16.8, 17.1 for the second, which has 16 rows;
+// for the first, which has 32, (12, 8), (8, 6), (16, 8), (8, 3), (24, 4), (4, 5) take 20.8, 21.7,
+// 21.7, 21.8, 23.5, 27.5.
 //
 // BLOCKS: pages of whole blocks of 16 rows, whose addresses are found once per block
-// instead of once per row: 64 x 512-8192 keys in pages of 16 take 71 us, 75.5 without.
+// instead of once per row: 64 x 512-8192 keys in pages of 16 take 61.5 us, 66.5 without.
 template <int DT, int D, int RB, bool BLOCKS>
 __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
     Fp4Args fa) {
@@ -868,8 +873,11 @@ __global__ __launch_bounds__(kD4Threads, 2) void fa2_decode_fp4_kernel(
     const int full = causal ? min(cur.kb, off + 1) : cur.kb;
     for (int n0 = cur.ka + turn * kD4Tile; n0 < cur.kb; n0 += kStep) {
       // The two waves of a SIMD (i and i + 4) take turns in going first: left to
-      // itself, the older one finishes its share early and the other is alone (4 x
-      // 300-600 keys 7.8 -> 7.5 us, 16 x 8200 with drafts 27.7 -> 27.3).
+      // itself, the older one finishes its share early and the other is alone.  Without /
+      // with, us, runs in turn within 0.1 of each other: 64 x 512-8192 keys 62.25 / 61.2, 33 x
+      // 100-4096 with 5 drafts 21.06 / 20.76, 16 x 2000-8192 of D256 26.65 / 26.32, 16 x 8200 with
+      // drafts 26.69 / 26.40, 4 x 1023 10.6 / 10.5, 16 x 16000-32768 44.5 both; 4 x 300-600, 8.1 /
+      // 8.3.
       if (((n0 / kStep) ^ (wave >> 2)) & 1)
         __builtin_amdgcn_s_setprio(1);
       else

@@ -144,7 +144,8 @@ int fp4_rows(const fa2_fp4_rows_params* p, void* stream, bool append) {
   hipStream_t st = static_cast<hipStream_t>(stream);
   // Gathered rows of more than 256 MB, which pass the caches: fewer writers at once write in
   // longer runs.  8 heads of D128 bf16, us at 8 / 6 / 5 / 4 / 3 waves per SIMD: 139 k rows (570
-  // MB) 153 / 147 / 141 / 145 / 168, 400 k 398 / 383 / 355; 17 k (71 MB) 18.6 at 8, 19.0 at 5.
+  // MB) 152 / 145 / 139.5 / 145 / 168, 400 k 407 / 391 / 364 / 375 / 446; 32 heads, 72 k rows 280 /
+  // 276 / 273 / 266 / 263; fp32 139 k rows 289 / - / 285 / 275 / 280; 17 k bf16 (71 MB) 17.4 at any.
   const bool large =
       p->num_rows > (int64_t(1) << 28) / (p->kv_heads * p->head_dim * eb * (has_v ? 2 : 1));
   auto go = [&](auto dt) {
@@ -163,13 +164,15 @@ int fp4_rows(const fa2_fp4_rows_params* p, void* stream, bool append) {
 }
 
 // The balanced walk's costs, in KV tiles of 64 keys (fa2_decode_walk.h).  A segment of
-// cut units has kD4MinTiles at least (2 instead of 4: 1 x 1023 keys of 8 kv heads 11.0 /
-// 11.3 us, 4 x 1023 12.3 / 11.7); the grid has a workgroup per kD4GridTiles at most (2 or
-// 4: the same).  Units stay whole where that costs at most kD4Whole tiles, in proportion
-// to the CUs that whole units leave idle and half of it at least, or they have kD4Short
-// at most.  Whole / cut (with 8 and 4 in their place), us, 8 kv heads of D128: 1 x 1023 keys 10.3
-// / 11.3, 8 x 700 9.4 / 11.5, 16 x 500-1000 10.8 / 13.2, 16 x 1500 13.2 / 14.5, 32 x
-// 1000-2000 17.2 / 17.8, 8 x 1500 12.9 / 12.3.
+// cut units has kD4MinTiles at least (2 instead of 4: 1 x 2500 keys 14.4 / 12.4 us, 4 x 2500
+// the same); the grid has a workgroup per kD4GridTiles at most (2 or 4: the same).
+// Units stay whole where that costs at most kD4Whole tiles, in proportion to the CUs
+// that whole units leave idle and half of it at least, or they have kD4Short at most.
+// Whole / cut, us, 8 kv heads of D128.  Whole by the rule: 1 x 1023 keys 9.9 / 11.3, 4 x 1023
+// 10.5 / 12.0, 8 x 700 9.1 / 11.4, 16 x 500-1000 10.2 / 12.5, 16 x 1500 12.7 / 14.2, 32 x
+// 1000-2000 15.9 / 16.5, and at its border 8 x 1500 12.5 / 11.7 to 12.5.  Cut: 8 x 1900 14.2 /
+// 13.1, 4 x 2500 16.9 / 14.2, 8 x 2500 17.1 / 14.0; but 24 x 1500-2500, whose 192 units nearly
+// fill the CUs, 17.3 / 22.1: the rule holds no cost of cutting unequal units.
 constexpr int64_t kD4MinTiles = 4;
 constexpr int64_t kD4GridTiles = 2;
 constexpr int64_t kD4Whole = 24, kD4Short = 12;
@@ -220,9 +223,9 @@ int fp4_plan(const fa2_fp4_decode_params* p, Fp4Plan* pl) {
   // More than 16 rows: q-blocks of 32 share K and V, q-blocks of 16 have less to add up
   // (D = 256 has no registers for 32).  16 where every unit of them still has a workgroup
   // and the tables hold kD4Wide tiles per workgroup at most.  20 rows of D128, q-blocks
-  // of 16 / 32, us: 8 kv heads, 4 x 1000 keys 11 / 15, 16 x 2048 (256 units, 16 tiles) 17 /
-  // 21, 16 x 8192 (64 tiles) 54 / 48, 32 x 1000-3000 (512 units) 40 / 37; 4 kv heads, 33 x
-  // 100-2000 (264 units, 17 tiles) 22 / 19.
+  // of 16 / 32, us: 8 kv heads, 4 x 1000 keys 10.6 / 14.6, 16 x 2048 (256 units, 16 tiles) 15.7
+  // / 19.6, 16 x 8192 (64 tiles) 47 / 39.7, 32 x 1000-3000 (512 units) 37.9 / 35.0; 4 kv heads,
+  // 33 x 100-2000 (264 units, 17 tiles) 23.6 / 18.6.
   const bool wide = p->head_dim <= 128 && pl->rows > 16 &&
                     (p->batch * p->kv_heads * cdiv(pl->rows, 16) > wgs ||
                      total * p->kv_heads > kD4Wide * wgs);
