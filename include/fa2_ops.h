@@ -30,8 +30,9 @@ extern "C" {
  *   (a cos - b sin, b cos + a sin),
  * with cos and sin of pair i of the row's token in rope[position][i] and
  * rope[position][rotary_dim / 2 + i].  Pairs are (i, i + rotary_dim / 2), or
- * with `interleaved` (2 i, 2 i + 1).  Computed in fp32, rounded once.  A token
- * whose position is outside [0, positions) gives NaN rows.
+ * with `interleaved` (2 i, 2 i + 1).  Computed in fp32, rounded once: a bf16 or fp32
+ * row whose sum of squares passes fp32's range gives zeros.  A token whose
+ * position is outside [0, positions) gives NaN rows.
  *
  * Token t of q is row t % q_rows of batch t / q_rows: token-major [T, H, D] has
  * q_rows = T (q_sb unused), [B, H, M, D] has q_rows = M; likewise k. */
@@ -130,7 +131,7 @@ typedef struct fa2_fp4_decode_params {
   const int32_t* kv_lens;       /* [batch]                                      */
   const int32_t* k_block_table; /* [batch, table_width]                         */
   const int32_t* v_block_table;
-  float softmax_scale;
+  float softmax_scale;          /* > 0, finite                                  */
   int32_t reserved0;
   void* workspace;          /* 16-byte aligned, any prior content; one per call in flight */
   size_t workspace_bytes;

@@ -225,3 +225,13 @@ def test_rope_table():
     for r in (0, 8, -16):
         with pytest.raises(ValueError):
             build_rope_table(10, r, device="cpu")
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.0, -0.1, float("nan"), float("inf"), -float("inf")])
+def test_decode_scale_refusals(scale):
+    """Refused before any launch; the workspace's size does not ask for one."""
+    n = ctypes.c_size_t(0)
+    p = decode_params(softmax_scale=scale)
+    assert _ops.lib().fa2_fp4_decode_workspace_size(ctypes.byref(p), ctypes.byref(n)) == 0
+    p.workspace_bytes = n.value
+    assert _ops.lib().fa2_fp4_decode(ctypes.byref(p), None) == 5

@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "fa2_host.h"
 #include "fa2_fp4_rows.h"
@@ -387,6 +388,8 @@ extern "C" int fa2_fp4_decode(const fa2_fp4_decode_params* p, void* stream) {
     return FA2_ERR_NULL_POINTER;
   if (!p->kv_lens || !p->k_block_table || !p->v_block_table || p->num_pages == 0)
     return FA2_ERR_PAGED_ARGS;
+  // (the kernel's running maximum is that of q . k, the scores' only for scales above 0)
+  if (!(p->softmax_scale > 0.f && std::isfinite(p->softmax_scale))) return FA2_ERR_BAD_SHAPE;
   const void* ptrs[] = {p->q, p->o, p->k_codes, p->v_codes};
   for (const void* x : ptrs)
     if (!aligned16(x)) return FA2_ERR_ALIGNMENT;

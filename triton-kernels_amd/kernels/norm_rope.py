@@ -11,9 +11,10 @@ keys.  For each head row x of ``head_dim`` values::
 over the pairs (i, i + R/2) of y's first R values, or (2i, 2i + 1) with
 ``interleaved``; cos and sin of the pair and the token's position come from a
 table (:func:`build_rope_table`), whose width is R.  The arithmetic is fp32
-whatever the tensors' type, rounded once at the end.  The computation runs in
-``libfa2.so`` (``fa2_norm_rope``, include/fa2_ops.h); no fallback, and no
-backward pass, like the rest of the package.
+whatever the tensors' type, rounded once at the end (so a bf16 or fp32 row whose
+sum of squares passes fp32's range, values around 2 ** 60, gives zeros).  The
+computation runs in ``libfa2.so`` (``fa2_norm_rope``, include/fa2_ops.h); no
+fallback, and no backward pass, like the rest of the package.
 """
 
 from __future__ import annotations
