@@ -85,7 +85,7 @@ typedef struct fa2_fp4_rows_params {
   int64_t batch, kv_heads, head_dim;
   int64_t num_rows;         /* rows of k / v                                    */
   int64_t page_size, num_pages;
-  int64_t table_width;      /* columns of the block tables                      */
+  int64_t table_width;      /* columns of the block tables (0: they may be NULL) */
   int64_t k_table_stride, v_table_stride;
   int64_t k_ts, k_hs, v_ts, v_hs; /* element strides (row, head) of k / v       */
   void* k;                  /* [num_rows, kv_heads, head_dim]                   */
@@ -129,7 +129,7 @@ typedef struct fa2_fp4_decode_params {
   const uint8_t* v_codes;
   const uint8_t* v_scales;
   const int32_t* kv_lens;       /* [batch]                                      */
-  const int32_t* k_block_table; /* [batch, table_width]                         */
+  const int32_t* k_block_table; /* [batch, table_width]; NULL where that is 0    */
   const int32_t* v_block_table;
   float softmax_scale;          /* > 0, finite                                  */
   int32_t reserved0;

@@ -493,3 +493,29 @@ def test_gather_in_fp16_of_other_rows(written):
         out = torch.empty(n, 1, 64, dtype=to, device="cuda")
         paged_kv_gather_fp4(kc, None, kt, None, ip, n, out=(out, None))  # (out's type)
         assert torch.equal(out, got)
+
+
+@pytest.mark.parametrize("use_ext", [True, False])
+@pytest.mark.parametrize("only_k", [False, True])
+def test_tables_without_columns(use_ext, only_k):
+    """No row has a place: nothing is written, rows are zeros, outputs NaN."""
+    import kernels.decode_fp4 as d
+    import kernels.fp4_cache as m
+    H, D = 2, 64
+    kc, vc = (m.allocate_fp4_cache(2, 16, H, D) for _ in range(2))
+    none = torch.empty(3, 0, dtype=torch.int32, device="cuda")
+    x = rows_of(9, H, D, torch.float16, 38).cuda()
+    ip = indptr([4, 0, 5]).cuda()
+    m.USE_EXT = d.USE_EXT = use_ext
+    args = (kc, None, none, None) if only_k else (kc, vc, none, none)
+    try:
+        m.paged_kv_append_fp4(*args, x, None if only_k else x, ip)
+        got = m.paged_kv_gather_fp4(*args, ip, 9, dtype=torch.float16)
+        out = d.decode_attention_fp4(x[:3], kc, vc, kv_indptr=ip[1:], k_block_table=none,
+                                     v_block_table=none)
+    finally:
+        m.USE_EXT = d.USE_EXT = True
+    for c in (kc, vc):
+        assert not c.codes.any() and not c.scales.any()
+    assert not got[0].any() and (only_k or not got[1].any())
+    assert torch.isnan(out).all()

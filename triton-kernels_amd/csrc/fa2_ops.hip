@@ -105,8 +105,9 @@ int fp4_rows(const fa2_fp4_rows_params* p, void* stream, bool append) {
   if (s != FA2_OK) return s;
   if (p->batch == 0 || p->num_rows == 0) return FA2_OK;
   const bool has_v = p->v || p->v_codes || p->v_scales || p->v_block_table;
-  if (!p->k || !p->k_codes || !p->k_scales || !p->indptr || !p->k_block_table ||
-      (has_v && (!p->v || !p->v_codes || !p->v_scales || !p->v_block_table)))
+  const bool tables = p->table_width > 0;  // (tables without columns may be null)
+  if (!p->k || !p->k_codes || !p->k_scales || !p->indptr || (tables && !p->k_block_table) ||
+      (has_v && (!p->v || !p->v_codes || !p->v_scales || (tables && !p->v_block_table))))
     return FA2_ERR_NULL_POINTER;
   if (!aligned16(p->k) || !aligned16(p->k_codes) ||
       (has_v && (!aligned16(p->v) || !aligned16(p->v_codes))))
@@ -386,7 +387,8 @@ extern "C" int fa2_fp4_decode(const fa2_fp4_decode_params* p, void* stream) {
   if (fp4_empty(p)) return FA2_OK;
   if (!p->q || !p->o || !p->k_codes || !p->k_scales || !p->v_codes || !p->v_scales)
     return FA2_ERR_NULL_POINTER;
-  if (!p->kv_lens || !p->k_block_table || !p->v_block_table || p->num_pages == 0)
+  if (!p->kv_lens || p->num_pages == 0 ||
+      (p->table_width > 0 && (!p->k_block_table || !p->v_block_table)))
     return FA2_ERR_PAGED_ARGS;
   // (the kernel's running maximum is that of q . k, the scores' only for scales above 0)
   if (!(p->softmax_scale > 0.f && std::isfinite(p->softmax_scale))) return FA2_ERR_BAD_SHAPE;
