@@ -19,16 +19,16 @@
 // moves the four words of the block in row i, and a 4 x 4 transpose within the quad
 // (DPP) turns them from or into a word of each row.  (A word and a scale byte per
 // lane and row takes three memory instructions for each KB of rows, not 1.5.)
-// Measured on MI355X, 8 heads of D128 bf16: 139 k rows gathered in 139.6 us (5.7 TB/s; a copy
+// Measured on MI355X, 8 heads of D128 bf16: 156 k rows gathered in 139.6 us (5.8 TB/s; a copy
 // of 1 GiB 5.05), calls back to back; by kernel traces, 10.7 k rows appended in 14.8 and
 // gathered in 12.1 (3.8 and 4.6 TB/s: one latency after another, all workgroups at once),
-// 64 rows in 5.0 and 4.8.  fp32: 139 k rows gathered in 285 (4.5 TB/s), 10.7 k appended in 22.
-// At 8 waves per SIMD, where 139 k rows take 152 us, a word at a time took 178 and
+// 64 rows in 5.0 and 4.8.  fp32: 156 k rows gathered in 285 (5.1 TB/s), 10.7 k appended in 22.
+// At 8 waves per SIMD, where 156 k rows take 152 us, a word at a time took 178 and
 // workgroups of 8 / 12 / 16 rows per thread 154 / 162 / 163.
-// Gathered rows of 16 bits are stored non-temporally (139 k rows 157.5 -> 139.6 us; with
+// Gathered rows of 16 bits are stored non-temporally (156 k rows 157.5 -> 139.6 us; with
 // attention of 16 queries per sequence after it 372 -> 375, which would rather find them
 // in the caches: 17 k rows 53.5 -> 54.5, 2 k rows and 64 queries 30.4 -> 33.3), fp32 rows
-// through the caches (139 k rows 558 -> 285).
+// through the caches (156 k rows 558 -> 285).
 #pragma once
 
 #include "fa2_values.h"

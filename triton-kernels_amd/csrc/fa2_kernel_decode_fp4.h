@@ -36,14 +36,14 @@
 //   * Running maxima and sums in fp32, raised only when a score passes the
 //     maximum by 2^8 (bf16, as in the 16-bit kernels) or 2^4.
 // Measured on MI355X, us per call, calls back to back (and the cache's bytes per s; under
-// the profiler the kernel alone takes 2 to 7 % more than such a call): 64 sequences of
-// 512-8192 keys, 32 / 8 heads of D128, 61 (5.0 TB/s), of D64 51.7 (3.1), of D256 109 (5.8);
-// 16 of 16000-32768, 32 / 4 heads, 44 (4.7); 16 of 8200 with 8 drafts, 8 / 8 heads of D64,
-// 25.3 (2.8); 33 of 100-4096 with 5 drafts, 16 / 4 heads, 20.8 (1.6); 4 of 1023, 10.5.  The
-// 16-bit decode reads 6.1 TB/s.  The long calls are bound by the loop's instructions as
-// much as by memory (8 % less with every page in L2, both under the profiler); the
-// short ones by what a workgroup does once: 3 us until its first tile is there, about 2
-// us per change of units, 4 us to count and merge cut units.
+// the profiler the kernel alone takes 3 to 12 % more than such a call): 64 sequences of
+// 512-8192 keys, 32 / 8 heads of D128, 61 (5.1 TB/s), of D64 52 (3.1), of D256 109 (5.8);
+// 16 of 16000-32768, 32 / 4 heads, 43 (4.8); 16 of 8200 with 8 drafts, 8 / 8 heads of D64, 25
+// (2.9); 33 of 100-4096 with 5 drafts, 16 / 4 heads, 21 (1.6); 4 of 1023, 10.5.  The 16-bit
+// decode reads 6.1 TB/s.  The long calls are bound by the loop's instructions as much as
+// by memory (6 to 8 % less with every page in L2, both under the profiler); the short
+// ones by what a workgroup does once: 3 us until its first tile is there, about 2 us
+// per change of units, 4 us to count and merge cut units.
 #pragma once
 
 #include "fa2_decode_walk.h"

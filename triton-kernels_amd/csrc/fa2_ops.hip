@@ -145,9 +145,9 @@ int fp4_rows(const fa2_fp4_rows_params* p, void* stream, bool append) {
   const dim3 grid(static_cast<uint32_t>(cdiv(p->num_rows, a.block_rows)));
   hipStream_t st = static_cast<hipStream_t>(stream);
   // Gathered rows of more than 256 MB, which pass the caches: fewer writers at once write in
-  // longer runs.  8 heads of D128 bf16, us at 8 / 6 / 5 / 4 / 3 waves per SIMD: 139 k rows (570
+  // longer runs.  8 heads of D128 bf16, us at 8 / 6 / 5 / 4 / 3 waves per SIMD: 156 k rows (638
   // MB) 152 / 145 / 139.5 / 145 / 168, 400 k 407 / 391 / 364 / 375 / 446; 32 heads, 72 k rows 280 /
-  // 276 / 273 / 266 / 263; fp32 139 k rows 289 / - / 285 / 275 / 280; 17 k bf16 (71 MB) 17.4 at any.
+  // 276 / 273 / 266 / 263; fp32 156 k rows 289 / - / 285 / 275 / 280; 17 k bf16 (71 MB) 17.4 at any.
   const bool large =
       p->num_rows > (int64_t(1) << 28) / (p->kv_heads * p->head_dim * eb * (has_v ? 2 : 1));
   auto go = [&](auto dt) {
