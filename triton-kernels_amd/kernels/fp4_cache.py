@@ -27,7 +27,9 @@ for bf16 and fp32 rows, so that every cached value is exact in the rows' type;
 past 49152 fp16 rows saturate.  Inside that range a value is off by at most 1/5 of
 its block's largest (5 steps become 4).  A block with an infinity or NaN is NaN.
 
-The computation runs in ``libfa2.so`` (include/fa2_ops.h); no fallback.
+Tables, lengths, starts and prefix sums are int32; other integer types are
+converted, int64 saturating, so that what is outside a pool stays outside.  The
+computation runs in ``libfa2.so`` (include/fa2_ops.h); no fallback.
 """
 
 from __future__ import annotations
