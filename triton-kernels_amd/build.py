@@ -18,7 +18,8 @@ ROOT = os.path.dirname(HERE)
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 CXX = os.environ.get("CXX", "g++")
 # translation units (compiled in parallel); they include the csrc/*.h
-SOURCES = [os.path.join(HERE, "csrc", n) for n in ("fa2_fwd.hip", "fa2_ops.hip")]
+SOURCES = [os.path.join(HERE, "csrc", n) for n in ("fa2_fwd.hip", "fa2_ops.hip",
+                                                   "fa2_latent.hip")]
 OUT_DIR = os.path.join(HERE, "kernels")
 OUT = os.path.join(OUT_DIR, "libfa2.so")
 EXT_NAME = "fa2_torch"

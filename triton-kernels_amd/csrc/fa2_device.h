@@ -158,6 +158,9 @@ struct KArgs {
   int32_t walk_streams, walk_segs, walk_min, walk_whole, walk_short;
   int32_t walk_rounds;       // whole units per workgroup at most
   int32_t walk_dj, walk_ds;  // gridDim.x / walk_streams, gridDim.x % walk_streams
+  // Latent attention, expanded form: the rows that all heads' keys share
+  const void* kr;
+  int64_t kr_sb, kr_ss;
 };
 
 constexpr int kMergeCountBits = 24;

@@ -188,21 +188,31 @@ __device__ void pp_bal_locate(const KArgs& a, int x, int upp, int ns, int k, int
 // kernel, one split; likewise separate.
 // F32: dense fp32 tensors (Plan::conv): q, k and v are fp16 copies, an unsplit
 // unit writes the fp32 output.
+// DR: the expanded form of latent attention (Hq == Hkv, KArgs::qpair): rows of q
+// have DR more values, the keys' DR more are those of the sequence's rows kr, which
+// all heads share; their tiles have LDS slots of their own, and partials go to slot
+// 2 * pair + group.
 template <int DT, int D, int MODE, bool BUF, bool CLAIM = false, bool INLINE = false,
-          bool BAL = false, bool F32 = false>
+          bool BAL = false, bool F32 = false, int DR = 0>
 __global__ __launch_bounds__(kPPThreads, 1) void fa2_fwd_pp_kernel(KArgs a) {
   static_assert(DT != FA2_DTYPE_F32, "fp32 uses the register-staged kernel");
   static_assert(!INLINE || (MODE == FA2_LAYOUT_RAGGED && !CLAIM), "inline plans: ragged, static walk");
   static_assert(!BAL || (MODE == FA2_LAYOUT_PAGED && !CLAIM && !INLINE), "balanced walk: paged");
+  static_assert(DR == 0 || (DR == 64 && MODE != FA2_LAYOUT_PAGED && !F32), "latent attention");
   constexpr bool BF = Elt<DT>::kBF;
-  constexpr int DC = D / 16;  // MFMA k-steps of S (16 head dims each)
+  constexpr int DK = D / 16;          // MFMA k-steps of S (16 head dims each)
+  constexpr int DC = DK + DR / 16;    // ... and of a row's shared part
   constexpr int DB = D / 32;  // 32-dim blocks of O^T
   constexpr int SB = kBN / 32;
   using G = SwzGeo<D>;
+  using GR = SwzGeo<64>;
   using LD = DirectLoader<D, MODE, BUF, DT, kWaves>;  // group 0 loads
+  using LR = DirectLoader<64, MODE, BUF, DT, kWaves>;
   constexpr int kI = LD::kInstr;
+  constexpr int kIK = kI + (DR ? LR::kInstr : 0);  // loads of K's part
   constexpr int kTile = G::kTileBytes;
-  constexpr int kSlotBytes = 2 * kPPSlots * kTile;
+  constexpr int kRTile = DR ? GR::kTileBytes : 0;
+  constexpr int kSlotBytes = kPPSlots * (2 * kTile + kRTile);
   constexpr int kStageDims = 64;  // output staged in passes of 64 dims
   constexpr int kStores = F32 ? kOStoreOpsF32<D> : kOStoreOps<D, kStageDims>;
 
@@ -267,6 +277,25 @@ __global__ __launch_bounds__(kPPThreads, 1) void fa2_fwd_pp_kernel(KArgs a) {
     voff0 = r * G::kRowBytes + (((dim >> 3) ^ G::v(r)) * 16) + (dim & 7) * 2;
   }
   const LD ld(a, wq, lane);
+  // the shared part's loads: those of a K of its own
+  KArgs ar = a;
+  if constexpr (DR > 0) {
+    ar.k = a.kr;
+    ar.k_ss = ar.v_ss = a.kr_ss;
+  }
+  const LR ldr(ar, wq, lane);
+  const uint32_t roff0 = l32 * GR::kRowBytes + ((hi ^ GR::k(l32)) * 16);
+  auto issue_k = [&](const Work& w, int k0, char* dst, char* rdst) {
+    ld.template issue<false>(a, w, k0, dst);
+    if constexpr (DR > 0) {
+      Work wr = w;
+      if constexpr (MODE == FA2_LAYOUT_DENSE)
+        wr.k_base = w.b * a.kr_sb;
+      else
+        wr.k_base = (ip ? __builtin_amdgcn_readfirstlane(ip->ki[w.b]) : a.kv_indptr[w.b]) * a.kr_ss;
+      ldr.template issue<false>(ar, wr, k0, rdst);
+    }
+  };
 
   // Persistent: gridDim.x workgroups walk the units (heaviest first) in
   // rounds; odd rounds run backwards over blocks of kXcds workgroups, which
@@ -365,14 +394,14 @@ __global__ __launch_bounds__(kPPThreads, 1) void fa2_fwd_pp_kernel(KArgs a) {
   // wait until at most n of this wave's vector memory operations are
   // outstanding; n is one of the counts this kernel produces
   auto wait_vm = [&](int n) {
-    if (n >= 2 * kI + kStores)
-      pp_wait_vm<2 * kI + kStores>();
+    if (n >= kI + kIK + kStores)
+      pp_wait_vm<kI + kIK + kStores>();
     else if (n >= kI + kStores)
       pp_wait_vm<kI + kStores>();
-    else if (n >= kStores && kStores > 2 * kI)
+    else if (n >= kStores && kStores > kI + kIK)
       pp_wait_vm<kStores>();
-    else if (n >= 2 * kI)
-      pp_wait_vm<2 * kI>();
+    else if (n >= kI + kIK)
+      pp_wait_vm<kI + kIK>();
     else if (n >= kI)
       pp_wait_vm<kI>();
     else if (n >= DC)
@@ -432,6 +461,9 @@ __global__ __launch_bounds__(kPPThreads, 1) void fa2_fwd_pp_kernel(KArgs a) {
 
     auto kslot = [&](int i) { return lds + ((gb + i) % kPPSlots) * kTile; };
     auto vslot = [&](int i) { return lds + (kPPSlots + (gb + i) % kPPSlots) * kTile; };
+    auto rslot = [&](int i) {
+      return lds + 2 * kPPSlots * kTile + ((gb + i) % kPPSlots) * kRTile;
+    };
     const int qrow = u.q0 + wq * kWaveRows + l32;
     const int wq_first = u.q0 + wq * kWaveRows;
 
@@ -450,6 +482,7 @@ __global__ __launch_bounds__(kPPThreads, 1) void fa2_fwd_pp_kernel(KArgs a) {
       // would otherwise sit between the reads the region is ordering)
       const uint32_t vbase = kPV ? lds_addr_of(vslot(i - 1)) : 0u;
       const uint32_t kbase = kS ? lds_addr_of(kslot(i)) : 0u;
+      const uint32_t rbase = kS && DR ? lds_addr_of(rslot(i)) : 0u;
       // a scheduling region of its own: nothing moves in or out
       __builtin_amdgcn_sched_barrier(0);
 #if FA2_PP_PRIO
@@ -466,6 +499,7 @@ __global__ __launch_bounds__(kPPThreads, 1) void fa2_fwd_pp_kernel(KArgs a) {
       constexpr int kAhead = FA2_PP_AHEAD < kN ? FA2_PP_AHEAD : kN;
       const lds_char_t* vl = lds_ptr(vbase);
       const lds_char_t* kl = lds_ptr(kbase);
+      const lds_char_t* rl = lds_ptr(rbase);
       auto frag = [&](auto kc) -> u32x4 {
         constexpr int k = decltype(kc)::value;
         if constexpr (k < kNPV) {
@@ -480,7 +514,11 @@ __global__ __launch_bounds__(kPPThreads, 1) void fa2_fwd_pp_kernel(KArgs a) {
           return (u32x4){l2[0], l2[1], h2[0], h2[1]};
         } else {
           constexpr int kk = k - kNPV, cc = kk / SB, sb = kk % SB;
-          return *(const lds_u32x4_t*)(kl + sb * 32 * G::kRowBytes + (koff0 ^ (32u * cc)));
+          if constexpr (cc >= DK)
+            return *(const lds_u32x4_t*)(rl + sb * 32 * GR::kRowBytes +
+                                         (roff0 ^ (32u * (cc - DK))));
+          else
+            return *(const lds_u32x4_t*)(kl + sb * 32 * G::kRowBytes + (koff0 ^ (32u * cc)));
         }
       };
       auto mma_k = [&](auto kc, const u32x4& f) {
@@ -597,8 +635,8 @@ __global__ __launch_bounds__(kPPThreads, 1) void fa2_fwd_pp_kernel(KArgs a) {
         n += kI;
       }
       if (i + 2 < T) {
-        ld.template issue<false>(a, w, (u.t_begin + i + 2) * kBN, kslot(i + 2));
-        n += kI;
+        issue_k(w, (u.t_begin + i + 2) * kBN, kslot(i + 2), rslot(i + 2));
+        n += kIK;
       }
       return n;
     };
@@ -608,8 +646,10 @@ __global__ __launch_bounds__(kPPThreads, 1) void fa2_fwd_pp_kernel(KArgs a) {
       char* k0s = lds + (g0 % kPPSlots) * kTile;
       char* k1s = lds + ((g0 + 1) % kPPSlots) * kTile;
       char* v0s = lds + (kPPSlots + g0 % kPPSlots) * kTile;
-      ld.template issue<false>(a, v.w, v.t_begin * kBN, k0s);
-      if (v.T > 1) ld.template issue<false>(a, v.w, (v.t_begin + 1) * kBN, k1s);
+      char* r0s = lds + 2 * kPPSlots * kTile + (g0 % kPPSlots) * kRTile;
+      char* r1s = lds + 2 * kPPSlots * kTile + ((g0 + 1) % kPPSlots) * kRTile;
+      issue_k(v.w, v.t_begin * kBN, k0s, r0s);
+      if (v.T > 1) issue_k(v.w, (v.t_begin + 1) * kBN, k1s, r1s);
       ld.template issue<true>(a, v.w, v.t_begin * kBN, v0s);
     };
 
@@ -623,14 +663,14 @@ __global__ __launch_bounds__(kPPThreads, 1) void fa2_fwd_pp_kernel(KArgs a) {
           // K(1) and V(0) go out once K(0) and Q have landed: at a launch
           // every workgroup fetches these at once, and the first MFMA phase
           // needs only K(0) and Q (c5 +1.5 %, c2 and c3 unchanged)
-          ld.template issue<false>(a, w, u.t_begin * kBN, kslot(0));
+          issue_k(w, u.t_begin * kBN, kslot(0), rslot(0));
           pp_wait_vm<0>();
-          if (T > 1) ld.template issue<false>(a, w, (u.t_begin + 1) * kBN, kslot(1));
+          if (T > 1) issue_k(w, (u.t_begin + 1) * kBN, kslot(1), rslot(1));
           ld.template issue<true>(a, w, u.t_begin * kBN, vslot(0));
         } else {
           // K(0) and Q have landed: what was issued after K(0) may be in
           // flight (K(1), V(0), and the previous unit's output stores)
-          wait_vm((T > 1 ? 2 * kI : kI) + kStores);
+          wait_vm((T > 1 ? kIK + kI : kI) + kStores);
         }
         if (claim_now) {
           pp_wait_vm<0>();
@@ -801,8 +841,8 @@ __global__ __launch_bounds__(kPPThreads, 1) void fa2_fwd_pp_kernel(KArgs a) {
       } else {
         // partials go to the slot the one-head-per-unit layout gives this
         // head (decode_work with heads = 1), which the combine kernel reads
-        const int unit =
-            ((w.pair / kXcds) * group + w.hg + grp) * kXcds + w.pair % kXcds;
+        const int unit = DR ? 2 * w.pair + grp
+                            : ((w.pair / kXcds) * group + w.hg + grp) * kXcds + w.pair % kXcds;
         const int64_t slot = static_cast<int64_t>(split) * a.part_slots + unit;
         const int rr = wq * kWaveRows + l32;
         if (INLINE && a.merge_ctr)

@@ -1,0 +1,510 @@
+// fa2_kernel_rows.h - decode attention with many query rows per K/V row: the
+// absorbed form of latent attention (every head reads the same cached row) and
+// trees of drafts over 16-bit K/V caches.
+#pragma once
+
+#include "fa2_decode_walk.h"
+#include "fa2_kernel_pp.h"
+
+namespace fa2 {
+
+constexpr int kRbWaves = 4;
+constexpr int kRbThreads = 64 * kRbWaves;
+constexpr int kRbTable = 2048;  // block-table entries in LDS (K and V share them)
+constexpr int kRbMaxTree = 64;  // drafts of a tree: bits of a mask word
+
+// Mask of a call beyond enum fa2_mask: the drafts that each draft sees.
+constexpr int kMaskTree = 3;
+
+struct RowsArgs {
+  KArgs a;  // q rows: token m of head h at h * q_sh + m * q_ss; o rows: o_ss apart
+  const uint8_t* tree;  // bool [batch, pack_m, pack_m]
+  int64_t tree_sb, tree_sr;
+  int32_t num_pages, table_width;
+  uint32_t page_mul, page_sh;  // n / page_size = umulhi(2 n, page_mul) >> page_sh, n < 2^30
+};
+
+// Rows of DK values in LDS: 16-byte chunks, chunk c of row r at c ^ swz(r) (in groups
+// of 8 chunks, or of 16 where a row is a multiple of 256 bytes).  Bits of r run
+// backwards through the swizzle, so that both reads hit distinct banks: 16 rows at one
+// chunk (K, one row per lane) and 4 rows at 4 neighbouring chunks (V, transposed).
+template <int DK>
+struct RowsGeo {
+  static constexpr int kNC = DK / 8;  // chunks of a row
+  static constexpr int kRowBytes = DK * 2;
+  static constexpr bool kWide = kNC % 16 == 0;
+  static constexpr int kGI = kNC / 8;  // 1 KB loads of 8 rows
+  static_assert(kNC % 8 == 0, "rows of whole swizzle groups");
+  static constexpr int kG = kWide ? 8 : 4;  // 32-byte steps of a swizzle group
+  __device__ __forceinline__ static uint32_t swz(int r) {
+    return kWide ? ((r & 1) << 3) | ((r & 2) << 1) | ((r & 4) >> 1) | ((r & 8) >> 3)
+                 : ((r & 2) << 1) | ((r & 4) >> 1) | ((r & 8) >> 3);
+  }
+};
+
+// Tile shape: keys of a tile and LDS slots.
+template <int DK, int DV, bool LAT>
+struct RowsTile {
+  using G = RowsGeo<DK>;
+  static constexpr int kRow = G::kRowBytes + (LAT ? 0 : DV * 2);
+  static constexpr int kKeys = kRow * 64 <= 40960 ? 64 : 32;
+  static constexpr int kSlot = kRow * kKeys;
+  static constexpr int kSlots = 150000 / kSlot < 6 ? 150000 / kSlot : 6;
+  static_assert(kSlots >= 3, "tiles in flight");
+};
+
+struct RowsPiece {
+  int b, kvh, qblk, Lk;
+  int t0, T;     // first tile of kBN keys and their count
+  int np, mine;  // pieces of the unit, this one's index
+  int us, W, unit;
+};
+
+// Wait until at most n tiles of IPT loads each are in flight (n <= MAXN, uniform).
+template <int IPT, int MAXN>
+__device__ __forceinline__ void rows_wait(int n) {
+  static_assert(MAXN * IPT <= 63 && MAXN <= 4, "vmcnt field");
+  if (MAXN >= 4 && n >= 4) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(MAXN >= 4 ? 4 * IPT : 0) : "memory");
+  else if (MAXN >= 3 && n >= 3) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(MAXN >= 3 ? 3 * IPT : 0) : "memory");
+  else if (MAXN >= 2 && n >= 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(MAXN >= 2 ? 2 * IPT : 0) : "memory");
+  else if (n >= 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(IPT) : "memory");
+  else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+// 16 bytes per lane to LDS from a scalar base and a 32-bit offset per lane (wait states
+// as dma_buffer_x4).
+__device__ __forceinline__ void rows_dma(uint64_t base, uint32_t off, uint32_t lds_addr) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1"
+               :
+               : "v"(off), "s"(base),
+                 "{m0}"(__builtin_amdgcn_readfirstlane(static_cast<int>(lds_addr))));
+}
+
+template <int DT, int DK, int DV, bool LAT, int RG, int MODE>
+__global__ __launch_bounds__(kRbThreads, 1) void fa2_decode_rows_kernel(RowsArgs ra) {
+  static_assert(DT != FA2_DTYPE_F32, "16-bit rows");
+  static_assert(RG == 1 || RG == 2 || RG == 4, "row groups");
+  constexpr bool BF = Elt<DT>::kBF;
+  constexpr bool kPaged = MODE == FA2_LAYOUT_PAGED;
+  constexpr int LM = kPaged ? kModePagedCapped : MODE;
+  using GK = RowsGeo<DK>;
+  using GV = RowsGeo<LAT ? DK : DV>;
+  using TL = RowsTile<DK, DV, LAT>;
+  constexpr int TK = TL::kKeys, NS = TL::kSlots, SB = TK / 32;
+  constexpr int DC = DK / 16;               // k-steps of S
+  constexpr int DG = kRbWaves / RG;         // waves that share a row group's dims
+  constexpr int DBW = DV / 32 / DG;         // 32-dim blocks of a wave's O^T
+  static_assert(DBW >= 1, "dims of a wave");
+  constexpr int GPW = TK / 32;              // 8-row groups a wave loads per tile
+  constexpr int IPT = GPW * (GK::kGI + (LAT ? 0 : GV::kGI));
+  constexpr int kVOff = LAT ? 0 : TK * GK::kRowBytes;  // V rows in a slot
+  constexpr int kTab = LAT ? kRbTable : kRbTable / 2;
+  // fp16 weights are scaled by 2^7 (at most 2^15 with the lazy maximum): small ones keep
+  // their bits in fp16's range
+  constexpr float kLift = BF ? 0.f : 7.f;
+
+  __shared__ __attribute__((aligned(1024))) char tiles[NS * TL::kSlot];
+  __shared__ int tab[kPaged ? kRbTable : 1];
+  __shared__ uint64_t tree_sh[kRbMaxTree];
+  __shared__ DecSegment seg_sh;
+  __shared__ int merge_flag;
+  static_assert(kMergePieceBytes<kRbThreads> <= NS * TL::kSlot, "merge area");
+
+  const KArgs& a = ra.a;
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31;
+  const int hi = lane >> 5;
+  const int rg = wave / DG;
+  const int dg = wave % DG;
+  const int d0 = dg * DBW;
+  const int stream = static_cast<int>(blockIdx.x) % a.walk_streams;
+  const int seg_k = static_cast<int>(blockIdx.x) / a.walk_streams;
+
+  if (wave == 0) walk_locate<LM>(a, seg_k, &seg_sh);
+  __syncthreads();
+  DecSegment sg;
+  sg.j = __builtin_amdgcn_readfirstlane(seg_sh.j);
+  sg.us = __builtin_amdgcn_readfirstlane(seg_sh.us);
+  sg.s0 = __builtin_amdgcn_readfirstlane(seg_sh.s0);
+  sg.s1 = __builtin_amdgcn_readfirstlane(seg_sh.s1);
+  sg.C = __builtin_amdgcn_readfirstlane(seg_sh.C);
+
+  // the piece of sequence j's unit (starting at us in its stream) of this segment
+  auto piece_at = [&](RowsPiece& p, int j, int us) -> bool {
+    const bool whole = sg.C == 0;
+    if (j >= a.batch || (!whole && us >= sg.s1)) return false;
+    p.b = j;
+    p.kvh = stream % a.hkv;
+    p.qblk = stream / a.hkv;
+    p.Lk = __builtin_amdgcn_readfirstlane(walk_len<LM>(a, j));
+    const int n = (p.Lk + kBN - 1) / kBN;
+    p.us = us;
+    p.W = n > 1 ? n : 1;
+    p.unit = j * a.walk_streams + stream;
+    if (whole) {
+      p.t0 = 0;
+      p.T = n;
+      p.np = 1;
+      p.mine = 0;
+      return true;
+    }
+    const int b = max(us, sg.s0), e = min(us + p.W, sg.s1);
+    p.t0 = b - us;
+    p.T = n > 0 ? e - b : 0;
+    const int kf = us / sg.C;
+    p.np = (us + p.W - 1) / sg.C - kf + 1;
+    p.mine = seg_k - kf;
+    return true;
+  };
+  auto page_of = [&](int n) -> int {
+    return static_cast<int>(__umulhi(2u * static_cast<uint32_t>(n), ra.page_mul) >> ra.page_sh);
+  };
+
+  // ---- LDS addresses ---------------------------------------------------------
+  const uint32_t tiles0 = lds_addr_of(tiles);
+  // K row l32 of a 32-key block, chunk 2 cc + hi
+  const uint32_t koff = l32 * GK::kRowBytes + ((hi ^ GK::swz(l32)) * 16);
+  // V: lane i of 16-lane group g reads row 16 c + 8 rr + 4 (g / 2) + i / 4, dims
+  // 32 d + 16 (g % 2) + 4 (i % 4); see RowsGeo for the place of a chunk
+  constexpr int KM = GV::kG / 2;  // 32-dim blocks of a swizzle group
+  uint32_t voff;
+  {
+    const int g = lane >> 4, i = lane & 15;
+    const int r = 4 * (g >> 1) + (i >> 2);
+    const uint32_t c = 4 * (d0 & (KM - 1)) + 2 * (g & 1) + ((i & 3) >> 1);
+    voff = kVOff + r * GV::kRowBytes + ((c ^ GV::swz(r)) * 16) + (i & 1) * 8 +
+           (d0 / KM) * KM * 64;
+  }
+  // loads: byte offset of this lane's chunk within the 8 rows of a group, whose rows
+  // are 8 (wave & 1) ..+7 in the swizzle
+  const uint32_t ksb = static_cast<uint32_t>(a.k_ss * 2), vsb = static_cast<uint32_t>(a.v_ss * 2);
+  auto lane_row = [&](auto geo, int i) -> int { return (i * 64 + lane) / decltype(geo)::kNC; };
+  auto lane_chunk = [&](auto geo, int i) -> uint32_t {
+    using G = decltype(geo);
+    return static_cast<uint32_t>((i * 64 + lane) % G::kNC) ^
+           G::swz(8 * (wave & 1) + (i * 64 + lane) / G::kNC);
+  };
+  uint32_t kl[GK::kGI], vl[LAT ? 1 : GV::kGI];
+#pragma unroll
+  for (int i = 0; i < GK::kGI; ++i) kl[i] = lane_row(GK{}, i) * ksb + lane_chunk(GK{}, i) * 16;
+  if constexpr (!LAT) {
+#pragma unroll
+    for (int i = 0; i < GV::kGI; ++i) vl[i] = lane_row(GV{}, i) * vsb + lane_chunk(GV{}, i) * 16;
+  }
+  const bool even_pages = !kPaged || a.page_size % 8 == 0;
+
+  RowsPiece p;
+  if (!piece_at(p, sg.j, sg.us)) return;
+  for (;;) {
+    // ---- the piece's rows, mask and first block-table entries -----------------
+    const int q0 = p.qblk * (32 * RG);
+    const int row = q0 + rg * 32 + l32;
+    const int m = row % a.pack_m;  // draft
+    const int nrows = min(a.q_len - q0, 32 * RG);
+    u32x4 qf[DC];
+    {
+      const int h = p.kvh * (a.hq / a.hkv) + row / a.pack_m;
+      const uint16_t* src = static_cast<const uint16_t*>(a.q) + p.b * a.q_sb + h * a.q_sh +
+                            m * a.q_ss + hi * 8;
+      const bool ok = row < a.q_len;
+#pragma unroll
+      for (int c = 0; c < DC; ++c)
+        qf[c] = ok ? *reinterpret_cast<const u32x4*>(src + c * 16) : (u32x4){0u, 0u, 0u, 0u};
+    }
+    if (a.mask == kMaskTree) {
+      for (int i = wave; i < a.pack_m; i += kRbWaves) {
+        const uint8_t sees =
+            lane < a.pack_m ? ra.tree[p.b * ra.tree_sb + i * ra.tree_sr + lane] : uint8_t(0);
+        const uint64_t word = __ballot(sees != 0);
+        if (lane == 0) tree_sh[i] = word;
+      }
+    }
+    int64_t kbase, vbase;
+    if constexpr (MODE == FA2_LAYOUT_DENSE) {
+      kbase = p.b * a.k_sb + p.kvh * a.k_sh;
+      vbase = p.b * a.v_sb + p.kvh * a.v_sh;
+    } else if constexpr (MODE == FA2_LAYOUT_RAGGED) {
+      const int ks = a.kv_indptr[p.b];
+      kbase = ks * a.k_ss + p.kvh * a.k_sh;
+      vbase = ks * a.v_ss + p.kvh * a.v_sh;
+    } else {
+      kbase = p.kvh * a.k_sh;
+      vbase = p.kvh * a.v_sh;
+    }
+    const char* kptr = static_cast<const char*>(a.k) + kbase * 2;
+    const char* vptr = static_cast<const char*>(a.v) + vbase * 2;
+
+    f32x16 o[DBW];
+#pragma unroll
+    for (int d = 0; d < DBW; ++d) o[d] = (f32x16){};
+    float m_run = -INFINITY, l_run = 0.f;
+    const int off = p.Lk - a.pack_m;  // keys that every row sees
+    const int full = a.mask == FA2_MASK_NONE ? p.Lk : min(off + (a.mask == kMaskTree ? 0 : 1), p.Lk);
+    const int kend = min((p.t0 + p.T) * kBN, p.Lk);
+    uint64_t word = 0;
+
+    // ---- windows: keys whose block-table entries lie in LDS --------------------
+    for (int ka = p.t0 * kBN; ka < kend;) {
+      int kb = kend, page0 = 0;
+      if constexpr (kPaged) {
+        page0 = page_of(ka);
+        const int64_t lim = (static_cast<int64_t>(page0) + kTab) * a.page_size;
+        if (lim < kend) kb = ka + max((static_cast<int>(lim) - ka) / kBN * kBN, kBN);
+        const int last = page_of(kb - 1) - page0;
+        for (int i = tid; i <= last; i += kRbThreads) {
+          const int e = a.k_table[p.b * a.k_table_stride + page0 + i];
+          tab[i] = min(max(e, 0), ra.num_pages - 1);
+          if constexpr (!LAT) {
+            const int f = a.v_table[p.b * a.v_table_stride + page0 + i];
+            tab[kTab + i] = min(max(f, 0), ra.num_pages - 1);
+          }
+        }
+      }
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0), which the compiler counts
+      __syncthreads();  // the table and the mask are in LDS, the slots are free
+      if (a.mask == kMaskTree) word = tree_sh[m];
+
+      const int T = (kb - ka + TK - 1) / TK;
+      auto issue_rows = [&](auto is_v, int n, uint32_t dst) {
+        constexpr bool V = decltype(is_v)::value;
+        using G = std::conditional_t<V, GV, GK>;
+        const char* base = V ? vptr : kptr;
+        const int64_t ss = V ? a.v_ss : a.k_ss;
+        const int* tb = tab + (V ? kTab : 0);
+        if (even_pages && n + 8 <= kb) {  // 8 rows of one page
+          int64_t r = n;
+          if constexpr (kPaged) {
+            const int pg = page_of(n);
+            r = static_cast<int64_t>(tb[pg - page0]) * a.page_size + (n - pg * a.page_size);
+          }
+          const uint64_t at = reinterpret_cast<uint64_t>(base + r * ss * 2);
+          const uint64_t sbase =
+              (static_cast<uint64_t>(static_cast<uint32_t>(
+                   __builtin_amdgcn_readfirstlane(static_cast<int>(at >> 32))))
+               << 32) |
+              static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(at)));
+#pragma unroll
+          for (int i = 0; i < G::kGI; ++i) {
+            if constexpr (V) rows_dma(sbase, vl[LAT ? 0 : i], dst + i * 1024);
+            else rows_dma(sbase, kl[i], dst + i * 1024);
+          }
+          return;
+        }
+        // a row per lane; rows past the window are its last one (finite data under a
+        // zero weight)
+#pragma unroll
+        for (int i = 0; i < G::kGI; ++i) {
+          const int nr = min(n + lane_row(G{}, i), kb - 1);
+          int64_t r = nr;
+          if constexpr (kPaged) {
+            const int pg = page_of(nr);
+            r = static_cast<int64_t>(tb[pg - page0]) * a.page_size + (nr - pg * a.page_size);
+          }
+          dma_global_x4(base + r * ss * 2 + lane_chunk(G{}, i) * 16, dst + i * 1024);
+        }
+      };
+      auto issue = [&](int t) {
+        const uint32_t slot = tiles0 + (t % NS) * TL::kSlot;
+#pragma unroll
+        for (int g = 0; g < GPW; ++g) {
+          const int grp = wave + 4 * g;
+          const int n = ka + t * TK + 8 * grp;
+          issue_rows(std::integral_constant<bool, false>{}, n, slot + grp * 8 * GK::kRowBytes);
+          if constexpr (!LAT)
+            issue_rows(std::integral_constant<bool, true>{}, n,
+                       slot + kVOff + grp * 8 * GV::kRowBytes);
+        }
+      };
+      for (int t = 0; t < NS - 1 && t < T; ++t) issue(t);
+
+      for (int t = 0; t < T; ++t) {
+        rows_wait<IPT, NS - 2>(T - 1 - t);
+        pp_barrier();  // tile t is there, and slot t - 1 has been read
+        if (t + NS - 1 < T) issue(t + NS - 1);
+        const uint32_t slot = tiles0 + (t % NS) * TL::kSlot;
+        const int n0 = ka + t * TK;
+
+        // ---- S^T = K Q^T -------------------------------------------------------
+        f32x16 s[SB];
+#pragma unroll
+        for (int sb = 0; sb < SB; ++sb) s[sb] = (f32x16){};
+        {
+          constexpr int kN = DC * SB, kAhead = 6 < kN ? 6 : kN;
+          auto frag = [&](auto kc) -> u32x4 {
+            constexpr int cc = decltype(kc)::value / SB, sb = decltype(kc)::value % SB;
+            return *(const lds_u32x4_t*)(lds_ptr(slot + (koff ^ (32u * (cc % GK::kG)))) +
+                                         sb * 32 * GK::kRowBytes + (cc / GK::kG) * GK::kG * 32);
+          };
+          f32x16 s2[SB];  // odd k-steps: two chains of MFMAs
+#pragma unroll
+          for (int sb = 0; sb < SB; ++sb) s2[sb] = (f32x16){};
+          u32x4 fr[kN];
+          static_for<kAhead>([&](auto kc) { fr[decltype(kc)::value] = frag(kc); });
+          static_for<kN>([&](auto kc) {
+            constexpr int k = decltype(kc)::value, cc = k / SB, sb = k % SB;
+            if constexpr (SB == 1 && (cc & 1))
+              s2[sb] = mma32<BF>(fr[k], qf[cc], s2[sb]);
+            else
+              s[sb] = mma32<BF>(fr[k], qf[cc], s[sb]);
+            if constexpr (k + kAhead < kN)
+              fr[k + kAhead] = frag(std::integral_constant<int, k + kAhead>{});
+          });
+          if constexpr (SB == 1) s[0] += s2[0];
+          __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+          for (int k = 0; k < kN - kAhead; ++k) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          }
+          __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+        }
+
+        // ---- mask: key n0 + 32 sb + 8 (i / 4) + 4 hi + i % 4 of element i --------
+        if (n0 + TK > full) {
+#pragma unroll
+          for (int sb = 0; sb < SB; ++sb) {
+            const int n = n0 + 32 * sb;
+            uint32_t sees;  // bit x: key n + x
+            if (a.mask == kMaskTree) {
+              const int x = n - off;  // the first key's place among the drafts
+              sees = x >= 64    ? 0u
+                     : x >= 0   ? static_cast<uint32_t>(word >> x)
+                     : x > -32  ? (static_cast<uint32_t>(word << -x) | ((1u << -x) - 1u))
+                                : ~0u;
+              // (a sequence shorter than its drafts has no key before the first)
+            } else {
+              const int c = (a.mask == FA2_MASK_NONE ? p.Lk : min(off + m + 1, p.Lk)) - n;
+              sees = c >= 32 ? ~0u : c <= 0 ? 0u : (1u << c) - 1u;
+            }
+            sees >>= 4 * hi;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (!(sees & (1u << ((i >> 2) * 8 + (i & 3))))) s[sb][i] = -INFINITY;
+          }
+        }
+
+        // ---- softmax -------------------------------------------------------------
+        float mx = -INFINITY;
+#pragma unroll
+        for (int sb = 0; sb < SB; ++sb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[sb][i]);
+        mx = max_xor32_valu(mx);
+        const float mt = mx * a.scale_log2;
+        const bool need = mt > m_run + kRescaleThreshold;
+        if (__any(need)) {
+          const float alpha = fast_exp2(need ? m_run - mt : 0.f);
+          m_run = need ? mt : m_run;
+          l_run *= alpha;
+#pragma unroll
+          for (int d = 0; d < DBW; ++d) o[d] *= alpha;
+        }
+        const float m_use = (m_run == -INFINITY ? 0.f : m_run) - kLift;
+        u32x4 pf[2 * SB];
+#pragma unroll
+        for (int sb = 0; sb < SB; ++sb) {
+          float e[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            e[i] = fast_exp2(__builtin_fmaf(s[sb][i], a.scale_log2, -m_use));
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            pf[sb * 2 + h] = (u32x4){pack2<BF>(e[h * 8 + 0], e[h * 8 + 1]),
+                                     pack2<BF>(e[h * 8 + 2], e[h * 8 + 3]),
+                                     pack2<BF>(e[h * 8 + 4], e[h * 8 + 5]),
+                                     pack2<BF>(e[h * 8 + 6], e[h * 8 + 7])};
+        }
+        // (the sum of the rounded weights, those that the product with V applies)
+#pragma unroll
+        for (int c = 0; c < 2 * SB; ++c)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) l_run = dot2_ones<BF>(pf[c][j], l_run);
+
+        // ---- O^T += V^T P^T --------------------------------------------------------
+        {
+          constexpr int kN = 2 * SB * DBW, kAhead = 4 < kN ? 4 : kN;
+          auto frag = [&](auto kc) -> u32x4 {
+            constexpr int c = decltype(kc)::value / DBW, d = decltype(kc)::value % DBW;
+            constexpr int kImm = 16 * c * GV::kRowBytes + (d / KM) * KM * 64;
+            const u32x2 lo = __builtin_bit_cast(
+                u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(
+                           lds_ptr(slot + (voff ^ (64u * (d % KM)))) + kImm)));
+            const u32x2 up = __builtin_bit_cast(
+                u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(
+                           lds_ptr(slot + (voff ^ (64u * (d % KM)) ^ 16u)) + kImm +
+                           8 * GV::kRowBytes)));
+            return (u32x4){lo[0], lo[1], up[0], up[1]};
+          };
+          u32x4 fr[kN];
+          static_for<kAhead>([&](auto kc) { fr[decltype(kc)::value] = frag(kc); });
+          static_for<kN>([&](auto kc) {
+            constexpr int k = decltype(kc)::value, c = k / DBW, d = k % DBW;
+            o[d] = mma32<BF>(fr[k], pf[c], o[d]);
+            if constexpr (k + kAhead < kN)
+              fr[k + kAhead] = frag(std::integral_constant<int, k + kAhead>{});
+          });
+          __builtin_amdgcn_sched_group_barrier(0x100, 2 * kAhead, 0);
+#pragma unroll
+          for (int k = 0; k < kN - kAhead; ++k) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+          }
+          __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+        }
+      }
+      __syncthreads();  // the window's table and slots have been read
+      ka = kb;
+    }
+
+    // ---- the piece's end ---------------------------------------------------------
+    const float l_tot = sum_xor32(l_run);
+    const int r = rg * 32 + l32;
+    const int64_t obase = p.b * a.o_sb + p.kvh * (a.hq / a.hkv) * a.o_sh;
+    if (p.np == 1) {
+      if (r < nrows) {
+        const float inv = 1.f / l_tot;  // 0/0 -> NaN for a row with no key
+        uint16_t* dst = static_cast<uint16_t*>(a.o) + obase +
+                        static_cast<int64_t>(q0 + r) * a.o_ss + d0 * 32 + hi * 4;
+#pragma unroll
+        for (int d = 0; d < DBW; ++d)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<u32x2*>(dst + d * 32 + g * 8) =
+                (u32x2){pack2<BF>(o[d][g * 4 + 0] * inv, o[d][g * 4 + 1] * inv),
+                        pack2<BF>(o[d][g * 4 + 2] * inv, o[d][g * 4 + 3] * inv)};
+      }
+    } else {
+      const int64_t slot = walk_slot(a, sg.C, p.us, stream, p.mine);
+      const uint32_t pr = static_cast<uint32_t>(a.part_rows);
+      const __amdgpu_buffer_rsrc_t rm = make_rsrc_uniform(a.part_ml + slot * pr * 2, pr * 8);
+      const __amdgpu_buffer_rsrc_t ro = make_rsrc_uniform(a.part_o + slot * pr * DV, pr * DV * 4);
+      if (r < nrows) {
+        if (dg == 0 && hi == 0)
+          __builtin_amdgcn_raw_buffer_store_b64(
+              (u32x2){__builtin_bit_cast(uint32_t, m_run), __builtin_bit_cast(uint32_t, l_tot)},
+              rm, static_cast<uint32_t>(r) * 8, 0, kCpolSc1);
+#pragma unroll
+        for (int d = 0; d < DBW; ++d)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            __builtin_amdgcn_raw_buffer_store_b128(
+                __builtin_bit_cast(u32x4, (f32x4){o[d][g * 4 + 0], o[d][g * 4 + 1],
+                                                  o[d][g * 4 + 2], o[d][g * 4 + 3]}),
+                ro, static_cast<uint32_t>(r * DV + (d0 + d) * 32 + g * 8 + hi * 4) * 4, 0,
+                kCpolSc1);
+      }
+      merge_publish();
+      __syncthreads();
+      if (merge_count(a, p.unit, p.np, &merge_flag))
+        merge_pieces<DT, DV, kRbThreads, 32 * RG>(
+            a, [&](int s) { return walk_slot(a, sg.C, p.us, stream, s); }, p.np, nrows, obase, q0,
+            tiles);
+    }
+    if (!piece_at(p, walk_next(a, sg, p.b), p.us + p.W)) return;
+    __syncthreads();  // the merge area, the mask and the flag are free
+  }
+}
+
+}  // namespace fa2

@@ -15,8 +15,10 @@
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "fa2.h"
+#include "fa2_latent.h"
 #include "fa2_ops.h"
 
 namespace {
@@ -594,6 +596,322 @@ std::tuple<int64_t, at::Tensor> fp4_decode(const at::Tensor& q, const at::Tensor
   return {fa2_fp4_decode(&p, st), out};
 }
 
+// ---- latent attention and trees of drafts (include/fa2_latent.h) ---------------
+
+constexpr int64_t kRope = 64;  // values of the key part that all heads share
+
+bool half_type(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }
+
+// latent_cache.check_cache and check_latent_dim
+bool latent_cache_ok(const at::Tensor& c, int64_t latent) {
+  return c.is_cuda() && half_type(c.scalar_type()) && c.dim() == 3 && c.is_contiguous() &&
+         c.numel() > 0 && reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 &&
+         (latent == 256 || latent == 512) && c.size(2) == latent + kRope;
+}
+
+// Workspace of a call (`Size`) into p; undefined where it takes none.
+template <typename P, typename Size>
+int64_t with_workspace(P& p, Size size, const at::TensorOptions& options, at::Tensor& ws) {
+  size_t n = 0;
+  const int rc = size(&p, &n);
+  if (rc != FA2_OK) return rc;
+  if (n) {
+    ws = at::empty({static_cast<int64_t>(n)}, options.dtype(at::kByte));
+    p.workspace = ws.data_ptr();
+    p.workspace_bytes = n;
+  }
+  return FA2_OK;
+}
+
+// paged_latent_append; (status, the finished rows where they are asked for).
+std::tuple<int64_t, OptTensor> latent_append(const at::Tensor& cache, const at::Tensor& block_table,
+                                             at::Tensor rows, const at::Tensor& indptr,
+                                             at::Tensor weight, at::Tensor rope,
+                                             const OptTensor& start_pos, double eps,
+                                             bool interleaved, bool return_rows) {
+  const int64_t latent = cache.dim() == 3 ? cache.size(2) - kRope : 0;
+  if (!latent_cache_ok(cache, latent)) return {kRefused, c10::nullopt};
+  const at::Device dev = cache.device();
+  const auto dt = cache.scalar_type();
+  const int64_t B = indptr.numel() - 1;
+  if (block_table.device() != dev || rows.device() != dev || indptr.device() != dev ||
+      weight.device() != dev || rope.device() != dev ||
+      (start_pos && (start_pos->device() != dev || start_pos->numel() < B)) ||
+      rows.scalar_type() != dt || rows.dim() != 2 || rows.size(1) != latent + kRope ||
+      (weight.scalar_type() != dt && weight.scalar_type() != at::kFloat) || weight.dim() != 1 ||
+      weight.size(0) != latent || rope.scalar_type() != at::kFloat || rope.dim() != 2 ||
+      rope.size(1) != kRope || !(eps >= 0) || B < 0 || block_table.dim() != 2 ||
+      block_table.size(0) < B)
+    return {kRefused, c10::nullopt};
+  const c10::DeviceGuard guard(dev);
+  rows = ready(rows);
+  weight = packed(weight);
+  rope = packed(rope);
+  const at::Tensor ip = fp4_index(indptr, dev);
+  const at::Tensor bt = fp4_table(block_table, dev);
+  at::Tensor sp;
+  OptTensor out;
+  fa2_latent_append_params p;
+  std::memset(&p, 0, sizeof(p));
+  if (return_rows) {
+    out = at::empty(rows.sizes(), rows.options());
+    p.rows_out = out->data_ptr();
+  }
+  if (start_pos) {
+    sp = fp4_index(*start_pos, dev);
+    p.start_pos = sp.data_ptr<int32_t>();
+  }
+  p.dtype = dtype_code(dt);
+  p.weight_dtype = dtype_code(weight.scalar_type());
+  p.interleaved = interleaved ? 1 : 0;
+  p.eps = static_cast<float>(eps);
+  p.batch = B;
+  p.num_rows = rows.size(0);
+  p.latent_dim = latent;
+  p.rope_dim = kRope;
+  p.page_size = cache.size(1);
+  p.num_pages = cache.size(0);
+  p.table_width = bt.size(1);
+  p.table_stride = bt.stride(0);
+  p.positions = rope.size(0);
+  p.rope_stride = kRope;
+  p.x_ts = stride_of(rows, 0);
+  p.x = rows.data_ptr();
+  p.cache = cache.data_ptr();
+  p.weight = weight.data_ptr();
+  p.rope = rope.data_ptr<float>();
+  p.indptr = ip.data_ptr<int32_t>();
+  p.block_table = bt.data_ptr<int32_t>();
+  const hipStream_t st = c10::hip::getCurrentHIPStream(dev.index()).stream();
+  return {fa2_latent_append(&p, st), out};
+}
+
+// latent_decode.check_tree; t becomes what the kernels take
+bool tree_ok(at::Tensor& t, int64_t B, int64_t M, const at::Device& dev) {
+  if (t.device() != dev || (t.scalar_type() != at::kBool && t.scalar_type() != at::kByte) ||
+      M > FA2_TREE_MAX || (t.dim() != 2 && t.dim() != 3) || t.size(-1) != M || t.size(-2) != M ||
+      (t.dim() == 3 && t.size(0) != B))
+    return false;
+  if (M > 1 && t.stride(-1) != 1) t = t.contiguous();
+  return true;
+}
+
+template <typename P>
+void set_tree(P& p, const at::Tensor& t) {
+  p.tree = static_cast<const uint8_t*>(t.data_ptr());
+  p.tree_sb = t.dim() == 3 ? stride_of(t, 0) : 0;
+  p.tree_sr = stride_of(t, t.dim() - 2);
+}
+
+// latent_decode_attention; (status, output).
+std::tuple<int64_t, at::Tensor> latent_decode(const at::Tensor& q, const at::Tensor& cache,
+                                              int64_t latent, double scale, const at::Tensor& lens,
+                                              const at::Tensor& block_table, bool causal,
+                                              const OptTensor& tree_mask) {
+  if ((q.dim() != 3 && q.dim() != 4) || !latent_cache_ok(cache, latent)) return {kRefused, q};
+  const at::Device dev = cache.device();
+  const int64_t B = q.size(0), M = q.dim() == 4 ? q.size(2) : 1;
+  if (q.device() != dev || q.scalar_type() != cache.scalar_type() ||
+      q.size(-1) != cache.size(2) || q.size(1) == 0 || lens.device() != dev ||
+      block_table.device() != dev || lens.numel() < B || block_table.dim() != 2 ||
+      block_table.size(0) < B || !(scale > 0) || !std::isfinite(scale))
+    return {kRefused, q};
+  const c10::DeviceGuard guard(dev);
+  at::Tensor tree;
+  if (tree_mask) {
+    tree = *tree_mask;
+    if (!tree_ok(tree, B, M, dev)) return {kRefused, q};
+  }
+  const at::Tensor q4 = ready(q.dim() == 3 ? q.unsqueeze(2) : q);
+  auto sizes = q.sizes().vec();
+  sizes.back() = latent;
+  at::Tensor out = at::empty(sizes, q.options());
+  const at::Tensor o4 = q.dim() == 3 ? out.unsqueeze(2) : out;
+  const at::Tensor li = fp4_index(lens, dev);
+  const at::Tensor bt = fp4_table(block_table, dev);
+  fa2_latent_decode_params p;
+  std::memset(&p, 0, sizeof(p));
+  p.dtype = dtype_code(q.scalar_type());
+  p.mask = tree_mask ? FA2_MASK_TREE : causal ? FA2_MASK_CAUSAL_BOTTOM_RIGHT : FA2_MASK_NONE;
+  p.batch = B;
+  p.q_heads = q.size(1);
+  p.q_len = M;
+  p.latent_dim = latent;
+  p.rope_dim = kRope;
+  p.page_size = cache.size(1);
+  p.num_pages = cache.size(0);
+  p.table_width = bt.size(1);
+  p.table_stride = bt.stride(0);
+  strides3(q4, p.q_sb, p.q_sh, p.q_ss);
+  strides3(o4, p.o_sb, p.o_sh, p.o_ss);
+  p.q = q4.data_ptr();
+  p.o = out.data_ptr();
+  p.cache = cache.data_ptr();
+  p.kv_lens = li.data_ptr<int32_t>();
+  p.block_table = bt.data_ptr<int32_t>();
+  if (tree_mask) set_tree(p, tree);
+  p.softmax_scale = static_cast<float>(scale);
+  at::Tensor ws;
+  const int64_t rc = with_workspace(p, fa2_latent_decode_workspace_size, q.options(), ws);
+  if (rc != FA2_OK) return {rc, out};
+  const hipStream_t st = c10::hip::getCurrentHIPStream(dev.index()).stream();
+  return {fa2_latent_decode(&p, st), out};
+}
+
+// tree_decode_attention; (status, output).
+std::tuple<int64_t, at::Tensor> tree_decode(const at::Tensor& q, at::Tensor k, at::Tensor v,
+                                            at::Tensor tree, const OptTensor& kv_indptr,
+                                            const OptTensor& k_table, const OptTensor& v_table,
+                                            c10::optional<int64_t> page_size) {
+  const at::Device dev = q.device();
+  const auto dt = q.scalar_type();
+  if (!q.is_cuda() || q.dim() != 4 || !half_type(dt) || k.scalar_type() != dt ||
+      v.scalar_type() != dt || k.device() != dev || v.device() != dev || k.sizes() != v.sizes() ||
+      (k.dim() != 3 && k.dim() != 4))
+    return {kRefused, q};
+  const int64_t B = q.size(0), QH = q.size(1), M = q.size(2), D = q.size(3);
+  if ((D != 64 && D != 128 && D != 256) || k.size(-1) != D) return {kRefused, q};
+  if (kv_indptr && kv_indptr->device() != dev) return {kRefused, q};
+  fa2_tree_decode_params p;
+  std::memset(&p, 0, sizeof(p));
+  if (k_table) {
+    if (!v_table || !page_size || !kv_indptr || *page_size <= 0 ||
+        (k.dim() == 4 && k.size(1) != *page_size) || k_table->dim() != 2 || v_table->dim() != 2 ||
+        k_table->device() != dev || v_table->device() != dev || kv_indptr->numel() < B ||
+        k_table->size(0) < B || v_table->size(0) < B)
+      return {kRefused, q};
+    p.layout = FA2_LAYOUT_PAGED;
+  } else if (kv_indptr) {
+    if (k.dim() != 3 || kv_indptr->numel() < B + 1) return {kRefused, q};
+    p.layout = FA2_LAYOUT_RAGGED;
+  } else {
+    if (k.dim() != 4 || k.size(0) != B) return {kRefused, q};
+    p.layout = FA2_LAYOUT_DENSE;
+  }
+  const c10::DeviceGuard guard(dev);
+  if (p.layout == FA2_LAYOUT_PAGED && k.dim() == 4) {
+    k = k.reshape({-1, k.size(2), k.size(3)});
+    v = v.reshape({-1, v.size(2), v.size(3)});
+  }
+  const int64_t KVH = k.size(1);
+  if (QH == 0 || KVH == 0 || QH % KVH != 0 || !tree_ok(tree, B, M, dev)) return {kRefused, q};
+  const at::Tensor qr = ready(q);
+  k = ready(k);
+  v = ready(v);
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  at::Tensor ki, kt, vt;
+  p.dtype = dtype_code(dt);
+  p.batch = B;
+  p.q_heads = QH;
+  p.kv_heads = KVH;
+  p.head_dim = D;
+  p.q_len = M;
+  p.kv_len = p.layout == FA2_LAYOUT_DENSE ? k.size(2) : k.size(0);
+  strides3(qr, p.q_sb, p.q_sh, p.q_ss);
+  strides3(k, p.k_sb, p.k_sh, p.k_ss);
+  strides3(v, p.v_sb, p.v_sh, p.v_ss);
+  strides3(out, p.o_sb, p.o_sh, p.o_ss);
+  p.q = qr.data_ptr();
+  p.k = k.data_ptr();
+  p.v = v.data_ptr();
+  p.o = out.data_ptr();
+  if (p.layout != FA2_LAYOUT_DENSE) {
+    ki = fp4_index(*kv_indptr, dev);
+    p.kv_indptr = ki.data_ptr<int32_t>();
+  }
+  if (p.layout == FA2_LAYOUT_PAGED) {
+    kt = fp4_table(*k_table, dev);
+    vt = fp4_table(*v_table, dev);
+    p.page_size = *page_size;
+    p.table_width = std::min(kt.size(1), vt.size(1));
+    p.k_table_stride = kt.stride(0);
+    p.v_table_stride = vt.stride(0);
+    p.k_block_table = kt.data_ptr<int32_t>();
+    p.v_block_table = vt.data_ptr<int32_t>();
+  }
+  set_tree(p, tree);
+  p.softmax_scale = static_cast<float>(std::pow(static_cast<double>(D), -0.5));
+  at::Tensor ws;
+  const int64_t rc = with_workspace(p, fa2_tree_decode_workspace_size, q.options(), ws);
+  if (rc != FA2_OK) return {rc, out};
+  const hipStream_t st = c10::hip::getCurrentHIPStream(dev.index()).stream();
+  return {fa2_tree_decode(&p, st), out};
+}
+
+// latent_attention; (status, output).
+std::tuple<int64_t, at::Tensor> latent_prefill(at::Tensor q, at::Tensor k, at::Tensor kr,
+                                               at::Tensor v, int64_t mask,
+                                               const OptTensor& q_indptr,
+                                               const OptTensor& kv_indptr,
+                                               c10::optional<double> scale) {
+  const at::Device dev = q.device();
+  const auto dt = q.scalar_type();
+  const bool ragged = q_indptr.has_value();
+  const int64_t dims = ragged ? 3 : 4;
+  if (!q.is_cuda() || !half_type(dt) || k.scalar_type() != dt || kr.scalar_type() != dt ||
+      v.scalar_type() != dt || k.device() != dev || kr.device() != dev || v.device() != dev ||
+      ragged != kv_indptr.has_value() || q.dim() != dims || k.dim() != dims ||
+      kr.dim() != dims - 1 || k.sizes() != v.sizes())
+    return {kRefused, q};
+  const int64_t H = q.size(1), D = k.size(-1);
+  if ((D != 64 && D != 128) || q.size(-1) != D + kRope || kr.size(-1) != kRope || H == 0 ||
+      k.size(1) != H || kr.size(0) != k.size(0) ||
+      (!ragged && (kr.size(1) != k.size(2) || k.size(0) != q.size(0))) ||
+      (ragged && (q_indptr->device() != dev || kv_indptr->device() != dev ||
+                  q_indptr->numel() != kv_indptr->numel() || q_indptr->numel() == 0)) ||
+      (scale && !(*scale > 0 && std::isfinite(*scale))))
+    return {kRefused, q};
+  const c10::DeviceGuard guard(dev);
+  q = ready(q);
+  k = ready(k);
+  kr = ready(kr);
+  v = ready(v);
+  auto sizes = q.sizes().vec();
+  sizes.back() = D;
+  at::Tensor out = at::empty(sizes, q.options());
+  at::Tensor qi, ki;
+  fa2_latent_prefill_params p;
+  std::memset(&p, 0, sizeof(p));
+  p.layout = ragged ? FA2_LAYOUT_RAGGED : FA2_LAYOUT_DENSE;
+  p.dtype = dtype_code(dt);
+  p.mask = static_cast<int32_t>(mask);
+  p.heads = H;
+  p.head_dim = D;
+  p.rope_dim = kRope;
+  if (ragged) {
+    qi = fp4_index(*q_indptr, dev);
+    ki = fp4_index(*kv_indptr, dev);
+    p.q_indptr = qi.data_ptr<int32_t>();
+    p.kv_indptr = ki.data_ptr<int32_t>();
+    p.batch = qi.numel() - 1;
+    p.q_len = q.size(0);
+    p.kv_len = k.size(0);
+    p.kr_ss = stride_of(kr, 0);
+  } else {
+    p.batch = q.size(0);
+    p.q_len = q.size(2);
+    p.kv_len = k.size(2);
+    p.kr_sb = stride_of(kr, 0);
+    p.kr_ss = stride_of(kr, 1);
+  }
+  strides3(q, p.q_sb, p.q_sh, p.q_ss);
+  strides3(k, p.k_sb, p.k_sh, p.k_ss);
+  strides3(v, p.v_sb, p.v_sh, p.v_ss);
+  strides3(out, p.o_sb, p.o_sh, p.o_ss);
+  p.q = q.data_ptr();
+  p.k = k.data_ptr();
+  p.kr = kr.data_ptr();
+  p.v = v.data_ptr();
+  p.o = out.data_ptr();
+  p.softmax_scale = static_cast<float>(
+      scale ? *scale : std::pow(static_cast<double>(D + kRope), -0.5));
+  at::Tensor ws;
+  const int64_t rc = with_workspace(p, fa2_latent_prefill_workspace_size, q.options(), ws);
+  if (rc != FA2_OK) return {rc, out};
+  const hipStream_t st = c10::hip::getCurrentHIPStream(dev.index()).stream();
+  return {fa2_latent_prefill(&p, st), out};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -606,4 +924,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fp4_gather_into", &fp4_gather_into, "enqueue fa2_fp4_gather; the fa2 status or -1");
   m.def("fp4_decode", &fp4_decode,
         "enqueue fa2_fp4_decode; (fa2 status or -1, output)");
+  m.def("latent_append", &latent_append,
+        "enqueue fa2_latent_append; (fa2 status or -1, rows or None)");
+  m.def("latent_decode", &latent_decode, "enqueue fa2_latent_decode; (fa2 status or -1, output)");
+  m.def("tree_decode", &tree_decode, "enqueue fa2_tree_decode; (fa2 status or -1, output)");
+  m.def("latent_prefill", &latent_prefill,
+        "enqueue fa2_latent_prefill; (fa2 status or -1, output)");
 }
