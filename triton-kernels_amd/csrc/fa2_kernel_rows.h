@@ -18,6 +18,7 @@ constexpr int kMaskTree = 3;
 
 struct RowsArgs {
   KArgs a;  // q rows: token m of head h at h * q_sh + m * q_ss; o rows: o_ss apart
+  int2* info;  // of each unit: its pieces and the part slot of the first (rows_info)
   const uint8_t* tree;  // bool [batch, pack_m, pack_m]
   int64_t tree_sb, tree_sr;
   int32_t num_pages, table_width;
@@ -42,14 +43,16 @@ struct RowsGeo {
   }
 };
 
-// Tile shape: keys of a tile and LDS slots.
-template <int DK, int DV, bool LAT>
+// Tile shape: workgroups per CU, keys of a tile and LDS slots.
+template <int DK, int DV, bool LAT, int RG>
 struct RowsTile {
   using G = RowsGeo<DK>;
   static constexpr int kRow = G::kRowBytes + (LAT ? 0 : DV * 2);
-  static constexpr int kKeys = kRow * 64 <= 40960 ? 64 : 32;
+  static constexpr int kOcc = kRow > 640 || (LAT && RG == 4) ? 1 : 2;
+  static constexpr int kBudget = kOcc == 2 ? 70000 : 150000;
+  static constexpr int kKeys = kRow * 64 * 4 <= kBudget ? 64 : 32;
   static constexpr int kSlot = kRow * kKeys;
-  static constexpr int kSlots = 150000 / kSlot < 6 ? 150000 / kSlot : 6;
+  static constexpr int kSlots = kBudget / kSlot < 6 ? kBudget / kSlot : 6;
   static_assert(kSlots >= 3, "tiles in flight");
 };
 
@@ -59,6 +62,150 @@ struct RowsPiece {
   int np, mine;  // pieces of the unit, this one's index
   int us, W, unit;
 };
+
+// The piece of sequence j's unit (starting at us in its stream) in segment sg; false past
+// the segment's end.
+template <int LM>
+__device__ __forceinline__ bool rows_piece(const KArgs& a, const DecSegment& sg, int stream,
+                                           int seg_k, int j, int us, RowsPiece& p) {
+  const bool whole = sg.C == 0;
+  if (j >= a.batch || (!whole && us >= sg.s1)) return false;
+  p.b = j;
+  p.kvh = stream % a.hkv;
+  p.qblk = stream / a.hkv;
+  p.Lk = __builtin_amdgcn_readfirstlane(walk_len<LM>(a, j));
+  const int n = (p.Lk + kBN - 1) / kBN;
+  p.us = us;
+  p.W = n > 1 ? n : 1;
+  p.unit = j * a.walk_streams + stream;
+  if (whole) {
+    p.t0 = 0;
+    p.T = n;
+    p.np = 1;
+    p.mine = 0;
+    return true;
+  }
+  const int b = max(us, sg.s0), e = min(us + p.W, sg.s1);
+  p.t0 = b - us;
+  p.T = n > 0 ? e - b : 0;
+  const int kf = us / sg.C;
+  p.np = (us + p.W - 1) / sg.C - kf + 1;
+  p.mine = seg_k - kf;
+  return true;
+}
+
+// What the merge of a unit has to know, by its first piece.
+__device__ __forceinline__ void rows_info(const RowsArgs& ra, const DecSegment& sg, int stream,
+                                          const RowsPiece& p) {
+  if (p.mine != 0) return;
+  const int slot =
+      p.np > 1 ? static_cast<int>(walk_slot(ra.a, sg.C, p.us, stream, 0)) : 0;
+  ra.info[p.unit] = make_int2(p.np, slot);
+}
+
+// The merge of cut units, launched behind the kernels that cut them: workgroup (x, y) takes
+// rows y * kCombineRows ..  of unit x, a thread 4 columns of a row over all pieces, in order,
+// kMergeAhead of them in flight.  (One workgroup per unit that merges in the first kernel, as
+// the 16-bit decode kernels do, takes a memory round trip for every 64 KB of partials, 32 to
+// 256 KB a piece here: 4 x 900 keys of 16 heads 36 us, with this launch XX.)
+constexpr int kMergeAhead = 8;
+template <int DV>
+constexpr int kMergeRows = DV >= 1024 ? 1 : 1024 / DV;  // rows of 256 threads
+
+template <int DT, int DV>
+__global__ __launch_bounds__(256) void fa2_rows_merge_kernel(RowsArgs ra) {
+  constexpr bool BF = Elt<DT>::kBF;
+  const KArgs& a = ra.a;
+  const int unit = blockIdx.x;
+  const int2 info = ra.info[unit];
+  if (info.x <= 1) return;  // the unit was whole
+  const int b = unit / a.walk_streams, stream = unit - b * a.walk_streams;
+  const int kvh = stream % a.hkv, q0 = stream / a.hkv * a.block_rows;
+  const int r = blockIdx.y * kMergeRows<DV> + threadIdx.x / (DV / 4);
+  const int col = (threadIdx.x % (DV / 4)) * 4;
+  if (r >= a.part_rows || q0 + r >= a.q_len) return;
+  auto row_of = [&](int s) -> int64_t {  // walk_slot
+    const int slot = s == 0 ? info.y : ((info.y >> 1) + s * a.walk_streams) * 2;
+    return static_cast<int64_t>(slot) * a.part_rows + r;
+  };
+  float m = -INFINITY, l = 0.f;
+  f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < info.x; s0 += kMergeAhead) {
+    f32x2 ml[kMergeAhead];
+    f32x4 x[kMergeAhead];
+#pragma unroll
+    for (int j = 0; j < kMergeAhead; ++j) {
+      const int64_t at = row_of(min(s0 + j, info.x - 1));
+      ml[j] = *reinterpret_cast<const f32x2*>(a.part_ml + at * 2);
+      x[j] = *reinterpret_cast<const f32x4*>(a.part_o + at * DV + col);
+    }
+    float mn = m;
+#pragma unroll
+    for (int j = 0; j < kMergeAhead; ++j) mn = fmaxf(mn, ml[j][0]);
+    const float mu = mn == -INFINITY ? 0.f : mn;
+    const float al = fast_exp2(m - mu);
+    l *= al;
+    acc *= al;
+    m = mn;
+#pragma unroll
+    for (int j = 0; j < kMergeAhead; ++j) {
+      const float m_j = ml[j][0], l_j = ml[j][1];
+      const float w = s0 + j < info.x ? fast_exp2(m_j - mu) : 0.f;
+      l += w * l_j;
+      acc += w * x[j];
+    }
+  }
+  const float inv = 1.f / l;  // 0/0 -> NaN for a row with no key
+  *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.o) + b * a.o_sb +
+                            static_cast<int64_t>(kvh) * (a.hq / a.hkv) * a.o_sh +
+                            static_cast<int64_t>(q0 + r) * a.o_ss + col) =
+      (u32x2){pack2<BF>(acc[0] * inv, acc[1] * inv), pack2<BF>(acc[2] * inv, acc[3] * inv)};
+}
+
+// Element offsets of a piece's K and V row 0 (paged: of its kv head).
+template <int MODE>
+__device__ __forceinline__ void rows_bases(const KArgs& a, const RowsPiece& p, int64_t& kbase,
+                                           int64_t& vbase) {
+  kbase = p.kvh * a.k_sh;
+  vbase = p.kvh * a.v_sh;
+  if constexpr (MODE == FA2_LAYOUT_DENSE) {
+    kbase += p.b * a.k_sb;
+    vbase += p.b * a.v_sb;
+  } else if constexpr (MODE == FA2_LAYOUT_RAGGED) {
+    const int64_t ks = a.kv_indptr[p.b];
+    kbase += ks * a.k_ss;
+    vbase += ks * a.v_ss;
+  }
+}
+
+// Block-table entries page0 .. page0 + last of sequence b into LDS, clamped into the pool;
+// V's behind K's.
+template <bool LAT, int NT>
+__device__ __forceinline__ void rows_table(const RowsArgs& ra, int b, int page0, int last,
+                                           int* tab) {
+  const KArgs& a = ra.a;
+  for (int i = threadIdx.x; i <= last; i += NT) {
+    tab[i] = min(max(a.k_table[b * a.k_table_stride + page0 + i], 0), ra.num_pages - 1);
+    if constexpr (!LAT)
+      tab[kRbTable / 2 + i] =
+          min(max(a.v_table[b * a.v_table_stride + page0 + i], 0), ra.num_pages - 1);
+  }
+}
+
+// Bit x: key n + x is seen by draft m; off: keys before the drafts (below zero where there
+// are fewer keys than drafts), word: the drafts that m sees (kMaskTree).
+__device__ __forceinline__ uint32_t rows_sees(const KArgs& a, int n, int Lk, int off, int m,
+                                              uint64_t word) {
+  if (a.mask == kMaskTree) {
+    const int x = n - off;  // the first key's place among the drafts
+    return x >= 64   ? 0u
+           : x >= 0  ? static_cast<uint32_t>(word >> x)
+           : x > -32 ? (static_cast<uint32_t>(word << -x) | ((1u << -x) - 1u))
+                     : ~0u;
+  }
+  const int c = (a.mask == FA2_MASK_NONE ? Lk : min(off + m + 1, Lk)) - n;
+  return c >= 32 ? ~0u : c <= 0 ? 0u : (1u << c) - 1u;
+}
 
 // Wait until at most n tiles of IPT loads each are in flight (n <= MAXN, uniform).
 template <int IPT, int MAXN>
@@ -73,15 +220,23 @@ __device__ __forceinline__ void rows_wait(int n) {
 
 // 16 bytes per lane to LDS from a scalar base and a 32-bit offset per lane (wait states
 // as dma_buffer_x4).
+template <bool NT = false>
 __device__ __forceinline__ void rows_dma(uint64_t base, uint32_t off, uint32_t lds_addr) {
-  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1"
-               :
-               : "v"(off), "s"(base),
-                 "{m0}"(__builtin_amdgcn_readfirstlane(static_cast<int>(lds_addr))));
+  if constexpr (NT)
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1 nt"
+                 :
+                 : "v"(off), "s"(base),
+                   "{m0}"(__builtin_amdgcn_readfirstlane(static_cast<int>(lds_addr))));
+  else
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :
+                 : "v"(off), "s"(base),
+                   "{m0}"(__builtin_amdgcn_readfirstlane(static_cast<int>(lds_addr))));
 }
 
 template <int DT, int DK, int DV, bool LAT, int RG, int MODE>
-__global__ __launch_bounds__(kRbThreads, 1) void fa2_decode_rows_kernel(RowsArgs ra) {
+__global__ __launch_bounds__(kRbThreads, (RowsTile<DK, DV, LAT, RG>::kOcc)) void
+fa2_decode_rows_kernel(RowsArgs ra) {
   static_assert(DT != FA2_DTYPE_F32, "16-bit rows");
   static_assert(RG == 1 || RG == 2 || RG == 4, "row groups");
   constexpr bool BF = Elt<DT>::kBF;
@@ -89,7 +244,7 @@ __global__ __launch_bounds__(kRbThreads, 1) void fa2_decode_rows_kernel(RowsArgs
   constexpr int LM = kPaged ? kModePagedCapped : MODE;
   using GK = RowsGeo<DK>;
   using GV = RowsGeo<LAT ? DK : DV>;
-  using TL = RowsTile<DK, DV, LAT>;
+  using TL = RowsTile<DK, DV, LAT, RG>;
   constexpr int TK = TL::kKeys, NS = TL::kSlots, SB = TK / 32;
   constexpr int DC = DK / 16;               // k-steps of S
   constexpr int DG = kRbWaves / RG;         // waves that share a row group's dims
@@ -107,8 +262,6 @@ __global__ __launch_bounds__(kRbThreads, 1) void fa2_decode_rows_kernel(RowsArgs
   __shared__ int tab[kPaged ? kRbTable : 1];
   __shared__ uint64_t tree_sh[kRbMaxTree];
   __shared__ DecSegment seg_sh;
-  __shared__ int merge_flag;
-  static_assert(kMergePieceBytes<kRbThreads> <= NS * TL::kSlot, "merge area");
 
   const KArgs& a = ra.a;
   const int tid = threadIdx.x;
@@ -131,33 +284,6 @@ __global__ __launch_bounds__(kRbThreads, 1) void fa2_decode_rows_kernel(RowsArgs
   sg.s1 = __builtin_amdgcn_readfirstlane(seg_sh.s1);
   sg.C = __builtin_amdgcn_readfirstlane(seg_sh.C);
 
-  // the piece of sequence j's unit (starting at us in its stream) of this segment
-  auto piece_at = [&](RowsPiece& p, int j, int us) -> bool {
-    const bool whole = sg.C == 0;
-    if (j >= a.batch || (!whole && us >= sg.s1)) return false;
-    p.b = j;
-    p.kvh = stream % a.hkv;
-    p.qblk = stream / a.hkv;
-    p.Lk = __builtin_amdgcn_readfirstlane(walk_len<LM>(a, j));
-    const int n = (p.Lk + kBN - 1) / kBN;
-    p.us = us;
-    p.W = n > 1 ? n : 1;
-    p.unit = j * a.walk_streams + stream;
-    if (whole) {
-      p.t0 = 0;
-      p.T = n;
-      p.np = 1;
-      p.mine = 0;
-      return true;
-    }
-    const int b = max(us, sg.s0), e = min(us + p.W, sg.s1);
-    p.t0 = b - us;
-    p.T = n > 0 ? e - b : 0;
-    const int kf = us / sg.C;
-    p.np = (us + p.W - 1) / sg.C - kf + 1;
-    p.mine = seg_k - kf;
-    return true;
-  };
   auto page_of = [&](int n) -> int {
     return static_cast<int>(__umulhi(2u * static_cast<uint32_t>(n), ra.page_mul) >> ra.page_sh);
   };
@@ -196,7 +322,7 @@ __global__ __launch_bounds__(kRbThreads, 1) void fa2_decode_rows_kernel(RowsArgs
   const bool even_pages = !kPaged || a.page_size % 8 == 0;
 
   RowsPiece p;
-  if (!piece_at(p, sg.j, sg.us)) return;
+  if (!rows_piece<LM>(a, sg, stream, seg_k, sg.j, sg.us, p)) return;
   for (;;) {
     // ---- the piece's rows, mask and first block-table entries -----------------
     const int q0 = p.qblk * (32 * RG);
@@ -222,17 +348,7 @@ __global__ __launch_bounds__(kRbThreads, 1) void fa2_decode_rows_kernel(RowsArgs
       }
     }
     int64_t kbase, vbase;
-    if constexpr (MODE == FA2_LAYOUT_DENSE) {
-      kbase = p.b * a.k_sb + p.kvh * a.k_sh;
-      vbase = p.b * a.v_sb + p.kvh * a.v_sh;
-    } else if constexpr (MODE == FA2_LAYOUT_RAGGED) {
-      const int ks = a.kv_indptr[p.b];
-      kbase = ks * a.k_ss + p.kvh * a.k_sh;
-      vbase = ks * a.v_ss + p.kvh * a.v_sh;
-    } else {
-      kbase = p.kvh * a.k_sh;
-      vbase = p.kvh * a.v_sh;
-    }
+    rows_bases<MODE>(a, p, kbase, vbase);
     const char* kptr = static_cast<const char*>(a.k) + kbase * 2;
     const char* vptr = static_cast<const char*>(a.v) + vbase * 2;
 
@@ -252,15 +368,7 @@ __global__ __launch_bounds__(kRbThreads, 1) void fa2_decode_rows_kernel(RowsArgs
         page0 = page_of(ka);
         const int64_t lim = (static_cast<int64_t>(page0) + kTab) * a.page_size;
         if (lim < kend) kb = ka + max((static_cast<int>(lim) - ka) / kBN * kBN, kBN);
-        const int last = page_of(kb - 1) - page0;
-        for (int i = tid; i <= last; i += kRbThreads) {
-          const int e = a.k_table[p.b * a.k_table_stride + page0 + i];
-          tab[i] = min(max(e, 0), ra.num_pages - 1);
-          if constexpr (!LAT) {
-            const int f = a.v_table[p.b * a.v_table_stride + page0 + i];
-            tab[kTab + i] = min(max(f, 0), ra.num_pages - 1);
-          }
-        }
+        rows_table<LAT, kRbThreads>(ra, p.b, page0, page_of(kb - 1) - page0, tab);
       }
       __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0), which the compiler counts
       __syncthreads();  // the table and the mask are in LDS, the slots are free
@@ -340,6 +448,7 @@ __global__ __launch_bounds__(kRbThreads, 1) void fa2_decode_rows_kernel(RowsArgs
           f32x16 s2[SB];  // odd k-steps: two chains of MFMAs
 #pragma unroll
           for (int sb = 0; sb < SB; ++sb) s2[sb] = (f32x16){};
+          __builtin_amdgcn_sched_barrier(0);
           u32x4 fr[kN];
           static_for<kAhead>([&](auto kc) { fr[decltype(kc)::value] = frag(kc); });
           static_for<kN>([&](auto kc) {
@@ -351,7 +460,6 @@ __global__ __launch_bounds__(kRbThreads, 1) void fa2_decode_rows_kernel(RowsArgs
             if constexpr (k + kAhead < kN)
               fr[k + kAhead] = frag(std::integral_constant<int, k + kAhead>{});
           });
-          if constexpr (SB == 1) s[0] += s2[0];
           __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
           for (int k = 0; k < kN - kAhead; ++k) {
@@ -359,26 +467,16 @@ __global__ __launch_bounds__(kRbThreads, 1) void fa2_decode_rows_kernel(RowsArgs
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
           }
           __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+          __builtin_amdgcn_sched_barrier(0);
+          if constexpr (SB == 1) s[0] += s2[0];
         }
 
         // ---- mask: key n0 + 32 sb + 8 (i / 4) + 4 hi + i % 4 of element i --------
         if (n0 + TK > full) {
 #pragma unroll
           for (int sb = 0; sb < SB; ++sb) {
-            const int n = n0 + 32 * sb;
-            uint32_t sees;  // bit x: key n + x
-            if (a.mask == kMaskTree) {
-              const int x = n - off;  // the first key's place among the drafts
-              sees = x >= 64    ? 0u
-                     : x >= 0   ? static_cast<uint32_t>(word >> x)
-                     : x > -32  ? (static_cast<uint32_t>(word << -x) | ((1u << -x) - 1u))
-                                : ~0u;
-              // (a sequence shorter than its drafts has no key before the first)
-            } else {
-              const int c = (a.mask == FA2_MASK_NONE ? p.Lk : min(off + m + 1, p.Lk)) - n;
-              sees = c >= 32 ? ~0u : c <= 0 ? 0u : (1u << c) - 1u;
-            }
-            sees >>= 4 * hi;
+            const uint32_t sees =
+                rows_sees(a, n0 + 32 * sb, p.Lk, off, m, word) >> (4 * hi);
 #pragma unroll
             for (int i = 0; i < 16; ++i)
               if (!(sees & (1u << ((i >> 2) * 8 + (i & 3))))) s[sb][i] = -INFINITY;
@@ -437,6 +535,7 @@ __global__ __launch_bounds__(kRbThreads, 1) void fa2_decode_rows_kernel(RowsArgs
                            8 * GV::kRowBytes)));
             return (u32x4){lo[0], lo[1], up[0], up[1]};
           };
+          __builtin_amdgcn_sched_barrier(0);
           u32x4 fr[kN];
           static_for<kAhead>([&](auto kc) { fr[decltype(kc)::value] = frag(kc); });
           static_for<kN>([&](auto kc) {
@@ -452,6 +551,7 @@ __global__ __launch_bounds__(kRbThreads, 1) void fa2_decode_rows_kernel(RowsArgs
             __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
           }
           __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
       __syncthreads();  // the window's table and slots have been read
@@ -477,33 +577,21 @@ __global__ __launch_bounds__(kRbThreads, 1) void fa2_decode_rows_kernel(RowsArgs
       }
     } else {
       const int64_t slot = walk_slot(a, sg.C, p.us, stream, p.mine);
-      const uint32_t pr = static_cast<uint32_t>(a.part_rows);
-      const __amdgpu_buffer_rsrc_t rm = make_rsrc_uniform(a.part_ml + slot * pr * 2, pr * 8);
-      const __amdgpu_buffer_rsrc_t ro = make_rsrc_uniform(a.part_o + slot * pr * DV, pr * DV * 4);
       if (r < nrows) {
-        if (dg == 0 && hi == 0)
-          __builtin_amdgcn_raw_buffer_store_b64(
-              (u32x2){__builtin_bit_cast(uint32_t, m_run), __builtin_bit_cast(uint32_t, l_tot)},
-              rm, static_cast<uint32_t>(r) * 8, 0, kCpolSc1);
+        float* ml = a.part_ml + (slot * a.part_rows + r) * 2;
+        float* po = a.part_o + (slot * a.part_rows + r) * DV + d0 * 32 + hi * 4;
+        if (dg == 0 && hi == 0) *reinterpret_cast<f32x2*>(ml) = (f32x2){m_run, l_tot};
 #pragma unroll
         for (int d = 0; d < DBW; ++d)
 #pragma unroll
           for (int g = 0; g < 4; ++g)
-            __builtin_amdgcn_raw_buffer_store_b128(
-                __builtin_bit_cast(u32x4, (f32x4){o[d][g * 4 + 0], o[d][g * 4 + 1],
-                                                  o[d][g * 4 + 2], o[d][g * 4 + 3]}),
-                ro, static_cast<uint32_t>(r * DV + (d0 + d) * 32 + g * 8 + hi * 4) * 4, 0,
-                kCpolSc1);
+            *reinterpret_cast<f32x4*>(po + d * 32 + g * 8) =
+                (f32x4){o[d][g * 4 + 0], o[d][g * 4 + 1], o[d][g * 4 + 2], o[d][g * 4 + 3]};
       }
-      merge_publish();
-      __syncthreads();
-      if (merge_count(a, p.unit, p.np, &merge_flag))
-        merge_pieces<DT, DV, kRbThreads, 32 * RG>(
-            a, [&](int s) { return walk_slot(a, sg.C, p.us, stream, s); }, p.np, nrows, obase, q0,
-            tiles);
     }
-    if (!piece_at(p, walk_next(a, sg, p.b), p.us + p.W)) return;
-    __syncthreads();  // the merge area, the mask and the flag are free
+    if (tid == 0) rows_info(ra, sg, stream, p);
+    if (!rows_piece<LM>(a, sg, stream, seg_k, walk_next(a, sg, p.b), p.us + p.W, p)) return;
+    __syncthreads();  // the mask is free
   }
 }
 

@@ -9,6 +9,7 @@
 
 #include "fa2_host.h"
 #include "fa2_kernel_rows.h"
+#include "fa2_kernel_rows16.h"
 #include "fa2_latent_append.h"
 #include "fa2_latent_prefill.h"
 
@@ -67,8 +68,9 @@ struct RowsCall {
 
 struct RowsPlan {
   int64_t rows;  // of a unit: heads of a kv head times tokens
-  int rg;        // 32-row groups of a q-block
+  int rg;        // 32-row groups of a q-block; 0: units of up to 16 rows
   int64_t part_rows, streams, segs, whole;
+  bool cut;      // units may be cut: the merge is launched
   size_t off_ml, off_o, total;
 };
 
@@ -79,11 +81,14 @@ constexpr int64_t kRbWhole = 16, kRbShort = 4;
 int rows_plan(const RowsCall& c, RowsPlan* pl) {
   pl->rows = c.q_heads / c.kv_heads * c.q_len;
   if (pl->rows > kLim) return FA2_ERR_TOO_LARGE;
-  const int64_t wgs = cu_count_current_device();
+  const int64_t cus = cu_count_current_device();
   const int64_t least = c.dv == 64 ? 2 : 1;  // (a wave has 32 dims at least)
-  pl->rg = static_cast<int>(std::max<int64_t>(least, pl->rows <= 32 ? 1 : pl->rows <= 64 ? 2 : 4));
-  const int64_t nqb = cdiv(pl->rows, 32 * pl->rg);
-  pl->part_rows = std::min<int64_t>(pl->rows, 32 * pl->rg);
+  pl->rg = static_cast<int>(pl->rows <= kR16Rows ? 0 : pl->rows <= 32 ? least : pl->rows <= 64 ? 2 : 4);
+  const int64_t block_rows = pl->rg ? 32 * pl->rg : kR16Rows;
+  const int64_t nqb = cdiv(pl->rows, block_rows);
+  // workgroups per CU (RowsTile::kOcc)
+  const int64_t wgs = cus * (pl->rg == 0 ? 1 : c.latent ? (c.dv == 256 && pl->rg < 4 ? 2 : 1) : c.dv < 256 ? 2 : 1);
+  pl->part_rows = std::min<int64_t>(pl->rows, block_rows);
   pl->streams = c.kv_heads * nqb;
   // tiles of the call at most (lengths are on the device)
   const int64_t keys = c.layout == FA2_LAYOUT_PAGED ? c.table_width * c.page_size : c.kv_len;
@@ -92,13 +97,14 @@ int rows_plan(const RowsCall& c, RowsPlan* pl) {
   if (total >= (int64_t(1) << 30)) return FA2_ERR_TOO_LARGE;
   pl->segs = std::min(std::max<int64_t>(1, wgs / pl->streams), cdiv(total, kRbMinTiles));
   const int64_t grid = pl->streams * pl->segs;
-  // (one segment per stream cuts no unit)
-  const int64_t slots = pl->segs > 1 ? 2 * grid : 0;
-  if (slots * pl->part_rows * c.dv * 4 >= (int64_t(1) << 31) || pl->streams * c.batch > kLim)
+  // (one segment per stream cuts no unit, and neither do short ones)
+  pl->cut = pl->segs > 1 && tiles > kRbShort;
+  const int64_t slots = pl->cut ? 2 * grid : 0;
+  if (pl->streams * c.batch > kLim || slots > kLim)
     return FA2_ERR_TOO_LARGE;
   const int64_t idle = std::max<int64_t>(0, grid - pl->streams * c.batch);
   pl->whole = std::max(kRbWhole / 2, kRbWhole * idle / grid);
-  size_t off = static_cast<size_t>(pl->streams * c.batch) * sizeof(uint64_t);
+  size_t off = static_cast<size_t>(pl->streams * c.batch) * sizeof(int2);
   off = (off + 255) & ~size_t(255);
   pl->off_ml = off;
   off += static_cast<size_t>(slots * pl->part_rows) * 2 * sizeof(float);
@@ -123,15 +129,11 @@ int rows_fill(const RowsCall& c, const RowsPlan& pl, float scale, void* workspac
   a.num_splits = 1;
   a.scale_log2 = scale * 1.4426950408889634f;
   char* ws = static_cast<char*>(workspace);
-  a.merge_ctr = reinterpret_cast<uint64_t*>(ws);
-  try {
-    a.merge_tag = next_merge_tag();
-  } catch (...) {  // (no random device: no tag, no call)
-    return FA2_ERR_HIP;
-  }
+  ra->info = reinterpret_cast<int2*>(ws);
   a.part_ml = reinterpret_cast<float*>(ws + pl.off_ml);
   a.part_o = reinterpret_cast<float*>(ws + pl.off_o);
   a.part_rows = static_cast<int32_t>(pl.part_rows);
+  a.block_rows = pl.rg ? 32 * pl.rg : kR16Rows;
   a.walk_streams = static_cast<int32_t>(pl.streams);
   a.walk_segs = static_cast<int32_t>(pl.segs);
   a.walk_min = kRbMinTiles;
@@ -156,40 +158,44 @@ int rows_fill(const RowsCall& c, const RowsPlan& pl, float scale, void* workspac
 }
 
 template <int DT, int DK, int DV, bool LAT, int MODE>
-void launch_rows(const RowsArgs& ra, int rg, hipStream_t st) {
-  const dim3 grid(static_cast<uint32_t>(ra.a.walk_streams * ra.a.walk_segs)), block(kRbThreads);
-  if (rg == 4) {
+void launch_rows(const RowsArgs& ra, const RowsPlan& pl, hipStream_t st) {
+  const dim3 grid(static_cast<uint32_t>(pl.streams * pl.segs)), block(kRbThreads);
+  constexpr int least = DV > 64 ? 1 : 2;
+  if (pl.rg == 0)
+    hipLaunchKernelGGL((fa2_decode_rows16_kernel<DT, DK, DV, LAT, MODE>), grid,
+                       dim3(Rows16Tile<DK, DV, LAT>::kThreads), 0, st, ra);
+  else if (pl.rg == 4)
     hipLaunchKernelGGL((fa2_decode_rows_kernel<DT, DK, DV, LAT, 4, MODE>), grid, block, 0, st, ra);
-    return;
-  }
-  if constexpr (DV > 64) {
-    if (rg == 1) {
-      hipLaunchKernelGGL((fa2_decode_rows_kernel<DT, DK, DV, LAT, 1, MODE>), grid, block, 0, st,
-                         ra);
-      return;
-    }
-  }
-  hipLaunchKernelGGL((fa2_decode_rows_kernel<DT, DK, DV, LAT, 2, MODE>), grid, block, 0, st, ra);
+  else if (pl.rg > least)
+    hipLaunchKernelGGL((fa2_decode_rows_kernel<DT, DK, DV, LAT, 2, MODE>), grid, block, 0, st, ra);
+  else
+    hipLaunchKernelGGL((fa2_decode_rows_kernel<DT, DK, DV, LAT, least, MODE>), grid, block, 0, st,
+                       ra);
+  if (pl.cut)
+    hipLaunchKernelGGL((fa2_rows_merge_kernel<DT, DV>),
+                       dim3(static_cast<uint32_t>(pl.streams * ra.a.batch),
+                            static_cast<uint32_t>(cdiv(pl.part_rows, kMergeRows<DV>))),
+                       dim3(256), 0, st, ra);
 }
 
 template <int DT, int MODE>
-void launch_tree_dim(int64_t d, const RowsArgs& ra, int rg, hipStream_t st) {
-  if (d == 64) launch_rows<DT, 64, 64, false, MODE>(ra, rg, st);
-  else if (d == 128) launch_rows<DT, 128, 128, false, MODE>(ra, rg, st);
-  else launch_rows<DT, 256, 256, false, MODE>(ra, rg, st);
+void launch_tree_dim(int64_t d, const RowsArgs& ra, const RowsPlan& pl, hipStream_t st) {
+  if (d == 64) launch_rows<DT, 64, 64, false, MODE>(ra, pl, st);
+  else if (d == 128) launch_rows<DT, 128, 128, false, MODE>(ra, pl, st);
+  else launch_rows<DT, 256, 256, false, MODE>(ra, pl, st);
 }
 
 template <int DT>
-void launch_tree(int layout, int64_t d, const RowsArgs& ra, int rg, hipStream_t st) {
-  if (layout == FA2_LAYOUT_DENSE) launch_tree_dim<DT, FA2_LAYOUT_DENSE>(d, ra, rg, st);
-  else if (layout == FA2_LAYOUT_RAGGED) launch_tree_dim<DT, FA2_LAYOUT_RAGGED>(d, ra, rg, st);
-  else launch_tree_dim<DT, FA2_LAYOUT_PAGED>(d, ra, rg, st);
+void launch_tree(int layout, int64_t d, const RowsArgs& ra, const RowsPlan& pl, hipStream_t st) {
+  if (layout == FA2_LAYOUT_DENSE) launch_tree_dim<DT, FA2_LAYOUT_DENSE>(d, ra, pl, st);
+  else if (layout == FA2_LAYOUT_RAGGED) launch_tree_dim<DT, FA2_LAYOUT_RAGGED>(d, ra, pl, st);
+  else launch_tree_dim<DT, FA2_LAYOUT_PAGED>(d, ra, pl, st);
 }
 
 template <int DT>
-void launch_latent(int64_t latent, const RowsArgs& ra, int rg, hipStream_t st) {
-  if (latent == 512) launch_rows<DT, 576, 512, true, FA2_LAYOUT_PAGED>(ra, rg, st);
-  else launch_rows<DT, 320, 256, true, FA2_LAYOUT_PAGED>(ra, rg, st);
+void launch_latent(int64_t latent, const RowsArgs& ra, const RowsPlan& pl, hipStream_t st) {
+  if (latent == 512) launch_rows<DT, 576, 512, true, FA2_LAYOUT_PAGED>(ra, pl, st);
+  else launch_rows<DT, 320, 256, true, FA2_LAYOUT_PAGED>(ra, pl, st);
 }
 
 bool scale_ok(float s) { return s > 0.f && std::isfinite(s); }
@@ -483,8 +489,8 @@ extern "C" int fa2_latent_decode(const fa2_latent_decode_params* p, void* stream
   a.k_table_stride = a.v_table_stride = p->table_stride;
   a.k_ss = a.v_ss = p->latent_dim + p->rope_dim;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (p->dtype == FA2_DTYPE_F16) launch_latent<FA2_DTYPE_F16>(p->latent_dim, ra, pl.rg, st);
-  else launch_latent<FA2_DTYPE_BF16>(p->latent_dim, ra, pl.rg, st);
+  if (p->dtype == FA2_DTYPE_F16) launch_latent<FA2_DTYPE_F16>(p->latent_dim, ra, pl, st);
+  else launch_latent<FA2_DTYPE_BF16>(p->latent_dim, ra, pl, st);
   return launched();
 }
 
@@ -520,8 +526,8 @@ extern "C" int fa2_tree_decode(const fa2_tree_decode_params* p, void* stream) {
   a.k_table_stride = p->k_table_stride;
   a.v_table_stride = p->v_table_stride;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (p->dtype == FA2_DTYPE_F16) launch_tree<FA2_DTYPE_F16>(p->layout, p->head_dim, ra, pl.rg, st);
-  else launch_tree<FA2_DTYPE_BF16>(p->layout, p->head_dim, ra, pl.rg, st);
+  if (p->dtype == FA2_DTYPE_F16) launch_tree<FA2_DTYPE_F16>(p->layout, p->head_dim, ra, pl, st);
+  else launch_tree<FA2_DTYPE_BF16>(p->layout, p->head_dim, ra, pl, st);
   return launched();
 }
 
