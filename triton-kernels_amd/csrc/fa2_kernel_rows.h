@@ -16,6 +16,9 @@ constexpr int kRbMaxTree = 64;  // drafts of a tree: bits of a mask word
 // Mask of a call beyond enum fa2_mask: the drafts that each draft sees.
 constexpr int kMaskTree = 3;
 
+// A second piece of a workgroup costs about as much as this many tiles of kBN keys.
+constexpr int kRbSwitch = 6;
+
 struct RowsArgs {
   KArgs a;  // q rows: token m of head h at h * q_sh + m * q_ss; o rows: o_ss apart
   int2* info;  // of each unit: its pieces and the part slot of the first (rows_info)
@@ -63,17 +66,88 @@ struct RowsPiece {
   int us, W, unit;
 };
 
-// The piece of sequence j's unit (starting at us in its stream) in segment sg; false past
+// A workgroup's segment and, for batches of up to 64, every length in the lanes of each
+// wave (which then locates the segment by itself: one load, no barrier, no load per piece).
+struct RowsWalk {
+  DecSegment sg;
+  int lens;
+  bool in_lanes;
+  bool aligned;  // units start at segments: they take whole segments of the stream
+};
+
+// walk_locate's rule; sh: LDS.  Every thread of the workgroup.
+template <int LM>
+__device__ __forceinline__ RowsWalk rows_locate(const KArgs& a, int k, DecSegment* sh) {
+  RowsWalk w;
+  const int lane = threadIdx.x & 63;
+  w.in_lanes = a.batch <= 64;
+  w.aligned = false;
+  w.lens = 0;
+  if (!w.in_lanes) {
+    if (threadIdx.x < 64) walk_locate<LM>(a, k, sh);
+    __syncthreads();
+    auto rd = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    w.sg = DecSegment{rd(sh->j), rd(sh->us), rd(sh->s0), rd(sh->s1), rd(sh->C)};
+    return w;
+  }
+  if (lane < a.batch) w.lens = walk_len<LM>(a, lane);
+  const int W = lane < a.batch ? walk_weight(w.lens) : 0;
+  int incl = W, longest = W;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(incl, d);
+    if (lane >= d) incl += y;
+    longest = max(longest, __shfl_xor(longest, d));
+  }
+  longest = __builtin_amdgcn_readfirstlane(longest);
+  int total = __builtin_amdgcn_readlane(incl, 63);
+  int C = max((total + a.walk_segs - 1) / a.walk_segs, a.walk_min);
+  if (longest <= a.walk_short || walk_keep_whole(a, longest, C, a.walk_whole)) {
+    w.sg = DecSegment{k, 0, 0, 0, 0};
+    return w;
+  }
+  // Units that start at segments: sum ceil(W / A) <= total / A + batch segments, so A = total /
+  // (segs - batch) will do; no workgroup has two pieces then, which is worth kRbSwitch tiles.
+  int room = W;
+  if (a.walk_segs > a.batch) {
+    const int free = a.walk_segs - a.batch;
+    const int A = max((total + free - 1) / free, a.walk_min);
+    if (A <= C + kRbSwitch) {
+      w.aligned = true;
+      C = A;
+      room = (W + A - 1) / A * A;
+      incl = room;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int y = __shfl_up(incl, d);
+        if (lane >= d) incl += y;
+      }
+      total = __builtin_amdgcn_readlane(incl, 63);
+    }
+  }
+  const int s0 = min(k * C, total);
+  if (s0 >= total) {
+    w.sg = DecSegment{a.batch, total, total, total, C};
+    return w;
+  }
+  const int j = __builtin_ctzll(__ballot(incl > s0));  // the first whose end is past s0
+  w.sg = DecSegment{j, __builtin_amdgcn_readlane(incl - room, j), s0, min(s0 + C, total), C};
+  return w;
+}
+
+// The piece of sequence j's unit (starting at us in its stream) in the segment; false past
 // the segment's end.
 template <int LM>
-__device__ __forceinline__ bool rows_piece(const KArgs& a, const DecSegment& sg, int stream,
+__device__ __forceinline__ bool rows_piece(const KArgs& a, const RowsWalk& w, int stream,
                                            int seg_k, int j, int us, RowsPiece& p) {
+  const DecSegment& sg = w.sg;
   const bool whole = sg.C == 0;
   if (j >= a.batch || (!whole && us >= sg.s1)) return false;
   p.b = j;
   p.kvh = stream % a.hkv;
   p.qblk = stream / a.hkv;
-  p.Lk = __builtin_amdgcn_readfirstlane(walk_len<LM>(a, j));
+  p.Lk = w.in_lanes ? __builtin_amdgcn_readlane(w.lens, j)
+                    : __builtin_amdgcn_readfirstlane(walk_len<LM>(a, j));
   const int n = (p.Lk + kBN - 1) / kBN;
   p.us = us;
   p.W = n > 1 ? n : 1;
@@ -91,6 +165,7 @@ __device__ __forceinline__ bool rows_piece(const KArgs& a, const DecSegment& sg,
   const int kf = us / sg.C;
   p.np = (us + p.W - 1) / sg.C - kf + 1;
   p.mine = seg_k - kf;
+  if (w.aligned) p.W = p.np * sg.C;  // (the room that it takes)
   return true;
 }
 
@@ -178,19 +253,33 @@ __device__ __forceinline__ void rows_bases(const KArgs& a, const RowsPiece& p, i
   }
 }
 
-// Block-table entries page0 .. page0 + last of sequence b into LDS, clamped into the pool;
-// V's behind K's.
+// Block-table entries page0 .. page0 + last of sequence b, clamped into the pool, on their
+// way to LDS: this thread's first ones in registers, the rest behind them.  (V's lie behind
+// K's.  What is loaded between load and store does not delay the entries.)
 template <bool LAT, int NT>
-__device__ __forceinline__ void rows_table(const RowsArgs& ra, int b, int page0, int last,
-                                           int* tab) {
-  const KArgs& a = ra.a;
-  for (int i = threadIdx.x; i <= last; i += NT) {
-    tab[i] = min(max(a.k_table[b * a.k_table_stride + page0 + i], 0), ra.num_pages - 1);
-    if constexpr (!LAT)
-      tab[kRbTable / 2 + i] =
-          min(max(a.v_table[b * a.v_table_stride + page0 + i], 0), ra.num_pages - 1);
+struct RowsTable {
+  int k, v;
+  __device__ __forceinline__ void load(const RowsArgs& ra, int b, int page0, int last) {
+    const KArgs& a = ra.a;
+    const int i = page0 + min(static_cast<int>(threadIdx.x), last);
+    k = a.k_table[b * a.k_table_stride + i];
+    if constexpr (!LAT) v = a.v_table[b * a.v_table_stride + i];
   }
-}
+  __device__ __forceinline__ void store(const RowsArgs& ra, int b, int page0, int last,
+                                        int* tab) const {
+    const KArgs& a = ra.a;
+    auto in = [&](int e) { return min(max(e, 0), ra.num_pages - 1); };
+    const int tid = threadIdx.x;
+    if (tid <= last) {
+      tab[tid] = in(k);
+      if constexpr (!LAT) tab[kRbTable / 2 + tid] = in(v);
+    }
+    for (int i = tid + NT; i <= last; i += NT) {
+      tab[i] = in(a.k_table[b * a.k_table_stride + page0 + i]);
+      if constexpr (!LAT) tab[kRbTable / 2 + i] = in(a.v_table[b * a.v_table_stride + page0 + i]);
+    }
+  }
+};
 
 // Bit x: key n + x is seen by draft m; off: keys before the drafts (below zero where there
 // are fewer keys than drafts), word: the drafts that m sees (kMaskTree).
@@ -275,15 +364,8 @@ fa2_decode_rows_kernel(RowsArgs ra) {
   const int stream = static_cast<int>(blockIdx.x) % a.walk_streams;
   const int seg_k = static_cast<int>(blockIdx.x) / a.walk_streams;
 
-  if (wave == 0) walk_locate<LM>(a, seg_k, &seg_sh);
-  __syncthreads();
-  DecSegment sg;
-  sg.j = __builtin_amdgcn_readfirstlane(seg_sh.j);
-  sg.us = __builtin_amdgcn_readfirstlane(seg_sh.us);
-  sg.s0 = __builtin_amdgcn_readfirstlane(seg_sh.s0);
-  sg.s1 = __builtin_amdgcn_readfirstlane(seg_sh.s1);
-  sg.C = __builtin_amdgcn_readfirstlane(seg_sh.C);
-
+  const RowsWalk walk = rows_locate<LM>(a, seg_k, &seg_sh);
+  const DecSegment& sg = walk.sg;
   auto page_of = [&](int n) -> int {
     return static_cast<int>(__umulhi(2u * static_cast<uint32_t>(n), ra.page_mul) >> ra.page_sh);
   };
@@ -322,23 +404,13 @@ fa2_decode_rows_kernel(RowsArgs ra) {
   const bool even_pages = !kPaged || a.page_size % 8 == 0;
 
   RowsPiece p;
-  if (!rows_piece<LM>(a, sg, stream, seg_k, sg.j, sg.us, p)) return;
+  if (!rows_piece<LM>(a, walk, stream, seg_k, sg.j, sg.us, p)) return;
   for (;;) {
     // ---- the piece's rows, mask and first block-table entries -----------------
     const int q0 = p.qblk * (32 * RG);
     const int row = q0 + rg * 32 + l32;
     const int m = row % a.pack_m;  // draft
     const int nrows = min(a.q_len - q0, 32 * RG);
-    u32x4 qf[DC];
-    {
-      const int h = p.kvh * (a.hq / a.hkv) + row / a.pack_m;
-      const uint16_t* src = static_cast<const uint16_t*>(a.q) + p.b * a.q_sb + h * a.q_sh +
-                            m * a.q_ss + hi * 8;
-      const bool ok = row < a.q_len;
-#pragma unroll
-      for (int c = 0; c < DC; ++c)
-        qf[c] = ok ? *reinterpret_cast<const u32x4*>(src + c * 16) : (u32x4){0u, 0u, 0u, 0u};
-    }
     if (a.mask == kMaskTree) {
       for (int i = wave; i < a.pack_m; i += kRbWaves) {
         const uint8_t sees =
@@ -362,15 +434,30 @@ fa2_decode_rows_kernel(RowsArgs ra) {
     uint64_t word = 0;
 
     // ---- windows: keys whose block-table entries lie in LDS --------------------
-    for (int ka = p.t0 * kBN; ka < kend;) {
-      int kb = kend, page0 = 0;
+    int ka = p.t0 * kBN, kb, page0;
+    RowsTable<LAT, kRbThreads> entries;
+    auto window = [&]() {
+      kb = kend;
+      page0 = 0;
       if constexpr (kPaged) {
         page0 = page_of(ka);
         const int64_t lim = (static_cast<int64_t>(page0) + kTab) * a.page_size;
         if (lim < kend) kb = ka + max((static_cast<int>(lim) - ka) / kBN * kBN, kBN);
-        rows_table<LAT, kRbThreads>(ra, p.b, page0, page_of(kb - 1) - page0, tab);
+        if (ka < kend) entries.load(ra, p.b, page0, page_of(kb - 1) - page0);
       }
-      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0), which the compiler counts
+    };
+    window();
+    u32x4 qf[DC];
+    {
+      const int qr = min(row, a.q_len - 1);  // (rows past the last repeat it: not stored)
+      const int h = p.kvh * (a.hq / a.hkv) + qr / a.pack_m;
+      const uint16_t* src = static_cast<const uint16_t*>(a.q) + p.b * a.q_sb + h * a.q_sh +
+                            (qr % a.pack_m) * a.q_ss + hi * 8;
+#pragma unroll
+      for (int c = 0; c < DC; ++c) qf[c] = *reinterpret_cast<const u32x4*>(src + c * 16);
+    }
+    for (; ka < kend; ka = kb, window()) {
+      if constexpr (kPaged) entries.store(ra, p.b, page0, page_of(kb - 1) - page0, tab);
       __syncthreads();  // the table and the mask are in LDS, the slots are free
       if (a.mask == kMaskTree) word = tree_sh[m];
 
@@ -426,6 +513,8 @@ fa2_decode_rows_kernel(RowsArgs ra) {
         }
       };
       for (int t = 0; t < NS - 1 && t < T; ++t) issue(t);
+      // Q and the first tiles: later waits of the compiler's would drain the tiles
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
 
       for (int t = 0; t < T; ++t) {
         rows_wait<IPT, NS - 2>(T - 1 - t);
@@ -496,8 +585,10 @@ fa2_decode_rows_kernel(RowsArgs ra) {
           const float alpha = fast_exp2(need ? m_run - mt : 0.f);
           m_run = need ? mt : m_run;
           l_run *= alpha;
+          if (n0 > p.t0 * kBN) {  // (nothing yet before the piece's first tile)
 #pragma unroll
-          for (int d = 0; d < DBW; ++d) o[d] *= alpha;
+            for (int d = 0; d < DBW; ++d) o[d] *= alpha;
+          }
         }
         const float m_use = (m_run == -INFINITY ? 0.f : m_run) - kLift;
         u32x4 pf[2 * SB];
@@ -555,7 +646,6 @@ fa2_decode_rows_kernel(RowsArgs ra) {
         }
       }
       __syncthreads();  // the window's table and slots have been read
-      ka = kb;
     }
 
     // ---- the piece's end ---------------------------------------------------------
@@ -590,7 +680,7 @@ fa2_decode_rows_kernel(RowsArgs ra) {
       }
     }
     if (tid == 0) rows_info(ra, sg, stream, p);
-    if (!rows_piece<LM>(a, sg, stream, seg_k, walk_next(a, sg, p.b), p.us + p.W, p)) return;
+    if (!rows_piece<LM>(a, walk, stream, seg_k, walk_next(a, sg, p.b), p.us + p.W, p)) return;
     __syncthreads();  // the mask is free
   }
 }

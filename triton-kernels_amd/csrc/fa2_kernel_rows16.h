@@ -44,7 +44,7 @@ fa2_decode_rows16_kernel(RowsArgs ra) {
   constexpr int R = kR16Rows;
 
   __shared__ __attribute__((aligned(1024))) char tiles[NW * TL::kSlot];
-  __shared__ float mrg_ml[NW][R][2];
+  __shared__ float mrg_ml[NW][R][2], sum_ml[R][2];
   __shared__ int tab[kPaged ? kRbTable : 1];
   __shared__ uint64_t tree_sh[R];
   __shared__ DecSegment seg_sh;
@@ -59,14 +59,8 @@ fa2_decode_rows16_kernel(RowsArgs ra) {
   const int stream = static_cast<int>(blockIdx.x) % a.walk_streams;
   const int seg_k = static_cast<int>(blockIdx.x) / a.walk_streams;
 
-  if (wave == 0) walk_locate<LM>(a, seg_k, &seg_sh);
-  __syncthreads();
-  DecSegment sg;
-  sg.j = __builtin_amdgcn_readfirstlane(seg_sh.j);
-  sg.us = __builtin_amdgcn_readfirstlane(seg_sh.us);
-  sg.s0 = __builtin_amdgcn_readfirstlane(seg_sh.s0);
-  sg.s1 = __builtin_amdgcn_readfirstlane(seg_sh.s1);
-  sg.C = __builtin_amdgcn_readfirstlane(seg_sh.C);
+  const RowsWalk walk = rows_locate<LM>(a, seg_k, &seg_sh);
+  const DecSegment& sg = walk.sg;
   auto page_of = [&](int n) -> int {
     return static_cast<int>(__umulhi(2u * static_cast<uint32_t>(n), ra.page_mul) >> ra.page_sh);
   };
@@ -100,20 +94,10 @@ fa2_decode_rows16_kernel(RowsArgs ra) {
   const bool even = (!kPaged || a.page_size % 8 == 0) && ksb % 32 == 0 && vsb % 32 == 0;
 
   RowsPiece p;
-  if (!rows_piece<LM>(a, sg, stream, seg_k, sg.j, sg.us, p)) return;
+  if (!rows_piece<LM>(a, walk, stream, seg_k, sg.j, sg.us, p)) return;
   for (;;) {
     const int m = l16 % a.pack_m;  // draft
     const int rows = a.q_len;
-    u32x4 qf[DJ];
-    {
-      const int h = p.kvh * (a.hq / a.hkv) + l16 / a.pack_m;
-      const uint16_t* src = static_cast<const uint16_t*>(a.q) + p.b * a.q_sb + h * a.q_sh +
-                            m * a.q_ss + g * 8;
-      const bool ok = l16 < rows;
-#pragma unroll
-      for (int j = 0; j < DJ; ++j)
-        qf[j] = ok ? *reinterpret_cast<const u32x4*>(src + j * 32) : (u32x4){0u, 0u, 0u, 0u};
-    }
     if (a.mask == kMaskTree) {
       for (int i = wave; i < a.pack_m; i += NW) {
         const uint8_t sees =
@@ -137,15 +121,30 @@ fa2_decode_rows16_kernel(RowsArgs ra) {
     const int kend = min((p.t0 + p.T) * kBN, p.Lk);
     uint64_t word = 0;
 
-    for (int ka = p.t0 * kBN; ka < kend;) {
-      int kb = kend, page0 = 0;
+    int ka = p.t0 * kBN, kb, page0;
+    RowsTable<LAT, NT> entries;
+    auto window = [&]() {  // keys whose block-table entries lie in LDS
+      kb = kend;
+      page0 = 0;
       if constexpr (kPaged) {
         page0 = page_of(ka);
         const int64_t lim = (static_cast<int64_t>(page0) + kTab) * a.page_size;
         if (lim < kend) kb = ka + max((static_cast<int>(lim) - ka) / kBN * kBN, kBN);
-        rows_table<LAT, NT>(ra, p.b, page0, page_of(kb - 1) - page0, tab);
+        if (ka < kend) entries.load(ra, p.b, page0, page_of(kb - 1) - page0);
       }
-      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0), which the compiler counts
+    };
+    window();
+    u32x4 qf[DJ];
+    {
+      const int qr = min(l16, rows - 1);  // (rows past the last repeat it: not stored)
+      const int h = p.kvh * (a.hq / a.hkv) + qr / a.pack_m;
+      const uint16_t* src = static_cast<const uint16_t*>(a.q) + p.b * a.q_sb + h * a.q_sh +
+                            (qr % a.pack_m) * a.q_ss + g * 8;
+#pragma unroll
+      for (int j = 0; j < DJ; ++j) qf[j] = *reinterpret_cast<const u32x4*>(src + j * 32);
+    }
+    for (; ka < kend; ka = kb, window()) {
+      if constexpr (kPaged) entries.store(ra, p.b, page0, page_of(kb - 1) - page0, tab);
       __syncthreads();  // the table and the mask are in LDS, the slots are free
       if (a.mask == kMaskTree) word = tree_sh[m];
 
@@ -202,6 +201,8 @@ fa2_decode_rows16_kernel(RowsArgs ra) {
         issue(IsK{}, n0);
         if constexpr (!LAT) issue(IsV{}, n0);
       }
+      // Q and the first tile: later waits of the compiler's would drain the tiles
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
       for (; n0 < kb; n0 += kStep) {
         const bool more = n0 + kStep < kb;
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kVOps) : "memory");  // K(t)
@@ -263,8 +264,10 @@ fa2_decode_rows16_kernel(RowsArgs ra) {
           const float alpha = fast_exp2(m_run - (mn == -INFINITY ? 0.f : mn));
           m_run = mn;
           l_run *= alpha;
+          if (n0 >= p.t0 * kBN + kStep) {  // (nothing yet before the wave's first tile)
 #pragma unroll
-          for (int d = 0; d < DB; ++d) o[d] *= alpha;
+            for (int d = 0; d < DB; ++d) o[d] *= alpha;
+          }
         }
         const float mu = (m_run == -INFINITY ? 0.f : m_run) - kLift;
         u32x4 pf[KK];
@@ -325,7 +328,6 @@ fa2_decode_rows16_kernel(RowsArgs ra) {
         }
       }
       __syncthreads();  // the window's table and slots have been read
-      ka = kb;
     }
 
     // ---- the piece's end: the waves' states meet in LDS, in wave order -----------------
@@ -339,42 +341,47 @@ fa2_decode_rows16_kernel(RowsArgs ra) {
     float mg = -INFINITY;
 #pragma unroll
     for (int x = 0; x < NW; ++x) mg = fmaxf(mg, mrg_ml[x][l16][0]);
-    const float f = fast_exp2(m_run - (mg == -INFINITY ? 0.f : mg));
+    const float mu = mg == -INFINITY ? 0.f : mg;
+    const float f = fast_exp2(m_run - mu);
     if (l16 < rows) {
       const uint32_t po = tiles0 + (wave * R + l16) * kPitch + 16 * g;
 #pragma unroll
       for (int d = 0; d < DB; ++d) *(lds_f32x4_t*)(lds_ptr(po) + 64 * d) = o[d] * f;
     }
+    if (wave == 0 && g == 0) {
+      float lt = 0.f;
+#pragma unroll
+      for (int x = 0; x < NW; ++x) lt += mrg_ml[x][l16][1] * fast_exp2(mrg_ml[x][l16][0] - mu);
+      sum_ml[l16][0] = mg;
+      sum_ml[l16][1] = lt;
+    }
     __syncthreads();
     const int64_t obase = p.b * a.o_sb + p.kvh * (a.hq / a.hkv) * a.o_sh;
     const int64_t part = p.np == 1 ? 0 : walk_slot(a, sg.C, p.us, stream, p.mine);
-    constexpr int kTPR = DV / 4;
+    constexpr int kTPR = DV / 4, kRP = NT / kTPR;  // threads of a row, rows at once
     const int col = (tid % kTPR) * 4;
-    for (int r = tid / kTPR; r < rows; r += NT / kTPR) {
-      float mt = -INFINITY;
 #pragma unroll
-      for (int x = 0; x < NW; ++x) mt = fmaxf(mt, mrg_ml[x][r][0]);
-      const float mu = mt == -INFINITY ? 0.f : mt;
-      float lt = 0.f;
+    for (int r0 = 0; r0 < R; r0 += kRP) {
+      const int r = r0 + tid / kTPR;
+      if (r >= rows) break;
       f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int x = 0; x < NW; ++x) {
-        lt += mrg_ml[x][r][1] * fast_exp2(mrg_ml[x][r][0] - mu);
+      for (int x = 0; x < NW; ++x)
         acc += *(const lds_f32x4_t*)(lds_ptr(tiles0 + (x * R + r) * kPitch + col * 4));
-      }
       if (p.np == 1) {  // 0/0 -> NaN for a row with no key
-        const float inv = 1.f / lt;
+        const float inv = 1.f / sum_ml[r][1];
         *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.o) + obase +
                                   static_cast<int64_t>(r) * a.o_ss + col) =
             (u32x2){pack2<BF>(acc[0] * inv, acc[1] * inv), pack2<BF>(acc[2] * inv, acc[3] * inv)};
       } else {
         const int64_t at = part * a.part_rows + r;
-        if (col == 0) *reinterpret_cast<f32x2*>(a.part_ml + at * 2) = (f32x2){mt, lt};
+        if (col == 0)
+          *reinterpret_cast<f32x2*>(a.part_ml + at * 2) = (f32x2){sum_ml[r][0], sum_ml[r][1]};
         *reinterpret_cast<f32x4*>(a.part_o + at * DV + col) = acc;
       }
     }
     if (tid == 0) rows_info(ra, sg, stream, p);
-    if (!rows_piece<LM>(a, sg, stream, seg_k, walk_next(a, sg, p.b), p.us + p.W, p)) return;
+    if (!rows_piece<LM>(a, walk, stream, seg_k, walk_next(a, sg, p.b), p.us + p.W, p)) return;
     __syncthreads();  // the merge area and the mask are free
   }
 }
