@@ -323,6 +323,37 @@ __device__ __forceinline__ void rows_dma(uint64_t base, uint32_t off, uint32_t l
                    "{m0}"(__builtin_amdgcn_readfirstlane(static_cast<int>(lds_addr))));
 }
 
+// x, whose uses are not computed ahead of this place (registers of the tile loop).
+__device__ __forceinline__ int here(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// MFMAs of the kernel whose accumulators fill the AGPRs (32 rows of 512 dims per wave): O^T
+// there (mma32_acc), S in VGPRs (mma32_vgpr), as the compiler left to itself moves both to and
+// fro and spills Q.  Two wait states stand between a VALU write of an operand and its MFMA; who
+// reads the result waits 24 (mma32_wait; the longest MFMA asks for 20).
+template <bool BF>
+__device__ __forceinline__ void mma32_acc(f32x16& c, u32x4 a, u32x4 b) {
+  if constexpr (BF)
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  else
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+template <bool BF>
+__device__ __forceinline__ void mma32_vgpr(f32x16& c, u32x4 a, u32x4 b) {
+  if constexpr (BF)
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+  else
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+}
+__device__ __forceinline__ void mma32_wait(f32x16& c) {
+  asm volatile("s_nop 15\n\ts_nop 7" : "+v"(c));
+}
+// c lies in AGPRs here: what scales or stores it takes its elements apart behind this, so that
+// the loops carry it whole.
+__device__ __forceinline__ void in_acc(f32x16& c) { asm volatile("" : "+a"(c)); }
+
 template <int DT, int DK, int DV, bool LAT, int RG, int MODE>
 __global__ __launch_bounds__(kRbThreads, (RowsTile<DK, DV, LAT, RG>::kOcc)) void
 fa2_decode_rows_kernel(RowsArgs ra) {
@@ -339,6 +370,7 @@ fa2_decode_rows_kernel(RowsArgs ra) {
   constexpr int DG = kRbWaves / RG;         // waves that share a row group's dims
   constexpr int DBW = DV / 32 / DG;         // 32-dim blocks of a wave's O^T
   static_assert(DBW >= 1, "dims of a wave");
+  constexpr bool kAcc = DBW == 16;          // O^T fills the AGPRs
   constexpr int GPW = TK / 32;              // 8-row groups a wave loads per tile
   constexpr int IPT = GPW * (GK::kGI + (LAT ? 0 : GV::kGI));
   constexpr int kVOff = LAT ? 0 : TK * GK::kRowBytes;  // V rows in a slot
@@ -388,18 +420,18 @@ fa2_decode_rows_kernel(RowsArgs ra) {
   // loads: byte offset of this lane's chunk within the 8 rows of a group, whose rows
   // are 8 (wave & 1) ..+7 in the swizzle
   const uint32_t ksb = static_cast<uint32_t>(a.k_ss * 2), vsb = static_cast<uint32_t>(a.v_ss * 2);
-  auto lane_row = [&](auto geo, int i) -> int { return (i * 64 + lane) / decltype(geo)::kNC; };
-  auto lane_chunk = [&](auto geo, int i) -> uint32_t {
+  auto lane_row = [&](auto geo, int i, int ln) -> int { return (i * 64 + ln) / decltype(geo)::kNC; };
+  auto lane_chunk = [&](auto geo, int i, int ln) -> uint32_t {
     using G = decltype(geo);
-    return static_cast<uint32_t>((i * 64 + lane) % G::kNC) ^
-           G::swz(8 * (wave & 1) + (i * 64 + lane) / G::kNC);
+    return static_cast<uint32_t>((i * 64 + ln) % G::kNC) ^
+           G::swz(8 * (wave & 1) + (i * 64 + ln) / G::kNC);
   };
   uint32_t kl[GK::kGI], vl[LAT ? 1 : GV::kGI];
 #pragma unroll
-  for (int i = 0; i < GK::kGI; ++i) kl[i] = lane_row(GK{}, i) * ksb + lane_chunk(GK{}, i) * 16;
+  for (int i = 0; i < GK::kGI; ++i) kl[i] = lane_row(GK{}, i, lane) * ksb + lane_chunk(GK{}, i, lane) * 16;
   if constexpr (!LAT) {
 #pragma unroll
-    for (int i = 0; i < GV::kGI; ++i) vl[i] = lane_row(GV{}, i) * vsb + lane_chunk(GV{}, i) * 16;
+    for (int i = 0; i < GV::kGI; ++i) vl[i] = lane_row(GV{}, i, lane) * vsb + lane_chunk(GV{}, i, lane) * 16;
   }
   const bool even_pages = !kPaged || a.page_size % 8 == 0;
 
@@ -426,7 +458,10 @@ fa2_decode_rows_kernel(RowsArgs ra) {
 
     f32x16 o[DBW];
 #pragma unroll
-    for (int d = 0; d < DBW; ++d) o[d] = (f32x16){};
+    for (int d = 0; d < DBW; ++d) {
+      o[d] = (f32x16){};
+      if constexpr (kAcc) in_acc(o[d]);
+    }
     float m_run = -INFINITY, l_run = 0.f;
     const int off = p.Lk - a.pack_m;  // keys that every row sees
     const int full = a.mask == FA2_MASK_NONE ? p.Lk : min(off + (a.mask == kMaskTree ? 0 : 1), p.Lk);
@@ -489,15 +524,16 @@ fa2_decode_rows_kernel(RowsArgs ra) {
         }
         // a row per lane; rows past the window are its last one (finite data under a
         // zero weight)
+        const int ln = here(lane);
 #pragma unroll
         for (int i = 0; i < G::kGI; ++i) {
-          const int nr = min(n + lane_row(G{}, i), kb - 1);
+          const int nr = min(n + lane_row(G{}, i, ln), kb - 1);
           int64_t r = nr;
           if constexpr (kPaged) {
             const int pg = page_of(nr);
             r = static_cast<int64_t>(tb[pg - page0]) * a.page_size + (nr - pg * a.page_size);
           }
-          dma_global_x4(base + r * ss * 2 + lane_chunk(G{}, i) * 16, dst + i * 1024);
+          dma_global_x4(base + r * ss * 2 + lane_chunk(G{}, i, ln) * 16, dst + i * 1024);
         }
       };
       auto issue = [&](int t) {
@@ -542,13 +578,17 @@ fa2_decode_rows_kernel(RowsArgs ra) {
           static_for<kAhead>([&](auto kc) { fr[decltype(kc)::value] = frag(kc); });
           static_for<kN>([&](auto kc) {
             constexpr int k = decltype(kc)::value, cc = k / SB, sb = k % SB;
-            if constexpr (SB == 1 && (cc & 1))
+            if constexpr (kAcc)
+              mma32_vgpr<BF>(s[sb], fr[k], qf[cc]);
+            else if constexpr (SB == 1 && (cc & 1))
               s2[sb] = mma32<BF>(fr[k], qf[cc], s2[sb]);
             else
               s[sb] = mma32<BF>(fr[k], qf[cc], s[sb]);
             if constexpr (k + kAhead < kN)
               fr[k + kAhead] = frag(std::integral_constant<int, k + kAhead>{});
+            if constexpr (kAcc) __builtin_amdgcn_sched_barrier(0);
           });
+          if constexpr (!kAcc) {
           __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
           for (int k = 0; k < kN - kAhead; ++k) {
@@ -556,8 +596,10 @@ fa2_decode_rows_kernel(RowsArgs ra) {
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
           }
           __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+          }
           __builtin_amdgcn_sched_barrier(0);
-          if constexpr (SB == 1) s[0] += s2[0];
+          if constexpr (kAcc) mma32_wait(s[0]);
+          else if constexpr (SB == 1) s[0] += s2[0];
         }
 
         // ---- mask: key n0 + 32 sb + 8 (i / 4) + 4 hi + i % 4 of element i --------
@@ -587,7 +629,14 @@ fa2_decode_rows_kernel(RowsArgs ra) {
           l_run *= alpha;
           if (n0 > p.t0 * kBN) {  // (nothing yet before the piece's first tile)
 #pragma unroll
-            for (int d = 0; d < DBW; ++d) o[d] *= alpha;
+            for (int d = 0; d < DBW; ++d) {
+              if constexpr (kAcc) in_acc(o[d]);
+              o[d] *= alpha;
+              if constexpr (kAcc) {
+                in_acc(o[d]);
+                __builtin_amdgcn_sched_barrier(0);
+              }
+            }
           }
         }
         const float m_use = (m_run == -INFINITY ? 0.f : m_run) - kLift;
@@ -631,10 +680,13 @@ fa2_decode_rows_kernel(RowsArgs ra) {
           static_for<kAhead>([&](auto kc) { fr[decltype(kc)::value] = frag(kc); });
           static_for<kN>([&](auto kc) {
             constexpr int k = decltype(kc)::value, c = k / DBW, d = k % DBW;
-            o[d] = mma32<BF>(fr[k], pf[c], o[d]);
+            if constexpr (kAcc) mma32_acc<BF>(o[d], fr[k], pf[c]);
+            else o[d] = mma32<BF>(fr[k], pf[c], o[d]);
             if constexpr (k + kAhead < kN)
               fr[k + kAhead] = frag(std::integral_constant<int, k + kAhead>{});
+            if constexpr (kAcc) __builtin_amdgcn_sched_barrier(0);
           });
+          if constexpr (!kAcc) {
           __builtin_amdgcn_sched_group_barrier(0x100, 2 * kAhead, 0);
 #pragma unroll
           for (int k = 0; k < kN - kAhead; ++k) {
@@ -642,15 +694,18 @@ fa2_decode_rows_kernel(RowsArgs ra) {
             __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
           }
           __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+          }
           __builtin_amdgcn_sched_barrier(0);
         }
       }
+      if constexpr (kAcc) asm volatile("s_nop 15\n\ts_nop 7" ::: "memory");  // the last MFMAs
       __syncthreads();  // the window's table and slots have been read
     }
 
     // ---- the piece's end ---------------------------------------------------------
     const float l_tot = sum_xor32(l_run);
-    const int r = rg * 32 + l32;
+    const int le = here(lane), hi = le >> 5;
+    const int r = rg * 32 + (le & 31);
     const int64_t obase = p.b * a.o_sb + p.kvh * (a.hq / a.hkv) * a.o_sh;
     if (p.np == 1) {
       if (r < nrows) {
@@ -658,12 +713,15 @@ fa2_decode_rows_kernel(RowsArgs ra) {
         uint16_t* dst = static_cast<uint16_t*>(a.o) + obase +
                         static_cast<int64_t>(q0 + r) * a.o_ss + d0 * 32 + hi * 4;
 #pragma unroll
-        for (int d = 0; d < DBW; ++d)
+        for (int d = 0; d < DBW; ++d) {
+          if constexpr (kAcc) in_acc(o[d]);
 #pragma unroll
           for (int g = 0; g < 4; ++g)
             *reinterpret_cast<u32x2*>(dst + d * 32 + g * 8) =
                 (u32x2){pack2<BF>(o[d][g * 4 + 0] * inv, o[d][g * 4 + 1] * inv),
                         pack2<BF>(o[d][g * 4 + 2] * inv, o[d][g * 4 + 3] * inv)};
+          if constexpr (kAcc) __builtin_amdgcn_sched_barrier(0);
+        }
       }
     } else {
       const int64_t slot = walk_slot(a, sg.C, p.us, stream, p.mine);
@@ -672,11 +730,14 @@ fa2_decode_rows_kernel(RowsArgs ra) {
         float* po = a.part_o + (slot * a.part_rows + r) * DV + d0 * 32 + hi * 4;
         if (dg == 0 && hi == 0) *reinterpret_cast<f32x2*>(ml) = (f32x2){m_run, l_tot};
 #pragma unroll
-        for (int d = 0; d < DBW; ++d)
+        for (int d = 0; d < DBW; ++d) {
+          if constexpr (kAcc) in_acc(o[d]);
 #pragma unroll
           for (int g = 0; g < 4; ++g)
             *reinterpret_cast<f32x4*>(po + d * 32 + g * 8) =
                 (f32x4){o[d][g * 4 + 0], o[d][g * 4 + 1], o[d][g * 4 + 2], o[d][g * 4 + 3]};
+          if constexpr (kAcc) __builtin_amdgcn_sched_barrier(0);
+        }
       }
     }
     if (tid == 0) rows_info(ra, sg, stream, p);
