@@ -8,6 +8,12 @@
 
 namespace fa2 {
 
+#ifndef FA2_RB_AHEAD_S
+#define FA2_RB_AHEAD_S 6
+#endif
+#ifndef FA2_RB_AHEAD_PV
+#define FA2_RB_AHEAD_PV 4
+#endif
 constexpr int kRbWaves = 4;
 constexpr int kRbThreads = 64 * kRbWaves;
 constexpr int kRbTable = 2048;  // block-table entries in LDS (K and V share them)
@@ -307,6 +313,14 @@ __device__ __forceinline__ void rows_wait(int n) {
   else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
+// A wave-uniform address in scalar registers.
+__device__ __forceinline__ uint64_t scalar_addr(const char* p) {
+  const uint64_t at = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<int>(at));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<int>(at >> 32));
+  return (static_cast<uint64_t>(hi) << 32) | lo;
+}
+
 // 16 bytes per lane to LDS from a scalar base and a 32-bit offset per lane (wait states
 // as dma_buffer_x4).
 template <bool NT = false>
@@ -497,33 +511,56 @@ fa2_decode_rows_kernel(RowsArgs ra) {
       if (a.mask == kMaskTree) word = tree_sh[m];
 
       const int T = (kb - ka + TK - 1) / TK;
-      auto issue_rows = [&](auto is_v, int n, uint32_t dst) {
+      // A tile goes out 8 rows at a time, each group of one page: its block-table entries are
+      // read from LDS a tile ahead (fetch), its bases are scalars (aim), and its loads stand
+      // between the MFMAs of S (send).
+      auto whole = [&](int t) { return even_pages && ka + (t + 1) * TK <= kb; };
+      int ek[GPW] = {}, ev[GPW] = {};
+      auto fetch = [&](int t) {
+        if constexpr (kPaged) {
+#pragma unroll
+          for (int g = 0; g < GPW; ++g) {
+            const int at = page_of(min(ka + t * TK + 8 * (wave + 4 * g), kb - 1)) - page0;
+            ek[g] = tab[at];
+            if constexpr (!LAT) ev[g] = tab[kTab + at];
+          }
+        }
+      };
+      uint64_t sk[GPW], sv[GPW];
+      auto aim = [&](int t) {
+#pragma unroll
+        for (int g = 0; g < GPW; ++g) {
+          const int n = ka + t * TK + 8 * (wave + 4 * g);
+          int64_t rk = n, rv = n;
+          if constexpr (kPaged) {
+            const int in = n - page_of(n) * a.page_size;
+            rk = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(ek[g])) * a.page_size + in;
+            if constexpr (!LAT)
+              rv = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(ev[g])) * a.page_size + in;
+          }
+          sk[g] = scalar_addr(kptr + rk * (a.k_ss * 2));
+          if constexpr (!LAT) sv[g] = scalar_addr(vptr + rv * (a.v_ss * 2));
+        }
+      };
+      auto send = [&](auto jc, uint32_t slot) {
+        constexpr int j = decltype(jc)::value, kPer = IPT / GPW;
+        constexpr int g = j / kPer, r = j % kPer;
+        constexpr bool V = r >= GK::kGI;
+        constexpr int i = V ? r - GK::kGI : r;
+        const uint32_t grp = wave + 4 * g;
+        if constexpr (V)
+          rows_dma(sv[g], vl[LAT ? 0 : i], slot + kVOff + grp * 8 * GV::kRowBytes + i * 1024);
+        else
+          rows_dma(sk[g], kl[i], slot + grp * 8 * GK::kRowBytes + i * 1024);
+      };
+      // The rest: a row per lane; rows past the window are its last one (finite data under a
+      // zero weight).
+      auto send_rows = [&](auto is_v, int n, uint32_t dst) {
         constexpr bool V = decltype(is_v)::value;
         using G = std::conditional_t<V, GV, GK>;
         const char* base = V ? vptr : kptr;
         const int64_t ss = V ? a.v_ss : a.k_ss;
         const int* tb = tab + (V ? kTab : 0);
-        if (even_pages && n + 8 <= kb) {  // 8 rows of one page
-          int64_t r = n;
-          if constexpr (kPaged) {
-            const int pg = page_of(n);
-            r = static_cast<int64_t>(tb[pg - page0]) * a.page_size + (n - pg * a.page_size);
-          }
-          const uint64_t at = reinterpret_cast<uint64_t>(base + r * ss * 2);
-          const uint64_t sbase =
-              (static_cast<uint64_t>(static_cast<uint32_t>(
-                   __builtin_amdgcn_readfirstlane(static_cast<int>(at >> 32))))
-               << 32) |
-              static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(at)));
-#pragma unroll
-          for (int i = 0; i < G::kGI; ++i) {
-            if constexpr (V) rows_dma(sbase, vl[LAT ? 0 : i], dst + i * 1024);
-            else rows_dma(sbase, kl[i], dst + i * 1024);
-          }
-          return;
-        }
-        // a row per lane; rows past the window are its last one (finite data under a
-        // zero weight)
         const int ln = here(lane);
 #pragma unroll
         for (int i = 0; i < G::kGI; ++i) {
@@ -536,26 +573,42 @@ fa2_decode_rows_kernel(RowsArgs ra) {
           dma_global_x4(base + r * ss * 2 + lane_chunk(G{}, i, ln) * 16, dst + i * 1024);
         }
       };
-      auto issue = [&](int t) {
+      auto send_part = [&](int t) {
         const uint32_t slot = tiles0 + (t % NS) * TL::kSlot;
 #pragma unroll
         for (int g = 0; g < GPW; ++g) {
-          const int grp = wave + 4 * g;
-          const int n = ka + t * TK + 8 * grp;
-          issue_rows(std::integral_constant<bool, false>{}, n, slot + grp * 8 * GK::kRowBytes);
+          const int grp = wave + 4 * g, n = ka + t * TK + 8 * grp;
+          send_rows(std::integral_constant<bool, false>{}, n, slot + grp * 8 * GK::kRowBytes);
           if constexpr (!LAT)
-            issue_rows(std::integral_constant<bool, true>{}, n,
-                       slot + kVOff + grp * 8 * GV::kRowBytes);
+            send_rows(std::integral_constant<bool, true>{}, n,
+                      slot + kVOff + grp * 8 * GV::kRowBytes);
         }
       };
-      for (int t = 0; t < NS - 1 && t < T; ++t) issue(t);
+      for (int t = 0; t < NS - 1 && t < T; ++t) {
+        if (whole(t)) {
+          fetch(t);
+          aim(t);
+          static_for<IPT>([&](auto jc) { send(jc, tiles0 + t * TL::kSlot); });
+        } else {
+          send_part(t);
+        }
+      }
+      if (NS - 1 < T) fetch(NS - 1);
       // Q and the first tiles: later waits of the compiler's would drain the tiles
       __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
 
       for (int t = 0; t < T; ++t) {
         rows_wait<IPT, NS - 2>(T - 1 - t);
         pp_barrier();  // tile t is there, and slot t - 1 has been read
-        if (t + NS - 1 < T) issue(t + NS - 1);
+        const int tn = t + NS - 1;
+        const bool ahead = tn < T && whole(tn);
+        if (ahead) {
+          aim(tn);
+          fetch(tn + 1);
+        } else if (tn < T) {
+          send_part(tn);
+        }
+        const uint32_t next = tiles0 + (tn % NS) * TL::kSlot;
         const uint32_t slot = tiles0 + (t % NS) * TL::kSlot;
         const int n0 = ka + t * TK;
 
@@ -563,16 +616,15 @@ fa2_decode_rows_kernel(RowsArgs ra) {
         f32x16 s[SB];
 #pragma unroll
         for (int sb = 0; sb < SB; ++sb) s[sb] = (f32x16){};
-        {
-          constexpr int kN = DC * SB, kAhead = 6 < kN ? 6 : kN;
+        auto scores = [&](auto dma) {
+          constexpr bool kDma = decltype(dma)::value;
+          constexpr int kN = DC * SB, kAhead = FA2_RB_AHEAD_S < kN ? FA2_RB_AHEAD_S : kN;
           auto frag = [&](auto kc) -> u32x4 {
             constexpr int cc = decltype(kc)::value / SB, sb = decltype(kc)::value % SB;
             return *(const lds_u32x4_t*)(lds_ptr(slot + (koff ^ (32u * (cc % GK::kG)))) +
                                          sb * 32 * GK::kRowBytes + (cc / GK::kG) * GK::kG * 32);
           };
-          f32x16 s2[SB];  // odd k-steps: two chains of MFMAs
-#pragma unroll
-          for (int sb = 0; sb < SB; ++sb) s2[sb] = (f32x16){};
+          f32x16 s2 = (f32x16){};  // odd k-steps of a single block: two chains of MFMAs
           __builtin_amdgcn_sched_barrier(0);
           u32x4 fr[kN];
           static_for<kAhead>([&](auto kc) { fr[decltype(kc)::value] = frag(kc); });
@@ -581,26 +633,34 @@ fa2_decode_rows_kernel(RowsArgs ra) {
             if constexpr (kAcc)
               mma32_vgpr<BF>(s[sb], fr[k], qf[cc]);
             else if constexpr (SB == 1 && (cc & 1))
-              s2[sb] = mma32<BF>(fr[k], qf[cc], s2[sb]);
+              s2 = mma32<BF>(fr[k], qf[cc], s2);
             else
               s[sb] = mma32<BF>(fr[k], qf[cc], s[sb]);
             if constexpr (k + kAhead < kN)
               fr[k + kAhead] = frag(std::integral_constant<int, k + kAhead>{});
+            if constexpr (kDma) {  // loads [k IPT / kN, (k + 1) IPT / kN)
+              constexpr int j0 = k * IPT / kN, j1 = (k + 1) * IPT / kN;
+              static_for<j1 - j0>([&](auto x) {
+                send(std::integral_constant<int, j0 + decltype(x)::value>{}, next);
+              });
+            }
             if constexpr (kAcc) __builtin_amdgcn_sched_barrier(0);
           });
           if constexpr (!kAcc) {
-          __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
-          for (int k = 0; k < kN - kAhead; ++k) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-          }
-          __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+            for (int k = 0; k < kN - kAhead; ++k) {
+              __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+              __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
           }
           __builtin_amdgcn_sched_barrier(0);
           if constexpr (kAcc) mma32_wait(s[0]);
-          else if constexpr (SB == 1) s[0] += s2[0];
-        }
+          else if constexpr (SB == 1) s[0] += s2;
+        };
+        if (ahead) scores(std::integral_constant<bool, true>{});
+        else scores(std::integral_constant<bool, false>{});
 
         // ---- mask: key n0 + 32 sb + 8 (i / 4) + 4 hi + i % 4 of element i --------
         if (n0 + TK > full) {
@@ -662,7 +722,7 @@ fa2_decode_rows_kernel(RowsArgs ra) {
 
         // ---- O^T += V^T P^T --------------------------------------------------------
         {
-          constexpr int kN = 2 * SB * DBW, kAhead = 4 < kN ? 4 : kN;
+          constexpr int kN = 2 * SB * DBW, kAhead = FA2_RB_AHEAD_PV < kN ? FA2_RB_AHEAD_PV : kN;
           auto frag = [&](auto kc) -> u32x4 {
             constexpr int c = decltype(kc)::value / DBW, d = decltype(kc)::value % DBW;
             constexpr int kImm = 16 * c * GV::kRowBytes + (d / KM) * KM * 64;

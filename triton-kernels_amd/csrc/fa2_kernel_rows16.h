@@ -162,14 +162,10 @@ fa2_decode_rows16_kernel(RowsArgs ra) {
             int64_t r = n;
             if constexpr (kPaged) {
               const int pg = page_of(n);
-              r = static_cast<int64_t>(tb[pg - page0]) * a.page_size + (n - pg * a.page_size);
+              r = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(tb[pg - page0])) * a.page_size +
+                  (n - pg * a.page_size);
             }
-            const uint64_t at = reinterpret_cast<uint64_t>(base + r * ss * 2);
-            const uint64_t sbase =
-                (static_cast<uint64_t>(static_cast<uint32_t>(
-                     __builtin_amdgcn_readfirstlane(static_cast<int>(at >> 32))))
-                 << 32) |
-                static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(at)));
+            const uint64_t sbase = scalar_addr(base + r * (ss * 2));
 #pragma unroll
             for (int i = 0; i < G::kGI; ++i)
               rows_dma<true>(sbase, (V ? vl[LAT ? 0 : i] : kl[V ? 0 : i]) ^ (16u * (grp & 1)),
