@@ -545,20 +545,28 @@ __device__ __forceinline__ void lds_fill_barrier() {
 #endif
 // F32: fp32 tensors (Plan::conv): K and V are fp16 copies, Q is fp32 and rounded
 // to fp16 here, an unsplit unit writes the fp32 output.
-template <int DT, int D, int MODE, bool BUF, bool F32 = false, bool PIPE = FA2_LDS_PIPE_DEFAULT(D)>
+// DR: the expanded form of latent attention (Hq == Hkv): rows of q have DR more values, the
+// keys' DR more are those of the sequence's rows kr, which all heads share.
+template <int DT, int D, int MODE, bool BUF, bool F32 = false, bool PIPE = FA2_LDS_PIPE_DEFAULT(D),
+          int DR = 0>
 __global__ __launch_bounds__(kThreads, D > 128 ? 1 : FA2_LDS_OCCUPANCY) void fa2_fwd_lds_kernel(KArgs a) {
   static_assert(DT != FA2_DTYPE_F32, "fp32 uses the register-staged kernel");
   constexpr bool BF = Elt<DT>::kBF;
-  constexpr int DC = D / 16;  // MFMA k-steps of S (16 head dims each)
+  static_assert(DR == 0 || (DR == 64 && MODE != FA2_LAYOUT_PAGED && !F32), "latent attention");
+  constexpr int DK = D / 16;        // MFMA k-steps of S (16 head dims each)
+  constexpr int DC = DK + DR / 16;  // ... and of a row's shared part
   constexpr int DB = D / 32;  // 32-dim blocks of O^T
   constexpr int SB = kBN / 32;
   using G = SwzGeo<D>;
 
-  __shared__ __attribute__((aligned(1024))) char lds[4 * G::kTileBytes];
+  using GR = SwzGeo<64>;
+  constexpr int kRTile = DR ? GR::kTileBytes : 0;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * G::kTileBytes + 2 * kRTile];
   // K buffers 0, 1 then V buffers 0, 1 (addresses computed, not read from an
   // array of LDS pointers, which a loop-carried index cannot select)
   auto kbuf = [&](int j) { return lds + (j & 1) * G::kTileBytes; };
   auto vbuf = [&](int j) { return lds + (2 + (j & 1)) * G::kTileBytes; };
+  auto rbuf = [&](int j) { return lds + 4 * G::kTileBytes + (j & 1) * kRTile; };
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -569,10 +577,18 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : FA2_LDS_OCCUPANCY) void fa2
   // a ragged launch without a plan kernel: the item list in LDS
   const InlinePlan* ip = nullptr;
   if constexpr (MODE == FA2_LAYOUT_RAGGED) {
-    __shared__ InlinePlan iplan;
-    if (a.inline_plan) {
-      build_inline_plan<MODE>(a, &iplan);
-      ip = &iplan;
+    if constexpr (DR > 0) {  // where the tiles will be: two workgroups fill a CU's LDS
+      static_assert(sizeof(InlinePlan) <= sizeof(lds), "plan");
+      if (a.inline_plan) {
+        ip = reinterpret_cast<InlinePlan*>(lds);
+        build_inline_plan<MODE>(a, reinterpret_cast<InlinePlan*>(lds));
+      }
+    } else {
+      __shared__ InlinePlan iplan;
+      if (a.inline_plan) {
+        build_inline_plan<MODE>(a, &iplan);
+        ip = &iplan;
+      }
     }
   }
   const Work w = decode_work<MODE>(a, blockIdx.x, 1, ip);
@@ -581,6 +597,18 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : FA2_LDS_OCCUPANCY) void fa2
   const int split = blockIdx.y;
   const int S = ip ? ip->splits : launch_splits(a);
   if (split >= S) return;
+  // the shared part of the keys: a K of its own
+  KArgs ar = a;
+  Work wr = w;
+  if constexpr (DR > 0) {
+    ar.k = a.kr;
+    ar.k_ss = ar.v_ss = a.kr_ss;
+    if constexpr (MODE == FA2_LAYOUT_DENSE)
+      wr.k_base = w.b * a.kr_sb;
+    else
+      wr.k_base = static_cast<int64_t>(ip ? ip->ki[w.b] : a.kv_indptr[w.b]) * a.kr_ss;
+    __syncthreads();  // the plan has been read
+  }
 
   const int kv_end = kv_end_for_unit(a, q0, w.Lq, w.Lk, w.off);
   const int ntiles = (kv_end + kBN - 1) / kBN;
@@ -638,11 +666,18 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : FA2_LDS_OCCUPANCY) void fa2
   const bool active = q0 + wave * kWaveRows < w.Lq;
 
   const DirectLoader<D, MODE, BUF, DT> ld(a, tid);
+  const DirectLoader<64, MODE, BUF, DT> ldr(ar, tid);
+  const uint32_t roff0 = l32 * GR::kRowBytes + ((hi ^ GR::k(l32)) * 16);
+  auto issue_k = [&](int k0, int j) {
+    ld.template issue<false>(a, w, k0, kbuf(j));
+    if constexpr (DR > 0) ldr.template issue<false>(ar, wr, k0, rbuf(j));
+  };
 
   // (no s_setprio here: it would end the scheduling region and undo the
   // interleaving of these MFMAs with the softmax)
-  auto compute_s = [&](f32x16 (&s)[SB], const char* kb) {
-    const lds_char_t* kl = to_lds(const_cast<char*>(kb));
+  auto compute_s = [&](f32x16 (&s)[SB], int j) {
+    const lds_char_t* kl = to_lds(kbuf(j));
+    const lds_char_t* rl = to_lds(rbuf(j));
     // accumulators interleaved (cc-major): back-to-back dependent MFMAs stall
 #pragma unroll
     for (int sb = 0; sb < SB; ++sb) s[sb] = (f32x16){};
@@ -651,7 +686,9 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : FA2_LDS_OCCUPANCY) void fa2
 #pragma unroll
       for (int sb = 0; sb < SB; ++sb) {
         const u32x4 kf =
-            *(const lds_u32x4_t*)(kl + sb * 32 * G::kRowBytes + (koff0 ^ (32u * cc)));
+            cc < DK ? *(const lds_u32x4_t*)(kl + sb * 32 * G::kRowBytes + (koff0 ^ (32u * cc)))
+                    : *(const lds_u32x4_t*)(rl + sb * 32 * GR::kRowBytes +
+                                            (roff0 ^ (32u * (cc - DK))));
         s[sb] = mma32<BF>(kf, qf[cc], s[sb]);
       }
     }
@@ -663,12 +700,12 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : FA2_LDS_OCCUPANCY) void fa2
     const int k0 = t * kBN;
     if constexpr (!kLast) {
       if (PIPE ? (i + 2 < T) : true)
-        ld.template issue<false>(a, w, k0 + (PIPE ? 2 : 1) * kBN, kbuf((PIPE ? i : i + 1) & 1));
+        issue_k(k0 + (PIPE ? 2 : 1) * kBN, PIPE ? i : i + 1);
       ld.template issue<true>(a, w, k0 + kBN, vbuf((i + 1) & 1));
     }
     if (active) {
     // scores of tile i must exist before they are masked
-    if constexpr (!PIPE) compute_s(s_cur, kbuf(i & 1));
+    if constexpr (!PIPE) compute_s(s_cur, i);
     if ((k0 + kBN > w.Lk) || (causal && (k0 + kBN - 1 > wq_diag + w.off))) {
       // key = k0 + 4*hi + c with c a compile-time offset per accumulator:
       // visible iff c <= lim (sequence end and, if causal, the diagonal)
@@ -683,7 +720,7 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : FA2_LDS_OCCUPANCY) void fa2
         }
       }
     }
-    if constexpr (!kLast && PIPE) compute_s(s_nxt, kbuf((i + 1) & 1));
+    if constexpr (!kLast && PIPE) compute_s(s_nxt, i + 1);
 
     float mx = -INFINITY;
 #pragma unroll
@@ -781,12 +818,12 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : FA2_LDS_OCCUPANCY) void fa2
 
   f32x16 sA[SB], sB[SB];
   if (T > 0) {
-    ld.template issue<false>(a, w, t_begin * kBN, kbuf(0));
+    issue_k(t_begin * kBN, 0);
     ld.template issue<true>(a, w, t_begin * kBN, vbuf(0));
-    if (PIPE && T > 1) ld.template issue<false>(a, w, (t_begin + 1) * kBN, kbuf(1));
+    if (PIPE && T > 1) issue_k((t_begin + 1) * kBN, 1);
     lds_fill_barrier();
     if constexpr (PIPE) {
-      if (active) compute_s(sA, kbuf(0));
+      if (active) compute_s(sA, 0);
       // step 0 refills kbuf(0) with K(t0+2): every wave must have finished
       // reading K(t0) first (the barrier also waits for the LDS reads)
       __syncthreads();
@@ -831,12 +868,13 @@ __global__ __launch_bounds__(kThreads, D > 128 ? 1 : FA2_LDS_OCCUPANCY) void fa2
     const int64_t slot = static_cast<int64_t>(split) * a.part_slots + blockIdx.x;
     const int r = wave * kWaveRows + l32;
     if (qrow < w.Lq && r < a.part_rows) {
-      if (MODE == FA2_LAYOUT_RAGGED && a.merge_ctr)
+      if (DR == 0 && MODE == FA2_LAYOUT_RAGGED && a.merge_ctr)
         store_partial_rows<true, D>(a, slot, r, hi, m_run, l_tot, o);
       else
         store_partial_rows<false, D>(a, slot, r, hi, m_run, l_tot, o);
     }
     // (only ragged launches merge here: KArgs::inline_plan)
+    if constexpr (DR > 0) return;
     if (MODE == FA2_LAYOUT_RAGGED && a.merge_ctr) {  // the split that completes the count merges
       __shared__ int merge_flag;
       merge_publish();

@@ -190,8 +190,7 @@ __device__ void pp_bal_locate(const KArgs& a, int x, int upp, int ns, int k, int
 // unit writes the fp32 output.
 // DR: the expanded form of latent attention (Hq == Hkv, KArgs::qpair): rows of q
 // have DR more values, the keys' DR more are those of the sequence's rows kr, which
-// all heads share; their tiles have LDS slots of their own, and partials go to slot
-// 2 * pair + group.
+// all heads share; their tiles have LDS slots of their own.  One split.
 template <int DT, int D, int MODE, bool BUF, bool CLAIM = false, bool INLINE = false,
           bool BAL = false, bool F32 = false, int DR = 0>
 __global__ __launch_bounds__(kPPThreads, 1) void fa2_fwd_pp_kernel(KArgs a) {
@@ -841,8 +840,8 @@ __global__ __launch_bounds__(kPPThreads, 1) void fa2_fwd_pp_kernel(KArgs a) {
       } else {
         // partials go to the slot the one-head-per-unit layout gives this
         // head (decode_work with heads = 1), which the combine kernel reads
-        const int unit = DR ? 2 * w.pair + grp
-                            : ((w.pair / kXcds) * group + w.hg + grp) * kXcds + w.pair % kXcds;
+        const int unit =
+            ((w.pair / kXcds) * group + w.hg + grp) * kXcds + w.pair % kXcds;
         const int64_t slot = static_cast<int64_t>(split) * a.part_slots + unit;
         const int rr = wq * kWaveRows + l32;
         if (INLINE && a.merge_ctr)

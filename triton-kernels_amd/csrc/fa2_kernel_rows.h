@@ -8,12 +8,6 @@
 
 namespace fa2 {
 
-#ifndef FA2_RB_AHEAD_S
-#define FA2_RB_AHEAD_S 6
-#endif
-#ifndef FA2_RB_AHEAD_PV
-#define FA2_RB_AHEAD_PV 4
-#endif
 constexpr int kRbWaves = 4;
 constexpr int kRbThreads = 64 * kRbWaves;
 constexpr int kRbTable = 2048;  // block-table entries in LDS (K and V share them)
@@ -23,7 +17,7 @@ constexpr int kRbMaxTree = 64;  // drafts of a tree: bits of a mask word
 constexpr int kMaskTree = 3;
 
 // A second piece of a workgroup costs about as much as this many tiles of kBN keys.
-constexpr int kRbSwitch = 6;
+constexpr int kRbSwitch = 2;
 
 struct RowsArgs {
   KArgs a;  // q rows: token m of head h at h * q_sh + m * q_ss; o rows: o_ss apart
@@ -368,7 +362,7 @@ __device__ __forceinline__ void mma32_wait(f32x16& c) {
 // the loops carry it whole.
 __device__ __forceinline__ void in_acc(f32x16& c) { asm volatile("" : "+a"(c)); }
 
-template <int DT, int DK, int DV, bool LAT, int RG, int MODE>
+template <int DT, int DK, int DV, bool LAT, int RG, int MODE, bool NT>
 __global__ __launch_bounds__(kRbThreads, (RowsTile<DK, DV, LAT, RG>::kOcc)) void
 fa2_decode_rows_kernel(RowsArgs ra) {
   static_assert(DT != FA2_DTYPE_F32, "16-bit rows");
@@ -549,9 +543,9 @@ fa2_decode_rows_kernel(RowsArgs ra) {
         constexpr int i = V ? r - GK::kGI : r;
         const uint32_t grp = wave + 4 * g;
         if constexpr (V)
-          rows_dma(sv[g], vl[LAT ? 0 : i], slot + kVOff + grp * 8 * GV::kRowBytes + i * 1024);
+          rows_dma<NT>(sv[g], vl[LAT ? 0 : i], slot + kVOff + grp * 8 * GV::kRowBytes + i * 1024);
         else
-          rows_dma(sk[g], kl[i], slot + grp * 8 * GK::kRowBytes + i * 1024);
+          rows_dma<NT>(sk[g], kl[i], slot + grp * 8 * GK::kRowBytes + i * 1024);
       };
       // The rest: a row per lane; rows past the window are its last one (finite data under a
       // zero weight).
@@ -570,7 +564,7 @@ fa2_decode_rows_kernel(RowsArgs ra) {
             const int pg = page_of(nr);
             r = static_cast<int64_t>(tb[pg - page0]) * a.page_size + (nr - pg * a.page_size);
           }
-          dma_global_x4(base + r * ss * 2 + lane_chunk(G{}, i, ln) * 16, dst + i * 1024);
+          dma_global_x4<NT>(base + r * ss * 2 + lane_chunk(G{}, i, ln) * 16, dst + i * 1024);
         }
       };
       auto send_part = [&](int t) {
@@ -618,7 +612,7 @@ fa2_decode_rows_kernel(RowsArgs ra) {
         for (int sb = 0; sb < SB; ++sb) s[sb] = (f32x16){};
         auto scores = [&](auto dma) {
           constexpr bool kDma = decltype(dma)::value;
-          constexpr int kN = DC * SB, kAhead = FA2_RB_AHEAD_S < kN ? FA2_RB_AHEAD_S : kN;
+          constexpr int kN = DC * SB, kAhead = 6 < kN ? 6 : kN;
           auto frag = [&](auto kc) -> u32x4 {
             constexpr int cc = decltype(kc)::value / SB, sb = decltype(kc)::value % SB;
             return *(const lds_u32x4_t*)(lds_ptr(slot + (koff ^ (32u * (cc % GK::kG)))) +
@@ -722,7 +716,7 @@ fa2_decode_rows_kernel(RowsArgs ra) {
 
         // ---- O^T += V^T P^T --------------------------------------------------------
         {
-          constexpr int kN = 2 * SB * DBW, kAhead = FA2_RB_AHEAD_PV < kN ? FA2_RB_AHEAD_PV : kN;
+          constexpr int kN = 2 * SB * DBW, kAhead = 4 < kN ? 4 : kN;
           auto frag = [&](auto kc) -> u32x4 {
             constexpr int c = decltype(kc)::value / DBW, d = decltype(kc)::value % DBW;
             constexpr int kImm = 16 * c * GV::kRowBytes + (d / KM) * KM * 64;

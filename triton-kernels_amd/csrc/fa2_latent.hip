@@ -11,7 +11,6 @@
 #include "fa2_kernel_rows.h"
 #include "fa2_kernel_rows16.h"
 #include "fa2_latent_append.h"
-#include "fa2_latent_prefill.h"
 
 namespace fa2 {
 namespace {
@@ -164,13 +163,18 @@ void launch_rows(const RowsArgs& ra, const RowsPlan& pl, hipStream_t st) {
   if (pl.rg == 0)
     hipLaunchKernelGGL((fa2_decode_rows16_kernel<DT, DK, DV, LAT, MODE>), grid,
                        dim3(Rows16Tile<DK, DV, LAT>::kThreads), 0, st, ra);
+  else if (pl.rg == 4 && pl.streams > ra.a.hkv)
+    hipLaunchKernelGGL((fa2_decode_rows_kernel<DT, DK, DV, LAT, 4, MODE, false>), grid, block, 0,
+                       st, ra);
   else if (pl.rg == 4)
-    hipLaunchKernelGGL((fa2_decode_rows_kernel<DT, DK, DV, LAT, 4, MODE>), grid, block, 0, st, ra);
-  else if (pl.rg > least)
-    hipLaunchKernelGGL((fa2_decode_rows_kernel<DT, DK, DV, LAT, 2, MODE>), grid, block, 0, st, ra);
-  else
-    hipLaunchKernelGGL((fa2_decode_rows_kernel<DT, DK, DV, LAT, least, MODE>), grid, block, 0, st,
+    hipLaunchKernelGGL((fa2_decode_rows_kernel<DT, DK, DV, LAT, 4, MODE, true>), grid, block, 0, st,
                        ra);
+  else if (pl.rg > least)
+    hipLaunchKernelGGL((fa2_decode_rows_kernel<DT, DK, DV, LAT, 2, MODE, true>), grid, block, 0, st,
+                       ra);
+  else
+    hipLaunchKernelGGL((fa2_decode_rows_kernel<DT, DK, DV, LAT, least, MODE, true>), grid, block, 0,
+                       st, ra);
   if (pl.cut)
     hipLaunchKernelGGL((fa2_rows_merge_kernel<DT, DV>),
                        dim3(static_cast<uint32_t>(pl.streams * ra.a.batch),
@@ -312,7 +316,8 @@ int rows_begin(const P* p, RowsPlan* pl, RowsArgs* ra) {
 constexpr size_t kClaimAt = 128;  // of the claim counters, in the 256 bytes of the counts
 
 struct PrefillPlan {
-  int64_t work_ub, npairs, grid, wgs;  // q-block pairs, times heads, unit slots, workgroups
+  bool pair;  // the two-head kernel over pairs of q-blocks; else the one-head kernel
+  int64_t work_ub, npairs, grid, wgs;  // items, times heads, unit slots, workgroups
   int splits;
   bool plan, inline_plan;  // ragged: the plan kernel's list, or each workgroup's own
   size_t off_work, off_count, off_ml, off_o, total;
@@ -343,20 +348,29 @@ int validate_prefill(const fa2_latent_prefill_params* p) {
 int prefill_plan(const fa2_latent_prefill_params* p, PrefillPlan* pl) {
   const bool ragged = p->layout == FA2_LAYOUT_RAGGED;
   const int64_t nqb = cdiv(p->q_len, kBM), cus = cu_count_current_device();
-  // (ragged: the sequences' pairs of q-blocks, at most one more each than all rows have)
-  pl->work_ub = ragged ? cdiv(p->q_len, 2 * kBM) + p->batch : cdiv(nqb, 2) * p->batch;
+  // items of `rows` rows (ragged: one more for each sequence at most)
+  auto items = [&](int64_t rows) {
+    return (ragged ? cdiv(p->q_len, rows) + p->batch : cdiv(p->q_len, rows) * p->batch);
+  };
+  if (items(kBM) * p->heads > kLim / 4) return FA2_ERR_TOO_LARGE;
+  // Pairs of q-blocks on one workgroup per CU where sequences have four q-blocks on average
+  // (a lone block leaves half of the workgroup without rows) and the pairs fill the CUs.
+  const bool many = ragged ? p->q_len >= 4 * kBM * p->batch : nqb >= 4;
+  pl->pair = many && items(2 * kBM) * p->heads >= cus;
+  pl->work_ub = items(pl->pair ? 2 * kBM : kBM);
   pl->npairs = pl->work_ub * p->heads;
-  if (pl->npairs > kLim / 4) return FA2_ERR_TOO_LARGE;
   pl->grid = cdiv(pl->npairs, kXcds) * kXcds;
   // Splits of the keys where the units leave CUs idle, kMinSplitTiles tiles each at least
   // (ragged: the plan kernel lowers the count to what the longest sequence takes).
   int64_t keys = p->kv_len;
   if (p->mask == FA2_MASK_CAUSAL_TOP_LEFT) keys = std::min(keys, p->q_len);
-  int64_t s = std::min(cus / std::max<int64_t>(pl->npairs, 1), cdiv(keys, kBN) / kMinSplitTiles);
-  s = std::max<int64_t>(1, std::min<int64_t>(s, FA2_MAX_SPLITS));
+  const int64_t slots = cus * (pl->pair ? 1 : 2);
+  int64_t s = std::min(cdiv(slots, std::max<int64_t>(pl->npairs, 1)),
+                       cdiv(keys, kBN) / kMinSplitTiles);
+  s = pl->pair ? 1 : std::max<int64_t>(1, std::min<int64_t>(s, FA2_MAX_SPLITS));
   pl->splits = static_cast<int>(s);
-  pl->wgs = s > 1 ? pl->grid : std::min(pl->grid, cus);
-  pl->inline_plan = ragged && s == 1 && p->batch <= kInlinePlanMaxBatch && pl->grid <= cus;
+  pl->wgs = pl->pair ? std::min(pl->grid, cus) : pl->grid;
+  pl->inline_plan = ragged && s == 1 && p->batch <= kInlinePlanMaxBatch && pl->grid <= slots;
   pl->plan = ragged && !pl->inline_plan;
   size_t off = 0;
   pl->off_work = off;
@@ -364,17 +378,15 @@ int prefill_plan(const fa2_latent_prefill_params* p, PrefillPlan* pl) {
   off = (off + 255) & ~size_t(255);
   pl->off_count = off;  // the item count, the split count, the claim counters at kClaimAt
   if (pl->plan) off += 256;
-  const size_t slots = s > 1 ? static_cast<size_t>(s) * 2 * pl->grid : 0;
+  const size_t parts = s > 1 ? static_cast<size_t>(s * pl->grid) : 0;
   pl->off_ml = off;
-  off += slots * kBM * 2 * sizeof(float);
+  off += parts * kBM * 2 * sizeof(float);
   off = (off + 255) & ~size_t(255);
   pl->off_o = off;
-  off += slots * kBM * p->head_dim * sizeof(float);
+  off += parts * kBM * p->head_dim * sizeof(float);
   pl->total = off;
   return FA2_OK;
 }
-
-
 
 template <int DT, int D, int MODE>
 void launch_prefill_typed(const KArgs& a, const PrefillPlan& pl, hipStream_t st) {
@@ -383,6 +395,18 @@ void launch_prefill_typed(const KArgs& a, const PrefillPlan& pl, hipStream_t st)
     if (pl.plan)
       hipLaunchKernelGGL((fa2_plan_kernel<MODE>), dim3(1), dim3(kPlanThreads), 0, st, a,
                          const_cast<int2*>(a.work), const_cast<int32_t*>(a.work_count));
+  }
+  if (!pl.pair) {
+    hipLaunchKernelGGL(
+        (fa2_fwd_lds_kernel<DT, D, MODE, true, false, false, kLaRope>), grid,
+        dim3(kThreads), 0, st, a);
+    if (pl.splits > 1)
+      hipLaunchKernelGGL((fa2_combine_kernel<DT, D, MODE>),
+                         dim3(static_cast<uint32_t>(pl.grid), kBM / kCombineRows<D>),
+                         dim3(kThreads), 0, st, a);
+    return;
+  }
+  if constexpr (MODE == FA2_LAYOUT_RAGGED) {
     if (a.claim) {
       hipLaunchKernelGGL((fa2_fwd_pp_kernel<DT, D, MODE, true, true, false, false, false, kLaRope>),
                          grid, block, 0, st, a);
@@ -396,10 +420,6 @@ void launch_prefill_typed(const KArgs& a, const PrefillPlan& pl, hipStream_t st)
   }
   hipLaunchKernelGGL((fa2_fwd_pp_kernel<DT, D, MODE, true, false, false, false, false, kLaRope>),
                      grid, block, 0, st, a);
-  if (pl.splits > 1)
-    hipLaunchKernelGGL((fa2_latent_combine_kernel<DT, D, MODE>),
-                       dim3(static_cast<uint32_t>(2 * pl.grid), kBM / kCombineRows<D>),
-                       dim3(kThreads), 0, st, a);
 }
 
 template <int DT>
@@ -577,14 +597,14 @@ extern "C" int fa2_latent_prefill(const fa2_latent_prefill_params* p, void* stre
   a.kv_len = static_cast<int32_t>(p->kv_len);
   a.page_size = 1;
   a.page_shift = 0;
-  a.nqb = static_cast<int32_t>(cdiv(cdiv(p->q_len, kBM), 2));  // q-block pairs
-  a.qpair = 1;
+  a.nqb = static_cast<int32_t>(cdiv(p->q_len, pl.pair ? 2 * kBM : kBM));
+  a.qpair = pl.pair ? 1 : 0;
   a.block_rows = kBM;
   a.work_ub = static_cast<int32_t>(pl.work_ub);
   a.npairs = static_cast<int32_t>(pl.npairs);
   a.mask = p->mask;
   a.num_splits = pl.splits;
-  a.part_slots = static_cast<int32_t>(2 * pl.grid);
+  a.part_slots = static_cast<int32_t>(pl.grid);
   a.part_rows = kBM;
   a.units = static_cast<int32_t>(pl.grid);
   a.scale_log2 = p->softmax_scale * 1.4426950408889634f;
@@ -598,7 +618,7 @@ extern "C" int fa2_latent_prefill(const fa2_latent_prefill_params* p, void* stre
     // Sequences of more than one q-block on average: units are claimed per XCD, so that its
     // workgroups run the q-blocks of one or two sequences at a time and share their K/V in
     // its L2, as in fa2_fwd.
-    if (pl.splits == 1 && pl.wgs >= kXcds && p->q_len > kBM * p->batch)
+    if (pl.pair && pl.wgs >= kXcds)
       a.claim = count + kClaimAt / sizeof(int32_t);
   }
   if (pl.splits > 1) {
