@@ -61,6 +61,7 @@ def append(**kw):
     (dict(rows_out=0x1008), ALIGN), (dict(weight=0x1004), ALIGN), (dict(rope=0x1008), ALIGN),
     (dict(x=None), NULL), (dict(cache=None), NULL), (dict(weight=None), NULL),
     (dict(indptr=None), NULL), (dict(rope=None), NULL), (dict(block_table=None), NULL),
+    (dict(num_rows=2 ** 26), LARGE), (dict(num_rows=2 ** 27, latent_dim=256), LARGE),  # the grid
 ])
 def test_append_refusals(kw, code):
     assert append(**kw) == code
@@ -180,7 +181,7 @@ def prefill(**kw):
     (dict(q_len=-1), SHAPE), (dict(kv_len=-1), SHAPE), (dict(layout=1, q_indptr=None), RAGGED),
     (dict(layout=1, kv_indptr=None), RAGGED), (dict(q_ss=194), ALIGN), (dict(kr_ss=2), ALIGN),
     (dict(heads=70000), LARGE), (dict(k_ss=2 ** 25), LARGE), (dict(kr_ss=-64), LARGE),
-    (dict(batch=2 ** 29), LARGE), (dict(q=None), NULL), (dict(kr=None), NULL), (dict(o=None), NULL),
+    (dict(batch=2 ** 29), LARGE), (dict(batch=2 ** 21), LARGE), (dict(q=None), NULL), (dict(kr=None), NULL), (dict(o=None), NULL),
     (dict(kr=0x1008), ALIGN), (dict(softmax_scale=0.0), SHAPE),
     (dict(kv_len=4096, batch=1), WORKSPACE),  # splits: partials
 ])

@@ -233,6 +233,8 @@ def test_decode(path, latent, dtype, lens, hq, m, page, causal, tree):
     ([3000, 100, 2500, 1], 16, 16),           # units cut by segments
     ([4097], 128, 16), ([20000], 16, 16), ([9000], 16, 3),  # windows of block-table entries
     ([600, 40, 1300, 90] * 70, 16, 16),       # more sequences than CUs
+    ([40] * 66 + [2600, 0, 1, 900], 48, 16),  # more than a wave's lanes, units cut
+    ([70] * 65 + [3000], 128, 16),
 ])
 def test_decode_shares(lens, hq, page):
     q, cache, table, _ = decode_case(256, BF, lens, hq, 0, page)
@@ -399,6 +401,7 @@ MASKS = [("none", {}), ("top_left", dict(is_causal=True)),
     (64, F16, [40], [2500], 2),                            # splits
     (128, BF, [500, 600, 300, 700, 40], [500, 700, 300, 900, 1100], 24),  # units claimed
     (128, F16, [2] * 40, [30] * 40, 16),                   # a plan, one q-block each
+    (64, BF, [1100, 30], [600, 90], 64),                   # pairs, some of one q-block
 ])
 def test_prefill_ragged(path, d, dtype, q_lens, kv_lens, h, mask, kw):
     q, k, kr, v = prefill_case(d, dtype, q_lens, kv_lens, h)
@@ -412,6 +415,7 @@ def test_prefill_ragged(path, d, dtype, q_lens, kv_lens, h, mask, kw):
 @pytest.mark.parametrize("b,h,m,n,d,dtype", [
     (1, 2, 1, 1, 128, BF), (2, 3, 100, 100, 64, F16), (3, 2, 65, 129, 128, BF),
     (1, 2, 40, 4500, 128, F16), (2, 4, 300, 260, 128, BF), (1, 1, 3, 0, 64, BF),
+    (2, 48, 520, 333, 64, BF), (1, 88, 513, 600, 128, F16),  # pairs of q-blocks
 ])
 def test_prefill_dense(path, b, h, m, n, d, dtype, mask, kw):
     q, k, kr, v = prefill_case(d, dtype, [m] * b, [n] * b, h)
@@ -450,6 +454,35 @@ def test_prefill_graph_streams_and_layouts():
     # rows behind the last sequence are left out
     more = torch.cat([q, q[:5]])
     assert torch.equal(kernels.latent_attention(more, k, kr, v, **f)[:317], ref)
+
+
+@pytest.mark.parametrize("mask,kw", MASKS, ids=[m for m, _ in MASKS])
+@pytest.mark.parametrize("q_lens,kv_lens,h", [
+    ([130, 40], [300, 70], 2), ([20], [2700], 2), ([1100, 1000], [590, 610], 52),
+])
+def test_prefill_neighbours(q_lens, kv_lens, h, mask, kw):
+    """What lies behind a sequence's rows is not seen: NaN between the sequences, ragged
+    (a sequence of nobody's queries) and dense (views of longer tensors)."""
+    d, gap = 64, 37
+    kn, qn = sum(kv_lens) + gap * len(kv_lens), sum(q_lens)
+    _, k, kr, v = prefill_case(d, BF, [1], [kn], h)
+    q = randn(qn, h, d + 64, dtype=BF, seed=4).cuda()
+    at, held = 0, torch.zeros(kn, dtype=torch.bool, device="cuda")
+    ki, qi = [0], [0]
+    for m, n in zip(q_lens, kv_lens):
+        held[at:at + n] = True
+        at += n + gap
+        ki += [at - gap, at]
+        qi += [qi[-1] + m] * 2
+    for x in (k, kr, v):
+        x[~held] = math.nan
+    o = kernels.latent_attention(q, k, kr, v, q_indptr=i32(qi), kv_indptr=i32(ki), **kw)
+    prefill_check(o, q, k[held], kr[held], v[held], q_lens, kv_lens, mask, 128 ** -0.5)
+    m, n = q_lens[0], kv_lens[0]
+    k, kr, v = k[:n + gap], kr[:n + gap], v[:n + gap]
+    dense = kernels.latent_attention(q[None, :m].transpose(1, 2), k[None, :n].transpose(1, 2),
+                                     kr[None, :n], v[None, :n].transpose(1, 2), **kw)
+    prefill_check(dense[0].transpose(0, 1), q[:m], k, kr, v, [m], [n], mask, 128 ** -0.5)
 
 
 # ---- refusals on the device, both paths ---------------------------------------------------

@@ -99,6 +99,8 @@ def test_layouts(path, layout, dtype, lens, hq, hkv, m, d, page):
     ([2500, 40, 3100, 16], 8, 2, 16, 128),   # units cut by segments
     ([1500, 900], 8, 8, 13, 64), ([5000], 16, 1, 61, 128), ([2000, 17], 8, 2, 20, 256),
     ([100 + i for i in range(150)], 2, 2, 3, 64),
+    ([30] * 66 + [2600, 0, 900], 4, 2, 24, 128),  # more than a wave's lanes, units cut
+    ([2600] + [64] * 70, 8, 1, 17, 64),
 ])
 def test_lengths(layout, lens, hq, hkv, m, d):
     q, ks, vs, t, (k, v), kw = make(layout, BF, lens, hq, hkv, m, d)

@@ -16,6 +16,8 @@ namespace fa2 {
 namespace {
 
 constexpr int64_t kLim = INT32_MAX / 2;  // 32-bit counters inside the kernels
+// Workgroups of 256 threads in a grid row: its threads are counted in 32 bits.
+constexpr int64_t kMaxGrid = (int64_t(1) << 24) - 1;
 
 int launched() { return hipGetLastError() == hipSuccess ? FA2_OK : FA2_ERR_HIP; }
 
@@ -26,6 +28,9 @@ bool latent_dims_ok(int64_t latent, int64_t rope) {
 bool half_type(int32_t dtype) { return dtype == FA2_DTYPE_F16 || dtype == FA2_DTYPE_BF16; }
 
 // ---- the writer ----------------------------------------------------------------
+
+// Rows of a workgroup.
+int64_t append_rows(int64_t latent) { return kLaThreads / 64 * (latent == 512 ? 1 : 2); }
 
 int validate_append(const fa2_latent_append_params* p) {
   if (!p) return FA2_ERR_NULL_POINTER;
@@ -39,14 +44,14 @@ int validate_append(const fa2_latent_append_params* p) {
   if (p->batch > kLim || p->num_rows > kLim || p->page_size > kLim || p->num_pages > kLim ||
       p->table_width > kLim || p->positions > kLim)
     return FA2_ERR_TOO_LARGE;
+  if (cdiv(p->num_rows, append_rows(p->latent_dim)) > kMaxGrid) return FA2_ERR_TOO_LARGE;
   if (!stride_ok(p->x_ts, 2) || p->rope_stride % 4) return FA2_ERR_ALIGNMENT;
   return FA2_OK;
 }
 
 template <int DT>
 void launch_append(int64_t latent, const LatentAppendArgs& a, hipStream_t st) {
-  const int rows = kLaThreads / 64 * (latent == 512 ? 1 : 2);
-  const dim3 grid(static_cast<uint32_t>(cdiv(a.num_rows, rows))), block(kLaThreads);
+  const dim3 grid(static_cast<uint32_t>(cdiv(a.num_rows, append_rows(latent)))), block(kLaThreads);
   if (latent == 512)
     hipLaunchKernelGGL((fa2_latent_append_kernel<DT, 512>), grid, block, 0, st, a);
   else
@@ -99,8 +104,7 @@ int rows_plan(const RowsCall& c, RowsPlan* pl) {
   // (one segment per stream cuts no unit, and neither do short ones)
   pl->cut = pl->segs > 1 && tiles > kRbShort;
   const int64_t slots = pl->cut ? 2 * grid : 0;
-  if (pl->streams * c.batch > kLim || slots > kLim)
-    return FA2_ERR_TOO_LARGE;
+  if (pl->streams * c.batch > kMaxGrid || grid > kMaxGrid) return FA2_ERR_TOO_LARGE;
   const int64_t idle = std::max<int64_t>(0, grid - pl->streams * c.batch);
   pl->whole = std::max(kRbWhole / 2, kRbWhole * idle / grid);
   size_t off = static_cast<size_t>(pl->streams * c.batch) * sizeof(int2);
@@ -352,11 +356,11 @@ int prefill_plan(const fa2_latent_prefill_params* p, PrefillPlan* pl) {
   auto items = [&](int64_t rows) {
     return (ragged ? cdiv(p->q_len, rows) + p->batch : cdiv(p->q_len, rows) * p->batch);
   };
-  if (items(kBM) * p->heads > kLim / 4) return FA2_ERR_TOO_LARGE;
+  if (items(kBM) * p->heads > kMaxGrid - kXcds) return FA2_ERR_TOO_LARGE;
   // Pairs of q-blocks on one workgroup per CU where sequences have four q-blocks on average
   // (a lone block leaves half of the workgroup without rows) and the pairs fill the CUs.
   const bool many = ragged ? p->q_len >= 4 * kBM * p->batch : nqb >= 4;
-  pl->pair = many && items(2 * kBM) * p->heads >= cus;
+  pl->pair = many && cus >= kXcds && items(2 * kBM) * p->heads >= cus;
   pl->work_ub = items(pl->pair ? 2 * kBM : kBM);
   pl->npairs = pl->work_ub * p->heads;
   pl->grid = cdiv(pl->npairs, kXcds) * kXcds;
@@ -370,7 +374,8 @@ int prefill_plan(const fa2_latent_prefill_params* p, PrefillPlan* pl) {
   s = pl->pair ? 1 : std::max<int64_t>(1, std::min<int64_t>(s, FA2_MAX_SPLITS));
   pl->splits = static_cast<int>(s);
   pl->wgs = pl->pair ? std::min(pl->grid, cus) : pl->grid;
-  pl->inline_plan = ragged && s == 1 && p->batch <= kInlinePlanMaxBatch && pl->grid <= slots;
+  pl->inline_plan =
+      ragged && !pl->pair && s == 1 && p->batch <= kInlinePlanMaxBatch && pl->grid <= slots;
   pl->plan = ragged && !pl->inline_plan;
   size_t off = 0;
   pl->off_work = off;
@@ -390,36 +395,24 @@ int prefill_plan(const fa2_latent_prefill_params* p, PrefillPlan* pl) {
 
 template <int DT, int D, int MODE>
 void launch_prefill_typed(const KArgs& a, const PrefillPlan& pl, hipStream_t st) {
-  const dim3 grid(static_cast<uint32_t>(pl.wgs), pl.splits), block(kPPThreads);
   if constexpr (MODE == FA2_LAYOUT_RAGGED) {
     if (pl.plan)
       hipLaunchKernelGGL((fa2_plan_kernel<MODE>), dim3(1), dim3(kPlanThreads), 0, st, a,
                          const_cast<int2*>(a.work), const_cast<int32_t*>(a.work_count));
   }
   if (!pl.pair) {
-    hipLaunchKernelGGL(
-        (fa2_fwd_lds_kernel<DT, D, MODE, true, false, false, kLaRope>), grid,
-        dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((fa2_fwd_lds_kernel<DT, D, MODE, true, false, false, kLaRope>),
+                       dim3(static_cast<uint32_t>(pl.wgs), pl.splits), dim3(kThreads), 0, st, a);
     if (pl.splits > 1)
       hipLaunchKernelGGL((fa2_combine_kernel<DT, D, MODE>),
                          dim3(static_cast<uint32_t>(pl.grid), kBM / kCombineRows<D>),
                          dim3(kThreads), 0, st, a);
     return;
   }
-  if constexpr (MODE == FA2_LAYOUT_RAGGED) {
-    if (a.claim) {
-      hipLaunchKernelGGL((fa2_fwd_pp_kernel<DT, D, MODE, true, true, false, false, false, kLaRope>),
-                         grid, block, 0, st, a);
-      return;
-    }
-    if (pl.inline_plan) {
-      hipLaunchKernelGGL((fa2_fwd_pp_kernel<DT, D, MODE, true, false, true, false, false, kLaRope>),
-                         grid, block, 0, st, a);
-      return;
-    }
-  }
-  hipLaunchKernelGGL((fa2_fwd_pp_kernel<DT, D, MODE, true, false, false, false, false, kLaRope>),
-                     grid, block, 0, st, a);
+  // (ragged units are claimed: KArgs::claim)
+  hipLaunchKernelGGL((fa2_fwd_pp_kernel<DT, D, MODE, true, MODE == FA2_LAYOUT_RAGGED, false, false,
+                                        false, kLaRope>),
+                     dim3(static_cast<uint32_t>(pl.wgs)), dim3(kPPThreads), 0, st, a);
 }
 
 template <int DT>
@@ -615,11 +608,9 @@ extern "C" int fa2_latent_prefill(const fa2_latent_prefill_params* p, void* stre
     a.work = reinterpret_cast<const int2*>(ws + pl.off_work);
     a.work_count = count;
     if (pl.splits > 1) a.split_count = count + 1;
-    // Sequences of more than one q-block on average: units are claimed per XCD, so that its
-    // workgroups run the q-blocks of one or two sequences at a time and share their K/V in
-    // its L2, as in fa2_fwd.
-    if (pl.pair && pl.wgs >= kXcds)
-      a.claim = count + kClaimAt / sizeof(int32_t);
+    // Units are claimed per XCD, so that its workgroups run the q-blocks of one or two
+    // sequences at a time and share their K/V in its L2, as in fa2_fwd.
+    if (pl.pair) a.claim = count + kClaimAt / sizeof(int32_t);
   }
   if (pl.splits > 1) {
     a.part_ml = reinterpret_cast<float*>(ws + pl.off_ml);
