@@ -378,7 +378,8 @@ fa2_decode_rows_kernel(RowsArgs ra) {
   constexpr int DG = kRbWaves / RG;         // waves that share a row group's dims
   constexpr int DBW = DV / 32 / DG;         // 32-dim blocks of a wave's O^T
   static_assert(DBW >= 1, "dims of a wave");
-  constexpr bool kAcc = DBW == 16;          // O^T fills the AGPRs
+  static_assert(DBW < 8 || SB == 1, "mma32_wait");
+  constexpr bool kAcc = DBW >= 8;           // O^T lies in the AGPRs
   constexpr int GPW = TK / 32;              // 8-row groups a wave loads per tile
   constexpr int IPT = GPW * (GK::kGI + (LAT ? 0 : GV::kGI));
   constexpr int kVOff = LAT ? 0 : TK * GK::kRowBytes;  // V rows in a slot
