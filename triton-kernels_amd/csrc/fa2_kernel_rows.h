@@ -94,13 +94,14 @@ __device__ __forceinline__ RowsWalk rows_locate(const KArgs& a, int k, DecSegmen
   const int W = lane < a.batch ? walk_weight(w.lens) : 0;
   int incl = W, longest = W;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
+  for (int d = 1; d < 64; d <<= 1) {  // (lanes past the batch count nothing)
+    if (d >= a.batch) break;
     const int y = __shfl_up(incl, d);
     if (lane >= d) incl += y;
     longest = max(longest, __shfl_xor(longest, d));
   }
   longest = __builtin_amdgcn_readfirstlane(longest);
-  int total = __builtin_amdgcn_readlane(incl, 63);
+  int total = __builtin_amdgcn_readlane(incl, a.batch - 1);
   int C = max((total + a.walk_segs - 1) / a.walk_segs, a.walk_min);
   if (longest <= a.walk_short || walk_keep_whole(a, longest, C, a.walk_whole)) {
     w.sg = DecSegment{k, 0, 0, 0, 0};
@@ -119,10 +120,11 @@ __device__ __forceinline__ RowsWalk rows_locate(const KArgs& a, int k, DecSegmen
       incl = room;
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) {
+        if (d >= a.batch) break;
         const int y = __shfl_up(incl, d);
         if (lane >= d) incl += y;
       }
-      total = __builtin_amdgcn_readlane(incl, 63);
+      total = __builtin_amdgcn_readlane(incl, a.batch - 1);
     }
   }
   const int s0 = min(k * C, total);
@@ -205,31 +207,37 @@ __global__ __launch_bounds__(256) void fa2_rows_merge_kernel(RowsArgs ra) {
   };
   float m = -INFINITY, l = 0.f;
   f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
-  for (int s0 = 0; s0 < info.x; s0 += kMergeAhead) {
-    f32x2 ml[kMergeAhead];
-    f32x4 x[kMergeAhead];
+  auto add = [&](auto nc, int s0) {  // pieces s0 ..+N - 1
+    constexpr int N = decltype(nc)::value;
+    f32x2 ml[N];
+    f32x4 x[N];
 #pragma unroll
-    for (int j = 0; j < kMergeAhead; ++j) {
-      const int64_t at = row_of(min(s0 + j, info.x - 1));
+    for (int j = 0; j < N; ++j) {
+      const int64_t at = row_of(s0 + j);
       ml[j] = *reinterpret_cast<const f32x2*>(a.part_ml + at * 2);
       x[j] = *reinterpret_cast<const f32x4*>(a.part_o + at * DV + col);
     }
     float mn = m;
 #pragma unroll
-    for (int j = 0; j < kMergeAhead; ++j) mn = fmaxf(mn, ml[j][0]);
+    for (int j = 0; j < N; ++j) mn = fmaxf(mn, ml[j][0]);
     const float mu = mn == -INFINITY ? 0.f : mn;
     const float al = fast_exp2(m - mu);
     l *= al;
     acc *= al;
     m = mn;
 #pragma unroll
-    for (int j = 0; j < kMergeAhead; ++j) {
-      const float m_j = ml[j][0], l_j = ml[j][1];
-      const float w = s0 + j < info.x ? fast_exp2(m_j - mu) : 0.f;
-      l += w * l_j;
+    for (int j = 0; j < N; ++j) {
+      const float w = fast_exp2(ml[j][0] - mu);
+      l += w * ml[j][1];
       acc += w * x[j];
     }
-  }
+  };
+  const int n = __builtin_amdgcn_readfirstlane(info.x);
+  int s0 = 0;
+  for (; s0 + 8 <= n; s0 += 8) add(std::integral_constant<int, 8>{}, s0);
+  if (n & 4) add(std::integral_constant<int, 4>{}, s0), s0 += 4;
+  if (n & 2) add(std::integral_constant<int, 2>{}, s0), s0 += 2;
+  if (n & 1) add(std::integral_constant<int, 1>{}, s0);
   const float inv = 1.f / l;  // 0/0 -> NaN for a row with no key
   *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.o) + b * a.o_sb +
                             static_cast<int64_t>(kvh) * (a.hq / a.hkv) * a.o_sh +
@@ -281,6 +289,52 @@ struct RowsTable {
   }
 };
 
+// x, whose uses are not computed ahead of this place (registers of the tile loop).
+__device__ __forceinline__ int here(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// The mask rows of sequence b's tree as words in LDS, a row per wave and step.  The loads of up
+// to 16 rows are in flight at once.  (A round trip for each, of 61: 6 us a piece.)
+template <int NW>
+struct RowsTree {
+  static constexpr int kMax = kRbMaxTree / NW;
+  uint8_t x[kMax];
+  // f(step, row) over the wave's rows; the last rows repeat
+  template <typename F>
+  __device__ __forceinline__ void each(const KArgs& a, int wave, F&& f) {
+    static_for<kMax / 4>([&](auto g) {
+      if (wave + decltype(g)::value * 4 * NW < a.pack_m) {
+        static_for<4>([&](auto j) {
+          constexpr int s = decltype(g)::value * 4 + decltype(j)::value;
+          f(std::integral_constant<int, s>{}, min(wave + s * NW, a.pack_m - 1));
+        });
+      }
+    });
+  }
+  __device__ __forceinline__ void load(const RowsArgs& ra, int b, int wave, int lane) {
+    const uint8_t* t = ra.tree + b * ra.tree_sb + min(lane, ra.a.pack_m - 1);
+    each(ra.a, wave, [&](auto s, int row) { x[decltype(s)::value] = t[row * ra.tree_sr]; });
+  }
+  // one row after the other, where the registers do not allow more
+  __device__ __forceinline__ static void fill(const RowsArgs& ra, int b, int wave, int lane,
+                                              uint64_t* sh) {
+    for (int i = wave; i < ra.a.pack_m; i += NW) {
+      const uint8_t sees =
+          lane < ra.a.pack_m ? ra.tree[b * ra.tree_sb + i * ra.tree_sr + lane] : uint8_t(0);
+      const uint64_t word = __ballot(sees != 0);
+      if (lane == 0) sh[i] = word;
+    }
+  }
+  __device__ __forceinline__ void store(const KArgs& a, int wave, int lane, uint64_t* sh) {
+    each(a, wave, [&](auto s, int row) {
+      const uint64_t word = __ballot(lane < a.pack_m && x[decltype(s)::value] != 0);
+      if (lane == 0) sh[row] = word;
+    });
+  }
+};
+
 // Bit x: key n + x is seen by draft m; off: keys before the drafts (below zero where there
 // are fewer keys than drafts), word: the drafts that m sees (kMaskTree).
 __device__ __forceinline__ uint32_t rows_sees(const KArgs& a, int n, int Lk, int off, int m,
@@ -329,12 +383,6 @@ __device__ __forceinline__ void rows_dma(uint64_t base, uint32_t off, uint32_t l
                  :
                  : "v"(off), "s"(base),
                    "{m0}"(__builtin_amdgcn_readfirstlane(static_cast<int>(lds_addr))));
-}
-
-// x, whose uses are not computed ahead of this place (registers of the tile loop).
-__device__ __forceinline__ int here(int x) {
-  asm volatile("" : "+v"(x));
-  return x;
 }
 
 // MFMAs of the kernel whose accumulators fill the AGPRs (32 rows of 512 dims per wave): O^T
@@ -452,14 +500,6 @@ fa2_decode_rows_kernel(RowsArgs ra) {
     const int row = q0 + rg * 32 + l32;
     const int m = row % a.pack_m;  // draft
     const int nrows = min(a.q_len - q0, 32 * RG);
-    if (a.mask == kMaskTree) {
-      for (int i = wave; i < a.pack_m; i += kRbWaves) {
-        const uint8_t sees =
-            lane < a.pack_m ? ra.tree[p.b * ra.tree_sb + i * ra.tree_sr + lane] : uint8_t(0);
-        const uint64_t word = __ballot(sees != 0);
-        if (lane == 0) tree_sh[i] = word;
-      }
-    }
     int64_t kbase, vbase;
     rows_bases<MODE>(a, p, kbase, vbase);
     const char* kptr = static_cast<const char*>(a.k) + kbase * 2;
@@ -490,6 +530,11 @@ fa2_decode_rows_kernel(RowsArgs ra) {
         if (ka < kend) entries.load(ra, p.b, page0, page_of(kb - 1) - page0);
       }
     };
+    RowsTree<kRbWaves> sees;
+    if (a.mask == kMaskTree) {
+      if constexpr (LAT) sees.fill(ra, p.b, wave, lane, tree_sh);
+      else sees.load(ra, p.b, wave, lane);
+    }
     window();
     u32x4 qf[DC];
     {
@@ -500,10 +545,15 @@ fa2_decode_rows_kernel(RowsArgs ra) {
 #pragma unroll
       for (int c = 0; c < DC; ++c) qf[c] = *reinterpret_cast<const u32x4*>(src + c * 16);
     }
+    if constexpr (!LAT)
+      if (a.mask == kMaskTree) sees.store(a, wave, lane, tree_sh);
     for (; ka < kend; ka = kb, window()) {
       if constexpr (kPaged) entries.store(ra, p.b, page0, page_of(kb - 1) - page0, tab);
       __syncthreads();  // the table and the mask are in LDS, the slots are free
       if (a.mask == kMaskTree) word = tree_sh[m];
+      // Q is there before the first tile goes out: a later wait of the compiler's would drain
+      // the tiles in flight
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
 
       const int T = (kb - ka + TK - 1) / TK;
       // A tile goes out 8 rows at a time, each group of one page: its block-table entries are
@@ -589,9 +639,6 @@ fa2_decode_rows_kernel(RowsArgs ra) {
         }
       }
       if (NS - 1 < T) fetch(NS - 1);
-      // Q and the first tiles: later waits of the compiler's would drain the tiles
-      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-
       for (int t = 0; t < T; ++t) {
         rows_wait<IPT, NS - 2>(T - 1 - t);
         pp_barrier();  // tile t is there, and slot t - 1 has been read

@@ -98,14 +98,6 @@ fa2_decode_rows16_kernel(RowsArgs ra) {
   for (;;) {
     const int m = l16 % a.pack_m;  // draft
     const int rows = a.q_len;
-    if (a.mask == kMaskTree) {
-      for (int i = wave; i < a.pack_m; i += NW) {
-        const uint8_t sees =
-            lane < a.pack_m ? ra.tree[p.b * ra.tree_sb + i * ra.tree_sr + lane] : uint8_t(0);
-        const uint64_t w = __ballot(sees != 0);
-        if (lane == 0) tree_sh[i] = w;
-      }
-    }
     int64_t kbase, vbase;
     rows_bases<MODE>(a, p, kbase, vbase);
     const char* kptr = static_cast<const char*>(a.k) + kbase * 2;
@@ -133,6 +125,11 @@ fa2_decode_rows16_kernel(RowsArgs ra) {
         if (ka < kend) entries.load(ra, p.b, page0, page_of(kb - 1) - page0);
       }
     };
+    RowsTree<NW> sees;
+    if (a.mask == kMaskTree) {
+      if constexpr (LAT) sees.fill(ra, p.b, wave, lane, tree_sh);
+      else sees.load(ra, p.b, wave, lane);
+    }
     window();
     u32x4 qf[DJ];
     {
@@ -143,10 +140,15 @@ fa2_decode_rows16_kernel(RowsArgs ra) {
 #pragma unroll
       for (int j = 0; j < DJ; ++j) qf[j] = *reinterpret_cast<const u32x4*>(src + j * 32);
     }
+    if constexpr (!LAT)
+      if (a.mask == kMaskTree) sees.store(a, wave, lane, tree_sh);
     for (; ka < kend; ka = kb, window()) {
       if constexpr (kPaged) entries.store(ra, p.b, page0, page_of(kb - 1) - page0, tab);
       __syncthreads();  // the table and the mask are in LDS, the slots are free
       if (a.mask == kMaskTree) word = tree_sh[m];
+      // Q is there before the first tile goes out: a later wait of the compiler's would drain
+      // the tiles in flight
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
 
       auto issue = [&](auto is_v, int n0) {
         constexpr bool V = decltype(is_v)::value;
@@ -197,8 +199,6 @@ fa2_decode_rows16_kernel(RowsArgs ra) {
         issue(IsK{}, n0);
         if constexpr (!LAT) issue(IsV{}, n0);
       }
-      // Q and the first tile: later waits of the compiler's would drain the tiles
-      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
       for (; n0 < kb; n0 += kStep) {
         const bool more = n0 + kStep < kb;
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kVOps) : "memory");  // K(t)
