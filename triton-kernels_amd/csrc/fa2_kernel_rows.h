@@ -1,6 +1,38 @@
 // fa2_kernel_rows.h - decode attention with many query rows per K/V row: the
 // absorbed form of latent attention (every head reads the same cached row) and
 // trees of drafts over 16-bit K/V caches.
+//
+//   s_rn = scale q_r . k_n (n visible to r),  p_rn = exp(s_rn - m_r),
+//   o_r = sum_n p_rn v_n / sum_n p_rn
+//
+// The rows of a unit (sequence, kv head) are its heads times its tokens: up to 128 in
+// latent attention's decode step, 8 to 16 times the decode kernels'.  Latent attention:
+// k_n is the whole cached row (DK = latent + 64), v_n its first DV = latent values, so a
+// row is read once for both products, from one LDS tile.  Per key the kernel reads
+// 2 DK (+ 2 DV) bytes and does 2 (DK + DV) FLOP a row: 16 rows of a latent are bound by
+// HBM, 128 rows (242 FLOP a byte) by neither alone, so loads and MFMAs have to overlap.
+//   * Workgroup = 4 waves.  RG row groups of 32 rows: a wave takes one of them and all
+//     DV dims (RG = 4), half (2) or a quarter (1) of them, S computed by each.  Up to 16
+//     rows: fa2_kernel_rows16.h.
+//   * S^T = K Q^T and O^T += V^T P^T by v_mfma_f32_32x32x16, so that a lane holds one
+//     row's scores: the softmax needs one cross-lane step, and P^T is the second
+//     product's operand as it lies in the registers.  V^T by ds_read_b64_tr_b16.
+//   * Tiles of 32 or 64 keys go straight to LDS (global_load_lds), 3 to 6 slots a
+//     workgroup, in groups of 8 rows whose base is a scalar: a page of 8 rows or more costs
+//     one block-table entry of LDS and no vector address.  The loads of a tile stand between
+//     the MFMAs of S.
+//   * fp32 scores, maxima, sums and O; the weights are rounded once, to the tensors' type,
+//     for the second product, and summed as rounded.  The maximum is raised when a score
+//     passes it by 2^8 only, so fp16 weights, lifted by 2^7, end at 2^15.
+//   * Workgroups share the tiles evenly (fa2_decode_walk.h, rows_locate); a unit cut by
+//     segments leaves fp32 partials, which a second launch merges in piece order
+//     (fa2_rows_merge_kernel): no atomics, the same bits every time.
+//
+// Measured on MI355X, us per call, against the first version of the kernel: 64 latents of
+// 512-8192 keys, 128 heads 1739 -> 126 (bound by power: 119 to 145 with the card's clock,
+// 625 TFLOP/s, 2.7 TB/s; the compiler's own allocation moved O^T between VGPRs and scratch),
+// 17 trees of 7 drafts over latents of 256 values 130 -> 48, 64 trees of 16 drafts Hq32/Hkv8
+// D128 237 -> 208 (4.6 TB/s), 16 trees of 61 drafts 129 -> 115 (615 TFLOP/s).
 #pragma once
 
 #include "fa2_decode_walk.h"
@@ -16,7 +48,9 @@ constexpr int kRbMaxTree = 64;  // drafts of a tree: bits of a mask word
 // Mask of a call beyond enum fa2_mask: the drafts that each draft sees.
 constexpr int kMaskTree = 3;
 
-// A second piece of a workgroup costs about as much as this many tiles of kBN keys.
+// A second piece of a workgroup costs about as much as this many tiles of kBN keys (1 to 6
+// measure the same; with 0, 17 trees of 7 drafts take 65 us instead of 55, 16 latents of
+// 16000-32768 keys 94 instead of 84).
 constexpr int kRbSwitch = 2;
 
 struct RowsArgs {
@@ -46,7 +80,9 @@ struct RowsGeo {
   }
 };
 
-// Tile shape: workgroups per CU, keys of a tile and LDS slots.
+// Tile shape: workgroups per CU, keys of a tile and LDS slots.  Two workgroups where their
+// tiles fit the CU's 160 KB and the registers 256 a lane: one's softmax runs under the other's
+// MFMAs.
 template <int DK, int DV, bool LAT, int RG>
 struct RowsTile {
   using G = RowsGeo<DK>;
@@ -181,11 +217,10 @@ __device__ __forceinline__ void rows_info(const RowsArgs& ra, const DecSegment& 
 }
 
 // The merge of cut units, launched behind the kernels that cut them: workgroup (x, y) takes
-// rows y * kCombineRows ..  of unit x, a thread 4 columns of a row over all pieces, in order,
-// kMergeAhead of them in flight.  (One workgroup per unit that merges in the first kernel, as
-// the 16-bit decode kernels do, takes a memory round trip for every 64 KB of partials, 32 to
-// 256 KB a piece here: 4 x 900 keys of 16 heads 36 us, with this launch XX.)
-constexpr int kMergeAhead = 8;
+// rows y * kMergeRows .. of unit x, a thread 4 columns of a row over all pieces, in order, up
+// to 8 of them in flight.  (One workgroup per unit that merges in the first kernel, as the
+// 16-bit decode kernels do, takes a memory round trip for every 64 KB of partials, 32 to 256 KB
+// a piece here: 4 x 900 keys of 16 heads 36 us, with this launch 26.)
 template <int DV>
 constexpr int kMergeRows = DV >= 1024 ? 1 : 1024 / DV;  // rows of 256 threads
 
@@ -385,9 +420,9 @@ __device__ __forceinline__ void rows_dma(uint64_t base, uint32_t off, uint32_t l
                    "{m0}"(__builtin_amdgcn_readfirstlane(static_cast<int>(lds_addr))));
 }
 
-// MFMAs of the kernel whose accumulators fill the AGPRs (32 rows of 512 dims per wave): O^T
-// there (mma32_acc), S in VGPRs (mma32_vgpr), as the compiler left to itself moves both to and
-// fro and spills Q.  Two wait states stand between a VALU write of an operand and its MFMA; who
+// MFMAs of the kernels with O^T of 256 dims or more a wave: O^T in AGPRs (mma32_acc), S in VGPRs
+// (mma32_vgpr), as the compiler left to itself moves O^T to and fro for every tile (17 trees of 7
+// drafts, 256 dims: 61 us, so 55) and spills Q (512 dims: 1739 us, so 130).  Two wait states stand between a VALU write of an operand and its MFMA; who
 // reads the result waits 24 (mma32_wait; the longest MFMA asks for 20).
 template <bool BF>
 __device__ __forceinline__ void mma32_acc(f32x16& c, u32x4 a, u32x4 b) {
@@ -410,6 +445,8 @@ __device__ __forceinline__ void mma32_wait(f32x16& c) {
 // the loops carry it whole.
 __device__ __forceinline__ void in_acc(f32x16& c) { asm volatile("" : "+a"(c)); }
 
+// NT: loads past the caches, where no other q-block reads the same K and V (64 trees of 16
+// drafts 237 -> 216 us; of 61 drafts, two q-blocks: 124 -> 129 with it).
 template <int DT, int DK, int DV, bool LAT, int RG, int MODE, bool NT>
 __global__ __launch_bounds__(kRbThreads, (RowsTile<DK, DV, LAT, RG>::kOcc)) void
 fa2_decode_rows_kernel(RowsArgs ra) {
@@ -789,13 +826,13 @@ fa2_decode_rows_kernel(RowsArgs ra) {
             if constexpr (kAcc) __builtin_amdgcn_sched_barrier(0);
           });
           if constexpr (!kAcc) {
-          __builtin_amdgcn_sched_group_barrier(0x100, 2 * kAhead, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2 * kAhead, 0);
 #pragma unroll
-          for (int k = 0; k < kN - kAhead; ++k) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-          }
-          __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+            for (int k = 0; k < kN - kAhead; ++k) {
+              __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+              __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
           }
           __builtin_amdgcn_sched_barrier(0);
         }

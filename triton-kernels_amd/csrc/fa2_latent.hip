@@ -78,7 +78,10 @@ struct RowsPlan {
   size_t off_ml, off_o, total;
 };
 
-// The balanced walk's costs, in tiles of 64 keys (fa2_decode_walk.h).
+// The balanced walk's costs, in tiles of 64 keys (fa2_decode_walk.h): units of up to kRbShort
+// tiles stay whole, as do all of them if that costs the longest workgroup no more than kRbWhole
+// (half of it where no workgroup would be idle): a cut unit's partials are 2 to 8 times those of
+// the other decode kernels.
 constexpr int64_t kRbMinTiles = 2;
 constexpr int64_t kRbWhole = 16, kRbShort = 4;
 
@@ -86,6 +89,8 @@ int rows_plan(const RowsCall& c, RowsPlan* pl) {
   pl->rows = c.q_heads / c.kv_heads * c.q_len;
   if (pl->rows > kLim) return FA2_ERR_TOO_LARGE;
   const int64_t cus = cu_count_current_device();
+  // The smallest q-block that holds the rows (4 x 900 keys of 16 heads: 17.8 us with up to 16
+  // rows, 26 with 32; 128-row blocks read K and V least often beyond that).
   const int64_t least = c.dv == 64 ? 2 : 1;  // (a wave has 32 dims at least)
   pl->rg = static_cast<int>(pl->rows <= kR16Rows ? 0 : pl->rows <= 32 ? least : pl->rows <= 64 ? 2 : 4);
   const int64_t block_rows = pl->rg ? 32 * pl->rg : kR16Rows;
@@ -358,7 +363,10 @@ int prefill_plan(const fa2_latent_prefill_params* p, PrefillPlan* pl) {
   };
   if (items(kBM) * p->heads > kMaxGrid - kXcds) return FA2_ERR_TOO_LARGE;
   // Pairs of q-blocks on one workgroup per CU where sequences have four q-blocks on average
-  // (a lone block leaves half of the workgroup without rows) and the pairs fill the CUs.
+  // (a lone block leaves half of the workgroup without rows) and the pairs fill the CUs: 854
+  // TFLOP/s on 16 prompts of 128-4096.  Else one q-block per workgroup, two workgroups per CU,
+  // the keys split over idle ones: one prompt of 333, 16 heads 15.1 us (pairs 19), 8 chunks of
+  // 100-512 over 4000 more 112 (pairs 133-166).
   const bool many = ragged ? p->q_len >= 4 * kBM * p->batch : nqb >= 4;
   pl->pair = many && cus >= kXcds && items(2 * kBM) * p->heads >= cus;
   pl->work_ub = items(pl->pair ? 2 * kBM : kBM);

@@ -8,7 +8,12 @@
 // part, whose pairs (i, i + 32) lie four lanes apart.  The row is loaded first; its
 // sequence is found meanwhile by a 64-way search of the prefix sums (one load for
 // up to 64 sequences, two up to 4096), then start, table entry and position's angles
-// follow one another.
+// follow one another.  The sum of squares, the norm and the rotation are fp32; each value is
+// rounded once, to the row's type.
+//
+// Measured on MI355X: 64 rows 3.5 us (a launch 2, the rest that chain of loads; 4.0 with the
+// host's call), 10754 rows of 16 sequences, rows returned as well, 11.4 (37 MB, 3.3 TB/s; a
+// copy of 1 GiB reaches 5.1).
 #pragma once
 
 #include "fa2_values.h"

@@ -19,7 +19,9 @@ reference's kernels/decode.py:203-331); lengths past the block table's width cou
 that.  ``softmax_scale`` is the model's, that of the expanded keys.  16-bit MFMA with fp32
 accumulation and softmax statistics; only the softmax weights are rounded to the
 tensors' type for the product with the latents, and summed as rounded.  A row that sees
-no key is NaN, as in the other decode calls.  The computation runs in ``libfa2.so``
+no key is NaN, as in the other decode calls; rows of a sequence that the mask hides are
+multiplied by zero, so their latents have to be finite (what lies behind the sequence's end
+need not be).  The computation runs in ``libfa2.so``
 (``fa2_latent_decode``, include/fa2_latent.h); no fallback.
 """
 

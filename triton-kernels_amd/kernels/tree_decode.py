@@ -17,8 +17,9 @@ itself).  A chain of drafts is the lower triangle.
 ``tree_mask``: bool ``[M, M]`` for all sequences or ``[B, M, M]``.  fp16 or bf16, D 64,
 128 or 256.  Masks, layouts and numerics are otherwise those of
 ``speculative_decode_attention``; lengths past the block table's width count as that,
-table entries are clamped into the caches, and a draft that sees no key is NaN.  The
-computation runs in ``libfa2.so`` (``fa2_tree_decode``, include/fa2_latent.h); no fallback.
+table entries are clamped into the caches, and a draft that sees no key is NaN; values that
+the mask hides are multiplied by zero, so they have to be finite (those behind a sequence's
+end need not be).  The computation runs in ``libfa2.so`` (``fa2_tree_decode``, include/fa2_latent.h); no fallback.
 """
 
 from __future__ import annotations
