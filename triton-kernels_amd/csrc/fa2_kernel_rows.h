@@ -421,9 +421,10 @@ __device__ __forceinline__ void rows_dma(uint64_t base, uint32_t off, uint32_t l
 }
 
 // MFMAs of the kernels with O^T of 256 dims or more a wave: O^T in AGPRs (mma32_acc), S in VGPRs
-// (mma32_vgpr), as the compiler left to itself moves O^T to and fro for every tile (17 trees of 7
-// drafts, 256 dims: 61 us, so 55) and spills Q (512 dims: 1739 us, so 130).  Two wait states stand between a VALU write of an operand and its MFMA; who
-// reads the result waits 24 (mma32_wait; the longest MFMA asks for 20).
+// (mma32_vgpr), as the compiler left to itself moves O^T to and fro for every tile (17 trees of
+// 7 drafts, 256 dims: 61 us, so 55) and spills Q (512 dims: 1739 us, so 130).  Two wait states
+// stand between a VALU write of an operand and its MFMA; who reads the result waits 24
+// (mma32_wait; the longest MFMA asks for 20).
 template <bool BF>
 __device__ __forceinline__ void mma32_acc(f32x16& c, u32x4 a, u32x4 b) {
   if constexpr (BF)

@@ -82,6 +82,8 @@ struct RowsPlan {
 // tiles stay whole, as do all of them if that costs the longest workgroup no more than kRbWhole
 // (half of it where no workgroup would be idle): a cut unit's partials are 2 to 8 times those of
 // the other decode kernels.
+// (4 x 900 keys of 16 heads: 17.2 us; segments of at least 1 tile 18.2, of 4 20.9; kRbWhole 32:
+// 30.0, as units stay whole on 4 workgroups.)
 constexpr int64_t kRbMinTiles = 2;
 constexpr int64_t kRbWhole = 16, kRbShort = 4;
 
@@ -92,11 +94,15 @@ int rows_plan(const RowsCall& c, RowsPlan* pl) {
   // The smallest q-block that holds the rows (4 x 900 keys of 16 heads: 17.8 us with up to 16
   // rows, 26 with 32; 128-row blocks read K and V least often beyond that).
   const int64_t least = c.dv == 64 ? 2 : 1;  // (a wave has 32 dims at least)
-  pl->rg = static_cast<int>(pl->rows <= kR16Rows ? 0 : pl->rows <= 32 ? least : pl->rows <= 64 ? 2 : 4);
+  pl->rg = static_cast<int>(pl->rows <= kR16Rows ? 0
+                            : pl->rows <= 32     ? least
+                            : pl->rows <= 64     ? 2
+                                                 : 4);
   const int64_t block_rows = pl->rg ? 32 * pl->rg : kR16Rows;
   const int64_t nqb = cdiv(pl->rows, block_rows);
   // workgroups per CU (RowsTile::kOcc)
-  const int64_t wgs = cus * (pl->rg == 0 ? 1 : c.latent ? (c.dv == 256 && pl->rg < 4 ? 2 : 1) : c.dv < 256 ? 2 : 1);
+  const bool two = pl->rg > 0 && (c.latent ? c.dv == 256 && pl->rg < 4 : c.dv < 256);
+  const int64_t wgs = two ? 2 * cus : cus;
   pl->part_rows = std::min<int64_t>(pl->rows, block_rows);
   pl->streams = c.kv_heads * nqb;
   // tiles of the call at most (lengths are on the device)
