@@ -6,7 +6,8 @@
 // makes rows 16-byte aligned, converts the index tensors, allocates the
 // output and the workspace from torch's caching allocator, fills
 // fa2_params and enqueues fa2_fwd (include/fa2.h) on torch's current HIP
-// stream (likewise fa2_decode_fwd and fa2_kv_append).  It replaces a chain of
+// stream (likewise fa2_decode_fwd, fa2_kv_append and the calls of
+// include/fa2_ops.h and include/fa2_latent.h).  It replaces a chain of
 // Python steps (strides, pointer fields, a ctypes call) that cost ~11 us per
 // call (prefill; decode with a workspace 15 to 18, append 14), more than small
 // calls take on the GPU.  No attention arithmetic here.
