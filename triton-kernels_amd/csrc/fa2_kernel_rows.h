@@ -324,6 +324,12 @@ struct RowsTable {
   }
 };
 
+// What a tile's places behind the last key take for V.  Their weights are zero; the last row
+// itself, repeated there, would turn its infinite values into NaN (0 * inf) for the rows that
+// see it.  (A latent's row needs none of this: an infinite value in it is NaN in the result
+// wherever a row sees it, by a score that is not finite and 0 * inf.)
+static __device__ const u32x4 kNoValue = {0, 0, 0, 0};
+
 // x, whose uses are not computed ahead of this place (registers of the tile loop).
 __device__ __forceinline__ int here(int x) {
   asm volatile("" : "+v"(x));
@@ -636,8 +642,8 @@ fa2_decode_rows_kernel(RowsArgs ra) {
         else
           rows_dma<NT>(sk[g], kl[i], slot + grp * 8 * GK::kRowBytes + i * 1024);
       };
-      // The rest: a row per lane; rows past the window are its last one (finite data under a
-      // zero weight).
+      // The rest: a row per lane; places past the window hold its last K row (masked) and
+      // zeros of V (kNoValue).
       auto send_rows = [&](auto is_v, int n, uint32_t dst) {
         constexpr bool V = decltype(is_v)::value;
         using G = std::conditional_t<V, GV, GK>;
@@ -647,13 +653,15 @@ fa2_decode_rows_kernel(RowsArgs ra) {
         const int ln = here(lane);
 #pragma unroll
         for (int i = 0; i < G::kGI; ++i) {
-          const int nr = min(n + lane_row(G{}, i, ln), kb - 1);
+          const int at = n + lane_row(G{}, i, ln), nr = min(at, kb - 1);
           int64_t r = nr;
           if constexpr (kPaged) {
             const int pg = page_of(nr);
             r = static_cast<int64_t>(tb[pg - page0]) * a.page_size + (nr - pg * a.page_size);
           }
-          dma_global_x4<NT>(base + r * ss * 2 + lane_chunk(G{}, i, ln) * 16, dst + i * 1024);
+          const char* src = base + r * ss * 2 + lane_chunk(G{}, i, ln) * 16;
+          if (V && at >= kb) src = reinterpret_cast<const char*>(&kNoValue);
+          dma_global_x4<NT>(src, dst + i * 1024);
         }
       };
       auto send_part = [&](int t) {

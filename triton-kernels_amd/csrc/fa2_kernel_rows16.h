@@ -188,19 +188,20 @@ fa2_decode_rows16_kernel(RowsArgs ra) {
           }
           return;
         }
-        // a row per lane; rows past the window are its last one (finite data under a zero
-        // weight)
+        // a row per lane; places past the window hold its last K row (masked) and zeros of V
+        // (kNoValue)
         for (int grp = 0; grp < TK / 8; ++grp) {
 #pragma unroll
           for (int i = 0; i < G::kGI; ++i) {
-            const int nr = min(n0 + 8 * grp + lane_row(G{}, i), kb - 1);
+            const int at = n0 + 8 * grp + lane_row(G{}, i), nr = min(at, kb - 1);
             int64_t r = nr;
             if constexpr (kPaged) {
               const int pg = page_of(nr);
               r = static_cast<int64_t>(tb[pg - page0]) * a.page_size + (nr - pg * a.page_size);
             }
-            dma_global_x4<true>(base + r * ss * 2 + lane_chunk(G{}, i, grp) * 16,
-                                dst + (grp * G::kGI + i) * 1024);
+            const char* src = base + r * ss * 2 + lane_chunk(G{}, i, grp) * 16;
+            if (V && at >= kb) src = reinterpret_cast<const char*>(&kNoValue);
+            dma_global_x4<true>(src, dst + (grp * G::kGI + i) * 1024);
           }
         }
       };
