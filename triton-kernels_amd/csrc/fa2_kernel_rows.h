@@ -58,7 +58,7 @@ struct RowsArgs {
   int2* info;  // of each unit: its pieces and the part slot of the first (rows_info)
   const uint8_t* tree;  // bool [batch, pack_m, pack_m]
   int64_t tree_sb, tree_sr;
-  int32_t num_pages, table_width;
+  int32_t num_pages;
   uint32_t page_mul, page_sh;  // n / page_size = umulhi(2 n, page_mul) >> page_sh, n < 2^30
 };
 

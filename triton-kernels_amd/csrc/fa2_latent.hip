@@ -60,12 +60,15 @@ void launch_append(int64_t latent, const LatentAppendArgs& a, hipStream_t st) {
 
 // ---- decode with many rows per key ------------------------------------------------
 
+static_assert(kMaskTree == FA2_MASK_TREE && kRbMaxTree == FA2_TREE_MAX,
+              "the kernels' mask words hold what the calls take");
+
 // What the two decode calls share.
 struct RowsCall {
   bool latent;
   int layout;
   int32_t dtype, mask;
-  int64_t batch, q_heads, kv_heads, q_len, dk, dv;
+  int64_t batch, q_heads, kv_heads, q_len, dv;
   int64_t kv_len;  // dense: keys; ragged: total rows
   int64_t page_size, num_pages, table_width;
 };
@@ -140,7 +143,6 @@ int rows_fill(const RowsCall& c, const RowsPlan& pl, float scale, void* workspac
                                                                : c.kv_len);
   a.page_size = static_cast<int32_t>(c.page_size);
   a.mask = c.mask;
-  a.num_splits = 1;
   a.scale_log2 = scale * 1.4426950408889634f;
   char* ws = static_cast<char*>(workspace);
   ra->info = reinterpret_cast<int2*>(ws);
@@ -153,12 +155,9 @@ int rows_fill(const RowsCall& c, const RowsPlan& pl, float scale, void* workspac
   a.walk_min = kRbMinTiles;
   a.walk_whole = static_cast<int32_t>(pl.whole);
   a.walk_short = kRbShort;
-  a.walk_dj = a.walk_segs;
   a.walk_rounds = static_cast<int32_t>(cdiv(c.batch, pl.segs));
   a.pack_m = static_cast<int32_t>(c.q_len);
-  a.dv = static_cast<int32_t>(c.dv);
   ra->num_pages = static_cast<int32_t>(c.num_pages);
-  ra->table_width = static_cast<int32_t>(c.table_width);
   // n / page_size for n < 2^30 as (2 n * page_mul) >> 32 >> page_sh, with page_sh =
   // floor(log2 page_size) and page_mul = ceil(2^(31 + page_sh) / page_size): page_mul
   // is off by less than 1, the quotient by less than n / 2^(31 + page_sh), which is
@@ -242,7 +241,7 @@ int validate_rows_sizes(const RowsCall& c) {
 
 RowsCall call_of(const fa2_latent_decode_params& p) {
   return {true,   FA2_LAYOUT_PAGED, p.dtype,      p.mask, p.batch,     p.q_heads,   1,
-          p.q_len, p.latent_dim + p.rope_dim, p.latent_dim, 0, p.page_size, p.num_pages, p.table_width};
+          p.q_len, p.latent_dim, 0, p.page_size, p.num_pages, p.table_width};
 }
 
 int validate_latent(const fa2_latent_decode_params* p) {
@@ -265,7 +264,7 @@ int validate_latent(const fa2_latent_decode_params* p) {
 RowsCall call_of(const fa2_tree_decode_params& p) {
   const bool paged = p.layout == FA2_LAYOUT_PAGED;
   return {false,   p.layout,   p.dtype,    FA2_MASK_TREE, p.batch, p.q_heads, p.kv_heads,
-          p.q_len, p.head_dim, p.head_dim, p.kv_len,
+          p.q_len, p.head_dim, p.kv_len,
           paged ? p.page_size : 1, paged && p.page_size > 0 ? p.kv_len / p.page_size : 0,
           paged ? p.table_width : 0};
 }
