@@ -100,7 +100,8 @@ int fa2_latent_decode(const fa2_latent_decode_params* p, void* stream);
  * fa2_fwd's masks.  The values have as many dims as k.  Dense: q [batch, heads, q_len,
  * head_dim + rope_dim], k, v and o [batch, heads, len, head_dim], kr [batch, kv_len,
  * rope_dim].  Ragged: [rows, heads, dims] and [rows, rope_dim] with prefix sums.  A row that
- * sees no key is NaN. */
+ * sees no key is NaN.  Values that a mask hides may be multiplied by zero, so they have to be
+ * finite (what lies behind a sequence's end need not be), in the decode calls too. */
 typedef struct fa2_latent_prefill_params {
   int32_t layout;           /* FA2_LAYOUT_DENSE or FA2_LAYOUT_RAGGED           */
   int32_t dtype;            /* FA2_DTYPE_F16 or FA2_DTYPE_BF16                 */

@@ -28,11 +28,11 @@
 //     segments leaves fp32 partials, which a second launch merges in piece order
 //     (fa2_rows_merge_kernel): no atomics, the same bits every time.
 //
-// Measured on MI355X, us per call, against the first version of the kernel: 64 latents of
-// 512-8192 keys, 128 heads 1739 -> 126 (bound by power: 119 to 145 with the card's clock,
-// 625 TFLOP/s, 2.7 TB/s; the compiler's own allocation moved O^T between VGPRs and scratch),
-// 17 trees of 7 drafts over latents of 256 values 130 -> 48, 64 trees of 16 drafts Hq32/Hkv8
-// D128 237 -> 208 (4.6 TB/s), 16 trees of 61 drafts 129 -> 115 (615 TFLOP/s).
+// Measured on MI355X, us per call: 64 latents of 512-8192 keys, 128 heads 128 to 131 (605
+// TFLOP/s, 2.6 TB/s; MFMAs busy for 29 % of the cycles, as S, softmax and PV of a tile follow one
+// another on one wave per SIMD; the kernel alone takes 116 in the first calls of a loop and 131
+// after 50), 17 trees of 7 drafts over latents of 256 values 48, 64 trees of 16 drafts Hq32/Hkv8
+// D128 207 (4.7 TB/s), 16 trees of 61 drafts 114 to 118 (610 TFLOP/s, MFMAs busy for 31 %).
 #pragma once
 
 #include "fa2_decode_walk.h"
@@ -49,8 +49,8 @@ constexpr int kRbMaxTree = 64;  // drafts of a tree: bits of a mask word
 constexpr int kMaskTree = 3;
 
 // A second piece of a workgroup costs about as much as this many tiles of kBN keys (1 to 6
-// measure the same; with 0, 17 trees of 7 drafts take 65 us instead of 55, 16 latents of
-// 16000-32768 keys 94 instead of 84).
+// measure the same; with 0, 17 trees of 7 drafts take 59 us instead of 53 in the same run, 16
+// latents of 16000-32768 keys 91 instead of 88).
 constexpr int kRbSwitch = 2;
 
 struct RowsArgs {
@@ -220,7 +220,8 @@ __device__ __forceinline__ void rows_info(const RowsArgs& ra, const DecSegment& 
 // rows y * kMergeRows .. of unit x, a thread 4 columns of a row over all pieces, in order, up
 // to 8 of them in flight.  (One workgroup per unit that merges in the first kernel, as the
 // 16-bit decode kernels do, takes a memory round trip for every 64 KB of partials, 32 to 256 KB
-// a piece here: 4 x 900 keys of 16 heads 36 us, with this launch 26.)
+// a piece of a latent: with blocks of 32 rows 4 x 900 keys of 16 heads took 36 us, with this
+// launch 26.  Pieces of a few KB were not measured.)
 template <int DV>
 constexpr int kMergeRows = DV >= 1024 ? 1 : 1024 / DV;  // rows of 256 threads
 
@@ -428,9 +429,9 @@ __device__ __forceinline__ void rows_dma(uint64_t base, uint32_t off, uint32_t l
 
 // MFMAs of the kernels with O^T of 256 dims or more a wave: O^T in AGPRs (mma32_acc), S in VGPRs
 // (mma32_vgpr), as the compiler left to itself moves O^T to and fro for every tile (17 trees of
-// 7 drafts, 256 dims: 61 us, so 55) and spills Q (512 dims: 1739 us, so 130).  Two wait states
-// stand between a VALU write of an operand and its MFMA; who reads the result waits 24
-// (mma32_wait; the longest MFMA asks for 20).
+// 7 drafts, 256 dims: 59 us, so 53 in the same run) and spills Q (512 dims: 1739 us in the first
+// version, so 130).  Two wait states stand between a VALU write of an operand and its MFMA; who
+// reads the result waits 24 (mma32_wait; the longest MFMA asks for 20).
 template <bool BF>
 __device__ __forceinline__ void mma32_acc(f32x16& c, u32x4 a, u32x4 b) {
   if constexpr (BF)
@@ -453,7 +454,7 @@ __device__ __forceinline__ void mma32_wait(f32x16& c) {
 __device__ __forceinline__ void in_acc(f32x16& c) { asm volatile("" : "+a"(c)); }
 
 // NT: loads past the caches, where no other q-block reads the same K and V (64 trees of 16
-// drafts 237 -> 216 us; of 61 drafts, two q-blocks: 124 -> 129 with it).
+// drafts 205 us, without it 227; of 61 drafts, two q-blocks, it cost 4 %).
 template <int DT, int DK, int DV, bool LAT, int RG, int MODE, bool NT>
 __global__ __launch_bounds__(kRbThreads, (RowsTile<DK, DV, LAT, RG>::kOcc)) void
 fa2_decode_rows_kernel(RowsArgs ra) {

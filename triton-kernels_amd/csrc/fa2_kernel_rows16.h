@@ -11,7 +11,7 @@
 //
 // Measured on MI355X: 16 latents of 16000-32768 keys, 16 heads, 83 us per call (5.3 TB/s; a
 // copy reaches 5.1, a plain read 6.9; equal shares end up to 10 % apart), 4 of 700-1100 keys
-// 17.5 (the 32-row kernel 26): 1.0 us to locate the segment, 1.4 and 2.2 for block table and Q,
+// 17.4 (the 32-row kernel 26): 1.0 us to locate the segment, 1.4 and 2.2 for block table and Q,
 // 4 for the states, 3.9 for the merge.
 #pragma once
 

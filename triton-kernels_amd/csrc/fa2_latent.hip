@@ -94,7 +94,7 @@ int rows_plan(const RowsCall& c, RowsPlan* pl) {
   pl->rows = c.q_heads / c.kv_heads * c.q_len;
   if (pl->rows > kLim) return FA2_ERR_TOO_LARGE;
   const int64_t cus = cu_count_current_device();
-  // The smallest q-block that holds the rows (4 x 900 keys of 16 heads: 17.8 us with up to 16
+  // The smallest q-block that holds the rows (4 x 900 keys of 16 heads: 17.4 us with up to 16
   // rows, 26 with 32; 128-row blocks read K and V least often beyond that).
   const int64_t least = c.dv == 64 ? 2 : 1;  // (a wave has 32 dims at least)
   pl->rg = static_cast<int>(pl->rows <= kR16Rows ? 0
@@ -368,10 +368,13 @@ int prefill_plan(const fa2_latent_prefill_params* p, PrefillPlan* pl) {
   };
   if (items(kBM) * p->heads > kMaxGrid - kXcds) return FA2_ERR_TOO_LARGE;
   // Pairs of q-blocks on one workgroup per CU where sequences have four q-blocks on average
-  // (a lone block leaves half of the workgroup without rows) and the pairs fill the CUs: 854
-  // TFLOP/s on 16 prompts of 128-4096.  Else one q-block per workgroup, two workgroups per CU,
-  // the keys split over idle ones: one prompt of 333, 16 heads 15.1 us (pairs 19), 8 chunks of
-  // 100-512 over 4000 more 112 (pairs 133-166).
+  // (a lone block leaves half of the workgroup without rows) and the pairs fill the CUs: 825 to
+  // 855 TFLOP/s on 16 prompts of 128-4096.  Else one q-block per workgroup, two workgroups per
+  // CU, the keys split over idle ones: one prompt of 333, 16 heads 15.1 us (pairs 19); in one
+  // run, 8 chunks of 100-512 rows over up to 4000 more, 16 heads, 118 (pairs 143), of 384-512 over
+  // none 28 (33), over up to 1000 58 (62), over up to 4000 141 (151).  Ragged pairs read the shared
+  // part's prefix sum anew for each tile and wait for all loads there, which dense ones and one
+  // q-block do not: 16 prompts of 2048 take 852 ragged and 835 dense.
   const bool many = ragged ? p->q_len >= 4 * kBM * p->batch : nqb >= 4;
   pl->pair = many && cus >= kXcds && items(2 * kBM) * p->heads >= cus;
   pl->work_ub = items(pl->pair ? 2 * kBM : kBM);

@@ -16,8 +16,9 @@ strides that start on 16 bytes are read in place, such as k and v as views of on
 up-projection and k_rope as a view of the finished rows.  ``is_causal`` and
 ``causal_alignment`` are those of ``flash_attention_v2`` (the reference's
 kernels/attention.py:749-927), whose kernel and numerics these are; ``softmax_scale``:
-``(D + 64) ** -0.5`` unless given.  The computation runs in ``libfa2.so``
-(``fa2_latent_prefill``, include/fa2_latent.h); no fallback.
+``(D + 64) ** -0.5`` unless given.  Values that the mask hides from a row may be multiplied by
+zero, so they have to be finite (what lies behind a sequence's end need not be).  The
+computation runs in ``libfa2.so`` (``fa2_latent_prefill``, include/fa2_latent.h); no fallback.
 """
 
 from __future__ import annotations
