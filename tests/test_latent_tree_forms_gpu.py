@@ -11,7 +11,8 @@ import torch
 
 import kernels
 from kernels import _fa2
-from test_latent_gpu import decode_case, i32, prefill_case, prefill_check, randn
+from test_latent_gpu import (append_case, decode_case, decode_check, i32, prefill_case,
+                             prefill_check, randn)
 from test_tree_decode_gpu import make, verify
 
 pytestmark = pytest.mark.gpu
@@ -206,3 +207,106 @@ def test_prefill_rows_past_4_gib(q_lens, kv_lens, h):
     up[..., :64], up[..., 64:] = k, v
     o = kernels.latent_attention(q, up[..., :64], kr, up[..., 64:], q_indptr=qi, kv_indptr=ki, **f)
     assert torch.equal(o, ref)
+
+
+# ---- graphs whose inputs change between replays ----------------------------------------
+
+def capture(f):
+    f()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = f()
+    return graph, out
+
+
+def test_append_in_a_graph():
+    """A captured append writes what its buffers hold at the replay."""
+    lens, starts, page = [1, 3, 0, 40], [0, 15, 7, 100], 16
+    x, w, rope, table, cache, _ = append_case(512, BF, [64] * 4, [200] * 4, page)
+    table, sp = table.cuda(), i32(starts)
+    ip = i32([0] + lens).cumsum(0).to(torch.int32)
+    first = cache.clone()
+    graph, rows = capture(lambda: kernels.paged_latent_append(cache, table, x, ip, w, rope, sp,
+                                                              return_rows=True))
+    for i, (ln, st) in enumerate([(lens, starts), ([2, 2, 2, 2], [9, 0, 31, 190]),
+                                  ([64] * 4, [100, 0, 199, 5]), ([0, 0, 0, 0], [1] * 4)]):
+        ip.copy_(i32([0] + ln).cumsum(0))
+        sp.copy_(i32(st))
+        x.copy_(randn(*x.shape, dtype=BF, seed=50 + i))
+        cache.copy_(first)
+        graph.replay()
+        eager = first.clone()
+        want = kernels.paged_latent_append(eager, table, x, ip, w, rope, sp, return_rows=True)
+        torch.cuda.synchronize()
+        assert torch.equal(cache, eager) and torch.equal(rows[:sum(ln)], want[:sum(ln)]), i
+
+
+@pytest.mark.parametrize("latent,hq,m", [(512, 128, 0), (512, 16, 0), (256, 32, 7)])
+def test_latent_decode_in_a_graph(latent, hq, m):
+    """A captured decode call goes by the lengths, the table, the queries and the mask of
+    the replay: whole units, cut ones and empty ones from one plan."""
+    page, b, width = 16, 4, 200
+    q, cache, table, t = decode_case(latent, BF, [width * page] * b, hq, m, page, tree=m > 0)
+    c, bt, li = cache.cuda(), table.cuda(), i32([1] * b)
+    t = t.cuda() if m else None
+    f = dict(latent_dim=latent, softmax_scale=0.07, kv_indptr=li, block_table=bt, tree_mask=t)
+    graph, out = capture(lambda: kernels.latent_decode_attention(q, c, **f))
+    for i, lens in enumerate([[3200] * 4, [1, 40, 64, 65], [3100, 0, 700, 2], [10] * 4,
+                              [5000, -1, 129, 3200]]):
+        li.copy_(i32(lens))
+        q.copy_(randn(*q.shape, dtype=BF, seed=90 + i))
+        bt.copy_(bt.roll(1, 0).clone())
+        if m:
+            t.copy_(t.roll(1, 0).clone())
+        out.zero_()
+        graph.replay()
+        want = kernels.latent_decode_attention(q, c, **f)
+        torch.cuda.synchronize()
+        assert torch.equal(out.nan_to_num(7.0), want.nan_to_num(7.0)), i
+        fresh = decode_case(latent, BF, [width * page] * b, hq, m, page, tree=m > 0)[1]
+        held = [min(max(n, 0), width * page) for n in lens]
+        decode_check(out, q, fresh, bt.cpu(), held, latent, 0.07, False,
+                     t.cpu() if m else None, page)
+
+
+@pytest.mark.parametrize("m,hq,hkv,d", [(9, 8, 2, 128), (3, 4, 4, 64), (20, 4, 1, 256)])
+def test_tree_decode_in_a_graph(m, hq, hkv, d):
+    q, ks, vs, t, (k, v), kw = make("paged", BF, [2600, 2600, 2600], hq, hkv, m, d)
+    t, li = t.cuda(), kw["kv_indptr"]
+    graph, out = capture(lambda: kernels.tree_decode_attention(q, k, v, t, **kw))
+    for i, lens in enumerate([[2600, 1, 300], [0, 64, 63], [2600] * 3, [30, 2000, 1000]]):
+        li.copy_(i32(lens))
+        q.copy_(randn(*q.shape, dtype=BF, seed=40 + i))
+        t.copy_(t.roll(1, 0).clone())
+        out.zero_()
+        graph.replay()
+        want = kernels.tree_decode_attention(q, k, v, t, **kw)
+        torch.cuda.synchronize()
+        assert torch.equal(out.nan_to_num(7.0), want.nan_to_num(7.0)), i
+        verify(out, q, [x[:n] for x, n in zip(ks, lens)], [x[:n] for x, n in zip(vs, lens)],
+               t.cpu())
+
+
+@pytest.mark.parametrize("h", [2, 24], ids=["blocks", "claimed"])
+def test_prefill_in_a_graph(h):
+    """A captured ragged prefill goes by the prefix sums of the replay."""
+    tq, tk = 2140, 3700
+    q, k, kr, v = prefill_case(128, BF, [tq], [tk], h)
+    qi, ki = torch.zeros(4, dtype=torch.int32, device="cuda"), i32([0] * 4)
+    f = dict(is_causal=True, causal_alignment="bottom_right", q_indptr=qi, kv_indptr=ki)
+    graph, out = capture(lambda: kernels.latent_attention(q, k, kr, v, **f))
+    for i, (ql, kl) in enumerate([([500, 600, 1040], [500, 700, 2500]), ([2140, 0, 0], [2140, 5, 0]),
+                                  ([1, 2, 3], [3000, 2, 600]), ([130, 300, 7], [130, 300, 9])]):
+        qi.copy_(i32([0] + ql).cumsum(0))
+        ki.copy_(i32([0] + kl).cumsum(0))
+        q.copy_(randn(*q.shape, dtype=BF, seed=60 + i))
+        out.zero_()
+        graph.replay()
+        want = kernels.latent_attention(q, k, kr, v, **f)
+        torch.cuda.synchronize()
+        n, nk = sum(ql), sum(kl)
+        assert torch.equal(out[:n].nan_to_num(7.0), want[:n].nan_to_num(7.0)), i
+        assert (out[n:] == 0).all()  # rows of nobody are left as they were
+        prefill_check(out[:n], q[:n], k[:nk], kr[:nk], v[:nk], ql, kl, "bottom_right",
+                      192 ** -0.5)
